@@ -699,6 +699,58 @@ int rk_kv_append(const void* k, int64_t skb, int64_t skh, int64_t sks, const voi
                  int64_t B, int64_t H, int64_t S, int64_t D, int64_t max_len, int64_t start,
                  int64_t clear_to, void* stream);
 
+/*
+ * The plan of an attention mask: for rows of S positions, documents (int32, or int64 with wide
+ * != 0; row stride sdb; NULL: one document per row) and marked positions prefix (0 / 1 bytes,
+ * row stride spb; NULL: none). A document is a run of equal ids >= 0; negative ids are padding.
+ * Query i sees key j of its document if j <= i, or if j lies in the run of marked positions that
+ * the document begins with. bounds: int32 [4][B][S], per position the keys [bounds[0],
+ * bounds[1]) a query there sees and the queries [bounds[2], bounds[3]) that see a key there
+ * (zeros: none); padding: one bit per position, [B][(S + 31) / 32] words. S <= 2^27.
+ * No counterpart in the reference (its windows hold one text each, model.py:117-123).
+ */
+int rk_attention_mask(const void* documents, int wide, int64_t sdb, const uint8_t* prefix,
+                      int64_t spb, int64_t B, int64_t S, int32_t* bounds, uint32_t* padding,
+                      void* stream);
+
+/*
+ * Attention with modified scores: bf16 q, o, g, dq [B, H, S, D], k, v, dk, dv [B, Hkv, S, D]
+ * (element strides batch, head, position; unit feature stride), H a multiple of Hkv (query head h
+ * reads key head h / (H / Hkv)), D = 64 or 128. With bounds as rk_attention_mask writes them
+ * (mask_batch 1 or B rows; NULL: causal),
+ *   s_ij = scale q_i . k_j;  softcap > 0: s = softcap tanh(s / softcap);
+ *   slopes (float32 [H]): s -= slopes[h] |i - j|;
+ *   o_i = sum_j softmax_j(s_ij over the keys i sees) v_j,  lse_i = log sum_j exp(s_ij).
+ * A query that sees nothing gets zeros (lse 0); what padding positions hold does not matter.
+ * The backward reads o, lse and the gradient g of o, and writes dq, dk, dv and, where given,
+ * dslopes (float32 [H]); work: rk_scored_attention_backward_work floats. Scores and softmax run
+ * in float32; probabilities and score gradients enter the products rounded to bf16; every sum
+ * has a fixed order. Inputs 16-byte aligned, outputs 8-byte, strides multiples of 8 elements, one
+ * head's positions under 2^31 bytes, fewer than 2^24 blocks of 128 positions; otherwise
+ * RK_ERR_UNSUPPORTED.
+ * No counterpart in the reference (it attends without cap, bias or mask, model.py:117-123).
+ */
+typedef struct rk_scored_attention_args {
+  const uint16_t *q, *k, *v;
+  uint16_t* o;
+  float* lse; /* [B, H, S] contiguous */
+  const int32_t* bounds;
+  const uint32_t* padding;
+  const float* slopes;
+  const uint16_t* g;
+  uint16_t *dq, *dk, *dv;
+  float* dslopes;
+  int64_t B, H, Hkv, S, D, mask_batch;
+  int64_t sqb, sqh, sqs, skb, skh, sks, svb, svh, svs, sob, soh, sos, sgb, sgh, sgs;
+  int64_t sxb, sxh, sxs; /* dq */
+  int64_t syb, syh, sys; /* dk and dv */
+  float scale, softcap;
+} rk_scored_attention_args;
+
+int rk_scored_attention_forward(const rk_scored_attention_args* args, void* stream);
+int64_t rk_scored_attention_backward_work(int64_t B, int64_t H, int64_t S, int slopes);
+int rk_scored_attention_backward(const rk_scored_attention_args* args, float* work, void* stream);
+
 /* HBM streaming probe (measurement only; no counterpart in the reference): reads `bytes`
  * (a multiple of 16) from src in 16-byte vectors, `unroll` (1, 2, 4, 8) loads in flight
  * per thread, `blocks` blocks of 256 threads in a grid-stride loop; copy != 0 writes them

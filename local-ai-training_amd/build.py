@@ -51,11 +51,12 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (ROCm is required to build libratchet_hip.so)")
 
 
-# Per-source flags. rk_attention.hip: MFMA results in VGPRs (the attention's softmax and
+# Per-source flags. The attention forwards: MFMA results in VGPRs (the attention's softmax and
 # output rescale read every accumulator with VALU instructions; in AGPRs each read and write
 # back is an extra copy, about as many instructions as the softmax itself).
 SOURCE_FLAGS = {
     "rk_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "rk_scored.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -1041,6 +1041,165 @@ void kv_append(const Tensor& k, const Tensor& v, Tensor& keys, Tensor& values, i
                "rk_kv_append");
 }
 
+// The plan of a mask (rk_attention_mask): bounds int32 [4, B, S], padding int32 [B, ceil(S / 32)].
+std::tuple<Tensor, Tensor> attention_mask(const OptTensor& documents, const OptTensor& prefix) {
+  TORCH_CHECK(documents.has_value() || prefix.has_value(),
+              "attention mask: documents or prefix must be given");
+  const Tensor& like = documents.has_value() ? *documents : *prefix;
+  require_gpu(like, "attention mask");
+  TORCH_CHECK(like.dim() == 2, "attention mask: documents and prefix must be [B, S]");
+  Tensor ids, marks;
+  const auto rows = [](const Tensor& t) {
+    return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
+  };
+  const c10::DeviceGuard guard(like.device());
+  if (documents.has_value()) {
+    TORCH_CHECK(documents->scalar_type() == at::kInt || documents->scalar_type() == at::kLong,
+                "attention mask: documents must be int32 or int64");
+    ids = rows(*documents);
+  }
+  if (prefix.has_value()) {
+    same_device(like, *prefix, "attention mask");
+    TORCH_CHECK(prefix->sizes() == like.sizes() && prefix->scalar_type() == at::kBool,
+                "attention mask: prefix must be a bool tensor of the documents' shape");
+    marks = rows(*prefix);
+  }
+  const int64_t B = like.size(0), S = like.size(1);
+  const auto i32 = like.options().dtype(at::kInt);
+  Tensor bounds = at::empty({4, B, S}, i32), padding = at::empty({B, (S + 31) / 32}, i32);
+  check_status(
+      rk_attention_mask(ids.defined() ? ids.data_ptr() : nullptr,
+                        ids.defined() && ids.scalar_type() == at::kLong,
+                        ids.defined() ? ids.stride(0) : 0,
+                        marks.defined() ? static_cast<const uint8_t*>(marks.data_ptr()) : nullptr,
+                        marks.defined() ? marks.stride(0) : 0, B, S, bounds.data_ptr<int32_t>(),
+                        static_cast<uint32_t*>(padding.data_ptr()), stream_of(like)),
+      "rk_attention_mask");
+  return {bounds, padding};
+}
+
+// What forward and backward of attention with modified scores share: checked operands as
+// rk_scored_attention_args. `keep` holds the copies of operands that the kernels' 16-byte loads do
+// not take as they lie.
+rk_scored_attention_args scored_args(const Tensor& q, const Tensor& k, const Tensor& v,
+                                     const OptTensor& bounds, const OptTensor& padding,
+                                     const OptTensor& slopes, double softcap, double scale,
+                                     std::vector<Tensor>& keep) {
+  constexpr const char* what = "scored attention";
+  require_gpu(q, what);
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+                  k.size(2) == q.size(2) && k.size(3) == q.size(3),
+              what, ": q must be [B, H, S, D] and k, v [B, Hkv, S, D]");
+  TORCH_CHECK(k.size(1) > 0 ? q.size(1) % k.size(1) == 0 : q.size(1) == 0, what,
+              ": query heads must be a multiple of the key heads");
+  rk_scored_attention_args a{};
+  a.B = q.size(0), a.H = q.size(1), a.Hkv = k.size(1), a.S = q.size(2), a.D = q.size(3);
+  const auto operand = [&](const Tensor& t) -> Tensor {
+    same_device(q, t, what);
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16, what, ": operands must be bfloat16");
+    bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
+    keep.push_back(ok ? t : t.clone(at::MemoryFormat::Contiguous));
+    return keep.back();
+  };
+  const c10::DeviceGuard guard(q.device());
+  const Tensor qq = operand(q), kk = operand(k), vv = operand(v);
+  const auto p16 = [](const Tensor& t) { return static_cast<const uint16_t*>(t.data_ptr()); };
+  a.q = p16(qq), a.sqb = qq.stride(0), a.sqh = qq.stride(1), a.sqs = qq.stride(2);
+  a.k = p16(kk), a.skb = kk.stride(0), a.skh = kk.stride(1), a.sks = kk.stride(2);
+  a.v = p16(vv), a.svb = vv.stride(0), a.svh = vv.stride(1), a.svs = vv.stride(2);
+  TORCH_CHECK(bounds.has_value() == padding.has_value(), what,
+              ": a mask's bounds and padding go together");
+  if (bounds.has_value()) {
+    same_device(q, *bounds, what);
+    same_device(q, *padding, what);
+    TORCH_CHECK(bounds->scalar_type() == at::kInt && bounds->dim() == 3 && bounds->size(0) == 4 &&
+                    (bounds->size(1) == 1 || bounds->size(1) == a.B) && bounds->size(2) == a.S &&
+                    bounds->is_contiguous(),
+                what, ": the mask must hold one row or one per sequence, of q's length");
+    TORCH_CHECK(padding->scalar_type() == at::kInt && padding->dim() == 2 &&
+                    padding->size(0) == bounds->size(1) &&
+                    padding->size(1) == (a.S + 31) / 32 && padding->is_contiguous(),
+                what, ": the mask's padding must be int32 [rows, ceil(S / 32)]");
+    a.bounds = bounds->data_ptr<int32_t>();
+    a.padding = static_cast<const uint32_t*>(padding->data_ptr());
+    a.mask_batch = bounds->size(1);
+  }
+  if (slopes.has_value()) {
+    same_device(q, *slopes, what);
+    keep.push_back(f32_vector(*slopes, a.H, "slopes"));
+    a.slopes = keep.back().data_ptr<float>();
+  }
+  a.softcap = static_cast<float>(softcap);
+  a.scale = static_cast<float>(scale);
+  return a;
+}
+
+// Attention with modified scores (rk_scored_attention_forward): (o, lse), o as a [B, H, S, D] view
+// of [B, S, H, D] memory.
+std::tuple<Tensor, Tensor> scored_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                                            const OptTensor& bounds, const OptTensor& padding,
+                                            const OptTensor& slopes, double softcap,
+                                            double scale) {
+  std::vector<Tensor> keep;
+  rk_scored_attention_args a = scored_args(q, k, v, bounds, padding, slopes, softcap, scale, keep);
+  const c10::DeviceGuard guard(q.device());
+  Tensor o = at::empty({a.B, a.S, a.H, a.D}, q.options()).permute({0, 2, 1, 3});
+  Tensor lse = at::empty({a.B, a.H, a.S}, q.options().dtype(at::kFloat));
+  a.o = static_cast<uint16_t*>(o.data_ptr());
+  a.sob = a.S * a.H * a.D, a.soh = a.D, a.sos = a.H * a.D;
+  a.lse = lse.data_ptr<float>();
+  check_status(rk_scored_attention_forward(&a, stream_of(q)), "rk_scored_attention_forward");
+  return {o, lse};
+}
+
+// Its backward (rk_scored_attention_backward): dq, dk, dv as [B, heads, S, D] views of
+// [B, S, heads, D] memory, and dslopes [H] (empty unless slope_grad).
+std::tuple<Tensor, Tensor, Tensor, Tensor> scored_attention_backward(
+    const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
+    const Tensor& lse, const OptTensor& bounds, const OptTensor& padding, const OptTensor& slopes,
+    double softcap, double scale, bool slope_grad) {
+  std::vector<Tensor> keep;
+  rk_scored_attention_args a = scored_args(q, k, v, bounds, padding, slopes, softcap, scale, keep);
+  const c10::DeviceGuard guard(q.device());
+  const auto rows = [&](const Tensor& t) -> Tensor {
+    same_device(q, t, "scored attention backward");
+    TORCH_CHECK(t.sizes() == q.sizes() && t.scalar_type() == at::kBFloat16,
+                "scored attention backward: o and its gradient must be bfloat16 of q's shape");
+    bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0;
+    keep.push_back(ok ? t : t.clone(at::MemoryFormat::Contiguous));
+    return keep.back();
+  };
+  const Tensor oo = rows(o), gg = rows(grad);
+  same_device(q, lse, "scored attention backward");
+  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.dim() == 3 && lse.size(0) == a.B &&
+                  lse.size(1) == a.H && lse.size(2) == a.S && lse.is_contiguous(),
+              "scored attention backward: lse must be a contiguous float32 [B, H, S] tensor");
+  TORCH_CHECK(!slope_grad || slopes.has_value(),
+              "scored attention backward: a slope gradient needs slopes");
+  const auto out = [&](int64_t heads) {
+    return at::empty_strided({a.B, heads, a.S, a.D}, {a.S * heads * a.D, a.D, heads * a.D, 1},
+                             q.options());
+  };
+  Tensor dq = out(a.H), dk = out(a.Hkv), dv = out(a.Hkv);
+  Tensor dslopes = at::empty({slope_grad ? a.H : 0}, lse.options());
+  if (q.numel() == 0) return {dq, dk, dv, dslopes.zero_()};
+  Tensor work = at::empty({rk_scored_attention_backward_work(a.B, a.H, a.S, slope_grad)},
+                          lse.options());
+  const auto w16 = [](const Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); };
+  a.o = w16(oo), a.sob = oo.stride(0), a.soh = oo.stride(1), a.sos = oo.stride(2);
+  a.g = w16(gg), a.sgb = gg.stride(0), a.sgh = gg.stride(1), a.sgs = gg.stride(2);
+  a.lse = lse.data_ptr<float>();
+  a.dq = w16(dq), a.dk = w16(dk), a.dv = w16(dv);
+  a.sxb = a.S * a.H * a.D, a.sxh = a.D, a.sxs = a.H * a.D;
+  a.syb = a.S * a.Hkv * a.D, a.syh = a.D, a.sys = a.Hkv * a.D;
+  a.dslopes = slope_grad ? dslopes.data_ptr<float>() : nullptr;
+  check_status(rk_scored_attention_backward(&a, work.data_ptr<float>(), stream_of(q)),
+               "rk_scored_attention_backward");
+  return {dq, dk, dv, dslopes};
+}
+
 // Means of segments [offsets[s], offsets[s + 1]) of a float32 row-rms buffer (rk_row_rms_means).
 Tensor row_rms_means(const Tensor& row_rms, const Tensor& offsets) {
   require_gpu(row_rms, "row rms means");
@@ -1190,6 +1349,12 @@ TORCH_LIBRARY(ratchet, m) {
   m.def("attention_forward(Tensor q, Tensor k, Tensor v, float scale) -> (Tensor, Tensor)");
   m.def("attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, "
         "float scale) -> (Tensor, Tensor, Tensor)");
+  m.def("attention_mask(Tensor? documents, Tensor? prefix) -> (Tensor, Tensor)");
+  m.def("scored_attention(Tensor q, Tensor k, Tensor v, Tensor? bounds, Tensor? padding, "
+        "Tensor? slopes, float softcap, float scale) -> (Tensor, Tensor)");
+  m.def("scored_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor o, "
+        "Tensor lse, Tensor? bounds, Tensor? padding, Tensor? slopes, float softcap, "
+        "float scale, bool slope_grad) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("kv_append(Tensor k, Tensor v, Tensor(a!) keys, Tensor(b!) values, int start, "
         "int clear_to) -> ()");
   m.def("cross_entropy_forward(Tensor logits, Tensor targets, int ignore_index=-100) -> "
@@ -1234,6 +1399,9 @@ TORCH_LIBRARY_IMPL(ratchet, CUDA, m) {
   m.impl("row_rms_means", &row_rms_means);
   m.impl("attention_forward", &attention_forward);
   m.impl("attention_backward", &attention_backward);
+  m.impl("attention_mask", &attention_mask);
+  m.impl("scored_attention", &scored_attention);
+  m.impl("scored_attention_backward", &scored_attention_backward);
   m.impl("kv_append", &kv_append);
   m.impl("cross_entropy_forward", &cross_entropy_forward);
   m.impl("cross_entropy_backward", &cross_entropy_backward);

@@ -1,0 +1,129 @@
+// Pieces shared by the forward and backward of attention with modified scores (rk_scored.hip,
+// rk_scored_bwd.hip): the arguments, the score's modification and the mask's intervals.
+//
+// A score in base-2 units, from the dot product x = q . k and the distance |i - j|:
+//   plain   t = x scale log2(e)
+//   capped  t = cap log2(e) tanh(x scale / cap) = C - 2 C r,  r = 1 / (exp2(x c) + 1),
+//           C = cap log2(e),  c = 2 log2(e) scale / cap;   1 - tanh^2 = 4 r (1 - r)
+//   biased  t - slope log2(e) |i - j|
+// exp2 and the reciprocal are the hardware's (1 ulp): the capped score is off by at most a few
+// 2^-24 of the cap, 2e-5 of a probability at cap 50 against the 2^-9 of its rounding to bf16.
+//
+// A mask is two intervals per position (rk_attention_mask): the keys [key_lo, key_hi) that a
+// query sees and the queries [query_lo, query_hi) that see a key. A position that sees nothing
+// has empty ones. Both kernels test the intervals of the rows they own, one per lane.
+#pragma once
+
+#include "rk_attention.h"
+
+namespace rk {
+
+struct ScoredArgs {
+  rk_scored_attention_args p;
+  int64_t G;        // query heads per key head
+  int64_t S32;      // padding words per row
+  int64_t Sp;       // S rounded up to 128 (row statistics)
+  float dot_scale;  // plain: scale log2(e); capped: 2 log2(e) scale / cap
+  float cap2;       // cap log2(e)
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Span {
+  int lo, hi;  // what this lane's row sees; rows without any see everything and are discarded
+  bool valid;
+};
+
+// The interval of row `row` (0 .. S - 1, or past it) of batch b; `kind` 0: keys of a query,
+// 2: queries of a key. Without a mask: causal.
+__device__ __forceinline__ Span row_span(const rk_scored_attention_args& p, int kind, int64_t b,
+                                         int row) {
+  const int S = static_cast<int>(p.S);
+  Span s{0, 0, row < S};
+  if (s.valid) {
+    if (p.bounds) {
+      const int32_t* at = p.bounds + (kind * p.mask_batch + (p.mask_batch > 1 ? b : 0)) * p.S + row;
+      s.lo = at[0] > 0 ? at[0] : 0;
+      s.hi = at[p.mask_batch * p.S];
+      s.hi = s.hi < S ? s.hi : S;
+    } else {
+      s.lo = kind == 0 ? 0 : row;
+      s.hi = kind == 0 ? row + 1 : S;
+    }
+    s.valid = s.hi > s.lo;
+  }
+  return s;
+}
+
+__device__ __forceinline__ int wave_min_int(int v) {
+  return wave_butterfly(v, [](int a, int b) { return a < b ? a : b; });
+}
+__device__ __forceinline__ int wave_max_int(int v) {
+  return wave_butterfly(v, [](int a, int b) { return a > b ? a : b; });
+}
+
+// What a wavefront's rows see: anything lies in [lo, hi), everything in [all_lo, all_hi).
+struct WaveSpan {
+  int lo, hi, all_lo, all_hi;
+  __device__ __forceinline__ explicit WaveSpan(Span& s) {
+    lo = __builtin_amdgcn_readfirstlane(wave_min_int(s.valid ? s.lo : 0x7fffffff));
+    hi = __builtin_amdgcn_readfirstlane(wave_max_int(s.valid ? s.hi : 0));
+    all_lo = __builtin_amdgcn_readfirstlane(wave_max_int(s.valid ? s.lo : 0));
+    all_hi = __builtin_amdgcn_readfirstlane(wave_min_int(s.valid ? s.hi : 0x7fffffff));
+    if (!s.valid) {
+      s.lo = 0;
+      s.hi = 0x7fffffff;
+    }
+  }
+  __device__ __forceinline__ bool none(int r0, int rows) const { return r0 >= hi || r0 + rows <= lo; }
+  __device__ __forceinline__ bool all(int r0, int rows) const {
+    return r0 >= all_lo && r0 + rows <= all_hi;
+  }
+};
+
+// The workgroup's range over its four wavefronts' (box: 8 ints of LDS).
+__device__ __forceinline__ void block_range(const WaveSpan& w, int wave, int lane, int* box,
+                                            int& lo, int& hi) {
+  if (lane == 0) {
+    box[wave] = w.lo;
+    box[4 + wave] = w.hi;
+  }
+  __syncthreads();
+  lo = box[0];
+  hi = box[4];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    lo = box[i] < lo ? box[i] : lo;
+    hi = box[4 + i] > hi ? box[4 + i] : hi;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+}
+
+// Padding bits of rows row0 .. row0 + R - 1 (row0 a multiple of 32) of batch b.
+template <int R>
+__device__ __forceinline__ uint64_t padding_bits(const ScoredArgs& a, int64_t b, int row0) {
+  if (!a.p.padding) return 0;
+  const uint32_t* at = a.p.padding + (a.p.mask_batch > 1 ? b : 0) * a.S32;
+  const int w = row0 / 32;
+  uint64_t bits = at[w];
+  if constexpr (R == 64) {
+    if (w + 1 < a.S32) bits |= static_cast<uint64_t>(at[w + 1]) << 32;
+  }
+  return bits;
+}
+
+// Zeros the padding rows of a staged tile: their values, which may be anything, meet
+// probabilities of zero. Every thread of the workgroup calls it, between two barriers.
+template <int D, int R>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, uint64_t bits, int tid) {
+  constexpr int SEGS = D / 8;
+  for (int i = tid; i < R * SEGS; i += 256)
+    if (bits >> (i / SEGS) & 1)
+      *reinterpret_cast<uint4*>(tile + 16 * i) = make_uint4(0, 0, 0, 0);
+}
+
+int check_scored(const rk_scored_attention_args& p, bool backward);
+ScoredArgs scored_args(const rk_scored_attention_args& p);
+
+}  // namespace rk

@@ -1,0 +1,434 @@
+// Causal self-attention whose scores are capped by a tanh, biased by the distance and masked by
+// documents and their prefixes: the mask's plan and the forward (gfx950). It stands beside
+// rk_attention_forward (model.py:117-123 attends without any of them) and shares its layout:
+//   s_ij = scale q_i . k_j,  s = cap tanh(s / cap),  s -= slope_h |i - j|,
+//   o_i = sum_j softmax_j(s_ij over the keys that i sees) v_j,  lse_i = log sum_j exp(s_ij).
+// A query that sees nothing gets o = 0. Query head h reads key head h / (H / Hkv).
+//
+// One workgroup = 128 queries of a head, one wavefront = 32, one lane = half the keys of one
+// query (rk_attention.hip describes the products). What differs:
+//  * the key range comes from the queries' intervals, so tiles outside every document of the
+//    workgroup are neither loaded nor computed; a wavefront skips tiles none of its rows sees and
+//    tests elements only in tiles that some row does not see whole;
+//  * capped or biased scores are modified before the running max, in base-2 units (rk_scored.h).
+#include "rk_scored.h"
+
+namespace rk {
+
+__device__ __forceinline__ float half_max2(float v) {
+  const uint32_t b = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum2(float v) {
+  const uint32_t b = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// R keys are staged per step, U of them make one update of the running max and sum.
+template <int D, int R, int U, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4)))
+void scored_fwd_kernel(ScoredArgs a) {
+  using T = AttnTile<D, R>;
+  constexpr int UT = U / 32;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kAttnStages * 2 * T::BYTES];
+  __shared__ int box[8];
+  const uint32_t lds0 = lds_address(smem);
+  const rk_scored_attention_args& p = a.p;
+  const int S = static_cast<int>(p.S);
+  const int64_t BH = p.B * p.H;
+  const int nqb = (S + kAttnRows - 1) / kAttnRows;
+  const int blk = static_cast<int>(blockIdx.x / BH);
+  const int qb = nqb - 1 - blk;  // longest causal rows first; heads fastest
+  const int64_t bh = blockIdx.x - blk * BH, b = bh / p.H, hd = bh - b * p.H, kvh = hd / a.G;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qw0 = qb * kAttnRows + 32 * wave, qi = qw0 + l32;  // this lane's query
+
+  v8bf_a qf[D / 16];
+  load_owned<D>(qf, p.q + b * p.sqb + hd * p.sqh, p.sqs, S, qi, h);
+  const TileDma<D, R> kd(p.k + b * p.skb + kvh * p.skh, p.sks, S, wave, lane);
+  const TileDma<D, R> vd(p.v + b * p.svb + kvh * p.svh, p.svs, S, wave, lane);
+  Span span = row_span(p, 0, b, qi);
+  const WaveSpan ws(span);
+  int lo, hi;
+  block_range(ws, wave, lane, box, lo, hi);
+  const int first = lo < hi ? lo / R : 0, end = lo < hi ? (hi + R - 1) / R : 0;
+  const uint32_t width = static_cast<uint32_t>(span.hi - span.lo);
+  float slope2 = 0.0f;
+  if constexpr (BIAS) slope2 = p.slopes[hd] * kLog2e;
+
+  auto issue = [&](int step) {
+    const uint32_t st = lds0 + (step & 1) * 2 * T::BYTES;
+    kd.issue(st, step * R, wave);
+    vd.issue(st + T::BYTES, step * R, wave);
+  };
+
+  float m = -INFINITY, l = 0.0f;
+  v16f_a o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) o[dt] = v16f_a{};
+  if (first < end) issue(first);
+  for (int step = first; step < end; ++step) {
+    const uint64_t pad = padding_bits<R>(a, b, step * R);
+    dma_wait_barrier<0>();
+    if (step + 1 < end) issue(step + 1);
+    uint8_t* const kt = smem + (step & 1) * 2 * T::BYTES;
+    uint8_t* const vt = kt + T::BYTES;
+    if (pad) {
+      clear_rows<D, R>(vt, pad, tid);
+      __syncthreads();
+    }
+    const int k0 = step * R;
+    if (ws.none(k0, R)) continue;
+    // S^T: lane holds keys k0 + 32 t + 8 (e / 4) + 4 h + e % 4 of its query
+    v16f_a sc[R / 32];
+#pragma unroll
+    for (int t = 0; t < R / 32; ++t) {
+      sc[t] = v16f_a{};
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, 32 * t, s, lane), qf[s],
+                                                        sc[t], 0, 0, 0);
+    }
+    // capped and biased scores in base-2 units here; plain ones are scaled with the max
+    const float mul = CAP || BIAS ? 1.0f : a.dot_scale;
+    if constexpr (CAP || BIAS) {
+      const float d0 = static_cast<float>(qi - k0 - 4 * h);
+#pragma unroll
+      for (int t = 0; t < R / 32; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float x = sc[t][e] * a.dot_scale;
+          if constexpr (CAP) {
+            const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f);
+            x = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
+          }
+          if constexpr (BIAS)
+            x = __builtin_fmaf(-slope2, fabsf(d0 - (32 * t + 8 * (e / 4) + (e % 4))), x);
+          sc[t][e] = x;
+        }
+    }
+    if (!ws.all(k0, R)) {
+      const int j0 = k0 + 4 * h - span.lo;
+#pragma unroll
+      for (int t = 0; t < R / 32; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (static_cast<uint32_t>(j0 + 32 * t + 8 * (e / 4) + (e % 4)) >= width)
+            sc[t][e] = -INFINITY;
+    }
+    // the updates' probabilities first, then their products
+    float alpha[R / U], ps[R / U];
+    uint4 pf[R / 32][2];
+#pragma unroll
+    for (int u = 0; u < R / U; ++u) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = u * UT; t < (u + 1) * UT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[t][e]);
+      mx = half_max2(mx);
+      const float mnew = fmaxf(m, mx * mul);
+      const float mref = mnew == -INFINITY ? 0.0f : mnew;  // a row with no key yet
+      alpha[u] = __builtin_amdgcn_exp2f(m - mref);
+      m = mnew;
+      ps[u] = 0.0f;
+#pragma unroll
+      for (int t = u * UT; t < (u + 1) * UT; ++t) {
+        float pr[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          pr[e] = __builtin_amdgcn_exp2f(CAP || BIAS ? sc[t][e] - mref
+                                                     : __builtin_fmaf(sc[t][e], mul, -mref));
+          ps[u] = ps[u] + pr[e];
+        }
+        pack16(pf[t], pr);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < R / U; ++u) {
+      // keys that no row of the wavefront sees: every p is zero, but their values may not be finite
+      if (ws.none(k0 + u * U, U)) continue;
+      if (__any(alpha[u] != 1.0f)) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * alpha[u];
+      }
+      l = l * alpha[u] + half_sum2(ps[u]);
+#pragma unroll
+      for (int t = u * UT; t < (u + 1) * UT; ++t)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt)
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                col_frag<D>(vt, 32 * t + 16 * s2, dt, lane), frag_of(pf[t][s2]), o[dt], 0, 0, 0);
+    }
+  }
+
+  if (qi < S) {
+    if (!span.valid) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[dt] = v16f_a{};
+    }
+    store_owned<D>(p.o + b * p.sob + hd * p.soh + static_cast<int64_t>(qi) * p.sos, o,
+                   span.valid ? 1.0f / l : 0.0f, h);
+    if (h == 0)
+      p.lse[bh * S + qi] = span.valid ? (m + __log2f(l)) * 0.69314718055994531f : 0.0f;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The plan: one workgroup per row, each thread 8 consecutive positions of a chunk of 8192, scans
+// over the threads' values by wavefront shuffles. The first pass takes, from the left, the
+// document's first position and whether the run of marked positions it begins with reaches here;
+// the second, from the right, the document's end and the end of that run.
+// ---------------------------------------------------------------------------
+constexpr int kMaskThreads = 1024, kMaskEach = 8, kMaskChunk = kMaskThreads * kMaskEach;
+
+struct MaskArgs {
+  const void* documents;  // int32 or int64 [B, S], or null (one document per row)
+  int wide;
+  const uint8_t* prefix;  // [B, S] 0 / 1, or null
+  int64_t sdb, spb;       // row strides
+  int64_t B, S, S32;
+  int32_t* bounds;        // [4][B][S]
+  uint8_t* padding;       // [B][S32][4]
+};
+
+// Inclusive max scan over the threads of the workgroup, left to right, two values at once;
+// returns the values before this thread (exclusive) and the totals. box: 32 ints.
+__device__ __forceinline__ void block_scan_max(int& x, int& y, int& tx, int& ty, int* box, int tid) {
+  const int lane = tid & 63, wave = tid >> 6;
+  int a = x, c = y;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int oa = __shfl_up(a, d, 64), oc = __shfl_up(c, d, 64);
+    if (lane >= d) {
+      a = a > oa ? a : oa;
+      c = c > oc ? c : oc;
+    }
+  }
+  __syncthreads();
+  if (lane == 63) {
+    box[wave] = a;
+    box[16 + wave] = c;
+  }
+  __syncthreads();
+  int ea = __shfl_up(a, 1, 64), ec = __shfl_up(c, 1, 64);
+  if (lane == 0) ea = ec = -0x7fffffff;
+  tx = ty = -0x7fffffff;
+  for (int w = 0; w < kMaskThreads / 64; ++w) {
+    const int ba = box[w], bc = box[16 + w];
+    if (w < wave) {
+      ea = ea > ba ? ea : ba;
+      ec = ec > bc ? ec : bc;
+    }
+    tx = tx > ba ? tx : ba;
+    ty = ty > bc ? ty : bc;
+  }
+  x = ea;
+  y = ec;
+}
+
+__device__ __forceinline__ int64_t document_of(const MaskArgs& a, int64_t b, int64_t i) {
+  if (!a.documents) return 0;
+  return a.wide ? static_cast<const int64_t*>(a.documents)[b * a.sdb + i]
+                : static_cast<const int32_t*>(a.documents)[b * a.sdb + i];
+}
+
+__global__ __launch_bounds__(kMaskThreads) void attention_mask_kernel(MaskArgs a) {
+  __shared__ int box[32];
+  const int64_t b = blockIdx.x;
+  const int tid = threadIdx.x, S = static_cast<int>(a.S);
+  int32_t* const key_lo = a.bounds + b * a.S;
+  int32_t* const key_hi = key_lo + a.B * a.S;
+  int32_t* const query_lo = key_hi + a.B * a.S;
+  int32_t* const query_hi = query_lo + a.B * a.S;
+  // left to right: key_lo = the document's first position, key_hi = 1 in its marked beginning
+  int begin0 = 0, broken0 = -1;
+  for (int c0 = 0; c0 < S; c0 += kMaskChunk) {
+    const int i0 = c0 + tid * kMaskEach;
+    int begin[kMaskEach], broken[kMaskEach];
+    uint32_t real = 0;
+    int bx = -0x7fffffff, by = -0x7fffffff;
+    if (i0 < S) {
+      int64_t before = i0 > 0 ? document_of(a, b, i0 - 1) : 0;
+#pragma unroll
+      for (int e = 0; e < kMaskEach; ++e) {
+        const int i = i0 + e;
+        const int64_t id = i < S ? document_of(a, b, i) : -1;
+        const bool mark = i < S && a.prefix && a.prefix[b * a.spb + i];
+        if (i == 0 || id != before) bx = i;
+        if (!mark) by = i;
+        before = id;
+        real |= static_cast<uint32_t>(id >= 0) << e;
+        begin[e] = bx;
+        broken[e] = by;
+      }
+    }
+    if (i0 < a.S32 * 32) {
+      const uint32_t inside = S - i0 >= 8 ? 0xffu : S > i0 ? (1u << (S - i0)) - 1u : 0u;
+      a.padding[b * a.S32 * 4 + i0 / 8] = static_cast<uint8_t>(~real & inside);
+    }
+    int ex = bx, ey = by, tx, ty;
+    block_scan_max(ex, ey, tx, ty, box, tid);
+    ex = ex > begin0 ? ex : begin0;
+    ey = ey > broken0 ? ey : broken0;
+#pragma unroll
+    for (int e = 0; e < kMaskEach; ++e) {
+      const int i = i0 + e;
+      if (i >= S) break;
+      const int bg = begin[e] > ex ? begin[e] : ex, br = broken[e] > ey ? broken[e] : ey;
+      const bool lead = br < bg;
+      key_lo[i] = bg;
+      key_hi[i] = lead;
+      query_lo[i] = lead ? bg : i;
+      query_hi[i] = real >> e & 1;
+    }
+    begin0 = tx > begin0 ? tx : begin0;
+    broken0 = ty > broken0 ? ty : broken0;
+  }
+  // right to left, as a max scan over mirrored positions: the least later position where a
+  // document begins (its end), and where one begins or the marked run is over.
+  __syncthreads();
+  int end0 = -S, stop0 = -S;
+  for (int c0 = 0; c0 < S; c0 += kMaskChunk) {
+    const int i0 = S - 1 - c0 - tid * kMaskEach;  // positions i0, i0 - 1, ..
+    int end[kMaskEach], stop[kMaskEach], lo[kMaskEach], lead[kMaskEach], real[kMaskEach];
+    int bx = -0x7fffffff, by = -0x7fffffff;
+#pragma unroll
+    for (int e = 0; e < kMaskEach; ++e) {
+      const int i = i0 - e;
+      end[e] = bx;  // over the later positions of this thread
+      stop[e] = by;
+      lo[e] = lead[e] = real[e] = 0;
+      if (i >= 0) {
+        lo[e] = key_lo[i];
+        lead[e] = key_hi[i];
+        real[e] = query_hi[i];
+        const bool begins = lo[e] == i;
+        if (begins) bx = -i;
+        if (begins || !lead[e]) by = -i;
+      }
+    }
+    int ex = bx, ey = by, tx, ty;
+    block_scan_max(ex, ey, tx, ty, box, tid);
+    ex = ex > end0 ? ex : end0;
+    ey = ey > stop0 ? ey : stop0;
+#pragma unroll
+    for (int e = 0; e < kMaskEach; ++e) {
+      const int i = i0 - e;
+      if (i < 0) break;
+      const int en = -(end[e] > ex ? end[e] : ex), st = -(stop[e] > ey ? stop[e] : ey);
+      if (real[e]) {
+        key_hi[i] = lead[e] ? st : i + 1;
+        query_hi[i] = en;
+      } else {
+        key_lo[i] = key_hi[i] = query_lo[i] = query_hi[i] = 0;
+      }
+    }
+    end0 = tx > end0 ? tx : end0;
+    stop0 = ty > stop0 ? ty : stop0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int check_scored(const rk_scored_attention_args& p, bool backward) {
+  if (p.B < 0 || p.H < 0 || p.Hkv < 0 || p.S < 0) return fail(RK_ERR_ARG, "negative size");
+  if (p.D != 64 && p.D != 128)
+    return fail(RK_ERR_UNSUPPORTED, "head size %lld (64 or 128 only)", static_cast<long long>(p.D));
+  if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
+  if (p.Hkv == 0 || p.H % p.Hkv != 0)
+    return fail(RK_ERR_ARG, "query heads must be a multiple of the key heads");
+  if (!(p.scale > 0.0f) || !(p.scale < INFINITY))
+    return fail(RK_ERR_ARG, "scale must be positive and finite");
+  if (!(p.softcap >= 0.0f) || !(p.softcap < INFINITY))
+    return fail(RK_ERR_ARG, "softcap must be finite and not negative (0: none)");
+  if (!p.q || !p.k || !p.v || !p.o || !p.lse) return fail(RK_ERR_ARG, "null pointer");
+  if (p.bounds && p.mask_batch != 1 && p.mask_batch != p.B)
+    return fail(RK_ERR_ARG, "a mask holds one row or one per sequence");
+  if ((p.bounds == nullptr) != (p.padding == nullptr))
+    return fail(RK_ERR_ARG, "a mask's intervals and padding bits go together");
+  const void* in16[] = {p.q, p.k, p.v, backward ? p.o : p.q, backward ? p.g : p.q};
+  for (const void* t : in16)
+    if (!t || !aligned16(t)) return fail(RK_ERR_UNSUPPORTED, "operands need 16-byte alignment");
+  const int64_t strides[] = {p.sqb, p.sqh, p.sqs, p.skb, p.skh, p.sks, p.svb, p.svh, p.svs,
+                             p.sob, p.soh, p.sos, backward ? p.sgb : 0, backward ? p.sgh : 0,
+                             backward ? p.sgs : 0, backward ? p.sxb : 0, backward ? p.sxh : 0,
+                             backward ? p.sxs : 0, backward ? p.syb : 0, backward ? p.syh : 0,
+                             backward ? p.sys : 0};
+  for (int64_t st : strides)
+    if (st < 0 || st % 8 != 0)
+      return fail(RK_ERR_UNSUPPORTED, "strides must be non-negative multiples of 8 elements");
+  // buffer offsets are 32-bit: the rows of one head up to the last tile's end, and its row
+  // statistics, lie below 2^31 bytes
+  const int64_t rows[] = {p.sqs, p.sks, p.svs, backward ? p.sos : 0, backward ? p.sgs : 0};
+  for (int64_t st : rows)
+    if (((p.S + 192) * st + p.D) * 2 >= (int64_t{1} << 31))
+      return fail(RK_ERR_UNSUPPORTED, "sequence extent exceeds 2^31 bytes per head");
+  const int64_t blocks = (p.S + kAttnRows - 1) / kAttnRows;
+  if (p.S > (int64_t{1} << 27) || p.B > (int64_t{1} << 24) || p.H > (int64_t{1} << 24) ||
+      p.B * p.H >= (int64_t{1} << 24) || p.B * p.H * blocks >= (int64_t{1} << 24))
+    return fail(RK_ERR_UNSUPPORTED, "2^24 blocks of 128 positions and more");
+  return RK_OK;
+}
+
+ScoredArgs scored_args(const rk_scored_attention_args& p) {
+  ScoredArgs a{};
+  a.p = p;
+  a.G = p.H / p.Hkv;
+  a.S32 = (p.S + 31) / 32;
+  a.Sp = (p.S + kAttnRows - 1) / kAttnRows * kAttnRows;
+  const bool cap = p.softcap > 0.0f;
+  a.dot_scale = cap ? 2.0f * kLog2e * (p.scale / p.softcap) : p.scale * kLog2e;
+  a.cap2 = p.softcap * kLog2e;
+  return a;
+}
+
+template <int D, int R, int U>
+static void launch_scored_fwd(const ScoredArgs& a, dim3 grid, hipStream_t st) {
+  const bool cap = a.p.softcap > 0.0f, bias = a.p.slopes != nullptr;
+  if (cap && bias) scored_fwd_kernel<D, R, U, true, true><<<grid, 256, 0, st>>>(a);
+  else if (cap) scored_fwd_kernel<D, R, U, true, false><<<grid, 256, 0, st>>>(a);
+  else if (bias) scored_fwd_kernel<D, R, U, false, true><<<grid, 256, 0, st>>>(a);
+  else scored_fwd_kernel<D, R, U, false, false><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace rk
+
+using namespace rk;
+
+extern "C" int rk_scored_attention_forward(const rk_scored_attention_args* args, void* stream) {
+  clear_error();
+  if (!args) return fail(RK_ERR_ARG, "null arguments");
+  const rk_scored_attention_args& p = *args;
+  if (int e = check_scored(p, false)) return e;
+  if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
+  if (reinterpret_cast<uintptr_t>(p.o) & 7) return fail(RK_ERR_UNSUPPORTED, "o needs 8-byte alignment");
+  const ScoredArgs a = scored_args(p);
+  const dim3 grid(static_cast<unsigned>(p.B * p.H * (a.Sp / kAttnRows)));
+  if (p.D == 64) launch_scored_fwd<64, 64, 64>(a, grid, as_stream(stream));
+  else launch_scored_fwd<128, 64, 32>(a, grid, as_stream(stream));
+  return launch_status("scored_attention_forward");
+}
+
+extern "C" int rk_attention_mask(const void* documents, int wide, int64_t sdb,
+                                 const uint8_t* prefix, int64_t spb, int64_t B, int64_t S,
+                                 int32_t* bounds, uint32_t* padding, void* stream) {
+  clear_error();
+  if (B < 0 || S < 0) return fail(RK_ERR_ARG, "negative size");
+  if (B == 0 || S == 0) return RK_OK;
+  if (!bounds || !padding) return fail(RK_ERR_ARG, "null pointer");
+  if (B > 0x7fffff || S > (int64_t{1} << 27)) return fail(RK_ERR_UNSUPPORTED, "mask too large");
+  const int64_t S32 = (S + 31) / 32;
+  MaskArgs a{documents, wide, prefix, sdb, spb, B, S, S32, bounds,
+             reinterpret_cast<uint8_t*>(padding)};
+  attention_mask_kernel<<<static_cast<unsigned>(B), kMaskThreads, 0, as_stream(stream)>>>(a);
+  return launch_status("attention_mask");
+}

@@ -1,0 +1,434 @@
+// The backward of attention with modified scores (rk_scored.hip; gfx950): from bf16 q, k, v, o,
+// the gradient g of o and the forward's log-sum-exp,
+//   p_ij = exp(s_ij - lse_i) where i sees j, else 0,     delta_i = g_i . o_i,
+//   d_ij = p_ij (g_i . v_j - delta_i)                    (gradient of the modified score)
+//   ds_ij = d_ij (1 - tanh^2)                            (of the plain one; no cap: d_ij)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij g_i,
+//   dslope_h = -sum_ij d_ij |i - j|.
+// Products of bf16 operands summed in float32; p and ds enter the second products rounded to
+// bf16 (half a step, 2^-9 relative); scores, exponentials, delta are float32. Two launches, as
+// at rk_attention_bwd.hip: the queries' (dq, and delta for the second) and the keys' (dk, dv; the
+// query heads that share a key head are summed by the one wavefront that owns the key, in order),
+// every output summed in a fixed order, so results repeat.
+//
+// The slopes' gradient takes three sums per query, of p dp, p |i - j| and p dp |i - j| with
+// dp = g . v - delta: with the first in place of what rounding o to bf16 left of it,
+// sum_j d_ij |i - j| = sum p dp |i - j| - (sum p dp)(sum p |i - j|). A third launch adds the
+// queries in 64 bits.
+#include "rk_scored.h"
+
+namespace rk {
+
+struct ScoredBwdArgs {
+  ScoredArgs f;
+  float inv_scale;  // 1 / scale
+  float* rows;      // [B H][2][Sp]: log-sum-exp term and -delta (zeros where a row is none)
+  float* slope_rows;  // [B H][Sp], or null
+};
+
+constexpr int kBwdRows = 32;  // staged rows per step
+
+// p and the factor of the score's gradient from the accumulated dot product. `term`: plain,
+// already in the accumulator (-lse / scale); otherwise lse log2(e), subtracted here.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ float score_p(const ScoredArgs& a, float x, float term, float slope2,
+                                         float dist, float& slack) {
+  if constexpr (CAP) {
+    const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.dot_scale) + 1.0f);
+    slack = 4.0f * r * (1.0f - r);
+    float t = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2 - term);
+    if constexpr (BIAS) t = __builtin_fmaf(-slope2, fabsf(dist), t);
+    return __builtin_amdgcn_exp2f(t);
+  } else {
+    slack = 1.0f;
+    if constexpr (BIAS)
+      return __builtin_amdgcn_exp2f(
+          __builtin_fmaf(-slope2, fabsf(dist), x * a.dot_scale));
+    return __builtin_amdgcn_exp2f(x * a.dot_scale);
+  }
+}
+
+template <int D, bool CAP, bool BIAS, bool SG>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void scored_dq_kernel(ScoredBwdArgs ba) {
+  using T = AttnTile<D, kBwdRows>;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kAttnStages * 2 * T::BYTES];
+  __shared__ int box[8];
+  const uint32_t lds0 = lds_address(smem);
+  const ScoredArgs& a = ba.f;
+  const rk_scored_attention_args& p = a.p;
+  const int S = static_cast<int>(p.S);
+  const int64_t BH = p.B * p.H;
+  const int nqb = (S + kAttnRows - 1) / kAttnRows;
+  const int blk = static_cast<int>(blockIdx.x / BH);  // heads fastest
+  const int qb = nqb - 1 - blk;                       // longest causal rows first
+  const int64_t bh = blockIdx.x - blk * BH, b = bh / p.H, hd = bh - b * p.H, kvh = hd / a.G;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qw0 = qb * kAttnRows + 32 * wave, qi = qw0 + l32;
+
+  v8bf_a qf[D / 16], gf[D / 16];
+  load_owned<D>(qf, p.q + b * p.sqb + hd * p.sqh, p.sqs, S, qi, h);
+  load_owned<D>(gf, p.g + b * p.sgb + hd * p.sgh, p.sgs, S, qi, h);
+  Span span = row_span(p, 0, b, qi);
+  const WaveSpan ws(span);
+  int lo, hi;
+  block_range(ws, wave, lane, box, lo, hi);
+  const int first = lo < hi ? lo / kBwdRows : 0;
+  const int end = lo < hi ? (hi + kBwdRows - 1) / kBwdRows : 0;
+  const uint32_t width = static_cast<uint32_t>(span.hi - span.lo);
+
+  // delta of this lane's query: half of the features here, the other half in lane ^ 32
+  float dot = 0.0f;
+  {
+    v8bf_a of[D / 16];
+    load_owned<D>(of, p.o + b * p.sob + hd * p.soh, p.sos, S, qi, h);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        dot = dot + static_cast<float>(gf[s][e]) * static_cast<float>(of[s][e]);
+  }
+  dot = dot + __shfl_xor(dot, 32, kWave);
+  const float lse = span.valid ? p.lse[bh * S + qi] : 0.0f;
+  const float term = CAP ? lse * kLog2e : -lse * ba.inv_scale;
+  const float ndelta = span.valid ? -dot : 0.0f;
+  if (h == 0) {  // Sp rows: the padded block's too
+    float* const rows = ba.rows + bh * 2 * a.Sp + qi;
+    rows[0] = term;
+    rows[a.Sp] = ndelta;
+  }
+  float slope2 = 0.0f;
+  if constexpr (BIAS) slope2 = p.slopes[hd] * kLog2e;
+
+  const TileDma<D, kBwdRows> kd(p.k + b * p.skb + kvh * p.skh, p.sks, S, wave, lane);
+  const TileDma<D, kBwdRows> vd(p.v + b * p.svb + kvh * p.svh, p.svs, S, wave, lane);
+  auto issue = [&](int step) {
+    const uint32_t st = lds0 + (step & 1) * 2 * T::BYTES;
+    kd.issue(st, step * kBwdRows, wave);
+    vd.issue(st + T::BYTES, step * kBwdRows, wave);
+  };
+
+  v16f_a dq[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) dq[dt] = v16f_a{};
+  float s_pd = 0.0f, s_pa = 0.0f, s_pda = 0.0f;  // sums of p dp, p |i - j|, p dp |i - j|
+  if (first < end) issue(first);
+  for (int step = first; step < end; ++step) {
+    const uint64_t pad = padding_bits<kBwdRows>(a, b, step * kBwdRows);
+    dma_wait_barrier<0>();
+    if (step + 1 < end) issue(step + 1);
+    uint8_t* const kt = smem + (step & 1) * 2 * T::BYTES;
+    uint8_t* const vt = kt + T::BYTES;
+    if (pad) {  // the keys meet gradients of zero
+      clear_rows<D, kBwdRows>(kt, pad, tid);
+      __syncthreads();
+    }
+    const int key0 = step * kBwdRows;
+    if (ws.none(key0, kBwdRows)) continue;
+    v16f_a st, dp;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      st[e] = CAP ? 0.0f : term;
+      dp[e] = ndelta;
+    }
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+      st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, 0, s, lane), qf[s], st,
+                                                   0, 0, 0);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+      dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(vt, 0, s, lane), gf[s], dp,
+                                                   0, 0, 0);
+    const float d0 = static_cast<float>(qi - key0 - 4 * h);
+    float ds[16], pr[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float slack;
+      pr[e] = score_p<CAP, BIAS>(a, st[e], term, slope2,
+                                 d0 - static_cast<float>(8 * (e / 4) + (e % 4)), slack);
+      st[e] = slack;
+    }
+    if (!ws.all(key0, kBwdRows)) {
+      const int j0 = key0 + 4 * h - span.lo;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) {
+          pr[e] = 0.0f;
+          dp[e] = 0.0f;
+          st[e] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      ds[e] = pr[e] * dp[e];
+      if constexpr (SG) {
+        const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
+        s_pd = s_pd + ds[e];
+        s_pa = __builtin_fmaf(pr[e], dist, s_pa);
+        s_pda = __builtin_fmaf(ds[e], dist, s_pda);
+      }
+      if constexpr (CAP) ds[e] = ds[e] * st[e];
+    }
+    uint4 dsf[2];
+    pack16(dsf, ds);
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+        dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            col_frag<D>(kt, 16 * s2, dt, lane), frag_of(dsf[s2]), dq[dt], 0, 0, 0);
+  }
+  if (!span.valid) {
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) dq[dt] = v16f_a{};
+  }
+  if (qi < S)
+    store_owned<D>(p.dq + b * p.sxb + hd * p.sxh + static_cast<int64_t>(qi) * p.sxs, dq, p.scale,
+                   h);
+  if constexpr (SG) {
+    s_pd = s_pd + __shfl_xor(s_pd, 32, kWave);
+    s_pa = s_pa + __shfl_xor(s_pa, 32, kWave);
+    s_pda = s_pda + __shfl_xor(s_pda, 32, kWave);
+    if (h == 0) ba.slope_rows[bh * a.Sp + qi] = span.valid ? s_pda - s_pd * s_pa : 0.0f;
+  }
+}
+
+// dslope[h] = -sum over the sequences and queries, in 64 bits and a fixed order.
+__global__ __launch_bounds__(256) void scored_slope_kernel(ScoredBwdArgs ba) {
+  __shared__ double red[256];
+  const ScoredArgs& a = ba.f;
+  const int64_t hd = blockIdx.x;
+  const int tid = threadIdx.x;
+  double sum = 0.0;
+  for (int64_t b = 0; b < a.p.B; ++b) {
+    const float* rows = ba.slope_rows + (b * a.p.H + hd) * a.Sp;
+    for (int64_t i = tid; i < a.Sp; i += 256) sum += rows[i];
+  }
+  red[tid] = sum;
+  for (int n = 128; n > 0; n >>= 1) {
+    __syncthreads();
+    if (tid < n) red[tid] += red[tid + n];
+  }
+  if (tid == 0) a.p.dslopes[hd] = static_cast<float>(-red[0]);
+}
+
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void scored_dkv_kernel(ScoredBwdArgs ba) {
+  using T = AttnTile<D, kBwdRows>;
+  constexpr int STAGE = 2 * T::BYTES + 256;  // two tiles, 32 log-sum-exp terms, 32 -delta
+  // the owned V rows stay in LDS (rk_attention_bwd.hip: in registers beside K the loop spills)
+  constexpr int VTILE = kAttnRows * T::ROWB;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[VTILE + kAttnStages * STAGE];
+  __shared__ int box[8];
+  const uint32_t lds0 = lds_address(smem) + VTILE;
+  const ScoredArgs& a = ba.f;
+  const rk_scored_attention_args& p = a.p;
+  const int S = static_cast<int>(p.S);
+  const int64_t BH = p.B * p.Hkv;
+  const int blk = static_cast<int>(blockIdx.x / BH);  // heads fastest
+  const int64_t bh = blockIdx.x - blk * BH, b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  const int k0 = blk * kAttnRows;  // the first keys have the longest walk
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kj = k0 + 32 * wave + l32;
+
+  v8bf_a kf[D / 16];
+  load_owned<D>(kf, p.k + b * p.skb + kvh * p.skh, p.sks, S, kj, h);
+  Span span = row_span(p, 2, b, kj);
+  const WaveSpan ws(span);
+  int lo, hi;
+  block_range(ws, wave, lane, box, lo, hi);
+  const int first = lo < hi ? lo / kBwdRows : 0;
+  const int steps = lo < hi ? (hi + kBwdRows - 1) / kBwdRows - first : 0;
+  const uint32_t width = static_cast<uint32_t>(span.hi - span.lo);
+
+  const TileDma<D, kBwdRows> vd(p.v + b * p.svb + kvh * p.svh, p.svs, S, wave, lane);
+#pragma unroll
+  for (int t = 0; t < kAttnRows / kBwdRows; ++t)
+    vd.issue(lds_address(smem) + t * T::BYTES, k0 + t * kBwdRows, wave);
+
+  // the group's query heads one after the other, the tiles of the next one behind the last of
+  // this one: tile n of all is step n % steps of head n / steps
+  const int total = steps * static_cast<int>(a.G);
+  int ihead = 0, istep = 0;  // the next tile to load
+  auto issue = [&](int n) {
+    const int64_t hd = kvh * a.G + ihead;
+    const uint32_t st = lds0 + (n & 1) * STAGE;
+    const int row0 = (first + istep) * kBwdRows;
+    const TileDma<D, kBwdRows> qd(p.q + b * p.sqb + hd * p.sqh, p.sqs, S, wave, lane);
+    const TileDma<D, kBwdRows> gd(p.g + b * p.sgb + hd * p.sgh, p.sgs, S, wave, lane);
+    // row statistics: lanes 0..31 take the first plane, lanes 32..63 the second (every wavefront
+    // writes the same bytes)
+    const __amdgpu_buffer_rsrc_t rbuf =
+        make_buffer(ba.rows + (b * p.H + hd) * 2 * a.Sp, 2 * a.Sp * 4);
+    dma4(rbuf, st + 2 * T::BYTES, static_cast<int>((h * a.Sp + l32) * 4), row0 * 4);
+    qd.issue(st, row0, wave);
+    gd.issue(st + T::BYTES, row0, wave);
+    if (++istep == steps) {
+      istep = 0;
+      ++ihead;
+    }
+  };
+
+  v16f_a dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) {
+    dk[dt] = v16f_a{};
+    dv[dt] = v16f_a{};
+  }
+  if (total > 0) issue(0);
+  int chead = 0, cstep = 0;  // the tile computed
+  float slope2 = 0.0f;
+  for (int n = 0; n < total; ++n) {
+    const int qs = (first + cstep) * kBwdRows;
+    const uint64_t pad = padding_bits<kBwdRows>(a, b, qs);
+    if constexpr (BIAS)
+      if (cstep == 0) slope2 = p.slopes[kvh * a.G + chead] * kLog2e;
+    if (++cstep == steps) {
+      cstep = 0;
+      ++chead;
+    }
+    dma_wait_barrier<0>();
+    if (n + 1 < total) issue(n + 1);
+    uint8_t* const qt = smem + VTILE + (n & 1) * STAGE;
+    uint8_t* const gt = qt + T::BYTES;
+    const float* rows = reinterpret_cast<const float*>(gt + T::BYTES);
+    if (pad) {  // the queries and their gradients meet probabilities of zero
+      clear_rows<D, kBwdRows>(qt, pad, tid);
+      clear_rows<D, kBwdRows>(gt, pad, tid);
+      __syncthreads();
+    }
+    if (ws.none(qs, kBwdRows)) continue;
+    v16f_a st, dp;
+    float term[16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float4 nl = *reinterpret_cast<const float4*>(rows + 8 * r + 4 * h);
+      const float4 nd = *reinterpret_cast<const float4*>(rows + kBwdRows + 8 * r + 4 * h);
+      term[4 * r] = nl.x; term[4 * r + 1] = nl.y; term[4 * r + 2] = nl.z; term[4 * r + 3] = nl.w;
+      dp[4 * r] = nd.x; dp[4 * r + 1] = nd.y; dp[4 * r + 2] = nd.z; dp[4 * r + 3] = nd.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st[e] = CAP ? 0.0f : term[e];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+      st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(qt, 0, s, lane), kf[s], st,
+                                                   0, 0, 0);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+      dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(gt, 0, s, lane),
+                                                   row_frag<D>(smem, 32 * wave, s, lane), dp,
+                                                   0, 0, 0);
+    const float d0 = static_cast<float>(qs + 4 * h - kj);
+    float pr[16], ds[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float slack;
+      pr[e] = score_p<CAP, BIAS>(a, st[e], term[e], slope2,
+                                 d0 + static_cast<float>(8 * (e / 4) + (e % 4)), slack);
+      st[e] = slack;
+    }
+    if (!ws.all(qs, kBwdRows)) {
+      const int i0 = qs + 4 * h - span.lo;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width) {
+          pr[e] = 0.0f;
+          dp[e] = 0.0f;
+          st[e] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      ds[e] = pr[e] * dp[e];
+      if constexpr (CAP) ds[e] = ds[e] * st[e];
+    }
+    uint4 pf[2], dsf[2];
+    pack16(pf, pr);
+    pack16(dsf, ds);
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+        dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            col_frag<D>(gt, 16 * s2, dt, lane), frag_of(pf[s2]), dv[dt], 0, 0, 0);
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+        dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            col_frag<D>(qt, 16 * s2, dt, lane), frag_of(dsf[s2]), dk[dt], 0, 0, 0);
+  }
+  // no load may still write this workgroup's LDS when it ends
+  if (total == 0) dma_wait_barrier<0>();
+  if (!span.valid) {
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      dk[dt] = v16f_a{};
+      dv[dt] = v16f_a{};
+    }
+  }
+  if (kj < S) {
+    const int64_t off = b * p.syb + kvh * p.syh + static_cast<int64_t>(kj) * p.sys;
+    store_owned<D>(p.dk + off, dk, p.scale, h);
+    store_owned<D>(p.dv + off, dv, 1.0f, h);
+  }
+}
+
+template <int D, bool CAP, bool BIAS>
+static void launch_scored_bwd(const ScoredBwdArgs& a, hipStream_t st) {
+  const rk_scored_attention_args& p = a.f.p;
+  const unsigned blocks = static_cast<unsigned>(a.f.Sp / kAttnRows);
+  const dim3 qgrid(static_cast<unsigned>(p.B * p.H) * blocks);
+  const dim3 kgrid(static_cast<unsigned>(p.B * p.Hkv) * blocks);
+  if (BIAS && a.slope_rows) {
+    scored_dq_kernel<D, CAP, BIAS, BIAS><<<qgrid, 256, 0, st>>>(a);
+    scored_slope_kernel<<<static_cast<unsigned>(p.H), 256, 0, st>>>(a);
+  } else {
+    scored_dq_kernel<D, CAP, BIAS, false><<<qgrid, 256, 0, st>>>(a);
+  }
+  scored_dkv_kernel<D, CAP, BIAS><<<kgrid, 256, 0, st>>>(a);
+}
+
+template <int D>
+static void dispatch_scored_bwd(const ScoredBwdArgs& a, hipStream_t st) {
+  const bool cap = a.f.p.softcap > 0.0f, bias = a.f.p.slopes != nullptr;
+  if (cap && bias) launch_scored_bwd<D, true, true>(a, st);
+  else if (cap) launch_scored_bwd<D, true, false>(a, st);
+  else if (bias) launch_scored_bwd<D, false, true>(a, st);
+  else launch_scored_bwd<D, false, false>(a, st);
+}
+
+}  // namespace rk
+
+using namespace rk;
+
+extern "C" int64_t rk_scored_attention_backward_work(int64_t B, int64_t H, int64_t S, int slopes) {
+  if (B <= 0 || H <= 0 || S <= 0) return 0;
+  return (slopes ? 3 : 2) * B * H * ((S + kAttnRows - 1) / kAttnRows * kAttnRows);
+}
+
+extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args, float* work,
+                                            void* stream) {
+  clear_error();
+  if (!args) return fail(RK_ERR_ARG, "null arguments");
+  const rk_scored_attention_args& p = *args;
+  if (int e = check_scored(p, true)) return e;
+  if (p.dslopes && !p.slopes) return fail(RK_ERR_ARG, "a slope gradient needs slopes");
+  if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
+  if (!p.dq || !p.dk || !p.dv || !work) return fail(RK_ERR_ARG, "null pointer");
+  const void* out8[] = {p.dq, p.dk, p.dv};
+  for (const void* t : out8)
+    if (reinterpret_cast<uintptr_t>(t) & 7)
+      return fail(RK_ERR_UNSUPPORTED, "dq, dk, dv need 8-byte alignment");
+  ScoredBwdArgs a{};
+  a.f = scored_args(p);
+  a.inv_scale = 1.0f / p.scale;
+  a.rows = work;
+  a.slope_rows = p.dslopes ? work + 2 * p.B * p.H * a.f.Sp : nullptr;
+  if (p.D == 64) dispatch_scored_bwd<64>(a, as_stream(stream));
+  else dispatch_scored_bwd<128>(a, as_stream(stream));
+  return launch_status("scored_attention_backward");
+}

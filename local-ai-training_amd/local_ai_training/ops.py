@@ -178,6 +178,29 @@ def _register_fakes() -> None:
         b, h, sl, d = q.shape
         return tuple(q.new_empty((b, sl, h, d)).permute(0, 2, 1, 3) for _ in range(3))
 
+    @fake("ratchet::attention_mask")
+    def _attention_mask(documents, prefix):
+        like = documents if documents is not None else prefix
+        b, sl = like.shape
+        return (like.new_empty((4, b, sl), dtype=torch.int32),
+                like.new_empty((b, (sl + 31) // 32), dtype=torch.int32))
+
+    @fake("ratchet::scored_attention")
+    def _scored_attention(q, k, v, bounds, padding, slopes, softcap, scale):
+        b, h, sl, d = q.shape
+        o = q.new_empty((b, sl, h, d)).permute(0, 2, 1, 3)
+        return o, q.new_empty((b, h, sl), dtype=torch.float32)
+
+    @fake("ratchet::scored_attention_backward")
+    def _scored_attention_backward(grad, q, k, v, o, lse, bounds, padding, slopes, softcap,
+                                   scale, slope_grad):
+        def rows(t):
+            b, h, sl, d = t.shape
+            return t.new_empty((b, sl, h, d)).permute(0, 2, 1, 3)
+
+        return (rows(q), rows(k), rows(k),
+                q.new_empty((q.shape[1] if slope_grad else 0,), dtype=torch.float32))
+
     @fake("ratchet::kv_append")
     def _kv_append(k, v, keys, values, start, clear_to):
         return None
@@ -198,7 +221,8 @@ def _register_fakes() -> None:
 
 
 # the operators the library defines (the opcheck tests walk this list), but for
-# attention_backward and kv_append, whose opchecks are beside their own tests
+# attention_backward, kv_append, attention_mask, the scored_attention and the int8_kv
+# operators, whose opchecks are beside their own tests
 OPERATORS = (
     "quantize_rows", "int8_mm_nt", "packed_mm", "packed_mm_residual", "packed_mm_accumulate",
     "packed_mm_t", "unpack_transpose", "unpack", "effective_bf16", "grad_input_bf16",
