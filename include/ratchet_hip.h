@@ -751,6 +751,52 @@ int rk_scored_attention_forward(const rk_scored_attention_args* args, void* stre
 int64_t rk_scored_attention_backward_work(int64_t B, int64_t H, int64_t S, int slopes);
 int rk_scored_attention_backward(const rk_scored_attention_args* args, float* work, void* stream);
 
+/*
+ * A key/value cache in 8 bits: keys int8 [B, H, blocks, 64, D], values int8 [B, H, blocks, D, 64]
+ * (by feature), float32 scales [B, H, blocks], one per block of 64 tokens and head; H key heads,
+ * D = 64, 128 or 256, 16-byte aligned. A code stands for code x scale.
+ */
+typedef struct rk_int8_kv {
+  int8_t *keys, *values;
+  float *key_scales, *value_scales;
+  int64_t B, H, blocks, D;
+} rk_int8_kv;
+
+/*
+ * Appends k and v (float32 or bf16 [B, H, S, D], element strides, unit feature stride; rows whole
+ * 16-byte vectors) at positions start .. of each sequence: start is a device int64, one or one per
+ * sequence (start_count 1 or B; negative: that sequence appends nothing); lengths (device int64
+ * [B], or NULL: S) says how many of a sequence's S tokens count. Positions past the cache are
+ * dropped. A block's scale is absmax / 127, its codes rint(x / scale) (IEEE float32); tokens
+ * appended to a block that holds some leave its scale or raise it, s = max(s_old, absmax / 127),
+ * and its codes are then rint(c (s_old / s)). A NaN or infinite value makes its block's scale one.
+ */
+int rk_int8_kv_append(const rk_int8_kv* cache, const void* k, int64_t skb, int64_t skh,
+                      int64_t sks, const void* v, int64_t svb, int64_t svh, int64_t svs, int dtype,
+                      int64_t S, const int64_t* start, int64_t start_count,
+                      const int64_t* lengths, void* stream);
+
+/* The values of positions begin .. end - 1 as float32 or bf16 [B, H, end - begin, D]. */
+int rk_int8_kv_read(const rk_int8_kv* cache, int64_t begin, int64_t end, int dtype, void* keys,
+                    void* values, void* stream);
+
+/*
+ * Attention of q (float32 or bf16 [B, Hq, S, D], element strides; Hq a multiple of H) over the
+ * cache: query i of a sequence stands at position start + i and sees positions 0 .. start + i,
+ * which must have been appended. Scores, softcap and slopes (float32 [Hq]) as in
+ * rk_scored_attention_forward. out: [B, S, Hq, D] contiguous, float32 or bf16; zeros for queries
+ * at or past lengths and for negative starts, NaN for positions past the cache. The products run
+ * in integers on the codes, with queries and probabilities rounded to 23 bits of their row's and
+ * block's largest. work: rk_int8_kv_attention_work floats (0: none), 16-byte aligned.
+ * No counterpart in the reference (its window is recomputed per token, generate.py:183-201).
+ */
+int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S);
+int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int qdtype, int64_t sqb,
+                         int64_t sqh, int64_t sqs, int64_t Hq, int64_t S, const int64_t* start,
+                         int64_t start_count, const int64_t* lengths, float scale, float softcap,
+                         const float* slopes, float* work, int64_t work_floats, void* out,
+                         int odtype, void* stream);
+
 /* HBM streaming probe (measurement only; no counterpart in the reference): reads `bytes`
  * (a multiple of 16) from src in 16-byte vectors, `unroll` (1, 2, 4, 8) loads in flight
  * per thread, `blocks` blocks of 256 threads in a grid-stride loop; copy != 0 writes them

@@ -1200,6 +1200,117 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> scored_attention_backward(
   return {dq, dk, dv, dslopes};
 }
 
+// The 8-bit cache of one layer as the library takes it.
+rk_int8_kv int8_kv(const Tensor& keys, const Tensor& values, const Tensor& key_scales,
+                   const Tensor& value_scales, const char* what) {
+  require_gpu(keys, what);
+  for (const Tensor* t : {&values, &key_scales, &value_scales}) same_device(keys, *t, what);
+  TORCH_CHECK(keys.dim() == 5 && keys.size(3) == 64 && keys.scalar_type() == at::kChar &&
+                  keys.is_contiguous(),
+              what, ": keys must be a contiguous int8 [B, H, blocks, 64, D] buffer");
+  const int64_t B = keys.size(0), H = keys.size(1), n = keys.size(2), D = keys.size(4);
+  TORCH_CHECK(values.sizes() == at::IntArrayRef({B, H, n, D, 64}) &&
+                  values.scalar_type() == at::kChar && values.is_contiguous(),
+              what, ": values must be a contiguous int8 [B, H, blocks, D, 64] buffer");
+  for (const Tensor* t : {&key_scales, &value_scales})
+    TORCH_CHECK(t->sizes() == at::IntArrayRef({B, H, n}) && t->scalar_type() == at::kFloat &&
+                    t->is_contiguous(),
+                what, ": scales must be contiguous float32 [B, H, blocks] buffers");
+  return rk_int8_kv{keys.data_ptr<int8_t>(), values.data_ptr<int8_t>(),
+                    key_scales.data_ptr<float>(), value_scales.data_ptr<float>(), B, H, n, D};
+}
+
+// Device positions: int64, one or one per sequence.
+const int64_t* positions(const Tensor& like, const Tensor& t, int64_t B, bool one,
+                         const char* what) {
+  same_device(like, t, what);
+  TORCH_CHECK(t.scalar_type() == at::kLong && t.dim() == 1 && t.is_contiguous() &&
+                  (t.size(0) == B || (one && t.size(0) == 1)),
+              what, ": positions must be int64, ", one ? "one or " : "", "one per sequence");
+  return t.data_ptr<int64_t>();
+}
+
+// Rows as 16-byte vectors: the tensor itself, or a copy where it does not lie so.
+Tensor vector_rows(const Tensor& t) {
+  const int64_t per = 16 / t.element_size();
+  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % per == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void int8_kv_append(const Tensor& k, const Tensor& v, Tensor& keys, Tensor& values,
+                    Tensor& key_scales, Tensor& value_scales, const Tensor& start,
+                    const OptTensor& lengths) {
+  constexpr const char* what = "int8 kv append";
+  const rk_int8_kv c = int8_kv(keys, values, key_scales, value_scales, what);
+  same_device(keys, k, what);
+  same_device(keys, v, what);
+  TORCH_CHECK(k.dim() == 4 && v.sizes() == k.sizes() && k.size(0) == c.B && k.size(1) == c.H &&
+                  k.size(3) == c.D && v.scalar_type() == k.scalar_type(),
+              what, ": k and v must share a dtype and the cache's [B, H, S, D] shape");
+  const int code = dtype_code(k, what);
+  const c10::DeviceGuard guard(k.device());
+  const Tensor kk = vector_rows(k), vv = vector_rows(v);
+  const int64_t* at = positions(keys, start, c.B, true, what);
+  const int64_t* len = lengths.has_value() ? positions(keys, *lengths, c.B, false, what) : nullptr;
+  check_status(rk_int8_kv_append(&c, kk.data_ptr(), kk.stride(0), kk.stride(1), kk.stride(2),
+                                 vv.data_ptr(), vv.stride(0), vv.stride(1), vv.stride(2), code,
+                                 k.size(2), at, start.size(0), len, stream_of(k)),
+               "rk_int8_kv_append");
+}
+
+std::tuple<Tensor, Tensor> int8_kv_read(const Tensor& keys, const Tensor& values,
+                                        const Tensor& key_scales, const Tensor& value_scales,
+                                        int64_t begin, int64_t end, at::ScalarType dtype) {
+  const rk_int8_kv c = int8_kv(keys, values, key_scales, value_scales, "int8 kv read");
+  const int code = dtype_code(dtype);
+  TORCH_CHECK(begin >= 0 && begin <= end && end <= c.blocks * 64,
+              "int8 kv read: positions past the cache");
+  const c10::DeviceGuard guard(keys.device());
+  const auto out = [&] { return at::empty({c.B, c.H, end - begin, c.D}, keys.options().dtype(dtype)); };
+  Tensor k = out(), v = out();
+  check_status(rk_int8_kv_read(&c, begin, end, code, k.data_ptr(), v.data_ptr(), stream_of(keys)),
+               "rk_int8_kv_read");
+  return {k, v};
+}
+
+// Attention over the 8-bit cache (rk_int8_kv_attention): [B, Hq, S, D] as a view of
+// [B, S, Hq, D] memory.
+Tensor int8_kv_attention(const Tensor& q, const Tensor& keys, const Tensor& values,
+                         const Tensor& key_scales, const Tensor& value_scales,
+                         const Tensor& start, const OptTensor& lengths, double scale,
+                         double softcap, const OptTensor& slopes, at::ScalarType out_dtype) {
+  constexpr const char* what = "int8 kv attention";
+  const rk_int8_kv c = int8_kv(keys, values, key_scales, value_scales, what);
+  same_device(keys, q, what);
+  TORCH_CHECK(q.dim() == 4 && q.size(0) == c.B && q.size(3) == c.D &&
+                  (c.H > 0 ? q.size(1) % c.H == 0 : q.size(1) == 0),
+              what, ": q must be [B, H, S, D] with heads a multiple of the cache's");
+  const int code = dtype_code(q, what), ocode = dtype_code(out_dtype);
+  const c10::DeviceGuard guard(q.device());
+  const Tensor qq = vector_rows(q);
+  const int64_t Hq = q.size(1), S = q.size(2);
+  const int64_t* at = positions(keys, start, c.B, true, what);
+  const int64_t* len = lengths.has_value() ? positions(keys, *lengths, c.B, false, what) : nullptr;
+  Tensor sl;
+  if (slopes.has_value()) {
+    same_device(keys, *slopes, what);
+    sl = f32_vector(*slopes, Hq, "slopes");
+  }
+  Tensor out = at::empty({c.B, S, Hq, c.D}, q.options().dtype(out_dtype));
+  const int64_t floats = rk_int8_kv_attention_work(&c, Hq, S);
+  Tensor work;
+  if (floats > 0) work = at::empty({floats}, key_scales.options());
+  check_status(rk_int8_kv_attention(&c, qq.data_ptr(), code, qq.stride(0), qq.stride(1),
+                                    qq.stride(2), Hq, S, at, start.size(0), len,
+                                    static_cast<float>(scale), static_cast<float>(softcap),
+                                    sl.defined() ? sl.data_ptr<float>() : nullptr,
+                                    floats > 0 ? work.data_ptr<float>() : nullptr, floats,
+                                    out.data_ptr(), ocode, stream_of(q)),
+               "rk_int8_kv_attention");
+  return out.permute({0, 2, 1, 3});
+}
+
 // Means of segments [offsets[s], offsets[s + 1]) of a float32 row-rms buffer (rk_row_rms_means).
 Tensor row_rms_means(const Tensor& row_rms, const Tensor& offsets) {
   require_gpu(row_rms, "row rms means");
@@ -1355,6 +1466,13 @@ TORCH_LIBRARY(ratchet, m) {
   m.def("scored_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor o, "
         "Tensor lse, Tensor? bounds, Tensor? padding, Tensor? slopes, float softcap, "
         "float scale, bool slope_grad) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("int8_kv_append(Tensor k, Tensor v, Tensor(a!) keys, Tensor(b!) values, "
+        "Tensor(c!) key_scales, Tensor(d!) value_scales, Tensor start, Tensor? lengths) -> ()");
+  m.def("int8_kv_read(Tensor keys, Tensor values, Tensor key_scales, Tensor value_scales, "
+        "int begin, int end, ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("int8_kv_attention(Tensor q, Tensor keys, Tensor values, Tensor key_scales, "
+        "Tensor value_scales, Tensor start, Tensor? lengths, float scale, float softcap, "
+        "Tensor? slopes, ScalarType out_dtype) -> Tensor");
   m.def("kv_append(Tensor k, Tensor v, Tensor(a!) keys, Tensor(b!) values, int start, "
         "int clear_to) -> ()");
   m.def("cross_entropy_forward(Tensor logits, Tensor targets, int ignore_index=-100) -> "
@@ -1402,6 +1520,9 @@ TORCH_LIBRARY_IMPL(ratchet, CUDA, m) {
   m.impl("attention_mask", &attention_mask);
   m.impl("scored_attention", &scored_attention);
   m.impl("scored_attention_backward", &scored_attention_backward);
+  m.impl("int8_kv_append", &int8_kv_append);
+  m.impl("int8_kv_read", &int8_kv_read);
+  m.impl("int8_kv_attention", &int8_kv_attention);
   m.impl("kv_append", &kv_append);
   m.impl("cross_entropy_forward", &cross_entropy_forward);
   m.impl("cross_entropy_backward", &cross_entropy_backward);

@@ -1,0 +1,759 @@
+// A key/value cache in 8 bits (gfx950): appended keys and values quantized per block of 64 tokens
+// and key head, attention of new tokens over it, and the values read back. It stands beside the
+// bf16 / float32 cache (rk_kv_append, rk_decode_attention) at half or a quarter of its bytes; the
+// reference keeps no cache (generate.py:183-201 recomputes the window).
+//
+// Layout: keys int8 [B, Hkv, NB, 64, D], values int8 [B, Hkv, NB, D, 64] (by feature), one
+// float32 scale per block and head for each. Both products of the attention then read their
+// operand as v_mfma_i32_16x16x64_i8 takes it, 16 bytes per lane straight from memory.
+//
+// Quantization: s = absmax / 127 over the block's tokens, code = rint(x / s) (IEEE float32
+// quotients, the rule of rk_quantize_rows). Tokens appended to a block that holds some can only
+// raise its scale; the codes there are then rounded again, rint(c (s_old / s)). A block's first
+// token starts it anew, whatever it held.
+#include "rk_common.h"
+
+#include <math.h>
+
+namespace rk {
+
+constexpr int kTok = 64;  // tokens of a block
+constexpr float kLog2e8 = 1.4426950408889634f;
+
+typedef int v4i8 __attribute__((ext_vector_type(4)));
+
+struct Kv8 {
+  int8_t* keys;
+  int8_t* values;
+  float* ks;
+  float* vs;
+  int64_t B, H, NB;  // H: key heads
+};
+
+struct Kv8Append {
+  Kv8 c;
+  const void* k;
+  const void* v;
+  int64_t skb, skh, sks, svb, svh, svs;
+  const int64_t* start;    // [1] or [B] (start_step 0 or 1)
+  const int64_t* lengths;  // [B] or null
+  int64_t start_step, S;
+};
+
+// The new tokens first .. last - 1 of block `blk` of sequence b, first past what it keeps.
+__device__ __forceinline__ bool append_range(const Kv8Append& a, int64_t b, int64_t touched,
+                                             int64_t& blk, int64_t& start, int& first, int& last) {
+  start = a.start[b * a.start_step];
+  if (start < 0) return false;
+  int64_t n = a.lengths ? a.lengths[b] : a.S;
+  n = n < a.S ? n : a.S;
+  blk = start / kTok + touched;
+  if (n <= 0 || blk >= a.c.NB) return false;
+  const int64_t base = blk * kTok, f = start - base, l = start + n - base;
+  first = static_cast<int>(f > 0 ? f : 0);
+  last = static_cast<int>(l < kTok ? l : kTok);
+  return first < last;
+}
+
+// code of x under scale s; only denormal scales reach the clamp, only NaN and infinite scales
+// the zero of a NaN quotient
+__device__ __forceinline__ int code_of(float x, float s) {
+  const float y = __builtin_rintf(x / s);
+  const int c = static_cast<int>(fminf(fmaxf(y, -127.0f), 127.0f));
+  return s > 0.0f && y == y ? c : 0;
+}
+__device__ __forceinline__ int code_again(int c, float ratio) {
+  return static_cast<int>(
+      fminf(fmaxf(__builtin_rintf(static_cast<float>(c) * ratio), -127.0f), 127.0f));
+}
+
+// grid (touched blocks, B * H, 2: keys, values), 256 threads; a thread takes D / 32 pieces of 8
+// features. The block's absmax by the bits of |x| (a NaN is the largest), so a block that takes
+// in a NaN or an infinity has such a scale and reads back as NaN.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
+  constexpr int PER = D / 8, EACH = kTok * PER / 256, PITCH = kTok + 4;
+  __shared__ uint32_t red[4];
+  __shared__ __attribute__((aligned(16))) uint8_t tile[D * PITCH];
+  const int64_t bh = blockIdx.y, b = bh / a.c.H, h = bh - b * a.c.H;
+  const int tid = threadIdx.x;
+  int64_t blk, start;
+  int first, last;
+  if (!append_range(a, b, blockIdx.x, blk, start, first, last)) return;
+  const bool val = blockIdx.z != 0;
+  const int64_t at = (bh * a.c.NB + blk);
+  float* const scale = (val ? a.c.vs : a.c.ks) + at;
+  int8_t* const codes = (val ? a.c.values : a.c.keys) + at * kTok * D;
+  const void* src = val ? a.v : a.k;
+  const int64_t ss = val ? a.svs : a.sks;
+  // element offset of the token at the block's first position (never read before `first`)
+  const int64_t off = b * (val ? a.svb : a.skb) + h * (val ? a.svh : a.skh) +
+                      (blk * kTok - start) * ss;
+  const float old = first > 0 ? *scale : 0.0f;
+
+  float x[EACH][8];
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int unit = tid + 256 * i, t = unit / PER, f = unit % PER * 8;
+    if (t >= first && t < last) {
+      const int64_t idx = off + t * ss + f;
+      load_vec16<DT>(src, idx, x[i]);
+      if constexpr (DT == RK_F32) load_vec16<DT>(src, idx + 4, x[i] + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t bits = __float_as_uint(x[i][e]) & 0x7fffffffu;
+        most = bits > most ? bits : most;
+      }
+    }
+  }
+  most = wave_butterfly(most, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
+  if ((tid & 63) == 0) red[tid >> 6] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) most = red[w] > most ? red[w] : most;
+  float s = __uint_as_float(most) / 127.0f;
+  if (first > 0 && __float_as_uint(old) > __float_as_uint(s)) s = old;
+  const bool grown = first > 0 && __float_as_uint(old) != __float_as_uint(s);
+  const float ratio = old / (s > 0.0f ? s : 1.0f);
+  if (tid == 0) *scale = s;
+
+  if (!val) {
+    if (grown) {
+      for (int i = tid; i < first * (D / 4); i += 256) {
+        uint32_t* const w = reinterpret_cast<uint32_t*>(codes) + i;
+        const uint32_t c = *w;
+        uint32_t r = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          r |= static_cast<uint32_t>(code_again(static_cast<int8_t>(c >> (8 * e)), ratio) & 255)
+               << (8 * e);
+        *w = r;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int unit = tid + 256 * i, t = unit / PER, f = unit % PER * 8;
+      if (t >= first && t < last) {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w[e / 4] |= static_cast<uint32_t>(code_of(x[i][e], s) & 255) << (8 * (e % 4));
+        *reinterpret_cast<uint2*>(codes + t * D + f) = make_uint2(w[0], w[1]);
+      }
+    }
+    return;
+  }
+  // values: the block by features in LDS, what it keeps first, then written whole
+  for (int i = tid; i < D * (kTok / 4); i += 256) {
+    const int f = i / (kTok / 4), w = i % (kTok / 4);
+    uint32_t r = 0;
+    if (4 * w < first) {
+      const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[i];
+      r = c;
+      if (grown) {
+        r = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          r |= static_cast<uint32_t>(code_again(static_cast<int8_t>(c >> (8 * e)), ratio) & 255)
+               << (8 * e);
+      }
+    }
+    *reinterpret_cast<uint32_t*>(tile + f * PITCH + 4 * w) = r;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int unit = tid + 256 * i, t = unit / PER, f = unit % PER * 8;
+    if (t >= first && t < last) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        tile[(f + e) * PITCH + t] = static_cast<uint8_t>(code_of(x[i][e], s) & 255);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < D * (kTok / 4); i += 256)
+    reinterpret_cast<uint32_t*>(codes)[i] =
+        *reinterpret_cast<const uint32_t*>(tile + i / (kTok / 4) * PITCH + 4 * (i % (kTok / 4)));
+}
+
+struct Kv8Read {
+  Kv8 c;
+  int64_t begin, n;
+  void* keys;  // [B, H, n, D] contiguous, float32 or bf16
+  void* values;
+};
+
+// grid (blocks, B * H, 2), 256 threads: the values codes stand for, code x scale in float32.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a) {
+  constexpr int PER = D / 8, PITCH = kTok + 4;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[D * PITCH];
+  const int64_t bh = blockIdx.y, blk = a.begin / kTok + blockIdx.x;
+  const int tid = threadIdx.x;
+  const bool val = blockIdx.z != 0;
+  const int64_t at = bh * a.c.NB + blk;
+  const float s = (val ? a.c.vs : a.c.ks)[at];
+  const int8_t* const codes = (val ? a.c.values : a.c.keys) + at * kTok * D;
+  if (val) {
+    for (int i = tid; i < D * (kTok / 4); i += 256)
+      *reinterpret_cast<uint32_t*>(tile + i / (kTok / 4) * PITCH + 4 * (i % (kTok / 4))) =
+          reinterpret_cast<const uint32_t*>(codes)[i];
+    __syncthreads();
+  }
+  char* const out = static_cast<char*>(val ? a.values : a.keys);
+  for (int unit = tid; unit < kTok * PER; unit += 256) {
+    const int t = unit / PER, f = unit % PER * 8;
+    const int64_t tok = blk * kTok + t - a.begin;
+    if (tok < 0 || tok >= a.n) continue;
+    float x[8];
+    if (val) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = static_cast<int8_t>(tile[(f + e) * PITCH + t]) * s;
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(codes + t * D + f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = static_cast<int8_t>((e < 4 ? w.x : w.y) >> (8 * (e % 4))) * s;
+    }
+    const int64_t idx = (bh * a.n + tok) * D + f;
+    if constexpr (DT == RK_F32) {
+      float4* const o = reinterpret_cast<float4*>(out + idx * 4);
+      o[0] = make_float4(x[0], x[1], x[2], x[3]);
+      o[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = f32_to_bf16(x[2 * e]) | (static_cast<uint32_t>(f32_to_bf16(x[2 * e + 1])) << 16);
+      *reinterpret_cast<uint4*>(out + idx * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention of S new tokens per sequence (positions start .. start + S - 1, their keys and values
+// appended before) over the cache: query i sees positions 0 .. start + i.
+//   s_j = scale q . k_j;  capped and biased as in rk_scored.h;  o = sum_j softmax(s_j) v_j
+// with k_j, v_j what the codes stand for. Columns of a product are the S * G queries that share a
+// key head (G = query heads per key head), 16 at a time; rows are keys, then features.
+//
+// Both products run on the codes as they are, in exact integers: the query is written as a fixed
+// point number of three signed base-256 digits relative to its largest feature (23 bits, the
+// rounding a float32 operand would have), the probabilities as three digits relative to the
+// block's largest, and each digit's product is its own MFMA. The matrix unit takes them at a
+// fraction of the time the codes need to arrive, and no code is ever converted: for one query
+// per head, 48 MFMAs and about 500 vector instructions per 16 KB of codes at D = 128.
+//
+// A wavefront walks blocks of 64 tokens with its own running max, sum and output. Lane l holds the
+// scores of column l % 16 against keys 16 (l / 16) .. + 15: key 16 g + 4 t + e is row 4 g + e of
+// product t, and the same 16 keys are the lane's k slots of the second product, whose other
+// operand, 16 tokens of one feature, lies side by side in the cache. The four wavefronts of a
+// workgroup are joined in LDS, splits of a long cache by a second launch.
+// ---------------------------------------------------------------------------
+struct Kv8Attn {
+  Kv8 c;
+  const void* q;
+  int64_t sqb, sqh, sqs;
+  const int64_t* start;
+  const int64_t* lengths;
+  const float* slopes;
+  int64_t start_step, S, Hq, G, nsplit, tiles;
+  float dot_scale, cap2;
+  float* work;  // [B * H * tiles][nsplit][16][D + 4]: max, sum, 2 pad, unnormalized output
+  void* out;    // [B, S, Hq, D], of type ODT
+};
+
+__device__ __forceinline__ float col_max(float v) {  // over the four lanes of a column
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float col_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ uint32_t col_umax(uint32_t v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = r[0] > r[1] ? r[0] : r[1];
+  const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return s[0] > s[1] ? s[0] : s[1];
+}
+
+constexpr float kFixed = 127.0f * 65536.0f;  // the largest three-digit number used
+
+// Digits of 4 numbers |x| <= kFixed, rounded, as bytes of one word each: x = 65536 a + 256 b + c.
+__device__ __forceinline__ void digits4(const float (&x)[4], int& a, int& b, int& c) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    // adding 128 to the two low digits makes them unsigned without a carry to take back
+    w[e] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(x[e])) + 0x8080);
+  }
+  const uint32_t p01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);  // c0 c1 b0 b1
+  const uint32_t p23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t h01 = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602u);  // a0 a1
+  const uint32_t h23 = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0602u);
+  c = static_cast<int>(__builtin_amdgcn_perm(p23, p01, 0x05040100u) ^ 0x80808080u);
+  b = static_cast<int>(__builtin_amdgcn_perm(p23, p01, 0x07060302u) ^ 0x80808080u);
+  a = static_cast<int>(__builtin_amdgcn_perm(h23, h01, 0x05040100u));
+}
+
+__device__ __forceinline__ float from_digits(int a, int b, int c) {
+  return __builtin_fmaf(static_cast<float>(a), 65536.0f,
+                        __builtin_fmaf(static_cast<float>(b), 256.0f, static_cast<float>(c)));
+}
+
+template <int QDT>
+__device__ __forceinline__ void store4(void* out, int64_t idx, const float (&x)[4]) {
+  if constexpr (QDT == RK_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + idx) =
+        make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    const uint32_t lo = f32_to_bf16(x[0]) | (static_cast<uint32_t>(f32_to_bf16(x[1])) << 16);
+    const uint32_t hi = f32_to_bf16(x[2]) | (static_cast<uint32_t>(f32_to_bf16(x[3])) << 16);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + idx) = make_uint2(lo, hi);
+  }
+}
+
+// What a row of the output holds where it is not a plain quotient: zeros for a sequence or token
+// that is switched off, NaN for a position past the cache.
+__device__ __forceinline__ float row_factor(const Kv8Attn& a, int64_t b, int64_t i, float l) {
+  const int64_t start = a.start[b * a.start_step];
+  if (start < 0 || (a.lengths && i >= a.lengths[b])) return 0.0f;
+  if (start + i >= a.c.NB * kTok) return __uint_as_float(0x7fc00000u);
+  return 1.0f / l;
+}
+
+template <int D, int QDT, int ODT, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
+  constexpr int KK = D / 64, FT = D / 16;
+  __shared__ __attribute__((aligned(16))) float so[4][16][D + 4];
+  __shared__ float sm[4][16], sl[4][16];
+  const int split = blockIdx.x;
+  const int64_t tile = blockIdx.y, bh = blockIdx.z;
+  const int64_t b = bh / a.c.H, kvh = bh - b * a.c.H;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t start = a.start[b * a.start_step];
+  const int64_t cols = a.S * a.G;
+  // this lane's column: query i of head kvh * G + hg; lanes past the last take the last's
+  const int64_t cc = tile * 16 + col < cols ? tile * 16 + col : cols - 1;
+  const int64_t i = cc / a.G, hd = kvh * a.G + (cc - i * a.G);
+  int64_t n = a.lengths ? a.lengths[b] : a.S;
+  n = n < a.S ? n : a.S;
+  // the blocks that the tile's last active query sees
+  const int64_t c_last = tile * 16 + 15 < cols ? tile * 16 + 15 : cols - 1;
+  int64_t i_last = c_last / a.G;
+  i_last = i_last < n ? i_last : n - 1;
+  int64_t nb = start < 0 || n <= 0 || tile * 16 / a.G >= n ? 0 : (start + i_last) / kTok + 1;
+  nb = nb < a.c.NB ? nb : a.c.NB;
+  const int64_t per = (nb + a.nsplit - 1) / a.nsplit;
+  const int64_t j0 = split * per, j1 = j0 + per < nb ? j0 + per : nb;
+
+  float m = -INFINITY, l = 0.0f, o[FT][4];
+#pragma unroll
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[f][e] = 0.0f;
+
+  if (j0 + wave < j1) {
+    // the query's digits: features 64 kk + 16 g .. + 15
+    v4i8 qd[3][KK];
+    float qscale;
+    {
+      float x[KK][16];
+      uint32_t most = 0;
+      const int64_t base = b * a.sqb + hd * a.sqh + i * a.sqs + 16 * g;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+        for (int v = 0; v < 16 / Vec<QDT>::N; ++v)
+          load_vec16<QDT>(a.q, base + 64 * kk + v * Vec<QDT>::N, x[kk] + v * Vec<QDT>::N);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t bits = __float_as_uint(x[kk][e]) & 0x7fffffffu;
+          most = bits > most ? bits : most;
+        }
+      }
+      most = col_umax(most);
+      const float big = __uint_as_float(most);
+      const float up = big > 0.0f ? kFixed / big : 0.0f;
+      qscale = big / kFixed;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            y[e] = fminf(fmaxf(x[kk][4 * w + e] * up, -kFixed), kFixed);
+          int d0, d1, d2;
+          digits4(y, d0, d1, d2);
+          qd[0][kk][w] = d0;
+          qd[1][kk][w] = d1;
+          qd[2][kk][w] = d2;
+        }
+    }
+    float slope2 = 0.0f;
+    if constexpr (BIAS) slope2 = a.slopes[hd] * kLog2e8;
+    const int64_t pos = start + i;
+    const int8_t* const kbase = a.c.keys + bh * a.c.NB * kTok * D;
+    const int8_t* const vbase = a.c.values + bh * a.c.NB * kTok * D;
+    const float* const ks = a.c.ks + bh * a.c.NB;
+    const float* const vs = a.c.vs + bh * a.c.NB;
+    const int koff = (16 * (col >> 2) + (col & 3)) * D + 16 * g;  // row 4 g' + e' of product 0
+    const int voff = col * kTok + 16 * g;
+
+    v4i8 kf[4][KK], vf[FT];
+    auto load_k = [&](int64_t j) {
+      const int8_t* p = kbase + j * (kTok * D) + koff;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+          kf[t][kk] = *reinterpret_cast<const v4i8*>(p + 4 * t * D + 64 * kk);
+    };
+    auto load_v = [&](int64_t j) {
+      const int8_t* p = vbase + j * (kTok * D) + voff;
+#pragma unroll
+      for (int f = 0; f < FT; ++f) vf[f] = *reinterpret_cast<const v4i8*>(p + 16 * f * kTok);
+    };
+    int64_t j = j0 + wave;
+    load_k(j);
+    load_v(j);
+    for (; j < j1; j += 4) {
+      const bool more = j + 4 < j1;
+      const float kscale = ks[j], vscale = vs[j];
+      float s[16];
+      const float mul = qscale * kscale * a.dot_scale;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        v4i8 acc[3];
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+          acc[d] = v4i8{0, 0, 0, 0};
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+            acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][kk], qd[d][kk], acc[d], 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[4 * t + e] = from_digits(acc[0][e], acc[1][e], acc[2][e]) * mul;
+      }
+      if (more) load_k(j + 4);
+      const int64_t ahead = pos - (j * kTok + 16 * g);
+      const int left = ahead > 16 ? 16 : ahead < -1 ? -1 : static_cast<int>(ahead);
+      const float d0 = static_cast<float>(ahead);  // key 16 g + x is seen for x <= left
+      float mx = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        float t = s[x];
+        if constexpr (CAP) {
+          const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(t) + 1.0f);
+          t = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
+        }
+        if constexpr (BIAS) t = __builtin_fmaf(-slope2, d0 - x, t);
+        s[x] = x <= left ? t : -INFINITY;
+        mx = fmaxf(mx, s[x]);
+      }
+      mx = col_max(mx);  // the block's own, the probabilities' unit
+      const float mnew = fmaxf(m, mx);
+      const float ref = mx == -INFINITY ? 0.0f : mx, nref = mnew == -INFINITY ? 0.0f : mnew;
+      const float alpha = __builtin_amdgcn_exp2f(m - nref);
+      const float beta = __builtin_amdgcn_exp2f(mx - nref);
+      m = mnew;
+      float sum = 0.0f;
+      v4i8 pd[3];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = __builtin_amdgcn_exp2f(s[4 * w + e] - ref);
+          sum = sum + p;
+          y[e] = fminf(p, 1.0f) * kFixed;
+        }
+        int d0i, d1i, d2i;
+        digits4(y, d0i, d1i, d2i);
+        pd[0][w] = d0i;
+        pd[1][w] = d1i;
+        pd[2][w] = d2i;
+      }
+      l = l * alpha + beta * col_sum(sum);
+      // a block that the column does not see at all adds nothing, whatever its scale
+      const float add = mx == -INFINITY && sum == 0.0f ? 0.0f : beta * vscale * (1.0f / kFixed);
+#pragma unroll
+      for (int f = 0; f < FT; ++f) {
+        v4i8 acc[3];
+#pragma unroll
+        for (int d = 0; d < 3; ++d)
+          acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[f], pd[d], v4i8{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[f][e] = __builtin_fmaf(from_digits(acc[0][e], acc[1][e], acc[2][e]), add,
+                                   o[f][e] * alpha);
+      }
+      if (more) load_v(j + 4);
+    }
+  }
+
+  // the four wavefronts
+  if (g == 0) {
+    sm[wave][col] = m;
+    sl[wave][col] = l;
+  }
+#pragma unroll
+  for (int f = 0; f < FT; ++f)
+    *reinterpret_cast<float4*>(&so[wave][col][16 * f + 4 * g]) =
+        make_float4(o[f][0], o[f][1], o[f][2], o[f][3]);
+  __syncthreads();
+  // a thread takes 4 features of one column at a time
+  for (int idx = tid; idx < 16 * (D / 4); idx += 256) {
+    const int c = idx / (D / 4), f = idx % (D / 4) * 4;
+    const int64_t ct = tile * 16 + c;
+    if (ct >= cols) break;
+    float mm = sm[0][c];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm[w][c]);
+    float ll = 0.0f, r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float x = sm[w][c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][c] - mm);
+      // a NaN sum with no maximum still has to be seen
+      ll = ll + (sl[w][c] == sl[w][c] ? x * sl[w][c] : sl[w][c]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = __builtin_fmaf(x, so[w][c][f + e], r[e]);
+    }
+    if (a.nsplit == 1) {
+      const int64_t qi = ct / a.G, h = kvh * a.G + (ct - qi * a.G);
+      const float factor = row_factor(a, b, qi, ll);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = factor == 0.0f ? 0.0f : r[e] * factor;
+      store4<ODT>(a.out, ((b * a.S + qi) * a.Hq + h) * D + f, r);
+    } else {
+      float* const w = a.work + (((bh * a.tiles + tile) * a.nsplit + split) * 16 + c) * (D + 4);
+      *reinterpret_cast<float4*>(w + 4 + f) = make_float4(r[0], r[1], r[2], r[3]);
+      if (f == 0) {
+        w[0] = mm;
+        w[1] = ll;
+      }
+    }
+  }
+}
+
+// grid (columns, B * H), D / 4 threads: the splits of one column.
+template <int D, int ODT>
+__global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
+  const int64_t ct = blockIdx.x, bh = blockIdx.y, b = bh / a.c.H, kvh = bh - b * a.c.H;
+  const int f = threadIdx.x * 4;
+  const float* w = a.work + (((bh * a.tiles + ct / 16) * a.nsplit) * 16 + ct % 16) * (D + 4);
+  const int64_t step = 16 * (D + 4);
+  float mm = -INFINITY;
+  for (int64_t s = 0; s < a.nsplit; ++s) mm = fmaxf(mm, w[s * step]);
+  float ll = 0.0f, r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t s = 0; s < a.nsplit; ++s) {
+    const float ms = w[s * step], ls = w[s * step + 1];
+    const float x = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - mm);
+    ll = ll + (ls == ls ? x * ls : ls);
+    const float4 v = *reinterpret_cast<const float4*>(w + s * step + 4 + f);
+    r[0] = __builtin_fmaf(x, v.x, r[0]);
+    r[1] = __builtin_fmaf(x, v.y, r[1]);
+    r[2] = __builtin_fmaf(x, v.z, r[2]);
+    r[3] = __builtin_fmaf(x, v.w, r[3]);
+  }
+  const int64_t qi = ct / a.G, h = kvh * a.G + (ct - qi * a.G);
+  const float factor = row_factor(a, b, qi, ll);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = factor == 0.0f ? 0.0f : r[e] * factor;
+  store4<ODT>(a.out, ((b * a.S + qi) * a.Hq + h) * D + f, r);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+static int check_cache(const rk_int8_kv& c) {
+  if (c.B < 0 || c.H < 0 || c.blocks < 0) return fail(RK_ERR_ARG, "negative size");
+  if (c.D != 64 && c.D != 128 && c.D != 256)
+    return fail(RK_ERR_UNSUPPORTED, "head size %lld (64, 128 or 256)", static_cast<long long>(c.D));
+  if (c.B == 0 || c.H == 0 || c.blocks == 0) return RK_OK;
+  if (!c.keys || !c.values || !c.key_scales || !c.value_scales)
+    return fail(RK_ERR_ARG, "null cache");
+  if (!aligned16(c.keys) || !aligned16(c.values))
+    return fail(RK_ERR_UNSUPPORTED, "the cache needs 16-byte alignment");
+  if (c.B * c.H > 65535) return fail(RK_ERR_UNSUPPORTED, "more than 65535 sequence heads");
+  if (c.blocks > (int64_t{1} << 30)) return fail(RK_ERR_UNSUPPORTED, "cache too long");
+  return RK_OK;
+}
+
+static Kv8 cache_args(const rk_int8_kv& c) {
+  return Kv8{c.keys, c.values, c.key_scales, c.value_scales, c.B, c.H, c.blocks};
+}
+
+static int64_t columns_tiles(int64_t S, int64_t G) { return (S * G + 15) / 16; }
+
+// Splits of the cache: about 1024 workgroups, and at least a block per wavefront of a split.
+static int64_t attention_splits(const rk_int8_kv& c, int64_t tiles) {
+  const int64_t have = c.B * c.H * tiles, want = have > 0 ? (1024 + have - 1) / have : 1;
+  const int64_t most = (c.blocks + 3) / 4;
+  return want < 1 ? 1 : (want < most ? want : (most > 0 ? most : 1));
+}
+
+template <int D, int QDT, int ODT>
+static void launch_kv8_attn(const Kv8Attn& a, bool cap, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.nsplit), static_cast<unsigned>(a.tiles),
+                  static_cast<unsigned>(a.c.B * a.c.H));
+  if (cap && a.slopes) kv8_attn_kernel<D, QDT, ODT, true, true><<<grid, 256, 0, st>>>(a);
+  else if (cap) kv8_attn_kernel<D, QDT, ODT, true, false><<<grid, 256, 0, st>>>(a);
+  else if (a.slopes) kv8_attn_kernel<D, QDT, ODT, false, true><<<grid, 256, 0, st>>>(a);
+  else kv8_attn_kernel<D, QDT, ODT, false, false><<<grid, 256, 0, st>>>(a);
+  if (a.nsplit > 1)
+    kv8_join_kernel<D, ODT><<<dim3(static_cast<unsigned>(a.S * a.G),
+                                   static_cast<unsigned>(a.c.B * a.c.H)), D / 4, 0, st>>>(a);
+}
+
+template <int D>
+static void dispatch_kv8_attn(const Kv8Attn& a, bool cap, int qdt, int odt, hipStream_t st) {
+  if (qdt == RK_F32) {
+    if (odt == RK_F32) launch_kv8_attn<D, RK_F32, RK_F32>(a, cap, st);
+    else launch_kv8_attn<D, RK_F32, RK_BF16>(a, cap, st);
+  } else {
+    if (odt == RK_F32) launch_kv8_attn<D, RK_BF16, RK_F32>(a, cap, st);
+    else launch_kv8_attn<D, RK_BF16, RK_BF16>(a, cap, st);
+  }
+}
+
+}  // namespace rk
+
+using namespace rk;
+
+extern "C" int rk_int8_kv_append(const rk_int8_kv* cache, const void* k, int64_t skb, int64_t skh,
+                                 int64_t sks, const void* v, int64_t svb, int64_t svh, int64_t svs,
+                                 int dtype, int64_t S, const int64_t* start, int64_t start_count,
+                                 const int64_t* lengths, void* stream) {
+  clear_error();
+  if (!cache) return fail(RK_ERR_ARG, "null cache");
+  const rk_int8_kv& c = *cache;
+  if (int e = check_cache(c)) return e;
+  if (S < 0) return fail(RK_ERR_ARG, "negative size");
+  if (dtype != RK_F32 && dtype != RK_BF16)
+    return fail(RK_ERR_ARG, "keys and values must be float32 or bfloat16");
+  if (start_count != 1 && start_count != c.B)
+    return fail(RK_ERR_ARG, "one start, or one per sequence");
+  if (c.B == 0 || c.H == 0 || c.blocks == 0 || S == 0) return RK_OK;
+  if (!k || !v || !start) return fail(RK_ERR_ARG, "null pointer");
+  const int64_t per = dtype == RK_F32 ? 4 : 8;
+  const int64_t strides[] = {skb, skh, sks, svb, svh, svs};
+  for (int64_t st : strides)
+    if (st < 0 || st % per != 0)
+      return fail(RK_ERR_UNSUPPORTED, "rows and strides must be whole 16-byte vectors");
+  if (!aligned16(k) || !aligned16(v))
+    return fail(RK_ERR_UNSUPPORTED, "keys and values need 16-byte alignment");
+  if (S > (int64_t{1} << 30)) return fail(RK_ERR_UNSUPPORTED, "too many tokens");
+  Kv8Append a{cache_args(c), k, v, skb, skh, sks, svb, svh, svs, start, lengths,
+              start_count > 1 ? 1 : 0, S};
+  // S tokens from any position touch at most this many blocks
+  const dim3 grid(static_cast<unsigned>((S + kTok - 2) / kTok + 1),
+                  static_cast<unsigned>(c.B * c.H), 2);
+  hipStream_t st = as_stream(stream);
+  const auto run = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (c.D == 64) kv8_append_kernel<DT, 64><<<grid, 256, 0, st>>>(a);
+    else if (c.D == 128) kv8_append_kernel<DT, 128><<<grid, 256, 0, st>>>(a);
+    else kv8_append_kernel<DT, 256><<<grid, 256, 0, st>>>(a);
+  };
+  if (dtype == RK_F32) run(std::integral_constant<int, RK_F32>{});
+  else run(std::integral_constant<int, RK_BF16>{});
+  return launch_status("int8_kv_append");
+}
+
+extern "C" int rk_int8_kv_read(const rk_int8_kv* cache, int64_t begin, int64_t end, int dtype,
+                               void* keys, void* values, void* stream) {
+  clear_error();
+  if (!cache) return fail(RK_ERR_ARG, "null cache");
+  const rk_int8_kv& c = *cache;
+  if (int e = check_cache(c)) return e;
+  if (begin < 0 || end < begin || end > c.blocks * kTok)
+    return fail(RK_ERR_ARG, "positions past the cache");
+  if (dtype != RK_F32 && dtype != RK_BF16)
+    return fail(RK_ERR_ARG, "values are read as float32 or bfloat16");
+  if (c.B == 0 || c.H == 0 || end == begin) return RK_OK;
+  if (!keys || !values) return fail(RK_ERR_ARG, "null pointer");
+  if (!aligned16(keys) || !aligned16(values))
+    return fail(RK_ERR_UNSUPPORTED, "keys and values need 16-byte alignment");
+  Kv8Read a{cache_args(c), begin, end - begin, keys, values};
+  const dim3 grid(static_cast<unsigned>((end + kTok - 1) / kTok - begin / kTok),
+                  static_cast<unsigned>(c.B * c.H), 2);
+  hipStream_t st = as_stream(stream);
+  const auto run = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (c.D == 64) kv8_read_kernel<DT, 64><<<grid, 256, 0, st>>>(a);
+    else if (c.D == 128) kv8_read_kernel<DT, 128><<<grid, 256, 0, st>>>(a);
+    else kv8_read_kernel<DT, 256><<<grid, 256, 0, st>>>(a);
+  };
+  if (dtype == RK_F32) run(std::integral_constant<int, RK_F32>{});
+  else run(std::integral_constant<int, RK_BF16>{});
+  return launch_status("int8_kv_read");
+}
+
+extern "C" int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S) {
+  if (!cache || cache->B <= 0 || cache->H <= 0 || Hq <= 0 || S <= 0 || Hq % cache->H) return 0;
+  const int64_t tiles = columns_tiles(S, Hq / cache->H), n = attention_splits(*cache, tiles);
+  return n == 1 ? 0 : cache->B * cache->H * tiles * n * 16 * (cache->D + 4);
+}
+
+extern "C" int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int qdtype, int64_t sqb,
+                                    int64_t sqh, int64_t sqs, int64_t Hq, int64_t S,
+                                    const int64_t* start, int64_t start_count,
+                                    const int64_t* lengths, float scale, float softcap,
+                                    const float* slopes, float* work, int64_t work_floats,
+                                    void* out, int odtype, void* stream) {
+  clear_error();
+  if (!cache) return fail(RK_ERR_ARG, "null cache");
+  const rk_int8_kv& c = *cache;
+  if (int e = check_cache(c)) return e;
+  if (S < 0 || Hq < 0) return fail(RK_ERR_ARG, "negative size");
+  if (c.H == 0 ? Hq != 0 : Hq % c.H != 0)
+    return fail(RK_ERR_ARG, "query heads must be a multiple of the key heads");
+  if ((qdtype != RK_F32 && qdtype != RK_BF16) || (odtype != RK_F32 && odtype != RK_BF16))
+    return fail(RK_ERR_ARG, "queries and outputs are float32 or bfloat16");
+  if (start_count != 1 && start_count != c.B)
+    return fail(RK_ERR_ARG, "one start, or one per sequence");
+  if (!(scale > 0.0f) || !(scale < INFINITY))
+    return fail(RK_ERR_ARG, "scale must be positive and finite");
+  if (!(softcap >= 0.0f) || !(softcap < INFINITY))
+    return fail(RK_ERR_ARG, "softcap must be finite and not negative (0: none)");
+  if (c.B == 0 || Hq == 0 || S == 0) return RK_OK;
+  if (c.blocks == 0) return fail(RK_ERR_ARG, "an empty cache");
+  if (!q || !start || !out) return fail(RK_ERR_ARG, "null pointer");
+  const int64_t per = qdtype == RK_F32 ? 4 : 8;
+  const int64_t strides[] = {sqb, sqh, sqs};
+  for (int64_t st : strides)
+    if (st < 0 || st % per != 0)
+      return fail(RK_ERR_UNSUPPORTED, "query rows and strides must be whole 16-byte vectors");
+  if (!aligned16(q) || !aligned16(out))
+    return fail(RK_ERR_UNSUPPORTED, "queries and outputs need 16-byte alignment");
+  const int64_t G = Hq / c.H, tiles = columns_tiles(S, G);
+  if (tiles > 65535 || S * G >= (int64_t{1} << 24))
+    return fail(RK_ERR_UNSUPPORTED, "too many queries for one launch");
+  const int64_t n = attention_splits(c, tiles);
+  if (n > 1 && (!work || !aligned16(work) || work_floats < rk_int8_kv_attention_work(&c, Hq, S)))
+    return fail(RK_ERR_ARG, "attention workspace too small");
+  const bool cap = softcap > 0.0f;
+  Kv8Attn a{cache_args(c), q, sqb, sqh, sqs, start, lengths, slopes, start_count > 1 ? 1 : 0, S,
+            Hq, G, n, tiles,
+            cap ? 2.0f * kLog2e8 * (scale / softcap) : scale * kLog2e8, softcap * kLog2e8, work,
+            out};
+  hipStream_t st = as_stream(stream);
+  if (c.D == 64) dispatch_kv8_attn<64>(a, cap, qdtype, odtype, st);
+  else if (c.D == 128) dispatch_kv8_attn<128>(a, cap, qdtype, odtype, st);
+  else dispatch_kv8_attn<256>(a, cap, qdtype, odtype, st);
+  return launch_status("int8_kv_attention");
+}

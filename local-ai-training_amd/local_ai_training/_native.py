@@ -131,6 +131,12 @@ SIGNATURES: dict[str, list] = {
     "rk_scored_attention_forward": [_p, _p],
     "rk_scored_attention_backward_work": [_i64, _i64, _i64, _i32],
     "rk_scored_attention_backward": [_p, _p, _p],
+    "rk_int8_kv_append": [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _i64, _p, _i64,
+                          _p, _p],
+    "rk_int8_kv_read": [_p, _i64, _i64, _i32, _p, _p, _p],
+    "rk_int8_kv_attention_work": [_p, _i64, _i64],
+    "rk_int8_kv_attention": [_p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _f32, _f32,
+                             _p, _p, _i64, _p, _i32, _p],
     "rk_kv_append": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i32, _i64, _i64,
                      _i64, _i64, _i64, _i64, _i64, _p],
     "rk_version": [],
@@ -142,6 +148,7 @@ RESTYPES = {
     "rk_last_error": ctypes.c_char_p,
     "rk_attention_backward_work": ctypes.c_int64,
     "rk_scored_attention_backward_work": ctypes.c_int64,
+    "rk_int8_kv_attention_work": ctypes.c_int64,
     "rk_int8_gemm_large_rows": ctypes.c_int64,
     "rk_decode_attention_splits": ctypes.c_int64,
     "rk_grad_weight_update_counters": ctypes.c_int64,

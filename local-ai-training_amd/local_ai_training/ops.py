@@ -201,6 +201,21 @@ def _register_fakes() -> None:
         return (rows(q), rows(k), rows(k),
                 q.new_empty((q.shape[1] if slope_grad else 0,), dtype=torch.float32))
 
+    @fake("ratchet::int8_kv_append")
+    def _int8_kv_append(k, v, keys, values, key_scales, value_scales, start, lengths):
+        return None
+
+    @fake("ratchet::int8_kv_read")
+    def _int8_kv_read(keys, values, key_scales, value_scales, begin, end, dtype):
+        b, h, _, _, d = keys.shape
+        return tuple(keys.new_empty((b, h, end - begin, d), dtype=dtype) for _ in range(2))
+
+    @fake("ratchet::int8_kv_attention")
+    def _int8_kv_attention(q, keys, values, key_scales, value_scales, start, lengths, scale,
+                           softcap, slopes, out_dtype):
+        b, h, sl, d = q.shape
+        return q.new_empty((b, sl, h, d), dtype=out_dtype).permute(0, 2, 1, 3)
+
     @fake("ratchet::kv_append")
     def _kv_append(k, v, keys, values, start, clear_to):
         return None
