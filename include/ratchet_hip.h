@@ -723,7 +723,7 @@ int rk_attention_mask(const void* documents, int wide, int64_t sdb, const uint8_
  *   o_i = sum_j softmax_j(s_ij over the keys i sees) v_j,  lse_i = log sum_j exp(s_ij).
  * A query that sees nothing gets zeros (lse 0); what padding positions hold does not matter.
  * The backward reads o, lse and the gradient g of o, and writes dq, dk, dv and, where given,
- * dslopes (float32 [H]); work: rk_scored_attention_backward_work floats. Scores and softmax run
+ * dslopes (float32 [H]); work: rk_scored_attention_backward_work floats, 16-byte aligned. Scores and softmax run
  * in float32; probabilities and score gradients enter the products rounded to bf16; every sum
  * has a fixed order. Inputs 16-byte aligned, outputs 8-byte, strides multiples of 8 elements, one
  * head's positions under 2^31 bytes, fewer than 2^24 blocks of 128 positions; otherwise
@@ -748,7 +748,8 @@ typedef struct rk_scored_attention_args {
 } rk_scored_attention_args;
 
 int rk_scored_attention_forward(const rk_scored_attention_args* args, void* stream);
-int64_t rk_scored_attention_backward_work(int64_t B, int64_t H, int64_t S, int slopes);
+int64_t rk_scored_attention_backward_work(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D,
+                                          int slopes);
 int rk_scored_attention_backward(const rk_scored_attention_args* args, float* work, void* stream);
 
 /*

@@ -1185,7 +1185,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> scored_attention_backward(
   Tensor dq = out(a.H), dk = out(a.Hkv), dv = out(a.Hkv);
   Tensor dslopes = at::empty({slope_grad ? a.H : 0}, lse.options());
   if (q.numel() == 0) return {dq, dk, dv, dslopes.zero_()};
-  Tensor work = at::empty({rk_scored_attention_backward_work(a.B, a.H, a.S, slope_grad)},
+  Tensor work = at::empty({rk_scored_attention_backward_work(a.B, a.H, a.Hkv, a.S, a.D,
+                                                            slope_grad)},
                           lse.options());
   const auto w16 = [](const Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); };
   a.o = w16(oo), a.sob = oo.stride(0), a.soh = oo.stride(1), a.sos = oo.stride(2);

@@ -24,9 +24,14 @@ struct ScoredBwdArgs {
   float inv_scale;  // 1 / scale
   float* rows;      // [B H][2][Sp]: log-sum-exp term and -delta (zeros where a row is none)
   float* slope_rows;  // [B H][Sp], or null
+  // the query heads of a key head in `parts` workgroups each: their float32 dk, dv [parts][2]
+  // [B Hkv][S][D], added by a launch of their own (1: written as they are)
+  int64_t parts;
+  float* part_rows;
 };
 
 constexpr int kBwdRows = 32;  // staged rows per step
+constexpr int64_t kBwdBlocks = 1024;  // workgroups wanted of the second launch (head_parts)
 
 // p and the factor of the score's gradient from the accumulated dot product. `term`: plain,
 // already in the accumulator (-lse / scale); otherwise lse log2(e), subtracted here.
@@ -126,49 +131,54 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
     }
     const int key0 = step * kBwdRows;
     if (ws.none(key0, kBwdRows)) continue;
-    v16f_a st, dp;
+    v16f_a st;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      st[e] = CAP ? 0.0f : term;
-      dp[e] = ndelta;
-    }
+    for (int e = 0; e < 16; ++e) st[e] = CAP ? 0.0f : term;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
       st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, 0, s, lane), qf[s], st,
                                                    0, 0, 0);
+    // the probabilities times the cap's slope (with slope gradients: apart)
+    const bool whole = ws.all(key0, kBwdRows);
+    const int j0 = key0 + 4 * h - span.lo;
+    const float d0 = static_cast<float>(qi - key0 - 4 * h);
+    float slack[CAP && SG ? 16 : 1];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float sl;
+      st[e] = score_p<CAP, BIAS>(a, st[e], term, slope2,
+                                 d0 - static_cast<float>(8 * (e / 4) + (e % 4)), sl);
+      if constexpr (CAP && SG) slack[e] = sl;
+      else if constexpr (CAP) st[e] = st[e] * sl;
+    }
+    if (!whole) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) st[e] = 0.0f;
+    }
+    v16f_a dp;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dp[e] = ndelta;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
       dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(vt, 0, s, lane), gf[s], dp,
                                                    0, 0, 0);
-    const float d0 = static_cast<float>(qi - key0 - 4 * h);
-    float ds[16], pr[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float slack;
-      pr[e] = score_p<CAP, BIAS>(a, st[e], term, slope2,
-                                 d0 - static_cast<float>(8 * (e / 4) + (e % 4)), slack);
-      st[e] = slack;
-    }
-    if (!ws.all(key0, kBwdRows)) {
-      const int j0 = key0 + 4 * h - span.lo;
+    if (!whole) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) {
-          pr[e] = 0.0f;
-          dp[e] = 0.0f;
-          st[e] = 0.0f;
-        }
+        if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) dp[e] = 0.0f;
     }
+    float ds[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      ds[e] = pr[e] * dp[e];
+      ds[e] = st[e] * dp[e];
       if constexpr (SG) {
         const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
         s_pd = s_pd + ds[e];
-        s_pa = __builtin_fmaf(pr[e], dist, s_pa);
+        s_pa = __builtin_fmaf(st[e], dist, s_pa);
         s_pda = __builtin_fmaf(ds[e], dist, s_pda);
+        if constexpr (CAP) ds[e] = ds[e] * slack[e];
       }
-      if constexpr (CAP) ds[e] = ds[e] * st[e];
     }
     uint4 dsf[2];
     pack16(dsf, ds);
@@ -227,8 +237,12 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
   const rk_scored_attention_args& p = a.p;
   const int S = static_cast<int>(p.S);
   const int64_t BH = p.B * p.Hkv;
-  const int blk = static_cast<int>(blockIdx.x / BH);  // heads fastest
-  const int64_t bh = blockIdx.x - blk * BH, b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  const int blk = static_cast<int>(blockIdx.x / (BH * ba.parts));  // heads fastest
+  const int64_t idx = blockIdx.x - blk * (BH * ba.parts);
+  const int64_t bh = idx / ba.parts, part = idx - bh * ba.parts;
+  const int64_t b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  const int heads = static_cast<int>(a.G / ba.parts);
+  const int64_t hq = kvh * a.G + part * heads;  // the first query head
   const int k0 = blk * kAttnRows;  // the first keys have the longest walk
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -249,26 +263,30 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
   for (int t = 0; t < kAttnRows / kBwdRows; ++t)
     vd.issue(lds_address(smem) + t * T::BYTES, k0 + t * kBwdRows, wave);
 
-  // the group's query heads one after the other, the tiles of the next one behind the last of
+  // the query heads one after the other, the tiles of the next one behind the last of
   // this one: tile n of all is step n % steps of head n / steps
-  const int total = steps * static_cast<int>(a.G);
+  const int total = steps * heads;
   int ihead = 0, istep = 0;  // the next tile to load
+  TileDma<D, kBwdRows> qd(p.q + b * p.sqb + hq * p.sqh, p.sqs, S, wave, lane);
+  TileDma<D, kBwdRows> gd(p.g + b * p.sgb + hq * p.sgh, p.sgs, S, wave, lane);
+  // row statistics: lanes 0..31 take the first plane, lanes 32..63 the second (every wavefront
+  // writes the same bytes)
+  const int rvoff = static_cast<int>((h * a.Sp + l32) * 4);
+  __amdgpu_buffer_rsrc_t rbuf = make_buffer(ba.rows + (b * p.H + hq) * 2 * a.Sp, 2 * a.Sp * 4);
   auto issue = [&](int n) {
-    const int64_t hd = kvh * a.G + ihead;
     const uint32_t st = lds0 + (n & 1) * STAGE;
     const int row0 = (first + istep) * kBwdRows;
-    const TileDma<D, kBwdRows> qd(p.q + b * p.sqb + hd * p.sqh, p.sqs, S, wave, lane);
-    const TileDma<D, kBwdRows> gd(p.g + b * p.sgb + hd * p.sgh, p.sgs, S, wave, lane);
-    // row statistics: lanes 0..31 take the first plane, lanes 32..63 the second (every wavefront
-    // writes the same bytes)
-    const __amdgpu_buffer_rsrc_t rbuf =
-        make_buffer(ba.rows + (b * p.H + hd) * 2 * a.Sp, 2 * a.Sp * 4);
-    dma4(rbuf, st + 2 * T::BYTES, static_cast<int>((h * a.Sp + l32) * 4), row0 * 4);
+    dma4(rbuf, st + 2 * T::BYTES, rvoff, row0 * 4);
     qd.issue(st, row0, wave);
     gd.issue(st + T::BYTES, row0, wave);
     if (++istep == steps) {
       istep = 0;
-      ++ihead;
+      const int64_t hd = hq + ++ihead;
+      if (ihead < heads) {
+        qd.buf = make_buffer(p.q + b * p.sqb + hd * p.sqh, ((p.S - 1) * p.sqs + D) * 2);
+        gd.buf = make_buffer(p.g + b * p.sgb + hd * p.sgh, ((p.S - 1) * p.sgs + D) * 2);
+        rbuf = make_buffer(ba.rows + (b * p.H + hd) * 2 * a.Sp, 2 * a.Sp * 4);
+      }
     }
   };
 
@@ -285,7 +303,7 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
     const int qs = (first + cstep) * kBwdRows;
     const uint64_t pad = padding_bits<kBwdRows>(a, b, qs);
     if constexpr (BIAS)
-      if (cstep == 0) slope2 = p.slopes[kvh * a.G + chead] * kLog2e;
+      if (cstep == 0) slope2 = p.slopes[hq + chead] * kLog2e;
     if (++cstep == steps) {
       cstep = 0;
       ++chead;
@@ -301,53 +319,66 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
       __syncthreads();
     }
     if (ws.none(qs, kBwdRows)) continue;
-    v16f_a st, dp;
-    float term[16];
+    // -lse / scale (plain: where the scores' sums begin), or lse log2(e)
+    const auto row_terms = [&](int plane, v16f_a& x) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float4 nl = *reinterpret_cast<const float4*>(rows + 8 * r + 4 * h);
-      const float4 nd = *reinterpret_cast<const float4*>(rows + kBwdRows + 8 * r + 4 * h);
-      term[4 * r] = nl.x; term[4 * r + 1] = nl.y; term[4 * r + 2] = nl.z; term[4 * r + 3] = nl.w;
-      dp[4 * r] = nd.x; dp[4 * r + 1] = nd.y; dp[4 * r + 2] = nd.z; dp[4 * r + 3] = nd.w;
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) st[e] = CAP ? 0.0f : term[e];
+      for (int r = 0; r < 4; ++r) {
+        const float4 v = *reinterpret_cast<const float4*>(rows + plane * kBwdRows + 8 * r + 4 * h);
+        x[4 * r] = v.x; x[4 * r + 1] = v.y; x[4 * r + 2] = v.z; x[4 * r + 3] = v.w;
+      }
+    };
+    v16f_a st{};
+    if constexpr (!CAP) row_terms(0, st);
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
       st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(qt, 0, s, lane), kf[s], st,
                                                    0, 0, 0);
+    const bool whole = ws.all(qs, kBwdRows);
+    const int i0 = qs + 4 * h - span.lo;
+    const float d0 = static_cast<float>(qs + 4 * h - kj);
+    // the probabilities, packed, and times the cap's slope
+    uint4 pf[2], dsf[2];
+    {
+      float pr[16];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float4 term{};
+        if constexpr (CAP) term = *reinterpret_cast<const float4*>(rows + 8 * r + 4 * h);
+        const float t4[4] = {term.x, term.y, term.z, term.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int e = 4 * r + x;
+          float sl;
+          pr[e] = score_p<CAP, BIAS>(a, st[e], t4[x], slope2,
+                                     d0 + static_cast<float>(8 * r + x), sl);
+          st[e] = CAP ? pr[e] * sl : pr[e];
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width) st[e] = pr[e] = 0.0f;
+      }
+      pack16(pf, pr);
+    }
+    v16f_a dp;
+    row_terms(1, dp);
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
       dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(gt, 0, s, lane),
                                                    row_frag<D>(smem, 32 * wave, s, lane), dp,
                                                    0, 0, 0);
-    const float d0 = static_cast<float>(qs + 4 * h - kj);
-    float pr[16], ds[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float slack;
-      pr[e] = score_p<CAP, BIAS>(a, st[e], term[e], slope2,
-                                 d0 + static_cast<float>(8 * (e / 4) + (e % 4)), slack);
-      st[e] = slack;
-    }
-    if (!ws.all(qs, kBwdRows)) {
-      const int i0 = qs + 4 * h - span.lo;
+    if (!whole) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width) {
-          pr[e] = 0.0f;
-          dp[e] = 0.0f;
-          st[e] = 0.0f;
-        }
+        if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width) dp[e] = 0.0f;
     }
+    {
+      float ds[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      ds[e] = pr[e] * dp[e];
-      if constexpr (CAP) ds[e] = ds[e] * st[e];
+      for (int e = 0; e < 16; ++e) ds[e] = st[e] * dp[e];
+      pack16(dsf, ds);
     }
-    uint4 pf[2], dsf[2];
-    pack16(pf, pr);
-    pack16(dsf, ds);
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
@@ -370,11 +401,55 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
       dv[dt] = v16f_a{};
     }
   }
-  if (kj < S) {
+  if (kj < S && ba.parts > 1) {
+    float* const to = ba.part_rows + ((part * 2 * BH + bh) * S + kj) * D + 4 * h;
+    const int64_t plane = BH * S * D;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float* const x = to + 32 * dt + 8 * r;
+        *reinterpret_cast<float4*>(x) =
+            make_float4(dk[dt][4 * r], dk[dt][4 * r + 1], dk[dt][4 * r + 2], dk[dt][4 * r + 3]);
+        *reinterpret_cast<float4*>(x + plane) =
+            make_float4(dv[dt][4 * r], dv[dt][4 * r + 1], dv[dt][4 * r + 2], dv[dt][4 * r + 3]);
+      }
+  } else if (kj < S) {
     const int64_t off = b * p.syb + kvh * p.syh + static_cast<int64_t>(kj) * p.sys;
     store_owned<D>(p.dk + off, dk, p.scale, h);
     store_owned<D>(p.dv + off, dv, 1.0f, h);
   }
+}
+
+// grid (S * D / 1024, B * Hkv, 2: dk, dv), 256 threads of 4 features: the parts, in order.
+__global__ __launch_bounds__(256) void scored_parts_kernel(ScoredBwdArgs ba) {
+  const rk_scored_attention_args& p = ba.f.p;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  const int64_t BH = p.B * p.Hkv, bh = blockIdx.y, plane = BH * p.S * p.D;
+  if (i >= p.S * p.D) return;
+  const float* at = ba.part_rows + blockIdx.z * plane + bh * p.S * p.D + i;
+  float4 sum = *reinterpret_cast<const float4*>(at);
+  for (int64_t n = 1; n < ba.parts; ++n) {
+    const float4 x = *reinterpret_cast<const float4*>(at + 2 * n * plane);
+    sum.x = sum.x + x.x;
+    sum.y = sum.y + x.y;
+    sum.z = sum.z + x.z;
+    sum.w = sum.w + x.w;
+  }
+  const int64_t row = i / p.D, b = bh / p.Hkv, kvh = bh - b * p.Hkv;
+  uint16_t* const to = (blockIdx.z ? p.dv : p.dk) + b * p.syb + kvh * p.syh + row * p.sys +
+                       (i - row * p.D);
+  const float f = blockIdx.z ? 1.0f : p.scale;
+  *reinterpret_cast<uint2*>(to) =
+      make_uint2(bf16_pair(sum.x * f, sum.y * f), bf16_pair(sum.z * f, sum.w * f));
+}
+
+// Parts of the query heads that share a key head: enough for about 1024 workgroups.
+static int64_t head_parts(int64_t B, int64_t H, int64_t Hkv, int64_t S) {
+  const int64_t G = H / Hkv, have = B * Hkv * ((S + kAttnRows - 1) / kAttnRows);
+  for (int64_t n = 1; n < G; ++n)
+    if (G % n == 0 && have * n >= kBwdBlocks) return n;
+  return G;
 }
 
 template <int D, bool CAP, bool BIAS>
@@ -382,7 +457,7 @@ static void launch_scored_bwd(const ScoredBwdArgs& a, hipStream_t st) {
   const rk_scored_attention_args& p = a.f.p;
   const unsigned blocks = static_cast<unsigned>(a.f.Sp / kAttnRows);
   const dim3 qgrid(static_cast<unsigned>(p.B * p.H) * blocks);
-  const dim3 kgrid(static_cast<unsigned>(p.B * p.Hkv) * blocks);
+  const dim3 kgrid(static_cast<unsigned>(p.B * p.Hkv * a.parts) * blocks);
   if (BIAS && a.slope_rows) {
     scored_dq_kernel<D, CAP, BIAS, BIAS><<<qgrid, 256, 0, st>>>(a);
     scored_slope_kernel<<<static_cast<unsigned>(p.H), 256, 0, st>>>(a);
@@ -390,6 +465,9 @@ static void launch_scored_bwd(const ScoredBwdArgs& a, hipStream_t st) {
     scored_dq_kernel<D, CAP, BIAS, false><<<qgrid, 256, 0, st>>>(a);
   }
   scored_dkv_kernel<D, CAP, BIAS><<<kgrid, 256, 0, st>>>(a);
+  if (a.parts > 1)
+    scored_parts_kernel<<<dim3(static_cast<unsigned>((p.S * D + 1023) / 1024),
+                               static_cast<unsigned>(p.B * p.Hkv), 2), 256, 0, st>>>(a);
 }
 
 template <int D>
@@ -405,9 +483,12 @@ static void dispatch_scored_bwd(const ScoredBwdArgs& a, hipStream_t st) {
 
 using namespace rk;
 
-extern "C" int64_t rk_scored_attention_backward_work(int64_t B, int64_t H, int64_t S, int slopes) {
-  if (B <= 0 || H <= 0 || S <= 0) return 0;
-  return (slopes ? 3 : 2) * B * H * ((S + kAttnRows - 1) / kAttnRows * kAttnRows);
+extern "C" int64_t rk_scored_attention_backward_work(int64_t B, int64_t H, int64_t Hkv, int64_t S,
+                                                     int64_t D, int slopes) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || S <= 0 || D <= 0 || H % Hkv != 0) return 0;
+  const int64_t parts = head_parts(B, H, Hkv, S);
+  return (slopes ? 3 : 2) * B * H * ((S + kAttnRows - 1) / kAttnRows * kAttnRows) +
+         (parts > 1 ? parts * 2 * B * Hkv * S * D : 0);
 }
 
 extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args, float* work,
@@ -419,6 +500,7 @@ extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args
   if (p.dslopes && !p.slopes) return fail(RK_ERR_ARG, "a slope gradient needs slopes");
   if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
   if (!p.dq || !p.dk || !p.dv || !work) return fail(RK_ERR_ARG, "null pointer");
+  if (!aligned16(work)) return fail(RK_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
   const void* out8[] = {p.dq, p.dk, p.dv};
   for (const void* t : out8)
     if (reinterpret_cast<uintptr_t>(t) & 7)
@@ -428,6 +510,10 @@ extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args
   a.inv_scale = 1.0f / p.scale;
   a.rows = work;
   a.slope_rows = p.dslopes ? work + 2 * p.B * p.H * a.f.Sp : nullptr;
+  a.parts = head_parts(p.B, p.H, p.Hkv, p.S);
+  a.part_rows = work + (p.dslopes ? 3 : 2) * p.B * p.H * a.f.Sp;
+  if (a.parts > 1 && p.B * p.Hkv > 65535)
+    return fail(RK_ERR_UNSUPPORTED, "more than 65535 sequence heads");
   if (p.D == 64) dispatch_scored_bwd<64>(a, as_stream(stream));
   else dispatch_scored_bwd<128>(a, as_stream(stream));
   return launch_status("scored_attention_backward");

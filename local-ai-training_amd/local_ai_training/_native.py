@@ -129,7 +129,7 @@ SIGNATURES: dict[str, list] = {
                               _p, _p, _p, _i64, _i64, _i64, _p, _p],
     "rk_attention_mask": [_p, _i32, _i64, _p, _i64, _i64, _i64, _p, _p, _p],
     "rk_scored_attention_forward": [_p, _p],
-    "rk_scored_attention_backward_work": [_i64, _i64, _i64, _i32],
+    "rk_scored_attention_backward_work": [_i64, _i64, _i64, _i64, _i64, _i32],
     "rk_scored_attention_backward": [_p, _p, _p],
     "rk_int8_kv_append": [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _i64, _p, _i64,
                           _p, _p],
