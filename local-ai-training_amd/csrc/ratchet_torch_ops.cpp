@@ -1135,12 +1135,12 @@ rk_scored_attention_args scored_args(const Tensor& q, const Tensor& k, const Ten
   return a;
 }
 
-// Attention with modified scores (rk_scored_attention_forward): (o, lse), o as a [B, H, S, D] view
-// of [B, S, H, D] memory.
-std::tuple<Tensor, Tensor> scored_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+// Attention with modified scores (rk_scored_attention_forward): (o, lse, rest), o as a
+// [B, H, S, D] view of [B, S, H, D] memory; rest, for the backward, is empty unless `grad`.
+std::tuple<Tensor, Tensor, Tensor> scored_attention(const Tensor& q, const Tensor& k, const Tensor& v,
                                             const OptTensor& bounds, const OptTensor& padding,
                                             const OptTensor& slopes, double softcap,
-                                            double scale) {
+                                            double scale, bool grad) {
   std::vector<Tensor> keep;
   rk_scored_attention_args a = scored_args(q, k, v, bounds, padding, slopes, softcap, scale, keep);
   const c10::DeviceGuard guard(q.device());
@@ -1148,17 +1148,20 @@ std::tuple<Tensor, Tensor> scored_attention(const Tensor& q, const Tensor& k, co
   Tensor lse = at::empty({a.B, a.H, a.S}, q.options().dtype(at::kFloat));
   a.o = static_cast<uint16_t*>(o.data_ptr());
   a.sob = a.S * a.H * a.D, a.soh = a.D, a.sos = a.H * a.D;
+  Tensor rest = grad ? at::empty({a.B, a.S, a.H, a.D}, q.options().dtype(at::kChar))
+                     : at::empty({0}, q.options().dtype(at::kChar));
   a.lse = lse.data_ptr<float>();
+  a.rest = grad ? rest.data_ptr<int8_t>() : nullptr;
   check_status(rk_scored_attention_forward(&a, stream_of(q)), "rk_scored_attention_forward");
-  return {o, lse};
+  return {o, lse, rest};
 }
 
 // Its backward (rk_scored_attention_backward): dq, dk, dv as [B, heads, S, D] views of
 // [B, S, heads, D] memory, and dslopes [H] (empty unless slope_grad).
 std::tuple<Tensor, Tensor, Tensor, Tensor> scored_attention_backward(
     const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
-    const Tensor& lse, const OptTensor& bounds, const OptTensor& padding, const OptTensor& slopes,
-    double softcap, double scale, bool slope_grad) {
+    const Tensor& lse, const Tensor& rest, const OptTensor& bounds, const OptTensor& padding,
+    const OptTensor& slopes, double softcap, double scale, bool slope_grad) {
   std::vector<Tensor> keep;
   rk_scored_attention_args a = scored_args(q, k, v, bounds, padding, slopes, softcap, scale, keep);
   const c10::DeviceGuard guard(q.device());
@@ -1176,6 +1179,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> scored_attention_backward(
   TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.dim() == 3 && lse.size(0) == a.B &&
                   lse.size(1) == a.H && lse.size(2) == a.S && lse.is_contiguous(),
               "scored attention backward: lse must be a contiguous float32 [B, H, S] tensor");
+  same_device(q, rest, "scored attention backward");
+  TORCH_CHECK(rest.scalar_type() == at::kChar && rest.is_contiguous() &&
+                  (rest.numel() == 0 || rest.numel() == q.numel()),
+              "scored attention backward: rest must be the forward's, or empty");
   TORCH_CHECK(!slope_grad || slopes.has_value(),
               "scored attention backward: a slope gradient needs slopes");
   const auto out = [&](int64_t heads) {
@@ -1192,6 +1199,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> scored_attention_backward(
   a.o = w16(oo), a.sob = oo.stride(0), a.soh = oo.stride(1), a.sos = oo.stride(2);
   a.g = w16(gg), a.sgb = gg.stride(0), a.sgh = gg.stride(1), a.sgs = gg.stride(2);
   a.lse = lse.data_ptr<float>();
+  a.rest = rest.numel() > 0 ? rest.data_ptr<int8_t>() : nullptr;
   a.dq = w16(dq), a.dk = w16(dk), a.dv = w16(dv);
   a.sxb = a.S * a.H * a.D, a.sxh = a.D, a.sxs = a.H * a.D;
   a.syb = a.S * a.Hkv * a.D, a.syh = a.D, a.sys = a.Hkv * a.D;
@@ -1463,10 +1471,10 @@ TORCH_LIBRARY(ratchet, m) {
         "float scale) -> (Tensor, Tensor, Tensor)");
   m.def("attention_mask(Tensor? documents, Tensor? prefix) -> (Tensor, Tensor)");
   m.def("scored_attention(Tensor q, Tensor k, Tensor v, Tensor? bounds, Tensor? padding, "
-        "Tensor? slopes, float softcap, float scale) -> (Tensor, Tensor)");
+        "Tensor? slopes, float softcap, float scale, bool grad) -> (Tensor, Tensor, Tensor)");
   m.def("scored_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor o, "
-        "Tensor lse, Tensor? bounds, Tensor? padding, Tensor? slopes, float softcap, "
-        "float scale, bool slope_grad) -> (Tensor, Tensor, Tensor, Tensor)");
+        "Tensor lse, Tensor rest, Tensor? bounds, Tensor? padding, Tensor? slopes, "
+        "float softcap, float scale, bool slope_grad) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("int8_kv_append(Tensor k, Tensor v, Tensor(a!) keys, Tensor(b!) values, "
         "Tensor(c!) key_scales, Tensor(d!) value_scales, Tensor start, Tensor? lengths) -> ()");
   m.def("int8_kv_read(Tensor keys, Tensor values, Tensor key_scales, Tensor value_scales, "

@@ -123,6 +123,16 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, uint64_t bits, int tid
       *reinterpret_cast<uint4*>(tile + 16 * i) = make_uint4(0, 0, 0, 0);
 }
 
+// What rounding x to bf16 left, in 256ths of the bf16 step (2^-16 of x): the difference of the
+// bit patterns, and the float32 value it restores.
+__device__ __forceinline__ int bf16_rest(float x, uint32_t bf16) {
+  const int d = static_cast<int>(__float_as_uint(x) - (bf16 << 16) + 128) >> 8;
+  return d > 127 ? 127 : d < -128 ? -128 : d;
+}
+__device__ __forceinline__ float with_rest(uint32_t bf16, int rest) {
+  return __uint_as_float((bf16 << 16) + static_cast<uint32_t>(rest * 256));
+}
+
 int check_scored(const rk_scored_attention_args& p, bool backward);
 ScoredArgs scored_args(const rk_scored_attention_args& p);
 

@@ -174,8 +174,24 @@ void scored_fwd_kernel(ScoredArgs a) {
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) o[dt] = v16f_a{};
     }
-    store_owned<D>(p.o + b * p.sob + hd * p.soh + static_cast<int64_t>(qi) * p.sos, o,
-                   span.valid ? 1.0f / l : 0.0f, h);
+    const float factor = span.valid ? 1.0f / l : 0.0f;
+    uint16_t* const row = p.o + b * p.sob + hd * p.soh + static_cast<int64_t>(qi) * p.sos;
+    store_owned<D>(row, o, factor, h);
+    if (p.rest) {
+      int8_t* const rest = p.rest + ((b * p.S + qi) * p.H + hd) * D + 4 * h;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = o[dt][4 * r + e] * factor;
+            w |= static_cast<uint32_t>(bf16_rest(x, f32_to_bf16(x)) & 255) << (8 * e);
+          }
+          *reinterpret_cast<uint32_t*>(rest + 32 * dt + 8 * r) = w;
+        }
+    }
     if (h == 0)
       p.lse[bh * S + qi] = span.valid ? (m + __log2f(l)) * 0.69314718055994531f : 0.0f;
   }
@@ -410,6 +426,8 @@ extern "C" int rk_scored_attention_forward(const rk_scored_attention_args* args,
   const rk_scored_attention_args& p = *args;
   if (int e = check_scored(p, false)) return e;
   if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
+  if (reinterpret_cast<uintptr_t>(p.rest) & 3)
+    return fail(RK_ERR_UNSUPPORTED, "rest needs 4-byte alignment");
   if (reinterpret_cast<uintptr_t>(p.o) & 7) return fail(RK_ERR_UNSUPPORTED, "o needs 8-byte alignment");
   const ScoredArgs a = scored_args(p);
   const dim3 grid(static_cast<unsigned>(p.B * p.H * (a.Sp / kAttnRows)));

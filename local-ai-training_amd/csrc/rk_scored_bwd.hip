@@ -6,7 +6,9 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij g_i,
 //   dslope_h = -sum_ij d_ij |i - j|.
 // Products of bf16 operands summed in float32; p and ds enter the second products rounded to
-// bf16 (half a step, 2^-9 relative); scores, exponentials, delta are float32. Two launches, as
+// bf16 (half a step); scores, exponentials, delta are float32, o with what its rounding left
+// (`rest`): with the bf16 o alone, dq and dk of concentrated rows were off by 2.7e-3 to 3.2e-3 of
+// their norm instead of XXX, the rounding of ds and of the results. Two launches, as
 // at rk_attention_bwd.hip: the queries' (dq, and delta for the second) and the keys' (dk, dv; the
 // query heads that share a key head are summed by the one wavefront that owns the key, in order),
 // every output summed in a fixed order, so results repeat.
@@ -88,11 +90,23 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   {
     v8bf_a of[D / 16];
     load_owned<D>(of, p.o + b * p.sob + hd * p.soh, p.sos, S, qi, h);
+    uint2 rest[D / 16] = {};
+    if (p.rest && qi < S) {
+      const int8_t* const at = p.rest + ((b * p.S + qi) * p.H + hd) * D + 8 * h;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s)
+      for (int s = 0; s < D / 16; ++s) rest[s] = *reinterpret_cast<const uint2*>(at + 16 * s);
+    }
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        dot = dot + static_cast<float>(gf[s][e]) * static_cast<float>(of[s][e]);
+    for (int s = 0; s < D / 16; ++s) {
+      const uint4 w = __builtin_bit_cast(uint4, of[s]);
+      const uint32_t pairs[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int8_t r = static_cast<int8_t>((e < 4 ? rest[s].x : rest[s].y) >> (8 * (e % 4)));
+        const float ov = with_rest(pairs[e / 2] >> (16 * (e % 2)) & 0xffffu, r);
+        dot = dot + static_cast<float>(gf[s][e]) * ov;
+      }
+    }
   }
   dot = dot + __shfl_xor(dot, 32, kWave);
   const float lse = span.valid ? p.lse[bh * S + qi] : 0.0f;
@@ -500,6 +514,8 @@ extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args
   if (p.dslopes && !p.slopes) return fail(RK_ERR_ARG, "a slope gradient needs slopes");
   if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
   if (!p.dq || !p.dk || !p.dv || !work) return fail(RK_ERR_ARG, "null pointer");
+  if (reinterpret_cast<uintptr_t>(p.rest) & 7)
+    return fail(RK_ERR_UNSUPPORTED, "rest needs 8-byte alignment");
   if (!aligned16(work)) return fail(RK_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
   const void* out8[] = {p.dq, p.dk, p.dv};
   for (const void* t : out8)

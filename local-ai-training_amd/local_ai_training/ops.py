@@ -186,14 +186,15 @@ def _register_fakes() -> None:
                 like.new_empty((b, (sl + 31) // 32), dtype=torch.int32))
 
     @fake("ratchet::scored_attention")
-    def _scored_attention(q, k, v, bounds, padding, slopes, softcap, scale):
+    def _scored_attention(q, k, v, bounds, padding, slopes, softcap, scale, grad):
         b, h, sl, d = q.shape
         o = q.new_empty((b, sl, h, d)).permute(0, 2, 1, 3)
-        return o, q.new_empty((b, h, sl), dtype=torch.float32)
+        rest = q.new_empty((b, sl, h, d) if grad else (0,), dtype=torch.int8)
+        return o, q.new_empty((b, h, sl), dtype=torch.float32), rest
 
     @fake("ratchet::scored_attention_backward")
-    def _scored_attention_backward(grad, q, k, v, o, lse, bounds, padding, slopes, softcap,
-                                   scale, slope_grad):
+    def _scored_attention_backward(grad, q, k, v, o, lse, rest, bounds, padding, slopes,
+                                   softcap, scale, slope_grad):
         def rows(t):
             b, h, sl, d = t.shape
             return t.new_empty((b, sl, h, d)).permute(0, 2, 1, 3)

@@ -105,8 +105,9 @@ class _ScoredBackwardFn(torch.autograd.Function):
     depend on q, k, v, the slopes and the gradient, and have no derivative."""
 
     @staticmethod
-    def forward(ctx, grad, q, k, v, slopes, out, lse, bounds, padding, softcap, scale, wanted):
-        return ratchet().scored_attention_backward(grad, q, k, v, out, lse, bounds, padding,
+    def forward(ctx, grad, q, k, v, slopes, out, lse, rest, bounds, padding, softcap, scale,
+                wanted):
+        return ratchet().scored_attention_backward(grad, q, k, v, out, lse, rest, bounds, padding,
                                                    slopes, softcap, scale, wanted)
 
     @staticmethod
@@ -119,21 +120,23 @@ class ScoredAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, slopes, bounds, padding, softcap, scale):
-        out, lse = ratchet().scored_attention(q, k, v, bounds, padding, slopes, softcap, scale)
-        ctx.save_for_backward(q, k, v, slopes, out, lse, bounds, padding)
+        out, lse, rest = ratchet().scored_attention(q, k, v, bounds, padding, slopes, softcap,
+                                                    scale, any(ctx.needs_input_grad[:4]))
+        ctx.save_for_backward(q, k, v, slopes, out, lse, rest, bounds, padding)
         ctx.softcap, ctx.scale = softcap, scale
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        q, k, v, slopes, out, lse, bounds, padding = ctx.saved_tensors
+        q, k, v, slopes, out, lse, rest, bounds, padding = ctx.saved_tensors
         wanted = slopes is not None and ctx.needs_input_grad[3]
         if torch.is_grad_enabled():
-            grads = _ScoredBackwardFn.apply(grad, q, k, v, slopes, out, lse, bounds, padding,
+            grads = _ScoredBackwardFn.apply(grad, q, k, v, slopes, out, lse, rest, bounds, padding,
                                             ctx.softcap, ctx.scale, wanted)
         else:
-            grads = ratchet().scored_attention_backward(grad, q, k, v, out, lse, bounds, padding,
-                                                        slopes, ctx.softcap, ctx.scale, wanted)
+            grads = ratchet().scored_attention_backward(grad, q, k, v, out, lse, rest, bounds,
+                                                        padding, slopes, ctx.softcap, ctx.scale,
+                                                        wanted)
         dq, dk, dv, dslopes = grads
         return dq, dk, dv, dslopes if wanted else None, None, None, None, None
 

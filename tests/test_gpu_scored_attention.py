@@ -297,20 +297,20 @@ def test_the_library_refuses(cuda):
     ops = ratchet()
     mask = attention_mask(torch.zeros(1, 8, dtype=torch.int32, device=cuda))
     with pytest.raises(RuntimeError, match="head size"):
-        ops.scored_attention(q[..., :32], q[..., :32], q[..., :32], None, None, None, 0.0, 1.0)
+        ops.scored_attention(q[..., :32], q[..., :32], q[..., :32], None, None, None, 0.0, 1.0, False)
     with pytest.raises(RuntimeError, match="scale"):
-        ops.scored_attention(q, q, q, None, None, None, 0.0, -1.0)
+        ops.scored_attention(q, q, q, None, None, None, 0.0, -1.0, False)
     with pytest.raises(RuntimeError, match="softcap"):
-        ops.scored_attention(q, q, q, None, None, None, -1.0, 1.0)
+        ops.scored_attention(q, q, q, None, None, None, -1.0, 1.0, False)
     with pytest.raises(RuntimeError, match="go together"):
-        ops.scored_attention(q, q, q, mask.bounds, None, None, 0.0, 1.0)
+        ops.scored_attention(q, q, q, mask.bounds, None, None, 0.0, 1.0, False)
     with pytest.raises(RuntimeError, match="bfloat16"):
-        ops.scored_attention(q.float(), q.float(), q.float(), None, None, None, 0.0, 1.0)
+        ops.scored_attention(q.float(), q.float(), q.float(), None, None, None, 0.0, 1.0, False)
     with pytest.raises(RuntimeError, match="multiple"):
-        ops.scored_attention(q, q[:, :0], q[:, :0], None, None, None, 0.0, 1.0)
+        ops.scored_attention(q, q[:, :0], q[:, :0], None, None, None, 0.0, 1.0, False)
     with pytest.raises(RuntimeError, match="slope gradient"):
-        o, lse = ops.scored_attention(q, q, q, None, None, None, 0.0, 1.0)
-        ops.scored_attention_backward(q, q, q, q, o, lse, None, None, None, 0.0, 1.0, True)
+        o, lse, rest = ops.scored_attention(q, q, q, None, None, None, 0.0, 1.0, False)
+        ops.scored_attention_backward(q, q, q, q, o, lse, rest, None, None, None, 0.0, 1.0, True)
     with pytest.raises(ValueError, match="device"):
         scored_attention(q, q, q, mask=AttentionMask(mask.bounds.cpu(), mask.padding.cpu()))
 
@@ -322,8 +322,9 @@ def test_opcheck(cuda):
     torch.library.opcheck(ops.attention_mask, (documents, prefix))
     mask = attention_mask(documents, prefix)
     slopes = slopes_of(cuda, 4)
-    torch.library.opcheck(ops.scored_attention, (q, k, v, *mask, slopes, 5.0, 0.125))
-    o, lse = ops.scored_attention(q, k, v, *mask, slopes, 5.0, 0.125)
+    for grad in (False, True):
+        torch.library.opcheck(ops.scored_attention, (q, k, v, *mask, slopes, 5.0, 0.125, grad))
+    o, lse, rest = ops.scored_attention(q, k, v, *mask, slopes, 5.0, 0.125, True)
     for wanted in (False, True):
         torch.library.opcheck(ops.scored_attention_backward,
-                              (g, q, k, v, o, lse, *mask, slopes, 5.0, 0.125, wanted))
+                              (g, q, k, v, o, lse, rest, *mask, slopes, 5.0, 0.125, wanted))
