@@ -192,6 +192,11 @@ def _register_fakes() -> None:
         rest = q.new_empty((b, sl, h, d) if grad else (0,), dtype=torch.int8)
         return o, q.new_empty((b, h, sl), dtype=torch.float32), rest
 
+    @fake("ratchet::scored_attend")
+    def _scored_attend(q, k, v, bounds, padding, slopes, softcap, scale):
+        b, h, sl, d = q.shape
+        return q.new_empty((b, sl, h, d)).permute(0, 2, 1, 3)
+
     @fake("ratchet::scored_attention_backward")
     def _scored_attention_backward(grad, q, k, v, o, lse, rest, bounds, padding, slopes,
                                    softcap, scale, slope_grad):

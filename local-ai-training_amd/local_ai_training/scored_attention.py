@@ -100,47 +100,6 @@ def _torch_mask(documents: Tensor | None, prefix: Tensor | None) -> AttentionMas
     return AttentionMask(bounds, torch.where(words >= 2**31, words - 2**32, words).to(torch.int32))
 
 
-class _ScoredBackwardFn(torch.autograd.Function):
-    """The backward as a function of its own where a graph of it is asked for: its results
-    depend on q, k, v, the slopes and the gradient, and have no derivative."""
-
-    @staticmethod
-    def forward(ctx, grad, q, k, v, slopes, out, lse, rest, bounds, padding, softcap, scale,
-                wanted):
-        return ratchet().scored_attention_backward(grad, q, k, v, out, lse, rest, bounds, padding,
-                                                   slopes, softcap, scale, wanted)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise RuntimeError("scored_attention has no second derivative")
-
-
-class ScoredAttentionFn(torch.autograd.Function):
-    """Attention with modified scores on the HIP kernels."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, slopes, bounds, padding, softcap, scale):
-        out, lse, rest = ratchet().scored_attention(q, k, v, bounds, padding, slopes, softcap,
-                                                    scale, any(ctx.needs_input_grad[:4]))
-        ctx.save_for_backward(q, k, v, slopes, out, lse, rest, bounds, padding)
-        ctx.softcap, ctx.scale = softcap, scale
-        return out
-
-    @staticmethod
-    def backward(ctx, grad):
-        q, k, v, slopes, out, lse, rest, bounds, padding = ctx.saved_tensors
-        wanted = slopes is not None and ctx.needs_input_grad[3]
-        if torch.is_grad_enabled():
-            grads = _ScoredBackwardFn.apply(grad, q, k, v, slopes, out, lse, rest, bounds, padding,
-                                            ctx.softcap, ctx.scale, wanted)
-        else:
-            grads = ratchet().scored_attention_backward(grad, q, k, v, out, lse, rest, bounds,
-                                                        padding, slopes, ctx.softcap, ctx.scale,
-                                                        wanted)
-        dq, dk, dv, dslopes = grads
-        return dq, dk, dv, dslopes if wanted else None, None, None, None, None
-
-
 def _torch_scored_attention(q: Tensor, k: Tensor, v: Tensor, mask: AttentionMask | None,
                             softcap: float, slopes: Tensor | None, scale: float) -> Tensor:
     work = torch.float64 if q.dtype == torch.float64 else torch.float32
@@ -213,6 +172,6 @@ def scored_attention(q: Tensor, k: Tensor, v: Tensor, *, mask: AttentionMask | N
             raise ValueError("the mask must be on the queries' device")
     if q.is_cuda and q.dtype == torch.bfloat16 and d in (64, 128):
         bounds, padding = mask if mask is not None else (None, None)
-        return ScoredAttentionFn.apply(q, k, v, slopes, bounds, padding, softcap, scale)
+        return ratchet().scored_attend(q, k, v, bounds, padding, slopes, softcap, scale)
     with torch.autocast(q.device.type, enabled=False):
         return _torch_scored_attention(q, k, v, mask, softcap, slopes, scale)

@@ -324,6 +324,9 @@ def test_opcheck(cuda):
     slopes = slopes_of(cuda, 4)
     for grad in (False, True):
         torch.library.opcheck(ops.scored_attention, (q, k, v, *mask, slopes, 5.0, 0.125, grad))
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    torch.library.opcheck(ops.scored_attend, (*leaves, *mask, slopes, 5.0, 0.125))
+    torch.library.opcheck(ops.scored_attend, (q, k, v, None, None, None, 0.0, 0.125))
     o, lse, rest = ops.scored_attention(q, k, v, *mask, slopes, 5.0, 0.125, True)
     for wanted in (False, True):
         torch.library.opcheck(ops.scored_attention_backward,
