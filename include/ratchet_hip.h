@@ -790,10 +790,12 @@ int rk_int8_kv_read(const rk_int8_kv* cache, int64_t begin, int64_t end, int dty
  * rk_scored_attention_forward. out: [B, S, Hq, D] contiguous, float32 or bf16; zeros for queries
  * at or past lengths and for negative starts, NaN for positions past the cache. The products run
  * in integers on the codes, with queries and probabilities rounded to 23 bits of their row's and
- * block's largest. work: rk_int8_kv_attention_work floats (0: none), 16-byte aligned.
+ * block's largest; chunks of 32 bf16 tokens and more with bf16 results take bf16 products, with
+ * the probabilities rounded to bf16. work: rk_int8_kv_attention_work floats (0: none), 16-byte aligned.
  * No counterpart in the reference (its window is recomputed per token, generate.py:183-201).
  */
-int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S);
+int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S, int qdtype,
+                                  int odtype);
 int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int qdtype, int64_t sqb,
                          int64_t sqh, int64_t sqs, int64_t Hq, int64_t S, const int64_t* start,
                          int64_t start_count, const int64_t* lengths, float scale, float softcap,

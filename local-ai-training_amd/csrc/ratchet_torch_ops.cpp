@@ -1405,7 +1405,7 @@ Tensor int8_kv_attention(const Tensor& q, const Tensor& keys, const Tensor& valu
     sl = f32_vector(*slopes, Hq, "slopes");
   }
   Tensor out = at::empty({c.B, S, Hq, c.D}, q.options().dtype(out_dtype));
-  const int64_t floats = rk_int8_kv_attention_work(&c, Hq, S);
+  const int64_t floats = rk_int8_kv_attention_work(&c, Hq, S, code, ocode);
   Tensor work;
   if (floats > 0) work = at::empty({floats}, key_scales.options());
   check_status(rk_int8_kv_attention(&c, qq.data_ptr(), code, qq.stride(0), qq.stride(1),

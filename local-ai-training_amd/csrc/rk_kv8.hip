@@ -11,13 +11,14 @@
 // quotients, the rule of rk_quantize_rows). Tokens appended to a block that holds some can only
 // raise its scale; the codes there are then rounded again, rint(c (s_old / s)). A block's first
 // token starts it anew, whatever it held.
-#include "rk_common.h"
+#include "rk_attention.h"
 
 #include <math.h>
 
 namespace rk {
 
 constexpr int kTok = 64;  // tokens of a block
+constexpr int64_t kChunkTokens = 32;  // chunks from here on take kv8_chunk_kernel
 constexpr float kLog2e8 = 1.4426950408889634f;
 
 typedef int v4i8 __attribute__((ext_vector_type(4)));
@@ -260,7 +261,7 @@ struct Kv8Attn {
   const float* slopes;
   int64_t start_step, S, Hq, G, nsplit, tiles;
   float dot_scale, cap2;
-  float* work;  // [B * H * tiles][nsplit][16][D + 4]: max, sum, 2 pad, unnormalized output
+  float* work;  // [B * H][S * G][nsplit][D + 4]: max, sum, 2 pad, unnormalized output
   void* out;    // [B, S, Hq, D], of type ODT
 };
 
@@ -405,8 +406,13 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
     float slope2 = 0.0f;
     if constexpr (BIAS) slope2 = a.slopes[hd] * kLog2e8;
     const int64_t pos = start + i;
-    const int8_t* const kbase = a.c.keys + bh * a.c.NB * kTok * D;
-    const int8_t* const vbase = a.c.values + bh * a.c.NB * kTok * D;
+    // loads past the split's last block return zeros without going to memory, so the next
+    // block's are issued without a branch (which doubled the registers that hold them)
+    const int bytes = static_cast<int>(j1 - j0) * (kTok * D);  // the host bounds a head's codes
+    const __amdgpu_buffer_rsrc_t kbuf =
+        make_buffer(a.c.keys + (bh * a.c.NB + j0) * kTok * D, bytes);
+    const __amdgpu_buffer_rsrc_t vbuf =
+        make_buffer(a.c.values + (bh * a.c.NB + j0) * kTok * D, bytes);
     const float* const ks = a.c.ks + bh * a.c.NB;
     const float* const vs = a.c.vs + bh * a.c.NB;
     const int koff = (16 * (col >> 2) + (col & 3)) * D + 16 * g;  // row 4 g' + e' of product 0
@@ -414,23 +420,25 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
 
     v4i8 kf[4][KK], vf[FT];
     auto load_k = [&](int64_t j) {
-      const int8_t* p = kbase + j * (kTok * D) + koff;
+      const int at = static_cast<int>(j - j0) * (kTok * D);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
-          kf[t][kk] = *reinterpret_cast<const v4i8*>(p + 4 * t * D + 64 * kk);
+          kf[t][kk] = __builtin_bit_cast(
+              v4i8, __builtin_amdgcn_raw_buffer_load_b128(kbuf, koff + 4 * t * D + 64 * kk, at, 0));
     };
     auto load_v = [&](int64_t j) {
-      const int8_t* p = vbase + j * (kTok * D) + voff;
+      const int at = static_cast<int>(j - j0) * (kTok * D);
 #pragma unroll
-      for (int f = 0; f < FT; ++f) vf[f] = *reinterpret_cast<const v4i8*>(p + 16 * f * kTok);
+      for (int f = 0; f < FT; ++f)
+        vf[f] = __builtin_bit_cast(
+            v4i8, __builtin_amdgcn_raw_buffer_load_b128(vbuf, voff + 16 * f * kTok, at, 0));
     };
     int64_t j = j0 + wave;
     load_k(j);
     load_v(j);
     for (; j < j1; j += 4) {
-      const bool more = j + 4 < j1;
       const float kscale = ks[j], vscale = vs[j];
       float s[16];
       const float mul = qscale * kscale * a.dot_scale;
@@ -448,7 +456,7 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
         for (int e = 0; e < 4; ++e)
           s[4 * t + e] = from_digits(acc[0][e], acc[1][e], acc[2][e]) * mul;
       }
-      if (more) load_k(j + 4);
+      load_k(j + 4);
       const int64_t ahead = pos - (j * kTok + 16 * g);
       const int left = ahead > 16 ? 16 : ahead < -1 ? -1 : static_cast<int>(ahead);
       const float d0 = static_cast<float>(ahead);  // key 16 g + x is seen for x <= left
@@ -501,7 +509,7 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
           o[f][e] = __builtin_fmaf(from_digits(acc[0][e], acc[1][e], acc[2][e]), add,
                                    o[f][e] * alpha);
       }
-      if (more) load_v(j + 4);
+      load_v(j + 4);
     }
   }
 
@@ -539,7 +547,7 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
       for (int e = 0; e < 4; ++e) r[e] = factor == 0.0f ? 0.0f : r[e] * factor;
       store4<ODT>(a.out, ((b * a.S + qi) * a.Hq + h) * D + f, r);
     } else {
-      float* const w = a.work + (((bh * a.tiles + tile) * a.nsplit + split) * 16 + c) * (D + 4);
+      float* const w = a.work + ((bh * cols + ct) * a.nsplit + split) * (D + 4);
       *reinterpret_cast<float4*>(w + 4 + f) = make_float4(r[0], r[1], r[2], r[3]);
       if (f == 0) {
         w[0] = mm;
@@ -554,8 +562,8 @@ template <int D, int ODT>
 __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
   const int64_t ct = blockIdx.x, bh = blockIdx.y, b = bh / a.c.H, kvh = bh - b * a.c.H;
   const int f = threadIdx.x * 4;
-  const float* w = a.work + (((bh * a.tiles + ct / 16) * a.nsplit) * 16 + ct % 16) * (D + 4);
-  const int64_t step = 16 * (D + 4);
+  const float* w = a.work + (bh * a.S * a.G + ct) * a.nsplit * (D + 4);
+  const int64_t step = D + 4;
   float mm = -INFINITY;
   for (int64_t s = 0; s < a.nsplit; ++s) mm = fmaxf(mm, w[s * step]);
   float ll = 0.0f, r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -577,6 +585,241 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
 }
 
 // ---------------------------------------------------------------------------
+// The same for chunks of many bf16 tokens with bf16 results (a prompt's next part): one workgroup
+// takes 128 queries of a head, a wavefront 32, and the products run on the bf16 MFMA as in
+// rk_attention.hip (scores transposed, a lane holds one query). The codes become bf16 once per
+// workgroup and block, exactly (8 bits), on their way into LDS; the key scale goes into the score,
+// the value scale into the probabilities before they are rounded to bf16. Values lie by feature, so
+// the second product's operand is a row read too: the tokens of a row are stored in the order in
+// which a lane holds its probabilities. The next block's codes are in registers meanwhile.
+//
+// Codes converted by each reader instead, or the digits of kv8_attn_kernel for chunks too, cost
+// more: the latter ZZZ us at 4 x 517 tokens behind 1500, 16 heads of 128.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  uint32_t f[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    f[e] = __float_as_uint(static_cast<float>(static_cast<int8_t>(w >> (8 * e))));
+  lo = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);  // small integers: the low halves are zero
+  hi = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
+}
+
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void kv8_chunk_kernel(Kv8Attn a) {
+  constexpr int TILE = kTok * D * 2;    // bf16 keys [64][D] or values [D][64]
+  constexpr int EACH = kTok * D / 16 / 256;  // 16-code pieces per thread and operand
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * 2 * TILE];
+  // the last queries, which see most, first; heads fastest
+  const int64_t BHq = a.c.B * a.Hq;
+  const int64_t qt = a.tiles - 1 - blockIdx.x / BHq;
+  const int64_t bhq = blockIdx.x % BHq, b = bhq / a.Hq, hd = bhq - b * a.Hq, kvh = hd / a.G;
+  const int64_t bh = b * a.c.H + kvh;
+  const int split = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t start = a.start[b * a.start_step];
+  int64_t n = a.lengths ? a.lengths[b] : a.S;
+  n = n < a.S ? n : a.S;
+  const int64_t i0 = qt * 128, iw = i0 + 32 * wave, i = iw + l32;
+  const bool on = start >= 0 && i0 < n;
+  const int64_t last = i0 + 128 < n ? i0 + 127 : n - 1;  // the last active query
+  int64_t nb = on ? (start + last) / kTok + 1 : 0;
+  nb = nb < a.c.NB ? nb : a.c.NB;
+  const int64_t per = (nb + a.nsplit - 1) / a.nsplit;
+  const int64_t j0 = split * per, j1 = j0 + per < nb ? j0 + per : nb;
+  // positions relative to the split's first key
+  const int64_t base = start - j0 * kTok;
+  const int64_t pw = base + iw;                       // of the wavefront's first query
+  const int64_t pos = base + (i < n ? i : n - 1);     // of this lane's
+
+  float m = -INFINITY, l = 0.0f;
+  v16f_a o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) o[dt] = v16f_a{};
+  if (j0 < j1) {
+    v8bf_a qf[D / 16];
+    {
+      const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.sqb + hd * a.sqh +
+                          (i < a.S ? i : a.S - 1) * a.sqs + 8 * h;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+        qf[s] = frag_of(*reinterpret_cast<const uint4*>(q + 16 * s));
+    }
+    float slope2 = 0.0f;
+    if constexpr (BIAS) slope2 = a.slopes[hd] * kLog2e8;
+    const uint4* const kc =
+        reinterpret_cast<const uint4*>(a.c.keys + (bh * a.c.NB + j0) * kTok * D) + tid;
+    const uint4* const vc =
+        reinterpret_cast<const uint4*>(a.c.values + (bh * a.c.NB + j0) * kTok * D) + tid;
+    const float* const ks = a.c.ks + bh * a.c.NB + j0;
+    const float* const vs = a.c.vs + bh * a.c.NB + j0;
+    uint4 rk[EACH], rv[EACH];
+    auto load = [&](int j) {
+#pragma unroll
+      for (int c = 0; c < EACH; ++c) {
+        rk[c] = kc[static_cast<int64_t>(j) * (kTok * D / 16) + 256 * c];
+        rv[c] = vc[static_cast<int64_t>(j) * (kTok * D / 16) + 256 * c];
+      }
+    };
+    auto store = [&](int j) {
+      uint8_t* const kt = smem + (j & 1) * 2 * TILE;
+      uint8_t* const vt = kt + TILE;
+#pragma unroll
+      for (int c = 0; c < EACH; ++c) {
+        const int p = tid + 256 * c;
+        uint4 x[2];
+        {
+          const int row = p / (D / 16), seg = p % (D / 16) * 2, sw = seg_swizzle<D>(row);
+          widen_codes(rk[c].x, x[0].x, x[0].y);
+          widen_codes(rk[c].y, x[0].z, x[0].w);
+          widen_codes(rk[c].z, x[1].x, x[1].y);
+          widen_codes(rk[c].w, x[1].z, x[1].w);
+          uint8_t* const to = kt + row * (2 * D);
+          *reinterpret_cast<uint4*>(to + 16 * (seg ^ sw)) = x[0];
+          *reinterpret_cast<uint4*>(to + 16 * ((seg + 1) ^ sw)) = x[1];
+        }
+        {  // tokens 0-3, 8-11 | 4-7, 12-15 of each 16: a lane's slots
+          const int row = p / 4, seg = p % 4 * 2, sw = seg_swizzle<64>(row);
+          widen_codes(rv[c].x, x[0].x, x[0].y);
+          widen_codes(rv[c].z, x[0].z, x[0].w);
+          widen_codes(rv[c].y, x[1].x, x[1].y);
+          widen_codes(rv[c].w, x[1].z, x[1].w);
+          uint8_t* const to = vt + row * (2 * kTok);
+          *reinterpret_cast<uint4*>(to + 16 * (seg ^ sw)) = x[0];
+          *reinterpret_cast<uint4*>(to + 16 * ((seg + 1) ^ sw)) = x[1];
+        }
+      }
+    };
+    const int blocks = static_cast<int>(j1 - j0);
+    load(0);
+    store(0);
+    if (blocks > 1) load(1);
+    __syncthreads();
+    for (int j = 0; j < blocks; ++j) {
+      const uint8_t* const kt = smem + (j & 1) * 2 * TILE;
+      const uint8_t* const vt = kt + TILE;
+      const int64_t k0 = static_cast<int64_t>(j) * kTok;
+      if (iw < n && k0 <= pw + 31) {  // some query of the wavefront sees some key
+        const float kscale = ks[j] * a.dot_scale, vscale = vs[j];
+        v16f_a sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          sc[t] = v16f_a{};
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s)
+            sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, 32 * t, s, lane),
+                                                            qf[s], sc[t], 0, 0, 0);
+        }
+        const int64_t ahead = pos - k0 - 4 * h;
+        const float d0 = static_cast<float>(ahead);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int x = 32 * t + 8 * (e / 4) + (e % 4);
+            float v = sc[t][e] * kscale;
+            if constexpr (CAP) {
+              const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v) + 1.0f);
+              v = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
+            }
+            if constexpr (BIAS) v = __builtin_fmaf(-slope2, d0 - x, v);
+            sc[t][e] = v;
+          }
+        const bool whole = k0 + kTok - 1 <= pw;
+        const int left = ahead > kTok ? kTok : ahead < -1 ? -1 : static_cast<int>(ahead);
+        if (!whole) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (32 * t + 8 * (e / 4) + (e % 4) > left) sc[t][e] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[t][e]);
+        {
+          const uint32_t bits = __float_as_uint(mx);
+          const auto r = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+          mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        }
+        const float mnew = fmaxf(m, mx);
+        const float mref = mnew == -INFINITY ? 0.0f : mnew;
+        const float alpha = __builtin_amdgcn_exp2f(m - mref);
+        m = mnew;
+        float sum = 0.0f;
+        uint4 pf[2][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(sc[t][e] - mref);
+            sum = sum + p[e];
+            p[e] = p[e] * vscale;
+          }
+          if (!whole) {  // a scale that is not finite stays with the queries that see the block
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (32 * t + 8 * (e / 4) + (e % 4) > left) p[e] = 0.0f;
+          }
+          pack16(pf[t], p);
+        }
+        {
+          const uint32_t bits = __float_as_uint(sum);
+          const auto r = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+          sum = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * alpha;
+        }
+        l = l * alpha + sum;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt)
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                row_frag<64>(vt, 32 * dt, s, lane), frag_of(pf[s / 2][s % 2]), o[dt], 0, 0, 0);
+      }
+      if (j + 1 < blocks) {
+        store(j + 1);
+        if (j + 2 < blocks) load(j + 2);
+        __syncthreads();
+      }
+    }
+  }
+  if (i >= a.S) return;
+  if (a.nsplit == 1) {
+    uint16_t* const row = static_cast<uint16_t*>(a.out) + ((b * a.S + i) * a.Hq + hd) * D;
+    const float factor = row_factor(a, b, i, l);
+    if (factor == 0.0f) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[dt] = v16f_a{};
+    }
+    store_owned<D>(row, o, factor, h);
+  } else {
+    float* const w = a.work + ((bh * a.S * a.G + i * a.G + (hd - kvh * a.G)) * a.nsplit + split) *
+                                  (D + 4);
+    if (h == 0) {
+      w[0] = m;
+      w[1] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<float4*>(w + 4 + 32 * dt + 8 * r + 4 * h) =
+            make_float4(o[dt][4 * r], o[dt][4 * r + 1], o[dt][4 * r + 2], o[dt][4 * r + 3]);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 static int check_cache(const rk_int8_kv& c) {
@@ -589,7 +832,8 @@ static int check_cache(const rk_int8_kv& c) {
   if (!aligned16(c.keys) || !aligned16(c.values))
     return fail(RK_ERR_UNSUPPORTED, "the cache needs 16-byte alignment");
   if (c.B * c.H > 65535) return fail(RK_ERR_UNSUPPORTED, "more than 65535 sequence heads");
-  if (c.blocks > (int64_t{1} << 30)) return fail(RK_ERR_UNSUPPORTED, "cache too long");
+  if (c.blocks * kTok * c.D >= (int64_t{1} << 31) - (int64_t{1} << 20))
+    return fail(RK_ERR_UNSUPPORTED, "a head's codes reach 2^31 bytes");
   return RK_OK;
 }
 
@@ -597,13 +841,24 @@ static Kv8 cache_args(const rk_int8_kv& c) {
   return Kv8{c.keys, c.values, c.key_scales, c.value_scales, c.B, c.H, c.blocks};
 }
 
-static int64_t columns_tiles(int64_t S, int64_t G) { return (S * G + 15) / 16; }
+// How a call is cut up: chunks of 128 queries of a head, or tiles of 16 columns; splits of the
+// cache up to about `want` workgroups, each at least `least` blocks.
+struct Kv8Plan {
+  bool chunk;
+  int64_t tiles, splits;
+};
 
-// Splits of the cache: about 1024 workgroups, and at least a block per wavefront of a split.
-static int64_t attention_splits(const rk_int8_kv& c, int64_t tiles) {
-  const int64_t have = c.B * c.H * tiles, want = have > 0 ? (1024 + have - 1) / have : 1;
-  const int64_t most = (c.blocks + 3) / 4;
-  return want < 1 ? 1 : (want < most ? want : (most > 0 ? most : 1));
+static Kv8Plan attention_plan(const rk_int8_kv& c, int64_t Hq, int64_t S, int qdtype, int odtype) {
+  const int64_t G = Hq / c.H;
+  Kv8Plan p{};
+  p.chunk = qdtype == RK_BF16 && odtype == RK_BF16 && c.D <= 128 && S >= kChunkTokens;
+  p.tiles = p.chunk ? (S + 127) / 128 : (S * G + 15) / 16;
+  const int64_t have = p.tiles * c.B * (p.chunk ? Hq : c.H);
+  const int64_t want = p.chunk ? 512 : 1024, least = 4;
+  const int64_t n = (want + have - 1) / have, most = (c.blocks + least - 1) / least;
+  p.splits = n < most ? n : most;
+  if (p.splits < 1) p.splits = 1;
+  return p;
 }
 
 template <int D, int QDT, int ODT>
@@ -614,19 +869,33 @@ static void launch_kv8_attn(const Kv8Attn& a, bool cap, hipStream_t st) {
   else if (cap) kv8_attn_kernel<D, QDT, ODT, true, false><<<grid, 256, 0, st>>>(a);
   else if (a.slopes) kv8_attn_kernel<D, QDT, ODT, false, true><<<grid, 256, 0, st>>>(a);
   else kv8_attn_kernel<D, QDT, ODT, false, false><<<grid, 256, 0, st>>>(a);
-  if (a.nsplit > 1)
-    kv8_join_kernel<D, ODT><<<dim3(static_cast<unsigned>(a.S * a.G),
-                                   static_cast<unsigned>(a.c.B * a.c.H)), D / 4, 0, st>>>(a);
 }
 
 template <int D>
-static void dispatch_kv8_attn(const Kv8Attn& a, bool cap, int qdt, int odt, hipStream_t st) {
-  if (qdt == RK_F32) {
+static void launch_kv8_chunk(const Kv8Attn& a, bool cap, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.tiles * a.c.B * a.Hq), static_cast<unsigned>(a.nsplit));
+  if (cap && a.slopes) kv8_chunk_kernel<D, true, true><<<grid, 256, 0, st>>>(a);
+  else if (cap) kv8_chunk_kernel<D, true, false><<<grid, 256, 0, st>>>(a);
+  else if (a.slopes) kv8_chunk_kernel<D, false, true><<<grid, 256, 0, st>>>(a);
+  else kv8_chunk_kernel<D, false, false><<<grid, 256, 0, st>>>(a);
+}
+
+template <int D>
+static void dispatch_kv8_attn(const Kv8Attn& a, const Kv8Plan& plan, bool cap, int qdt, int odt,
+                              hipStream_t st) {
+  if (plan.chunk) {
+    if constexpr (D <= 128) launch_kv8_chunk<D>(a, cap, st);
+  } else if (qdt == RK_F32) {
     if (odt == RK_F32) launch_kv8_attn<D, RK_F32, RK_F32>(a, cap, st);
     else launch_kv8_attn<D, RK_F32, RK_BF16>(a, cap, st);
   } else {
     if (odt == RK_F32) launch_kv8_attn<D, RK_BF16, RK_F32>(a, cap, st);
     else launch_kv8_attn<D, RK_BF16, RK_BF16>(a, cap, st);
+  }
+  if (a.nsplit > 1) {
+    const dim3 grid(static_cast<unsigned>(a.S * a.G), static_cast<unsigned>(a.c.B * a.c.H));
+    if (odt == RK_F32) kv8_join_kernel<D, RK_F32><<<grid, D / 4, 0, st>>>(a);
+    else kv8_join_kernel<D, RK_BF16><<<grid, D / 4, 0, st>>>(a);
   }
 }
 
@@ -703,10 +972,11 @@ extern "C" int rk_int8_kv_read(const rk_int8_kv* cache, int64_t begin, int64_t e
   return launch_status("int8_kv_read");
 }
 
-extern "C" int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S) {
+extern "C" int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S,
+                                             int qdtype, int odtype) {
   if (!cache || cache->B <= 0 || cache->H <= 0 || Hq <= 0 || S <= 0 || Hq % cache->H) return 0;
-  const int64_t tiles = columns_tiles(S, Hq / cache->H), n = attention_splits(*cache, tiles);
-  return n == 1 ? 0 : cache->B * cache->H * tiles * n * 16 * (cache->D + 4);
+  const int64_t n = attention_plan(*cache, Hq, S, qdtype, odtype).splits;
+  return n == 1 ? 0 : cache->B * Hq * S * n * (cache->D + 4);
 }
 
 extern "C" int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int qdtype, int64_t sqb,
@@ -740,20 +1010,24 @@ extern "C" int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int 
       return fail(RK_ERR_UNSUPPORTED, "query rows and strides must be whole 16-byte vectors");
   if (!aligned16(q) || !aligned16(out))
     return fail(RK_ERR_UNSUPPORTED, "queries and outputs need 16-byte alignment");
-  const int64_t G = Hq / c.H, tiles = columns_tiles(S, G);
-  if (tiles > 65535 || S * G >= (int64_t{1} << 24))
+  const int64_t G = Hq / c.H;
+  const Kv8Plan plan = attention_plan(c, Hq, S, qdtype, odtype);
+  // a launch holds fewer than 2^24 blocks of 256 threads
+  if (S * G >= (int64_t{1} << 24) || (!plan.chunk && plan.tiles > 65535) ||
+      plan.tiles * c.B * Hq * plan.splits >= (int64_t{1} << 24))
     return fail(RK_ERR_UNSUPPORTED, "too many queries for one launch");
-  const int64_t n = attention_splits(c, tiles);
-  if (n > 1 && (!work || !aligned16(work) || work_floats < rk_int8_kv_attention_work(&c, Hq, S)))
+  const int64_t n = plan.splits;
+  if (n > 1 && (!work || !aligned16(work) ||
+                work_floats < rk_int8_kv_attention_work(&c, Hq, S, qdtype, odtype)))
     return fail(RK_ERR_ARG, "attention workspace too small");
   const bool cap = softcap > 0.0f;
   Kv8Attn a{cache_args(c), q, sqb, sqh, sqs, start, lengths, slopes, start_count > 1 ? 1 : 0, S,
-            Hq, G, n, tiles,
+            Hq, G, n, plan.tiles,
             cap ? 2.0f * kLog2e8 * (scale / softcap) : scale * kLog2e8, softcap * kLog2e8, work,
             out};
   hipStream_t st = as_stream(stream);
-  if (c.D == 64) dispatch_kv8_attn<64>(a, cap, qdtype, odtype, st);
-  else if (c.D == 128) dispatch_kv8_attn<128>(a, cap, qdtype, odtype, st);
-  else dispatch_kv8_attn<256>(a, cap, qdtype, odtype, st);
+  if (c.D == 64) dispatch_kv8_attn<64>(a, plan, cap, qdtype, odtype, st);
+  else if (c.D == 128) dispatch_kv8_attn<128>(a, plan, cap, qdtype, odtype, st);
+  else dispatch_kv8_attn<256>(a, plan, cap, qdtype, odtype, st);
   return launch_status("int8_kv_attention");
 }

@@ -134,7 +134,7 @@ SIGNATURES: dict[str, list] = {
     "rk_int8_kv_append": [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _i64, _p, _i64,
                           _p, _p],
     "rk_int8_kv_read": [_p, _i64, _i64, _i32, _p, _p, _p],
-    "rk_int8_kv_attention_work": [_p, _i64, _i64],
+    "rk_int8_kv_attention_work": [_p, _i64, _i64, _i32, _i32],
     "rk_int8_kv_attention": [_p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _f32, _f32,
                              _p, _p, _i64, _p, _i32, _p],
     "rk_kv_append": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i32, _i64, _i64,
