@@ -57,6 +57,7 @@ def hipcc() -> str:
 SOURCE_FLAGS = {
     "rk_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "rk_scored.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "rk_kv8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -12,6 +12,7 @@
 // raise its scale; the codes there are then rounded again, rint(c (s_old / s)). A block's first
 // token starts it anew, whatever it held.
 #include "rk_attention.h"
+#include "rk_rowquant.h"
 
 #include <math.h>
 
@@ -56,12 +57,28 @@ __device__ __forceinline__ bool append_range(const Kv8Append& a, int64_t b, int6
   return first < last;
 }
 
+__device__ __forceinline__ float fmed3(float x) {
+  return __builtin_amdgcn_fmed3f(x, -127.0f, 127.0f);
+}
+
 // code of x under scale s; only denormal scales reach the clamp, only NaN and infinite scales
 // the zero of a NaN quotient
 __device__ __forceinline__ int code_of(float x, float s) {
   const float y = __builtin_rintf(x / s);
   const int c = static_cast<int>(fminf(fmaxf(y, -127.0f), 127.0f));
   return s > 0.0f && y == y ? c : 0;
+}
+// The same for 8 values, by the reciprocal r of s where that decides (rk_rowquant.h: the rounded
+// product, redone by the quotient when one of the 8 lies near a rounding boundary). With the IEEE
+// quotient for every value the divisions bounded the kernel (VVV).
+__device__ __forceinline__ void codes_of(const float (&x)[8], float s, float r, int (&c)[8]) {
+  bool exact = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = static_cast<int>(fmed3(round_fast(x[e], r, exact)));
+  if (exact) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = code_of(x[e], s);
+  }
 }
 __device__ __forceinline__ int code_again(int c, float ratio) {
   return static_cast<int>(
@@ -92,22 +109,24 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
                       (blk * kTok - start) * ss;
   const float old = first > 0 ? *scale : 0.0f;
 
+  // every thread loads, tokens outside first .. last - 1 the nearest one inside: a condition
+  // around the loads let only one be in flight (16 -> NNN us at 4 x 777 tokens, 16 heads of 128)
   float x[EACH][8];
-  uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int unit = tid + 256 * i, t = unit / PER, f = unit % PER * 8;
-    if (t >= first && t < last) {
-      const int64_t idx = off + t * ss + f;
-      load_vec16<DT>(src, idx, x[i]);
-      if constexpr (DT == RK_F32) load_vec16<DT>(src, idx + 4, x[i] + 4);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t bits = __float_as_uint(x[i][e]) & 0x7fffffffu;
-        most = bits > most ? bits : most;
-      }
-    }
+    const int tc = t < first ? first : t < last ? t : last - 1;
+    load_vec16<DT>(src, off + tc * ss + f, x[i]);
+    if constexpr (DT == RK_F32) load_vec16<DT>(src, off + tc * ss + f + 4, x[i] + 4);
   }
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t bits = __float_as_uint(x[i][e]) & 0x7fffffffu;
+      most = bits > most ? bits : most;
+    }
   most = wave_butterfly(most, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
   if ((tid & 63) == 0) red[tid >> 6] = most;
   __syncthreads();
@@ -116,7 +135,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   float s = __uint_as_float(most) / 127.0f;
   if (first > 0 && __float_as_uint(old) > __float_as_uint(s)) s = old;
   const bool grown = first > 0 && __float_as_uint(old) != __float_as_uint(s);
-  const float ratio = old / (s > 0.0f ? s : 1.0f);
+  const float ratio = old / (s > 0.0f ? s : 1.0f), recip = 1.0f / s;
   if (tid == 0) *scale = s;
 
   if (!val) {
@@ -136,11 +155,10 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
     for (int i = 0; i < EACH; ++i) {
       const int unit = tid + 256 * i, t = unit / PER, f = unit % PER * 8;
       if (t >= first && t < last) {
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w[e / 4] |= static_cast<uint32_t>(code_of(x[i][e], s) & 255) << (8 * (e % 4));
-        *reinterpret_cast<uint2*>(codes + t * D + f) = make_uint2(w[0], w[1]);
+        int c[8];
+        codes_of(x[i], s, recip, c);
+        *reinterpret_cast<uint2*>(codes + t * D + f) =
+            make_uint2(pack_bytes4(c[0], c[1], c[2], c[3]), pack_bytes4(c[4], c[5], c[6], c[7]));
       }
     }
     return;
@@ -167,9 +185,10 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   for (int i = 0; i < EACH; ++i) {
     const int unit = tid + 256 * i, t = unit / PER, f = unit % PER * 8;
     if (t >= first && t < last) {
+      int c[8];
+      codes_of(x[i], s, recip, c);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        tile[(f + e) * PITCH + t] = static_cast<uint8_t>(code_of(x[i][e], s) & 255);
+      for (int e = 0; e < 8; ++e) tile[(f + e) * PITCH + t] = static_cast<uint8_t>(c[e]);
     }
   }
   __syncthreads();
@@ -240,9 +259,10 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a) {
 // key head (G = query heads per key head), 16 at a time; rows are keys, then features.
 //
 // Both products run on the codes as they are, in exact integers: the query is written as a fixed
-// point number of three signed base-256 digits relative to its largest feature (23 bits, the
-// rounding a float32 operand would have), the probabilities as three digits relative to the
-// block's largest, and each digit's product is its own MFMA. The matrix unit takes them at a
+// point number of signed base-256 digits relative to its largest feature, the probabilities
+// relative to the block's largest, and each digit's product is its own MFMA. Three digits (23
+// bits, about a float32 operand's rounding) for float32 results, two (15 bits, against the 8 of
+// the result) for bf16. The matrix unit takes them at a
 // fraction of the time the codes need to arrive, and no code is ever converted: for one query
 // per head, 48 MFMAs and about 500 vector instructions per 16 KB of codes at D = 128.
 //
@@ -260,8 +280,10 @@ struct Kv8Attn {
   const int64_t* lengths;
   const float* slopes;
   int64_t start_step, S, Hq, G, nsplit, tiles;
+  int64_t nfull;  // chunks: splits of whole tiles (1 or nsplit; the last, partial one has nsplit)
+  int64_t col0;   // the first column that is joined
   float dot_scale, cap2;
-  float* work;  // [B * H][S * G][nsplit][D + 4]: max, sum, 2 pad, unnormalized output
+  float* work;  // [B * H][S * G - col0][nsplit][D + 4]: max, sum, 2 pad, unnormalized output
   void* out;    // [B, S, Hq, D], of type ODT
 };
 
@@ -288,28 +310,36 @@ __device__ __forceinline__ uint32_t col_umax(uint32_t v) {
   return s[0] > s[1] ? s[0] : s[1];
 }
 
-constexpr float kFixed = 127.0f * 65536.0f;  // the largest three-digit number used
+// A number of ND signed base-256 digits, the largest 127 256^(ND - 1).
+template <int ND>
+constexpr float kFixed = ND == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
 
-// Digits of 4 numbers |x| <= kFixed, rounded, as bytes of one word each: x = 65536 a + 256 b + c.
-__device__ __forceinline__ void digits4(const float (&x)[4], int& a, int& b, int& c) {
-  uint32_t w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    // adding 128 to the two low digits makes them unsigned without a carry to take back
-    w[e] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(x[e])) + 0x8080);
-  }
-  const uint32_t p01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);  // c0 c1 b0 b1
+// Digits of 4 numbers, each given as the word whose low bytes are the number plus 128 in every
+// digit but the first (which makes them unsigned, without a carry to take back), as one word a
+// digit, the first digit first.
+template <int ND>
+__device__ __forceinline__ void digits4(const uint32_t (&w)[4], int (&d)[ND]) {
+  const uint32_t p01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);  // low bytes, second bytes
   const uint32_t p23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
-  const uint32_t h01 = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602u);  // a0 a1
-  const uint32_t h23 = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0602u);
-  c = static_cast<int>(__builtin_amdgcn_perm(p23, p01, 0x05040100u) ^ 0x80808080u);
-  b = static_cast<int>(__builtin_amdgcn_perm(p23, p01, 0x07060302u) ^ 0x80808080u);
-  a = static_cast<int>(__builtin_amdgcn_perm(h23, h01, 0x05040100u));
+  const uint32_t low = __builtin_amdgcn_perm(p23, p01, 0x05040100u);
+  const uint32_t mid = __builtin_amdgcn_perm(p23, p01, 0x07060302u);
+  d[ND - 1] = static_cast<int>(low ^ 0x80808080u);
+  if constexpr (ND == 3) {
+    const uint32_t h01 = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602u);
+    const uint32_t h23 = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0602u);
+    d[1] = static_cast<int>(mid ^ 0x80808080u);
+    d[0] = static_cast<int>(__builtin_amdgcn_perm(h23, h01, 0x05040100u));
+  } else {
+    d[0] = static_cast<int>(mid);
+  }
 }
 
-__device__ __forceinline__ float from_digits(int a, int b, int c) {
-  return __builtin_fmaf(static_cast<float>(a), 65536.0f,
-                        __builtin_fmaf(static_cast<float>(b), 256.0f, static_cast<float>(c)));
+// The sum that the digits' sums make (each below 2^22, so two of them fit an integer).
+template <int ND>
+__device__ __forceinline__ float from_digits(const v4i8 (&d)[ND], int e) {
+  const float low = static_cast<float>(d[ND - 2][e] * 256 + d[ND - 1][e]);
+  if constexpr (ND == 3) return __builtin_fmaf(static_cast<float>(d[0][e]), 65536.0f, low);
+  return low;
 }
 
 template <int QDT>
@@ -333,11 +363,11 @@ __device__ __forceinline__ float row_factor(const Kv8Attn& a, int64_t b, int64_t
   return 1.0f / l;
 }
 
-template <int D, int QDT, int ODT, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
-  constexpr int KK = D / 64, FT = D / 16;
-  __shared__ __attribute__((aligned(16))) float so[4][16][D + 4];
-  __shared__ float sm[4][16], sl[4][16];
+template <int D, int QDT, int ODT, int NW, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
+  constexpr int KK = D / 64, FT = D / 16, ND = ODT == RK_F32 ? 3 : 2, NT = 64 * NW;
+  __shared__ __attribute__((aligned(16))) float so[NW][16][D + 4];
+  __shared__ float sm[NW][16], sl[NW][16];
   const int split = blockIdx.x;
   const int64_t tile = blockIdx.y, bh = blockIdx.z;
   const int64_t b = bh / a.c.H, kvh = bh - b * a.c.H;
@@ -366,43 +396,6 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
     for (int e = 0; e < 4; ++e) o[f][e] = 0.0f;
 
   if (j0 + wave < j1) {
-    // the query's digits: features 64 kk + 16 g .. + 15
-    v4i8 qd[3][KK];
-    float qscale;
-    {
-      float x[KK][16];
-      uint32_t most = 0;
-      const int64_t base = b * a.sqb + hd * a.sqh + i * a.sqs + 16 * g;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-#pragma unroll
-        for (int v = 0; v < 16 / Vec<QDT>::N; ++v)
-          load_vec16<QDT>(a.q, base + 64 * kk + v * Vec<QDT>::N, x[kk] + v * Vec<QDT>::N);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t bits = __float_as_uint(x[kk][e]) & 0x7fffffffu;
-          most = bits > most ? bits : most;
-        }
-      }
-      most = col_umax(most);
-      const float big = __uint_as_float(most);
-      const float up = big > 0.0f ? kFixed / big : 0.0f;
-      qscale = big / kFixed;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          float y[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            y[e] = fminf(fmaxf(x[kk][4 * w + e] * up, -kFixed), kFixed);
-          int d0, d1, d2;
-          digits4(y, d0, d1, d2);
-          qd[0][kk][w] = d0;
-          qd[1][kk][w] = d1;
-          qd[2][kk][w] = d2;
-        }
-    }
     float slope2 = 0.0f;
     if constexpr (BIAS) slope2 = a.slopes[hd] * kLog2e8;
     const int64_t pos = start + i;
@@ -438,15 +431,54 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
     int64_t j = j0 + wave;
     load_k(j);
     load_v(j);
-    for (; j < j1; j += 4) {
+    // the query's digits: features 64 kk + 16 g .. + 15
+    v4i8 qd[ND][KK];
+    float qscale;
+    {
+      float x[KK][16];
+      uint32_t most = 0;
+      const int64_t base = b * a.sqb + hd * a.sqh + i * a.sqs + 16 * g;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+        for (int v = 0; v < 16 / Vec<QDT>::N; ++v)
+          load_vec16<QDT>(a.q, base + 64 * kk + v * Vec<QDT>::N, x[kk] + v * Vec<QDT>::N);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t bits = __float_as_uint(x[kk][e]) & 0x7fffffffu;
+          most = bits > most ? bits : most;
+        }
+      }
+      most = col_umax(most);
+      const float big = __uint_as_float(most);
+      const float up = big > 0.0f ? kFixed<ND> / big : 0.0f;
+      qscale = big / kFixed<ND>;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t y[4];
+          int d[ND];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = fminf(fmaxf(x[kk][4 * w + e] * up, -kFixed<ND>), kFixed<ND>);
+            y[e] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v)) +
+                                         (ND == 3 ? 0x8080 : 0x80));
+          }
+          digits4<ND>(y, d);
+#pragma unroll
+          for (int n = 0; n < ND; ++n) qd[n][kk][w] = d[n];
+        }
+    }
+    for (; j < j1; j += NW) {
       const float kscale = ks[j], vscale = vs[j];
       float s[16];
       const float mul = qscale * kscale * a.dot_scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        v4i8 acc[3];
+        v4i8 acc[ND];
 #pragma unroll
-        for (int d = 0; d < 3; ++d) {
+        for (int d = 0; d < ND; ++d) {
           acc[d] = v4i8{0, 0, 0, 0};
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk)
@@ -454,9 +486,9 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          s[4 * t + e] = from_digits(acc[0][e], acc[1][e], acc[2][e]) * mul;
+          s[4 * t + e] = from_digits<ND>(acc, e) * mul;
       }
-      load_k(j + 4);
+      load_k(j + NW);
       const int64_t ahead = pos - (j * kTok + 16 * g);
       const int left = ahead > 16 ? 16 : ahead < -1 ? -1 : static_cast<int>(ahead);
       const float d0 = static_cast<float>(ahead);  // key 16 g + x is seen for x <= left
@@ -478,42 +510,50 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
       const float alpha = __builtin_amdgcn_exp2f(m - nref);
       const float beta = __builtin_amdgcn_exp2f(mx - nref);
       m = mnew;
+      // p as a fixed-point number: 2^23 and the digits' 128s are added in float32, which rounds
+      // it and leaves the digits in the low bytes of the sum
       float sum = 0.0f;
-      v4i8 pd[3];
+      v4i8 pd[ND];
+      constexpr float kUnit = ND == 3 ? 8388608.0f + 32896.0f : 8388608.0f + 128.0f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        float y[4];
+        uint32_t y[4];
+        int d[ND];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float p = __builtin_amdgcn_exp2f(s[4 * w + e] - ref);
           sum = sum + p;
-          y[e] = fminf(p, 1.0f) * kFixed;
+          y[e] = __float_as_uint(__builtin_fmaf(p, kFixed<ND>, kUnit));
         }
-        int d0i, d1i, d2i;
-        digits4(y, d0i, d1i, d2i);
-        pd[0][w] = d0i;
-        pd[1][w] = d1i;
-        pd[2][w] = d2i;
+        digits4<ND>(y, d);
+#pragma unroll
+        for (int n = 0; n < ND; ++n) pd[n][w] = d[n];
       }
       l = l * alpha + beta * col_sum(sum);
       // a block that the column does not see at all adds nothing, whatever its scale
-      const float add = mx == -INFINITY && sum == 0.0f ? 0.0f : beta * vscale * (1.0f / kFixed);
+      const float add =
+          mx == -INFINITY && sum == 0.0f ? 0.0f : beta * vscale * (1.0f / kFixed<ND>);
+      if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int f = 0; f < FT; ++f)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[f][e] = o[f][e] * alpha;
+      }
 #pragma unroll
       for (int f = 0; f < FT; ++f) {
-        v4i8 acc[3];
+        v4i8 acc[ND];
 #pragma unroll
-        for (int d = 0; d < 3; ++d)
+        for (int d = 0; d < ND; ++d)
           acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[f], pd[d], v4i8{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          o[f][e] = __builtin_fmaf(from_digits(acc[0][e], acc[1][e], acc[2][e]), add,
-                                   o[f][e] * alpha);
+          o[f][e] = __builtin_fmaf(from_digits<ND>(acc, e), add, o[f][e]);
       }
-      load_v(j + 4);
+      load_v(j + NW);
     }
   }
 
-  // the four wavefronts
+  // the wavefronts
   if (g == 0) {
     sm[wave][col] = m;
     sl[wave][col] = l;
@@ -524,16 +564,16 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
         make_float4(o[f][0], o[f][1], o[f][2], o[f][3]);
   __syncthreads();
   // a thread takes 4 features of one column at a time
-  for (int idx = tid; idx < 16 * (D / 4); idx += 256) {
+  for (int idx = tid; idx < 16 * (D / 4); idx += NT) {
     const int c = idx / (D / 4), f = idx % (D / 4) * 4;
     const int64_t ct = tile * 16 + c;
     if (ct >= cols) break;
     float mm = sm[0][c];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm[w][c]);
+    for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm[w][c]);
     float ll = 0.0f, r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float x = sm[w][c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][c] - mm);
       // a NaN sum with no maximum still has to be seen
       ll = ll + (sl[w][c] == sl[w][c] ? x * sl[w][c] : sl[w][c]);
@@ -560,22 +600,39 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(Kv8Attn a) {
 // grid (columns, B * H), D / 4 threads: the splits of one column.
 template <int D, int ODT>
 __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
-  const int64_t ct = blockIdx.x, bh = blockIdx.y, b = bh / a.c.H, kvh = bh - b * a.c.H;
+  const int64_t ct = a.col0 + blockIdx.x, bh = blockIdx.y, b = bh / a.c.H, kvh = bh - b * a.c.H;
   const int f = threadIdx.x * 4;
-  const float* w = a.work + (bh * a.S * a.G + ct) * a.nsplit * (D + 4);
+  const float* w = a.work + (bh * (a.S * a.G - a.col0) + blockIdx.x) * a.nsplit * (D + 4);
   const int64_t step = D + 4;
-  float mm = -INFINITY;
-  for (int64_t s = 0; s < a.nsplit; ++s) mm = fmaxf(mm, w[s * step]);
-  float ll = 0.0f, r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t s = 0; s < a.nsplit; ++s) {
-    const float ms = w[s * step], ls = w[s * step + 1];
-    const float x = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - mm);
-    ll = ll + (ls == ls ? x * ls : ls);
-    const float4 v = *reinterpret_cast<const float4*>(w + s * step + 4 + f);
-    r[0] = __builtin_fmaf(x, v.x, r[0]);
-    r[1] = __builtin_fmaf(x, v.y, r[1]);
-    r[2] = __builtin_fmaf(x, v.z, r[2]);
-    r[3] = __builtin_fmaf(x, v.w, r[3]);
+  float mm = -INFINITY, ll = 0.0f, r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  // eight splits' loads in flight, in one pass with a running maximum
+  for (int64_t s0 = 0; s0 < a.nsplit; s0 += 8) {
+    float ms[8], ls[8];
+    float4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float* at = w + (s0 + u < a.nsplit ? s0 + u : s0) * step;
+      ms[u] = s0 + u < a.nsplit ? at[0] : -INFINITY;
+      ls[u] = s0 + u < a.nsplit ? at[1] : 0.0f;
+      v[u] = *reinterpret_cast<const float4*>(at + 4 + f);
+    }
+    float mn = mm;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) mn = fmaxf(mn, ms[u]);
+    const float c = mm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mm - mn);
+    mm = mn;
+    ll = ll == ll ? ll * c : ll;  // a NaN sum with no maximum still has to be seen
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = r[e] * c;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float x = ms[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[u] - mm);
+      ll = ll + (ls[u] == ls[u] ? x * ls[u] : ls[u]);
+      const float o4[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        r[e] = ms[u] == -INFINITY ? r[e] : __builtin_fmaf(x, o4[e], r[e]);
+    }
   }
   const int64_t qi = ct / a.G, h = kvh * a.G + (ct - qi * a.G);
   const float factor = row_factor(a, b, qi, ll);
@@ -596,29 +653,53 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
 // Codes converted by each reader instead, or the digits of kv8_attn_kernel for chunks too, cost
 // more: the latter ZZZ us at 4 x 517 tokens behind 1500, 16 heads of 128.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+template <bool SCALED = false>
+__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi,
+                                            float power = 1.0f) {
   uint32_t f[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    f[e] = __float_as_uint(static_cast<float>(static_cast<int8_t>(w >> (8 * e))));
+  for (int e = 0; e < 4; ++e) {
+    const float x = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
+    f[e] = __float_as_uint(SCALED ? x * power : x);
+  }
   lo = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);  // small integers: the low halves are zero
   hi = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
 }
 
+// A block's value scale: `fold` goes into the exponent of its probabilities, whose sum is
+// multiplied by `inv`, and `rest` into its values. Scales whose products could leave float32's
+// range leave a power of two to the values; one that is not finite makes its values zero and the
+// sum NaN, which only the queries that see the block take over.
+struct ValueScale {
+  float fold, inv, rest;
+  __device__ __forceinline__ explicit ValueScale(float s) : fold(s), inv(0.0f), rest(1.0f) {
+    const bool finite = s <= 3.4028235e38f;
+    if (!(s >= 0x1p-60f && s <= 0x1p60f)) {
+      fold = !finite || s == 0.0f ? 1.0f : s < 1.0f ? s * 0x1p96f : s * 0x1p-96f;
+      rest = !finite || s == 0.0f ? 0.0f : s < 1.0f ? 0x1p-96f : 0x1p96f;
+    }
+    inv = finite ? 1.0f / fold : __uint_as_float(0x7fc00000u);
+  }
+};
+
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void kv8_chunk_kernel(Kv8Attn a) {
   constexpr int TILE = kTok * D * 2;    // bf16 keys [64][D] or values [D][64]
   constexpr int EACH = kTok * D / 16 / 256;  // 16-code pieces per thread and operand
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * 2 * TILE];
-  // the last queries, which see most, first; heads fastest
-  const int64_t BHq = a.c.B * a.Hq;
-  const int64_t qt = a.tiles - 1 - blockIdx.x / BHq;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * 2 * 2 * TILE];
+  // whole tiles first, the last queries, which see most, before the others; heads fastest
+  const int64_t BHq = a.c.B * a.Hq, full = a.S / 128, turn = blockIdx.x / BHq;
+  const bool whole_tile = turn < full * a.nfull;
+  const int64_t qt = whole_tile ? full - 1 - turn / a.nfull : full;
+  const int64_t split = whole_tile ? turn % a.nfull : turn - full * a.nfull;
+  const int64_t nsplit = whole_tile ? a.nfull : a.nsplit;
   const int64_t bhq = blockIdx.x % BHq, b = bhq / a.Hq, hd = bhq - b * a.Hq, kvh = hd / a.G;
   const int64_t bh = b * a.c.H + kvh;
-  const int split = blockIdx.y;
-  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x & 255, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);  // blocks half, half + 2, ..
+  uint8_t* const smem = lds + half * 2 * 2 * TILE;
   const int64_t start = a.start[b * a.start_step];
   int64_t n = a.lengths ? a.lengths[b] : a.S;
   n = n < a.S ? n : a.S;
@@ -627,7 +708,7 @@ void kv8_chunk_kernel(Kv8Attn a) {
   const int64_t last = i0 + 128 < n ? i0 + 127 : n - 1;  // the last active query
   int64_t nb = on ? (start + last) / kTok + 1 : 0;
   nb = nb < a.c.NB ? nb : a.c.NB;
-  const int64_t per = (nb + a.nsplit - 1) / a.nsplit;
+  const int64_t per = (nb + nsplit - 1) / nsplit;
   const int64_t j0 = split * per, j1 = j0 + per < nb ? j0 + per : nb;
   // positions relative to the split's first key
   const int64_t base = start - j0 * kTok;
@@ -664,8 +745,9 @@ void kv8_chunk_kernel(Kv8Attn a) {
       }
     };
     auto store = [&](int j) {
-      uint8_t* const kt = smem + (j & 1) * 2 * TILE;
+      uint8_t* const kt = smem + (j >> 1 & 1) * 2 * TILE;
       uint8_t* const vt = kt + TILE;
+      const float power = ValueScale(vs[j]).rest;
 #pragma unroll
       for (int c = 0; c < EACH; ++c) {
         const int p = tid + 256 * c;
@@ -682,10 +764,17 @@ void kv8_chunk_kernel(Kv8Attn a) {
         }
         {  // tokens 0-3, 8-11 | 4-7, 12-15 of each 16: a lane's slots
           const int row = p / 4, seg = p % 4 * 2, sw = seg_swizzle<64>(row);
-          widen_codes(rv[c].x, x[0].x, x[0].y);
-          widen_codes(rv[c].z, x[0].z, x[0].w);
-          widen_codes(rv[c].y, x[1].x, x[1].y);
-          widen_codes(rv[c].w, x[1].z, x[1].w);
+          if (power == 1.0f) {
+            widen_codes(rv[c].x, x[0].x, x[0].y);
+            widen_codes(rv[c].z, x[0].z, x[0].w);
+            widen_codes(rv[c].y, x[1].x, x[1].y);
+            widen_codes(rv[c].w, x[1].z, x[1].w);
+          } else {
+            widen_codes<true>(rv[c].x, x[0].x, x[0].y, power);
+            widen_codes<true>(rv[c].z, x[0].z, x[0].w, power);
+            widen_codes<true>(rv[c].y, x[1].x, x[1].y, power);
+            widen_codes<true>(rv[c].w, x[1].z, x[1].w, power);
+          }
           uint8_t* const to = vt + row * (2 * kTok);
           *reinterpret_cast<uint4*>(to + 16 * (seg ^ sw)) = x[0];
           *reinterpret_cast<uint4*>(to + 16 * ((seg + 1) ^ sw)) = x[1];
@@ -693,40 +782,50 @@ void kv8_chunk_kernel(Kv8Attn a) {
       }
     };
     const int blocks = static_cast<int>(j1 - j0);
-    load(0);
-    store(0);
-    if (blocks > 1) load(1);
+    if (half < blocks) {
+      load(half);
+      store(half);
+      if (half + 2 < blocks) load(half + 2);
+    }
     __syncthreads();
-    for (int j = 0; j < blocks; ++j) {
-      const uint8_t* const kt = smem + (j & 1) * 2 * TILE;
+    for (int n2 = 0; n2 < blocks; n2 += 2) {
+      const int j = n2 + half;
+      const uint8_t* const kt = smem + (j >> 1 & 1) * 2 * TILE;
       const uint8_t* const vt = kt + TILE;
       const int64_t k0 = static_cast<int64_t>(j) * kTok;
-      if (iw < n && k0 <= pw + 31) {  // some query of the wavefront sees some key
-        const float kscale = ks[j] * a.dot_scale, vscale = vs[j];
-        v16f_a sc[2];
+      if (j < blocks && iw < n && k0 <= pw + 31) {  // some query of the wavefront sees some key
+        const float kscale = ks[j] * a.dot_scale;
+        const ValueScale v(vs[j]);
+        const float vlog = __log2f(v.fold);
+        v16f_a sc[2] = {v16f_a{}, v16f_a{}};
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          sc[t] = v16f_a{};
+        for (int s = 0; s < D / 16; ++s)
 #pragma unroll
-          for (int s = 0; s < D / 16; ++s)
+          for (int t = 0; t < 2; ++t)
             sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, 32 * t, s, lane),
                                                             qf[s], sc[t], 0, 0, 0);
-        }
         const int64_t ahead = pos - k0 - 4 * h;
         const float d0 = static_cast<float>(ahead);
+        // capped and biased scores in base-2 units here; plain ones are scaled with the max
+        const float mul = CAP || BIAS ? 1.0f : kscale;
+        if constexpr (CAP || BIAS) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int x = 32 * t + 8 * (e / 4) + (e % 4);
-            float v = sc[t][e] * kscale;
-            if constexpr (CAP) {
-              const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v) + 1.0f);
-              v = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
+            for (int e = 0; e < 16; ++e) {
+              const int x = 32 * t + 8 * (e / 4) + (e % 4);
+              float y = sc[t][e];
+              if constexpr (CAP) {
+                const float r =
+                    __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * kscale) + 1.0f);
+                y = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
+                if constexpr (BIAS) y = __builtin_fmaf(-slope2, d0 - x, y);
+              } else {
+                y = __builtin_fmaf(y, kscale, -slope2 * (d0 - x));
+              }
+              sc[t][e] = y;
             }
-            if constexpr (BIAS) v = __builtin_fmaf(-slope2, d0 - x, v);
-            sc[t][e] = v;
-          }
+        }
         const bool whole = k0 + kTok - 1 <= pw;
         const int left = ahead > kTok ? kTok : ahead < -1 ? -1 : static_cast<int>(ahead);
         if (!whole) {
@@ -746,9 +845,10 @@ void kv8_chunk_kernel(Kv8Attn a) {
           const auto r = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
           mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
         }
-        const float mnew = fmaxf(m, mx);
+        // a zero key scale: every score is zero, also times a maximum of -inf
+        const float mnew = fmaxf(m, mx == -INFINITY ? mx : mx * mul);
         const float mref = mnew == -INFINITY ? 0.0f : mnew;
-        const float alpha = __builtin_amdgcn_exp2f(m - mref);
+        const float alpha = __builtin_amdgcn_exp2f(m - mref), shift = vlog - mref;
         m = mnew;
         float sum = 0.0f;
         uint4 pf[2][2];
@@ -756,16 +856,16 @@ void kv8_chunk_kernel(Kv8Attn a) {
         for (int t = 0; t < 2; ++t) {
           float p[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(sc[t][e] - mref);
-            sum = sum + p[e];
-            p[e] = p[e] * vscale;
-          }
-          if (!whole) {  // a scale that is not finite stays with the queries that see the block
+          for (int e = 0; e < 16; ++e)
+            p[e] = __builtin_amdgcn_exp2f(CAP || BIAS ? sc[t][e] + shift
+                                                      : __builtin_fmaf(sc[t][e], mul, shift));
+          if (!whole) {  // (a zero key scale makes NaN of a masked score)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               if (32 * t + 8 * (e / 4) + (e % 4) > left) p[e] = 0.0f;
           }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum = sum + p[e];
           pack16(pf[t], p);
         }
         {
@@ -779,7 +879,7 @@ void kv8_chunk_kernel(Kv8Attn a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * alpha;
         }
-        l = l * alpha + sum;
+        l = l * alpha + (sum == 0.0f ? 0.0f : sum * v.inv);
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -787,15 +887,41 @@ void kv8_chunk_kernel(Kv8Attn a) {
             o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 row_frag<64>(vt, 32 * dt, s, lane), frag_of(pf[s / 2][s % 2]), o[dt], 0, 0, 0);
       }
-      if (j + 1 < blocks) {
-        store(j + 1);
-        if (j + 2 < blocks) load(j + 2);
-        __syncthreads();
+      if (j + 2 < blocks) {
+        store(j + 2);
+        if (j + 4 < blocks) load(j + 4);
       }
+      if (n2 + 2 < blocks) __syncthreads();
     }
   }
+  // the second half's state into the first's
+  {
+    float* const box = reinterpret_cast<float*>(lds) + tid;
+    __syncthreads();
+    if (half == 1) {
+      box[0] = m;
+      box[256] = l;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) box[256 * (2 + 16 * dt + e)] = o[dt][e];
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const float m1 = box[0], l1 = box[256], mn = fmaxf(m, m1);
+    const float c0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float c1 = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - mn);
+    // a NaN sum with no maximum still has to be seen
+    l = (l == l ? l * c0 : l) + (l1 == l1 ? l1 * c1 : l1);
+    m = mn;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        o[dt][e] = __builtin_fmaf(box[256 * (2 + 16 * dt + e)], c1, o[dt][e] * c0);
+  }
   if (i >= a.S) return;
-  if (a.nsplit == 1) {
+  if (nsplit == 1) {
     uint16_t* const row = static_cast<uint16_t*>(a.out) + ((b * a.S + i) * a.Hq + hd) * D;
     const float factor = row_factor(a, b, i, l);
     if (factor == 0.0f) {
@@ -804,8 +930,9 @@ void kv8_chunk_kernel(Kv8Attn a) {
     }
     store_owned<D>(row, o, factor, h);
   } else {
-    float* const w = a.work + ((bh * a.S * a.G + i * a.G + (hd - kvh * a.G)) * a.nsplit + split) *
-                                  (D + 4);
+    const int64_t ct = i * a.G + (hd - kvh * a.G);
+    float* const w =
+        a.work + ((bh * (a.S * a.G - a.col0) + ct - a.col0) * a.nsplit + split) * (D + 4);
     if (h == 0) {
       w[0] = m;
       w[1] = l;
@@ -845,7 +972,8 @@ static Kv8 cache_args(const rk_int8_kv& c) {
 // cache up to about `want` workgroups, each at least `least` blocks.
 struct Kv8Plan {
   bool chunk;
-  int64_t tiles, splits;
+  int waves;  // of a workgroup
+  int64_t tiles, splits, full_splits, col0;
 };
 
 static Kv8Plan attention_plan(const rk_int8_kv& c, int64_t Hq, int64_t S, int qdtype, int odtype) {
@@ -854,30 +982,50 @@ static Kv8Plan attention_plan(const rk_int8_kv& c, int64_t Hq, int64_t S, int qd
   p.chunk = qdtype == RK_BF16 && odtype == RK_BF16 && c.D <= 128 && S >= kChunkTokens;
   p.tiles = p.chunk ? (S + 127) / 128 : (S * G + 15) / 16;
   const int64_t have = p.tiles * c.B * (p.chunk ? Hq : c.H);
-  const int64_t want = p.chunk ? 512 : 1024, least = 4;
-  const int64_t n = (want + have - 1) / have, most = (c.blocks + least - 1) / least;
-  p.splits = n < most ? n : most;
-  if (p.splits < 1) p.splits = 1;
+  const auto splits = [&](int64_t want, int64_t least) {
+    const int64_t n = want / (have > 0 ? have : 1), most = (c.blocks + least - 1) / least;
+    return n < 1 || most < 1 ? 1 : n < most ? n : most;
+  };
+  if (!p.chunk) {
+    p.waves = have <= 128 ? 8 : 4;
+    p.splits = splits(c.D == 64 ? 1024 : 512, p.waves == 8 ? 16 : 4);
+    return p;
+  }
+  p.splits = p.full_splits = splits(256, 8);
+  // a last tile of less than 64 queries behind whole ones: its few busy wavefronts would be the
+  // launch's tail, so its keys are split
+  const int64_t full = S / 128, rest = S % 128;
+  if (p.splits == 1 && full > 0 && rest > 0 && rest < 64 && c.blocks >= 16) {
+    p.splits = c.blocks / 8 < 8 ? c.blocks / 8 : 8;
+    p.col0 = full * 128 * G;
+  }
   return p;
 }
 
-template <int D, int QDT, int ODT>
+template <int D, int QDT, int ODT, int NW>
 static void launch_kv8_attn(const Kv8Attn& a, bool cap, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(a.nsplit), static_cast<unsigned>(a.tiles),
                   static_cast<unsigned>(a.c.B * a.c.H));
-  if (cap && a.slopes) kv8_attn_kernel<D, QDT, ODT, true, true><<<grid, 256, 0, st>>>(a);
-  else if (cap) kv8_attn_kernel<D, QDT, ODT, true, false><<<grid, 256, 0, st>>>(a);
-  else if (a.slopes) kv8_attn_kernel<D, QDT, ODT, false, true><<<grid, 256, 0, st>>>(a);
-  else kv8_attn_kernel<D, QDT, ODT, false, false><<<grid, 256, 0, st>>>(a);
+  if (cap && a.slopes) kv8_attn_kernel<D, QDT, ODT, NW, true, true><<<grid, 64 * NW, 0, st>>>(a);
+  else if (cap) kv8_attn_kernel<D, QDT, ODT, NW, true, false><<<grid, 64 * NW, 0, st>>>(a);
+  else if (a.slopes) kv8_attn_kernel<D, QDT, ODT, NW, false, true><<<grid, 64 * NW, 0, st>>>(a);
+  else kv8_attn_kernel<D, QDT, ODT, NW, false, false><<<grid, 64 * NW, 0, st>>>(a);
+}
+
+template <int D, int QDT, int ODT>
+static void launch_kv8_waves(const Kv8Attn& a, const Kv8Plan& plan, bool cap, hipStream_t st) {
+  if (plan.waves == 8) launch_kv8_attn<D, QDT, ODT, 8>(a, cap, st);
+  else launch_kv8_attn<D, QDT, ODT, 4>(a, cap, st);
 }
 
 template <int D>
 static void launch_kv8_chunk(const Kv8Attn& a, bool cap, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.tiles * a.c.B * a.Hq), static_cast<unsigned>(a.nsplit));
-  if (cap && a.slopes) kv8_chunk_kernel<D, true, true><<<grid, 256, 0, st>>>(a);
-  else if (cap) kv8_chunk_kernel<D, true, false><<<grid, 256, 0, st>>>(a);
-  else if (a.slopes) kv8_chunk_kernel<D, false, true><<<grid, 256, 0, st>>>(a);
-  else kv8_chunk_kernel<D, false, false><<<grid, 256, 0, st>>>(a);
+  const int64_t turns = a.S / 128 * a.nfull + (a.S % 128 ? a.nsplit : 0);
+  const dim3 grid(static_cast<unsigned>(turns * a.c.B * a.Hq));
+  if (cap && a.slopes) kv8_chunk_kernel<D, true, true><<<grid, 512, 0, st>>>(a);
+  else if (cap) kv8_chunk_kernel<D, true, false><<<grid, 512, 0, st>>>(a);
+  else if (a.slopes) kv8_chunk_kernel<D, false, true><<<grid, 512, 0, st>>>(a);
+  else kv8_chunk_kernel<D, false, false><<<grid, 512, 0, st>>>(a);
 }
 
 template <int D>
@@ -886,14 +1034,15 @@ static void dispatch_kv8_attn(const Kv8Attn& a, const Kv8Plan& plan, bool cap, i
   if (plan.chunk) {
     if constexpr (D <= 128) launch_kv8_chunk<D>(a, cap, st);
   } else if (qdt == RK_F32) {
-    if (odt == RK_F32) launch_kv8_attn<D, RK_F32, RK_F32>(a, cap, st);
-    else launch_kv8_attn<D, RK_F32, RK_BF16>(a, cap, st);
+    if (odt == RK_F32) launch_kv8_waves<D, RK_F32, RK_F32>(a, plan, cap, st);
+    else launch_kv8_waves<D, RK_F32, RK_BF16>(a, plan, cap, st);
   } else {
-    if (odt == RK_F32) launch_kv8_attn<D, RK_BF16, RK_F32>(a, cap, st);
-    else launch_kv8_attn<D, RK_BF16, RK_BF16>(a, cap, st);
+    if (odt == RK_F32) launch_kv8_waves<D, RK_BF16, RK_F32>(a, plan, cap, st);
+    else launch_kv8_waves<D, RK_BF16, RK_BF16>(a, plan, cap, st);
   }
   if (a.nsplit > 1) {
-    const dim3 grid(static_cast<unsigned>(a.S * a.G), static_cast<unsigned>(a.c.B * a.c.H));
+    const dim3 grid(static_cast<unsigned>(a.S * a.G - a.col0),
+                    static_cast<unsigned>(a.c.B * a.c.H));
     if (odt == RK_F32) kv8_join_kernel<D, RK_F32><<<grid, D / 4, 0, st>>>(a);
     else kv8_join_kernel<D, RK_BF16><<<grid, D / 4, 0, st>>>(a);
   }
@@ -975,8 +1124,9 @@ extern "C" int rk_int8_kv_read(const rk_int8_kv* cache, int64_t begin, int64_t e
 extern "C" int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S,
                                              int qdtype, int odtype) {
   if (!cache || cache->B <= 0 || cache->H <= 0 || Hq <= 0 || S <= 0 || Hq % cache->H) return 0;
-  const int64_t n = attention_plan(*cache, Hq, S, qdtype, odtype).splits;
-  return n == 1 ? 0 : cache->B * Hq * S * n * (cache->D + 4);
+  const Kv8Plan p = attention_plan(*cache, Hq, S, qdtype, odtype);
+  return p.splits == 1 ? 0
+                       : cache->B * (Hq * S - cache->H * p.col0) * p.splits * (cache->D + 4);
 }
 
 extern "C" int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int qdtype, int64_t sqb,
@@ -1022,7 +1172,7 @@ extern "C" int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int 
     return fail(RK_ERR_ARG, "attention workspace too small");
   const bool cap = softcap > 0.0f;
   Kv8Attn a{cache_args(c), q, sqb, sqh, sqs, start, lengths, slopes, start_count > 1 ? 1 : 0, S,
-            Hq, G, n, plan.tiles,
+            Hq, G, n, plan.tiles, plan.full_splits, plan.col0,
             cap ? 2.0f * kLog2e8 * (scale / softcap) : scale * kLog2e8, softcap * kLog2e8, work,
             out};
   hipStream_t st = as_stream(stream);

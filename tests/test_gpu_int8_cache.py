@@ -1,16 +1,18 @@
 """The 8-bit key/value cache against plain forms: its codes to the last one (float32 quotients are
 IEEE on either side), its attention against 64 bits over the values the codes stand for.
 
-Tolerance of the attention. A query is rounded to 2^-24 of its largest feature, the float32
-combination of its digits' sums to 2^-22 of |q| . |k| <= max|q| sum|k|, a capped score to 2^-21 of
-the cap and the scaled, biased score to 2^-21 of itself and of the bias: a score is off by at most
-    delta = 2^-21 (scale max|q| sum|k| + |s| + cap + slope |i - j|),
+Tolerance of the attention. Queries and probabilities are fixed-point numbers of r = 23 bits for
+float32 results and 15 for bfloat16 ones (127 256^2 and 127 256 steps, so half a step is below
+2^-(r + 1) of the largest). A query is off by that of its row's largest feature, the float32
+combination of its digits' sums by 2^-22 of |q| . |k| <= max|q| sum|k|, a capped score by 2^-21 of
+the cap and the scaled, biased score by 2^-21 of itself and of the bias: a score is off by at most
+    delta = (2^-21 + 2^-(r + 1)) scale max|q| sum|k| + 2^-21 (|s| + cap + slope |i - j|),
 a probability by 2 max(delta) of itself, plus 2^-20 for the exponentials and sums. The fixed-point
-probabilities are off by 2^-24 of their block's largest each, over 64 tokens 2^-18 of the values'
-largest. bfloat16 results are rounded once, by 2^-8 of themselves. Chunks of 32 bfloat16 tokens and
-more with bfloat16 results take bfloat16 products: each probability times its block's value scale
-is rounded to bfloat16, by at most 2^-8 of itself, which moves a result by at most 2^-8 of the sum
-of p |v| more (the codes and the queries enter as they are)."""
+probabilities are off by 2^-(r + 1) of their block's largest each, over 64 tokens 2^(5 - r) of the
+values' largest. bfloat16 results are rounded once, by 2^-8 of themselves. Chunks of 32 bfloat16
+tokens and more with bfloat16 results take bfloat16 products: each probability times its block's
+value scale is rounded to bfloat16, by at most 2^-8 of itself, which moves a result by at most
+2^-8 of the sum of p |v| more (the codes and the queries enter as they are)."""
 
 from __future__ import annotations
 
@@ -147,6 +149,7 @@ def check_attention(q, cache, start, lengths=None, cap=0.0, slopes=None, out_dty
     group = q.shape[1] // keys.shape[1]
     keys, values = (t.repeat_interleave(group, dim=1) for t in (keys, values))
     step = torch.finfo(got.dtype).eps / 2
+    r = 23 if got.dtype == torch.float32 else 15
     rounded = q.dtype == got.dtype == torch.bfloat16 and q.shape[2] >= 32 and q.shape[3] <= 128
     for b in range(q.shape[0]):
         p0 = int(start[b % len(start)])
@@ -165,13 +168,13 @@ def check_attention(q, cache, start, lengths=None, cap=0.0, slopes=None, out_dty
             s = cap * torch.tanh(s / cap)
         bias = slopes.double()[:, None, None] * dist.abs() if slopes is not None else 0.0
         s = s - bias
-        delta = 2.0**-21 * (scale * x.abs().amax(-1, keepdim=True)
-                            * k.abs().sum(-1)[:, None] + s.abs() + cap + bias)
+        products = scale * x.abs().amax(-1, keepdim=True) * k.abs().sum(-1)[:, None]
+        delta = 2.0**-21 * (products + s.abs() + cap + bias) + 2.0**-(r + 1) * products
         unseen = dist < 0
         p = s.masked_fill(unseen, -math.inf).softmax(-1)
         want = p @ v
         bound = ((2 * delta.masked_fill(unseen, 0.0).amax(-1, keepdim=True) + 2.0**-20
-                  + (2.0**-8 if rounded else 0.0)) * (p @ v.abs()) + 2.0**-18 * v.abs().amax() + step * want.abs())
+                  + (2.0**-8 if rounded else 0.0)) * (p @ v.abs()) + 2.0**(5 - r) * v.abs().amax() + step * want.abs())
         worst = ((got[b, :, :n].double() - want).abs() - bound).max().item()
         assert worst <= 0.0, (b, p0, worst)
 
