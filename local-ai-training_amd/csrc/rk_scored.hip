@@ -198,12 +198,14 @@ void scored_fwd_kernel(ScoredArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The plan: one workgroup per row, each thread 8 consecutive positions of a chunk of 8192, scans
-// over the threads' values by wavefront shuffles. The first pass takes, from the left, the
-// document's first position and whether the run of marked positions it begins with reaches here;
-// the second, from the right, the document's end and the end of that run.
+// The plan: one workgroup per row, a thread 8 consecutive positions of a chunk of 8 * NT, scans over
+// the threads' values by wavefront shuffles. From the left: the document's first position and
+// whether the run of marked positions it begins with reaches here; from the right: the
+// document's end and the end of that run. Up to one chunk the first pass stays in registers.
+// (In 8-byte loads and stores of one position each, and through memory between the passes, a row
+// of 8192 positions took 39 us; MMM us this way.)
 // ---------------------------------------------------------------------------
-constexpr int kMaskThreads = 1024, kMaskEach = 8, kMaskChunk = kMaskThreads * kMaskEach;
+constexpr int kMaskEach = 8;
 
 struct MaskArgs {
   const void* documents;  // int32 or int64 [B, S], or null (one document per row)
@@ -215,31 +217,38 @@ struct MaskArgs {
   uint8_t* padding;       // [B][S32][4]
 };
 
-// Inclusive max scan over the threads of the workgroup, left to right, two values at once;
-// returns the values before this thread (exclusive) and the totals. box: 32 ints.
+// Two max scans over the threads of the workgroup, left to right or (BACK) right to left: each
+// thread's x, y become those of the threads before it, tx, ty those of all. box: 2 NT / 64 ints.
+template <int NT, bool BACK>
 __device__ __forceinline__ void block_scan_max(int& x, int& y, int& tx, int& ty, int* box, int tid) {
+  constexpr int NW = NT / 64, kNone = -0x7fffffff;
   const int lane = tid & 63, wave = tid >> 6;
+  const int turn = BACK ? 63 - lane : lane, place = BACK ? NW - 1 - wave : wave;
+  const auto before = [&](int v, int d) {
+    return BACK ? __shfl_down(v, d, 64) : __shfl_up(v, d, 64);
+  };
   int a = x, c = y;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int oa = __shfl_up(a, d, 64), oc = __shfl_up(c, d, 64);
-    if (lane >= d) {
+    const int oa = before(a, d), oc = before(c, d);
+    if (turn >= d) {
       a = a > oa ? a : oa;
       c = c > oc ? c : oc;
     }
   }
   __syncthreads();
-  if (lane == 63) {
-    box[wave] = a;
-    box[16 + wave] = c;
+  if (turn == 63) {
+    box[place] = a;
+    box[NW + place] = c;
   }
   __syncthreads();
-  int ea = __shfl_up(a, 1, 64), ec = __shfl_up(c, 1, 64);
-  if (lane == 0) ea = ec = -0x7fffffff;
-  tx = ty = -0x7fffffff;
-  for (int w = 0; w < kMaskThreads / 64; ++w) {
-    const int ba = box[w], bc = box[16 + w];
-    if (w < wave) {
+  int ea = before(a, 1), ec = before(c, 1);
+  if (turn == 0) ea = ec = kNone;
+  tx = ty = kNone;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const int ba = box[w], bc = box[NW + w];
+    if (w < place) {
       ea = ea > ba ? ea : ba;
       ec = ec > bc ? ec : bc;
     }
@@ -250,39 +259,92 @@ __device__ __forceinline__ void block_scan_max(int& x, int& y, int& tx, int& ty,
   y = ec;
 }
 
+// 4-byte aligned vectors (rows of any length)
+typedef int32_t v4i_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef int64_t v2l_u __attribute__((ext_vector_type(2), aligned(8)));
+
 __device__ __forceinline__ int64_t document_of(const MaskArgs& a, int64_t b, int64_t i) {
   if (!a.documents) return 0;
   return a.wide ? static_cast<const int64_t*>(a.documents)[b * a.sdb + i]
                 : static_cast<const int32_t*>(a.documents)[b * a.sdb + i];
 }
 
-__global__ __launch_bounds__(kMaskThreads) void attention_mask_kernel(MaskArgs a) {
-  __shared__ int box[32];
+// Ids of positions i0 .. i0 + 7 (-1 past the row).
+__device__ __forceinline__ void documents_of(const MaskArgs& a, int64_t b, int i0, int S,
+                                             int64_t (&id)[kMaskEach]) {
+  if (a.documents && i0 + kMaskEach <= S) {
+    if (a.wide) {
+      const int64_t* at = static_cast<const int64_t*>(a.documents) + b * a.sdb + i0;
+#pragma unroll
+      for (int e = 0; e < kMaskEach; e += 2) {
+        const v2l_u v = *reinterpret_cast<const v2l_u*>(at + e);
+        id[e] = v.x;
+        id[e + 1] = v.y;
+      }
+    } else {
+      const int32_t* at = static_cast<const int32_t*>(a.documents) + b * a.sdb + i0;
+#pragma unroll
+      for (int e = 0; e < kMaskEach; e += 4) {
+        const v4i_u v = *reinterpret_cast<const v4i_u*>(at + e);
+        id[e] = v.x;
+        id[e + 1] = v.y;
+        id[e + 2] = v.z;
+        id[e + 3] = v.w;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kMaskEach; ++e) id[e] = i0 + e < S ? document_of(a, b, i0 + e) : -1;
+  }
+}
+
+__device__ __forceinline__ void store8(int32_t* to, const int (&v)[kMaskEach], int n) {
+  if (n >= kMaskEach) {
+    *reinterpret_cast<v4i_u*>(to) = v4i_u{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<v4i_u*>(to + 4) = v4i_u{v[4], v[5], v[6], v[7]};
+  } else {
+#pragma unroll
+    for (int e = 0; e < kMaskEach; ++e)
+      if (e < n) to[e] = v[e];
+  }
+}
+
+template <int NT>
+__global__ __launch_bounds__(NT) void attention_mask_kernel(MaskArgs a) {
+  constexpr int CHUNK = NT * kMaskEach, kNone = -0x7fffffff;
+  __shared__ int box[2 * NT / 64];
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, S = static_cast<int>(a.S);
+  const int chunks = (S + CHUNK - 1) / CHUNK;
   int32_t* const key_lo = a.bounds + b * a.S;
   int32_t* const key_hi = key_lo + a.B * a.S;
   int32_t* const query_lo = key_hi + a.B * a.S;
   int32_t* const query_hi = query_lo + a.B * a.S;
-  // left to right: key_lo = the document's first position, key_hi = 1 in its marked beginning
+  // left to right: the document's first position; bits: marked beginning, not padding
+  int lo[kMaskEach] = {};
+  uint32_t lead = 0, real = 0;
   int begin0 = 0, broken0 = -1;
-  for (int c0 = 0; c0 < S; c0 += kMaskChunk) {
-    const int i0 = c0 + tid * kMaskEach;
-    int begin[kMaskEach], broken[kMaskEach];
-    uint32_t real = 0;
-    int bx = -0x7fffffff, by = -0x7fffffff;
+  for (int c = 0; c < chunks; ++c) {
+    const int i0 = c * CHUNK + tid * kMaskEach;
+    int broken[kMaskEach] = {};
+    int bx = kNone, by = kNone;
+    lead = real = 0;
     if (i0 < S) {
+      int64_t id[kMaskEach];
+      documents_of(a, b, i0, S, id);
       int64_t before = i0 > 0 ? document_of(a, b, i0 - 1) : 0;
+      uint32_t marks = 0;
+#pragma unroll
+      for (int e = 0; e < kMaskEach; ++e)
+        marks |= static_cast<uint32_t>(a.prefix && i0 + e < S && a.prefix[b * a.spb + i0 + e]) << e;
 #pragma unroll
       for (int e = 0; e < kMaskEach; ++e) {
         const int i = i0 + e;
-        const int64_t id = i < S ? document_of(a, b, i) : -1;
-        const bool mark = i < S && a.prefix && a.prefix[b * a.spb + i];
-        if (i == 0 || id != before) bx = i;
-        if (!mark) by = i;
-        before = id;
-        real |= static_cast<uint32_t>(id >= 0) << e;
-        begin[e] = bx;
+        if (i == 0 || id[e] != before) bx = i;
+        if (!(marks >> e & 1)) by = i;
+        before = id[e];
+        real |= static_cast<uint32_t>(i < S && id[e] >= 0) << e;
+        lo[e] = bx;
         broken[e] = by;
       }
     }
@@ -291,61 +353,65 @@ __global__ __launch_bounds__(kMaskThreads) void attention_mask_kernel(MaskArgs a
       a.padding[b * a.S32 * 4 + i0 / 8] = static_cast<uint8_t>(~real & inside);
     }
     int ex = bx, ey = by, tx, ty;
-    block_scan_max(ex, ey, tx, ty, box, tid);
+    block_scan_max<NT, false>(ex, ey, tx, ty, box, tid);
     ex = ex > begin0 ? ex : begin0;
     ey = ey > broken0 ? ey : broken0;
 #pragma unroll
     for (int e = 0; e < kMaskEach; ++e) {
-      const int i = i0 + e;
-      if (i >= S) break;
-      const int bg = begin[e] > ex ? begin[e] : ex, br = broken[e] > ey ? broken[e] : ey;
-      const bool lead = br < bg;
-      key_lo[i] = bg;
-      key_hi[i] = lead;
-      query_lo[i] = lead ? bg : i;
-      query_hi[i] = real >> e & 1;
+      lo[e] = lo[e] > ex ? lo[e] : ex;
+      const int br = broken[e] > ey ? broken[e] : ey;
+      lead |= static_cast<uint32_t>(br < lo[e]) << e;
     }
     begin0 = tx > begin0 ? tx : begin0;
     broken0 = ty > broken0 ? ty : broken0;
+    if (chunks > 1) {  // the same thread takes them up again
+      store8(key_lo + i0, lo, S - i0);
+      if (i0 < S) key_hi[i0] = static_cast<int>(lead | real << 8);
+    }
   }
-  // right to left, as a max scan over mirrored positions: the least later position where a
-  // document begins (its end), and where one begins or the marked run is over.
-  __syncthreads();
+  // right to left, as a max scan of negated positions: the least later position where a
+  // document begins (its end), and where one begins or the marked run is over
   int end0 = -S, stop0 = -S;
-  for (int c0 = 0; c0 < S; c0 += kMaskChunk) {
-    const int i0 = S - 1 - c0 - tid * kMaskEach;  // positions i0, i0 - 1, ..
-    int end[kMaskEach], stop[kMaskEach], lo[kMaskEach], lead[kMaskEach], real[kMaskEach];
-    int bx = -0x7fffffff, by = -0x7fffffff;
+  for (int c = chunks - 1; c >= 0; --c) {
+    const int i0 = c * CHUNK + tid * kMaskEach;
+    if (chunks > 1 && i0 < S) {
 #pragma unroll
-    for (int e = 0; e < kMaskEach; ++e) {
-      const int i = i0 - e;
+      for (int e = 0; e < kMaskEach; ++e) lo[e] = i0 + e < S ? key_lo[i0 + e] : 0;
+      lead = static_cast<uint32_t>(key_hi[i0]);
+      real = lead >> 8;
+    }
+    int end[kMaskEach], stop[kMaskEach];
+    int bx = kNone, by = kNone;
+#pragma unroll
+    for (int e = kMaskEach - 1; e >= 0; --e) {
+      const int i = i0 + e;
       end[e] = bx;  // over the later positions of this thread
       stop[e] = by;
-      lo[e] = lead[e] = real[e] = 0;
-      if (i >= 0) {
-        lo[e] = key_lo[i];
-        lead[e] = key_hi[i];
-        real[e] = query_hi[i];
-        const bool begins = lo[e] == i;
-        if (begins) bx = -i;
-        if (begins || !lead[e]) by = -i;
+      if (i < S) {
+        if (lo[e] == i) bx = -i;
+        if (lo[e] == i || !(lead >> e & 1)) by = -i;
       }
     }
     int ex = bx, ey = by, tx, ty;
-    block_scan_max(ex, ey, tx, ty, box, tid);
+    block_scan_max<NT, true>(ex, ey, tx, ty, box, tid);
     ex = ex > end0 ? ex : end0;
     ey = ey > stop0 ? ey : stop0;
+    int v[4][kMaskEach];
 #pragma unroll
     for (int e = 0; e < kMaskEach; ++e) {
-      const int i = i0 - e;
-      if (i < 0) break;
+      const int i = i0 + e;
       const int en = -(end[e] > ex ? end[e] : ex), st = -(stop[e] > ey ? stop[e] : ey);
-      if (real[e]) {
-        key_hi[i] = lead[e] ? st : i + 1;
-        query_hi[i] = en;
-      } else {
-        key_lo[i] = key_hi[i] = query_lo[i] = query_hi[i] = 0;
-      }
+      const bool r = real >> e & 1, ld = lead >> e & 1;
+      v[0][e] = r ? lo[e] : 0;
+      v[1][e] = r ? (ld ? st : i + 1) : 0;
+      v[2][e] = r ? (ld ? lo[e] : i) : 0;
+      v[3][e] = r ? en : 0;
+    }
+    if (i0 < S) {
+      store8(key_lo + i0, v[0], S - i0);
+      store8(key_hi + i0, v[1], S - i0);
+      store8(query_lo + i0, v[2], S - i0);
+      store8(query_hi + i0, v[3], S - i0);
     }
     end0 = tx > end0 ? tx : end0;
     stop0 = ty > stop0 ? ty : stop0;
@@ -447,6 +513,8 @@ extern "C" int rk_attention_mask(const void* documents, int wide, int64_t sdb,
   const int64_t S32 = (S + 31) / 32;
   MaskArgs a{documents, wide, prefix, sdb, spb, B, S, S32, bounds,
              reinterpret_cast<uint8_t*>(padding)};
-  attention_mask_kernel<<<static_cast<unsigned>(B), kMaskThreads, 0, as_stream(stream)>>>(a);
+  const unsigned grid = static_cast<unsigned>(B);
+  if (S <= 256 * kMaskEach) attention_mask_kernel<256><<<grid, 256, 0, as_stream(stream)>>>(a);
+  else attention_mask_kernel<1024><<<grid, 1024, 0, as_stream(stream)>>>(a);
   return launch_status("attention_mask");
 }

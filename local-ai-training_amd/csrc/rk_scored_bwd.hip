@@ -218,19 +218,23 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   }
 }
 
-// dslope[h] = -sum over the sequences and queries, in 64 bits and a fixed order.
-__global__ __launch_bounds__(256) void scored_slope_kernel(ScoredBwdArgs ba) {
-  __shared__ double red[256];
+// dslope[h] = -sum over the sequences and queries, in 64 bits and a fixed order; four loads in
+// flight.
+__global__ __launch_bounds__(1024) void scored_slope_kernel(ScoredBwdArgs ba) {
+  __shared__ double red[1024];
   const ScoredArgs& a = ba.f;
   const int64_t hd = blockIdx.x;
   const int tid = threadIdx.x;
   double sum = 0.0;
   for (int64_t b = 0; b < a.p.B; ++b) {
     const float* rows = ba.slope_rows + (b * a.p.H + hd) * a.Sp;
-    for (int64_t i = tid; i < a.Sp; i += 256) sum += rows[i];
+    for (int64_t i = 4 * tid; i < a.Sp; i += 4096) {  // Sp is a multiple of 128
+      const float4 x = *reinterpret_cast<const float4*>(rows + i);
+      sum += (static_cast<double>(x.x) + x.y) + (static_cast<double>(x.z) + x.w);
+    }
   }
   red[tid] = sum;
-  for (int n = 128; n > 0; n >>= 1) {
+  for (int n = 512; n > 0; n >>= 1) {
     __syncthreads();
     if (tid < n) red[tid] += red[tid + n];
   }
@@ -474,7 +478,7 @@ static void launch_scored_bwd(const ScoredBwdArgs& a, hipStream_t st) {
   const dim3 kgrid(static_cast<unsigned>(p.B * p.Hkv * a.parts) * blocks);
   if (BIAS && a.slope_rows) {
     scored_dq_kernel<D, CAP, BIAS, BIAS><<<qgrid, 256, 0, st>>>(a);
-    scored_slope_kernel<<<static_cast<unsigned>(p.H), 256, 0, st>>>(a);
+    scored_slope_kernel<<<static_cast<unsigned>(p.H), 1024, 0, st>>>(a);
   } else {
     scored_dq_kernel<D, CAP, BIAS, false><<<qgrid, 256, 0, st>>>(a);
   }
