@@ -85,6 +85,15 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   const int end = lo < hi ? (hi + kBwdRows - 1) / kBwdRows : 0;
   const uint32_t width = static_cast<uint32_t>(span.hi - span.lo);
 
+  const TileDma<D, kBwdRows> kd(p.k + b * p.skb + kvh * p.skh, p.sks, S, wave, lane);
+  const TileDma<D, kBwdRows> vd(p.v + b * p.svb + kvh * p.svh, p.svs, S, wave, lane);
+  auto issue = [&](int step) {
+    const uint32_t st = lds0 + (step & 1) * 2 * T::BYTES;
+    kd.issue(st, step * kBwdRows, wave);
+    vd.issue(st + T::BYTES, step * kBwdRows, wave);
+  };
+  if (first < end) issue(first);  // under way while delta is formed
+
   // delta of this lane's query: half of the features here, the other half in lane ^ 32
   float dot = 0.0f;
   {
@@ -120,19 +129,10 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   float slope2 = 0.0f;
   if constexpr (BIAS) slope2 = p.slopes[hd] * kLog2e;
 
-  const TileDma<D, kBwdRows> kd(p.k + b * p.skb + kvh * p.skh, p.sks, S, wave, lane);
-  const TileDma<D, kBwdRows> vd(p.v + b * p.svb + kvh * p.svh, p.svs, S, wave, lane);
-  auto issue = [&](int step) {
-    const uint32_t st = lds0 + (step & 1) * 2 * T::BYTES;
-    kd.issue(st, step * kBwdRows, wave);
-    vd.issue(st + T::BYTES, step * kBwdRows, wave);
-  };
-
   v16f_a dq[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) dq[dt] = v16f_a{};
   float s_pd = 0.0f, s_pa = 0.0f, s_pda = 0.0f;  // sums of p dp, p |i - j|, p dp |i - j|
-  if (first < end) issue(first);
   for (int step = first; step < end; ++step) {
     const uint64_t pad = padding_bits<kBwdRows>(a, b, step * kBwdRows);
     dma_wait_barrier<0>();
