@@ -19,7 +19,9 @@ equal what the training kernels compute for the same float rows (``rk_rmsnorm_qu
 equal ``rk_int8_gemm_packed``'s; the attention runs in float32 with its positions split
 across workgroups, so its result differs from the window forward's attention only by
 float summation order. Every kernel reads the position from ``cache.pos`` on the device,
-so the step can be captured once as a HIP graph and replayed.
+so the step can be captured once as a HIP graph and replayed. With an 8-bit cache the
+attention's launches are those of ``int8_cache.py`` (append, attention, and their join for long
+caches), which also take capped and biased scores.
 """
 
 from __future__ import annotations
@@ -30,6 +32,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _native as nat
+from .int8_cache import int8_kv_append, int8_kv_attention
 from .ratchet import DiscreteRatchetLinear
 
 PRO_INT8, PRO_PLAIN, PRO_RMSNORM = 0, 1, 2
@@ -73,6 +76,23 @@ def decode_attention(qkv: Tensor, keys: Tensor, values: Tensor, pos: Tensor, n_h
     return out
 
 
+def _int8_cache():
+    from .model import Int8KVCache
+
+    return Int8KVCache
+
+
+def int8_decode_attention(qkv: Tensor, store, pos: Tensor, attention) -> Tensor:
+    """The same over an 8-bit cache (``int8_cache.py``), with the layer's cap and bias: appends
+    this step's k, v, returns the attention rows [B, H*D] float32."""
+    batch, heads, _, _, head = store.keys.shape
+    q, k, v = (t.view(batch, 1, heads, head).transpose(1, 2) for t in qkv.chunk(3, dim=1))
+    int8_kv_append(store, k, v, pos)
+    out = int8_kv_attention(q, store, pos, softcap=attention.softcap, slopes=attention.slopes,
+                            out_dtype=torch.float32)
+    return out.transpose(1, 2).reshape(batch, heads * head)
+
+
 def decode_greedy(logits: Tensor, tokens: Tensor, pos: Tensor | None = None) -> Tensor:
     """tokens[b, 0] = argmax of logits row b (torch.argmax's pick: the first largest value,
     NaN above every number), then ``pos += 1`` when `pos` is given: the greedy choice of
@@ -111,6 +131,8 @@ def fused_decode_supported(model, cache) -> bool:
     config = model.config
     if cache.device.type != "cuda" or cache.batch > MAX_ROWS or model.training:
         return False
+    if config.modified_scores and not isinstance(cache, _int8_cache()):
+        return False  # capped and biased scores are read from the 8-bit cache
     if not isinstance(model.token_embedding, nn.Embedding):
         return False
     if model.token_embedding.weight.dtype != torch.float32:
@@ -161,6 +183,7 @@ def fused_decode_logits(model, tokens: Tensor, cache) -> Tensor:
         ids = bufs["tokens"]
         ids.copy_(tokens.reshape(batch))
     hidden, qkv, ffn = bufs["hidden"], bufs["qkv"], bufs["ffn"]
+    int8 = isinstance(cache, _int8_cache())
     stream = nat.stream_handle(hidden.device)
     table = model.token_embedding.weight
     positions = model.position_encoding
@@ -171,9 +194,12 @@ def fused_decode_logits(model, tokens: Tensor, cache) -> Tensor:
         attention, feed_forward = block.attention, block.feed_forward
         decode_gemv(attention.qkv, qkv, prologue=PRO_RMSNORM, epilogue=EPI_STORE, x=hidden,
                     norm_weight=block.attention_norm.weight, eps=BLOCK_NORM_EPS)
-        keys, values = cache.buffers(index, qkv)
-        att = decode_attention(qkv, keys, values, cache.pos, config.n_head, bufs["work"],
-                               bufs["attn"])
+        if int8:
+            att = int8_decode_attention(qkv, cache.store(index), cache.pos, attention)
+        else:
+            keys, values = cache.buffers(index, qkv)
+            att = decode_attention(qkv, keys, values, cache.pos, config.n_head, bufs["work"],
+                                   bufs["attn"])
         decode_gemv(attention.projection, hidden, prologue=PRO_PLAIN, epilogue=EPI_ADD, x=att)
         decode_gemv(feed_forward.expand, ffn, prologue=PRO_RMSNORM, epilogue=EPI_GELU,
                     x=hidden, norm_weight=block.feed_forward_norm.weight, eps=BLOCK_NORM_EPS)

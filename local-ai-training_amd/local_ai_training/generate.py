@@ -25,7 +25,7 @@ import torch
 from torch import Tensor
 
 from .decode import decode_greedy
-from .model import KVCache, ModelConfig, RatchetGPT, build_seeded_model
+from .model import Int8KVCache, KVCache, ModelConfig, RatchetGPT, build_seeded_model
 from .ratchet import DiscreteRatchetLinear
 
 
@@ -121,11 +121,17 @@ class DecodeGraph:
     def __init__(self, model: RatchetGPT, cache: KVCache, greedy: bool = False) -> None:
         self.model, self.cache, self.greedy = model, cache, greedy
         self.tokens = torch.zeros((cache.batch, 1), dtype=torch.long, device=cache.device)
-        # warm-up step (allocates the cache buffers), then undo its position advance
+        # warm-up step (allocates the cache buffers), then undo its position advance. Into an
+        # 8-bit cache it appends nothing (position -1): its token could raise a block's scale.
         stream = torch.cuda.Stream(device=cache.device)
         stream.wait_stream(torch.cuda.current_stream(cache.device))
+        position = cache.pos.clone() if isinstance(cache, Int8KVCache) else None
         with torch.cuda.stream(stream), torch.no_grad():
+            if position is not None:
+                cache.pos.fill_(-1)
             model.decode_logits(self.tokens, cache)
+            if position is not None:
+                cache.pos.copy_(position)
         torch.cuda.current_stream(cache.device).wait_stream(stream)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph), torch.no_grad():
@@ -187,10 +193,12 @@ def generate(
     seed: int | None = None,
     device: str | torch.device | None = None,
     use_graph: bool = False,
+    cache_dtype: torch.dtype | None = None,
 ) -> str:
     """Sample `max_new_tokens` characters continuing `prompt` and return only the new text
     (``generate.py:135-206``: same arguments, validation and sampling). `use_graph` replays
-    the decode step as a HIP graph (GPU only)."""
+    the decode step as a HIP graph (GPU only); `cache_dtype` is the key/value cache's
+    (``RatchetGPT.new_cache``: e.g. torch.bfloat16, or torch.int8 for codes with scales)."""
     if max_new_tokens < 0:
         raise ValueError("max_new_tokens must be non-negative")
     if temperature < 0:
@@ -205,7 +213,7 @@ def generate(
     # an empty prompt starts from token 0, so there is always a position to predict from
     history = [index[character] for character in prompt] or [0]
     history = history[-window:]
-    cache = model.new_cache(1)
+    cache = model.new_cache(1, dtype=cache_dtype)
     logits = model.prefill(torch.tensor([history], dtype=torch.long, device=device), cache)
     graph: DecodeGraph | None = None
     produced: list[int] = []

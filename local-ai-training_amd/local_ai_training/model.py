@@ -7,7 +7,10 @@ update fused into backward. In ``matmul_mode="int8"`` the RMSNorm / GELU / head-
 prologues quantize on the GPU and hand int8 rows straight to the ratchet GEMMs.
 
 Additions: ``ffn_hidden`` (default ``4 * n_embd``, the reference's hard-coded width,
-``model.py:137``) so 1B-class shapes with FFN 5632 can be built.
+``model.py:137``) so 1B-class shapes with FFN 5632 can be built; ``attention_softcap`` and
+``distance_bias`` (scores capped by a tanh, and falling with the distance), masks of packed
+documents and their prefixes in ``forward`` (``scored_attention.py``), and a key/value cache in
+8 bits (``new_cache(dtype=torch.int8)``, ``int8_cache.py``).
 """
 
 from __future__ import annotations
@@ -23,6 +26,8 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from .attention import CausalAttentionFn, attention_supported
 from .cross_entropy import cross_entropy
+from .int8_cache import HEAD_SIZES as INT8_HEAD_SIZES
+from .int8_cache import Int8KV, int8_kv, int8_kv_append, int8_kv_attention
 from .int8_fused import (
     FusedGELUQuantizeFn,
     FusedRMSNormQuantizeFn,
@@ -30,6 +35,7 @@ from .int8_fused import (
     FusedTransposeQuantizeFn,
 )
 from .ratchet import DiscreteRatchetLinear, RatchetEmbedding, RatchetUpdateStats, UpdateQueue
+from .scored_attention import AttentionMask, scored_attention, torch_scores
 
 
 @dataclass(frozen=True)
@@ -53,6 +59,8 @@ class ModelConfig:
     qat: bool = False
     ratchet_embedding: bool = False
     ffn_hidden: int | None = None
+    attention_softcap: float = 0.0
+    distance_bias: bool = False
 
     def __post_init__(self) -> None:
         if min(self.vocab_size, self.block_size, self.n_layer, self.n_head, self.n_embd) <= 0:
@@ -65,8 +73,16 @@ class ModelConfig:
             raise ValueError("matmul_mode must be fp32, bf16, or int8")
         if self.ffn_hidden is not None and self.ffn_hidden <= 0:
             raise ValueError("ffn_hidden must be positive")
+        if not 0.0 <= self.attention_softcap < math.inf:
+            raise ValueError("attention_softcap must be finite and not negative")
+        if self.modified_scores and self.dropout:
+            raise ValueError("capped or biased scores take no attention dropout")
         if self.qat:
             raise ValueError("the QAT control arm is not part of the ratchet-linear build")
+
+    @property
+    def modified_scores(self) -> bool:
+        return self.attention_softcap > 0.0 or self.distance_bias
 
     @property
     def hidden_size(self) -> int:
@@ -208,6 +224,43 @@ class KVCache:
         self.pos.add_(steps)
 
 
+class Int8KVCache(KVCache):
+    """A KVCache whose keys and values are held in 8 bits (``int8_cache.py``): GPU only, head
+    sizes 64, 128 and 256. The attention of a prompt's first part reads the keys and values as
+    they are; what comes later reads the cache."""
+
+    def __init__(self, n_layer: int, batch: int, n_head: int, head_size: int, max_len: int,
+                 device: torch.device) -> None:
+        if torch.device(device).type != "cuda":
+            raise RuntimeError("an 8-bit cache requires CUDA (a ROCm GPU)")
+        if head_size not in INT8_HEAD_SIZES:
+            raise ValueError(f"an 8-bit cache takes head sizes {INT8_HEAD_SIZES}")
+        super().__init__(n_layer, batch, n_head, head_size, max_len, device, torch.int8)
+        self.stores: list[Int8KV | None] = [None] * n_layer
+
+    def store(self, layer: int) -> Int8KV:
+        """The layer's codes and scales, allocated on first use."""
+        if self.stores[layer] is None:
+            self.stores[layer] = int8_kv(self.batch, self.n_head, self.max_len, self.head_size,
+                                         self.device)
+        return self.stores[layer]
+
+    def buffers(self, layer: int, like: Tensor) -> tuple[Tensor, Tensor]:
+        raise TypeError("an 8-bit cache has no key and value tensors; see store()")
+
+    def append(self, layer: int, k: Tensor, v: Tensor) -> Int8KV:
+        """Writes k and v [B, H, S, D] at positions ``pos`` .. (the host's ``length``)."""
+        if self.length + k.shape[2] > self.max_len:
+            raise ValueError("KV cache is full")
+        store = self.store(layer)
+        int8_kv_append(store, k, v, self.pos)
+        return store
+
+    def stores_bf16(self, layer: int) -> bool:
+        # what it stores is rounded further: bf16 projections are handed over as they are
+        return True
+
+
 # causal training attention: the HIP kernels where they apply (attention.py; False: torch's)
 hip_attention_forward = True
 _FAST_ATTENTION = [SDPBackend.EFFICIENT_ATTENTION, SDPBackend.FLASH_ATTENTION]
@@ -296,13 +349,19 @@ class CausalSelfAttention(nn.Module):
         self.n_head = config.n_head
         self.head_size = config.n_embd // config.n_head
         self.dropout = config.dropout
+        self.softcap = config.attention_softcap
+        slopes = None
+        if config.distance_bias:
+            # a fixed slope per head, falling geometrically from 2^(-8 / n_head) to 2^-8
+            slopes = torch.exp2(torch.arange(1, config.n_head + 1) * (-8.0 / config.n_head))
+        self.register_buffer("slopes", slopes, persistent=False)
 
     def forward(self, inputs: Tensor, *, inputs_int8: Tensor | None = None,
                 inputs_scale: Tensor | None = None, cache: KVCache | None = None,
-                layer: int = 0, decode: bool = False,
+                layer: int = 0, decode: bool = False, mask: AttentionMask | None = None,
                 residual: Tensor | None = None) -> Tensor:
         """``residual``: return residual + attention output (int8 projection: added in the
-        GEMM epilogue)."""
+        GEMM epilogue). ``mask``: the documents of the batch (``attention_mask``)."""
         batch_size, sequence_length, channels = inputs.shape
         projection_kw = {}
         if inputs_int8 is not None:
@@ -331,7 +390,11 @@ class CausalSelfAttention(nn.Module):
         q, k, v = heads(query), heads(key), heads(value)
         dropout_p = self.dropout if self.training else 0.0
         if cache is not None:
-            attended = self._cached_attention(q, k, v, cache, layer, decode)
+            attended = self._cached_attention(q, k, v, cache, layer, decode, mask)
+        elif self._scored(mask):
+            if dropout_p:
+                raise ValueError("a masked attention takes no dropout")
+            attended = self._score(q, k, v, mask)
         else:
             attended = _attend(q, k, v, dropout_p=dropout_p, is_causal=True)
         if _is_int8(self.projection):
@@ -342,31 +405,74 @@ class CausalSelfAttention(nn.Module):
         out = self.projection(joined)
         return out if residual is None else residual + out
 
+    def _scored(self, mask: AttentionMask | None) -> bool:
+        return mask is not None or self.softcap > 0.0 or self.slopes is not None
+
+    def _score(self, q: Tensor, k: Tensor, v: Tensor, mask: AttentionMask | None) -> Tensor:
+        """Attention with this layer's cap and bias under `mask`; in bfloat16 under autocast, as
+        the attention without them."""
+        cast = _autocast_bf16(q)
+        if cast is not None:
+            q, k, v = q.to(cast), k.to(cast), v.to(cast)
+        return scored_attention(q, k, v, mask=mask, softcap=self.softcap, slopes=self.slopes)
+
     def _cached_attention(self, q: Tensor, k: Tensor, v: Tensor, cache: KVCache, layer: int,
-                          decode: bool) -> Tensor:
+                          decode: bool, mask: AttentionMask | None = None) -> Tensor:
         """Attention of the new positions against the cache, after appending their keys and
         values. ``decode``: one token at the device-side position ``cache.pos``, attending
         over the whole buffer under a mask (fixed shapes); otherwise a prompt of S tokens
-        written at the host-side ``cache.length`` (causal among themselves)."""
+        written at the host-side ``cache.length`` (causal among themselves; ``mask``, at the
+        start of the cache only, as in training)."""
         out_dtype = q.dtype
+        scored = self._scored(mask)
+        start, length = cache.length, q.shape[2]
+        if mask is not None and (decode or start):
+            raise ValueError("a mask applies to a prompt at the start of the cache")
+        if isinstance(cache, Int8KVCache):
+            if decode:
+                store = cache.store(layer)
+                int8_kv_append(store, k, v, cache.pos)
+            else:
+                store = cache.append(layer, k, v)
+                if start == 0:
+                    out = self._score(q, k, v, mask) if scored else _attend(q, k, v,
+                                                                            is_causal=True)
+                    return out.to(out_dtype)
+            return int8_kv_attention(q, store, cache.pos, softcap=self.softcap,
+                                     slopes=self.slopes)
         if decode:
             keys, values = cache.buffers(layer, k)
             if keys.dtype != q.dtype:
                 q, k, v = q.to(keys.dtype), k.to(keys.dtype), v.to(keys.dtype)
             keys.index_copy_(2, cache.pos, k)
             values.index_copy_(2, cache.pos, v)
+            if scored:
+                return self._score_buffer(q, keys, values, cache.pos, cache._arange).to(out_dtype)
             out = _attend(q, keys, values, attn_mask=cache.decode_mask(q.dtype))
             return out.to(out_dtype)
-        start, length = cache.length, q.shape[2]
         end = start + length
         k, v, keys, values = cache.append(layer, k, v)
         if keys.dtype != q.dtype:
             q = q.to(keys.dtype)
         if start == 0:
+            if scored:
+                return self._score(q, k, v, mask).to(out_dtype)
             return _attend(q, k, v, is_causal=True).to(out_dtype)
+        if scored:
+            at = cache._arange[start:end]
+            return self._score_buffer(q, keys[:, :, :end], values[:, :, :end], at,
+                                      cache._arange[:end]).to(out_dtype)
         mask = torch.ones(length, end, dtype=torch.bool, device=q.device).tril(diagonal=start)
         out = _attend(q, keys[:, :, :end], values[:, :, :end], attn_mask=mask)
         return out.to(out_dtype)
+
+    def _score_buffer(self, q: Tensor, keys: Tensor, values: Tensor, at: Tensor,
+                      key_at: Tensor) -> Tensor:
+        """Capped and biased attention of positions `at` over a bf16 / float32 buffer, in torch
+        operations (the kernels for cached tokens read the 8-bit cache)."""
+        return torch_scores(q, keys, values, key_at[None, :] <= at[:, None],
+                            (at[:, None] - key_at[None, :]).abs(), self.softcap, self.slopes,
+                            1.0 / math.sqrt(self.head_size))
 
 
 class FeedForward(nn.Module):
@@ -435,8 +541,10 @@ class TransformerBlock(nn.Module):
         self.feed_forward = FeedForward(config, max_code=max_code)
 
     def forward(self, inputs: Tensor, *, cache: KVCache | None = None, layer: int = 0,
-                decode: bool = False) -> Tensor:
+                decode: bool = False, mask: AttentionMask | None = None) -> Tensor:
         kv = dict(cache=cache, layer=layer, decode=decode) if cache is not None else {}
+        if mask is not None:
+            kv["mask"] = mask
         fuse_grad = self.fuse_residual and self.fuse_residual_grad
         if _is_int8(self.attention.qkv):
             if fuse_grad:
@@ -537,8 +645,10 @@ class RatchetGPT(nn.Module):
             return False
         return not (self.hip_embedding_backward and _hip_lookup_config_ok(emb))
 
-    def forward(self, tokens: Tensor, targets: Tensor | None = None
-                ) -> tuple[Tensor, Tensor | None]:
+    def forward(self, tokens: Tensor, targets: Tensor | None = None, *,
+                mask: AttentionMask | None = None) -> tuple[Tensor, Tensor | None]:
+        """``mask``: the documents the rows hold, and their prefixes (``attention_mask``; padding
+        positions attend to nothing, and are left out of the loss by targets of -100)."""
         if tokens.ndim != 2:
             raise ValueError("tokens must have shape (batch, sequence)")
         sequence_length = tokens.shape[1]
@@ -551,13 +661,14 @@ class RatchetGPT(nn.Module):
         else:
             looked_up = self.token_embedding(tokens)
         hidden = looked_up + self.position_encoding[:sequence_length]
+        masked = {} if mask is None else {"mask": mask}
         for block in self.blocks:
             if self.config.gradient_checkpointing and self.training:
                 from torch.utils.checkpoint import checkpoint
 
-                hidden = checkpoint(block, hidden, use_reentrant=False)
+                hidden = checkpoint(block, hidden, use_reentrant=False, **masked)
             else:
-                hidden = block(hidden)
+                hidden = block(hidden, **masked)
         if targets is not None and targets.shape != tokens.shape:
             raise ValueError("targets must have the same shape as tokens")
         fused_loss = (targets is not None and self.fused_cross_entropy and hidden.is_cuda
@@ -580,22 +691,26 @@ class RatchetGPT(nn.Module):
                   dtype: torch.dtype | None = None) -> KVCache:
         """An empty KV cache for `batch` sequences of up to `max_len` (<= block_size) tokens.
         `dtype` (e.g. bfloat16) stores keys/values and runs the cached attention in that
-        type; by default they keep the activations' dtype."""
+        type; by default they keep the activations' dtype. torch.int8: codes with a scale per
+        64 tokens and head (``Int8KVCache``)."""
         max_len = max_len or self.config.block_size
         if max_len > self.config.block_size:
             raise ValueError("a cache cannot outgrow block_size (positions are absolute)")
         device = self.position_encoding.device
-        return KVCache(self.config.n_layer, batch, self.config.n_head,
-                       self.config.n_embd // self.config.n_head, max_len, device, dtype)
+        shape = (self.config.n_layer, batch, self.config.n_head,
+                 self.config.n_embd // self.config.n_head, max_len, device)
+        return Int8KVCache(*shape) if dtype == torch.int8 else KVCache(*shape, dtype)
 
     @torch.no_grad()
-    def prefill(self, tokens: Tensor, cache: KVCache) -> Tensor:
+    def prefill(self, tokens: Tensor, cache: KVCache, *,
+                mask: AttentionMask | None = None) -> Tensor:
         """Run `tokens` [B, S] at positions cache.length .. +S, append their keys/values, and
-        return the logits of the last position [B, vocab]."""
+        return the logits of the last position [B, vocab]. `mask`: of a prompt at the start of
+        the cache, for a model trained so (e.g. its prompt as a prefix)."""
         start, length = cache.length, tokens.shape[1]
         hidden = self.token_embedding(tokens) + self.position_encoding[start:start + length]
         for index, block in enumerate(self.blocks):
-            hidden = block(hidden, cache=cache, layer=index)
+            hidden = block(hidden, cache=cache, layer=index, mask=mask)
         cache.advance(length)
         return self.lm_head(self.final_norm(hidden[:, -1:]))[:, 0]
 

@@ -100,28 +100,35 @@ def _torch_mask(documents: Tensor | None, prefix: Tensor | None) -> AttentionMas
     return AttentionMask(bounds, torch.where(words >= 2**31, words - 2**32, words).to(torch.int32))
 
 
+def torch_scores(q: Tensor, k: Tensor, v: Tensor, seen: Tensor, distance: Tensor,
+                 softcap: float, slopes: Tensor | None, scale: float) -> Tensor:
+    """The formulas in torch operations, in float32 (float64 for float64 operands): `seen` and
+    `distance` broadcast to the scores [B, H, Q, K]."""
+    with torch.autocast(q.device.type, enabled=False):
+        work = torch.float64 if q.dtype == torch.float64 else torch.float32
+        group = q.shape[1] // k.shape[1] if k.shape[1] else 1
+        kk, vv = (t.to(work).repeat_interleave(group, dim=1) for t in (k, v))
+        scores = q.to(work) @ kk.transpose(2, 3).contiguous() * scale
+        if softcap:
+            scores = softcap * torch.tanh(scores / softcap)
+        if slopes is not None:
+            scores = scores - slopes.to(work)[:, None, None] * distance
+        weights = scores.masked_fill(~seen, -math.inf)
+        weights = torch.where(seen.any(-1, keepdim=True), weights, 0.0).softmax(-1)
+        return (weights.masked_fill(~seen, 0.0) @ vv).to(q.dtype)
+
+
 def _torch_scored_attention(q: Tensor, k: Tensor, v: Tensor, mask: AttentionMask | None,
                             softcap: float, slopes: Tensor | None, scale: float) -> Tensor:
-    work = torch.float64 if q.dtype == torch.float64 else torch.float32
-    group = q.shape[1] // k.shape[1] if k.shape[1] else 1
-    s = q.shape[2]
-    at = torch.arange(s, device=q.device)
+    at = torch.arange(q.shape[2], device=q.device)
     if mask is None:
-        seen = (at[None, :] <= at[:, None])[None, None]
+        seen = at[None, :] <= at[:, None]
     else:
         seen = ((at >= mask.bounds[0][..., None]) & (at < mask.bounds[1][..., None]))[:, None]
-        # padding may hold anything: its products are masked below, its values are cleared here
+        # padding may hold anything: its products are masked, its values are cleared here
         used = (mask.bounds[1] > mask.bounds[0])[:, None, :, None]
         q, k, v = (torch.where(used, t, 0) for t in (q, k, v))
-    kk, vv = (t.to(work).repeat_interleave(group, dim=1) for t in (k, v))
-    scores = q.to(work) @ kk.transpose(2, 3).contiguous() * scale
-    if softcap:
-        scores = softcap * torch.tanh(scores / softcap)
-    if slopes is not None:
-        scores = scores - slopes.to(work)[:, None, None] * (at[:, None] - at[None, :]).abs()
-    weights = scores.masked_fill(~seen, -math.inf)
-    weights = torch.where(seen.any(-1, keepdim=True), weights, 0.0).softmax(-1)
-    return (weights.masked_fill(~seen, 0.0) @ vv).to(q.dtype)
+    return torch_scores(q, k, v, seen, (at[:, None] - at[None, :]).abs(), softcap, slopes, scale)
 
 
 def score_arguments(q: Tensor, softcap: float | None, slopes: Tensor | None,
@@ -173,5 +180,4 @@ def scored_attention(q: Tensor, k: Tensor, v: Tensor, *, mask: AttentionMask | N
     if q.is_cuda and q.dtype == torch.bfloat16 and d in (64, 128):
         bounds, padding = mask if mask is not None else (None, None)
         return ratchet().scored_attend(q, k, v, bounds, padding, slopes, softcap, scale)
-    with torch.autocast(q.device.type, enabled=False):
-        return _torch_scored_attention(q, k, v, mask, softcap, slopes, scale)
+    return _torch_scored_attention(q, k, v, mask, softcap, slopes, scale)
