@@ -24,6 +24,9 @@ namespace rk {
 struct ScoredBwdArgs {
   ScoredArgs f;
   float inv_scale;  // 1 / scale
+  // capped scores, with slope gradients: scale log2(e), the largest |x| of the polynomial below,
+  // its coefficients by C^-2, C^-4, .. (C = cap log2(e)), and 1 / C
+  float near_scale, near_limit, near[4], inv_cap2;
   float* rows;      // [B H][2][Sp]: log-sum-exp term and -delta (zeros where a row is none)
   float* slope_rows;  // [B H][Sp], or null
   // the query heads of a key head in `parts` workgroups each: their float32 dk, dv [parts][2]
@@ -53,6 +56,22 @@ __device__ __forceinline__ float score_p(const ScoredArgs& a, float x, float ter
           __builtin_fmaf(-slope2, fabsf(dist), x * a.dot_scale));
     return __builtin_amdgcn_exp2f(x * a.dot_scale);
   }
+}
+
+// The capped score in base-2 units by an odd polynomial, y + y z (c1 + c2 z + c3 z^2 + c4 z^3) with
+// y = x scale log2(e), z = y^2: tanh(u) / u fitted by least squares at Chebyshev nodes of
+// |u| <= 1/2, off by 2e-8 there. The exponential form is off by 2^-24 of the cap whatever the
+// score, which the slopes' gradient, a float32 sum over all pairs, shows (3e-6 of its norm at cap
+// 50 to 100, against 1.0e-6 to 1.4e-6). The other kernels, whose results are bf16, keep the exponential: with
+// a branch between the two forms they were slower, the forward by a fifth.
+__device__ __forceinline__ float near_capped(const ScoredBwdArgs& a, float x, float& slack) {
+  const float y = x * a.near_scale, z = y * y;
+  float q = __builtin_fmaf(a.near[3], z, a.near[2]);
+  q = __builtin_fmaf(q, z, a.near[1]);
+  q = __builtin_fmaf(q, z, a.near[0]);
+  const float t = __builtin_fmaf(y, z * q, y), th = t * a.inv_cap2;
+  slack = __builtin_fmaf(-th, th, 1.0f);
+  return t;
 }
 
 template <int D, bool CAP, bool BIAS, bool SG>
@@ -157,13 +176,31 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
     const int j0 = key0 + 4 * h - span.lo;
     const float d0 = static_cast<float>(qi - key0 - 4 * h);
     float slack[CAP && SG ? 16 : 1];
+    bool near = false;
+    if constexpr (CAP && SG) {
+      float most = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float sl;
-      st[e] = score_p<CAP, BIAS>(a, st[e], term, slope2,
-                                 d0 - static_cast<float>(8 * (e / 4) + (e % 4)), sl);
-      if constexpr (CAP && SG) slack[e] = sl;
-      else if constexpr (CAP) st[e] = st[e] * sl;
+      for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(st[e]));
+      near = !__any(most > ba.near_limit);
+    }
+    if (near) {  // (never without slope gradients)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float sl;
+        const float t = near_capped(ba, st[e], sl) - term;
+        const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
+        st[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(-slope2, dist, t));
+        if constexpr (CAP && SG) slack[e] = sl;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float sl;
+        st[e] = score_p<CAP, BIAS>(a, st[e], term, slope2,
+                                   d0 - static_cast<float>(8 * (e / 4) + (e % 4)), sl);
+        if constexpr (CAP && SG) slack[e] = sl;
+        else if constexpr (CAP) st[e] = st[e] * sl;
+      }
     }
     if (!whole) {
 #pragma unroll
@@ -528,6 +565,18 @@ extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args
   ScoredBwdArgs a{};
   a.f = scored_args(p);
   a.inv_scale = 1.0f / p.scale;
+  if (p.softcap > 0.0f) {
+    const double c2 = static_cast<double>(a.f.cap2), step = 1.0 / (c2 * c2);
+    const double fit[4] = {-0.3333323001861572, 0.13327749073505402, -0.053165826946496964,
+                           0.0174802765250206};
+    double power = step;
+    for (int i = 0; i < 4; ++i, power *= step) a.near[i] = static_cast<float>(fit[i] * power);
+    a.near_scale = p.scale * kLog2e;
+    // caps whose powers leave float32's range: always the exponential
+    const bool fits = p.softcap > 1e-3f && p.softcap < 1e3f;
+    a.near_limit = fits ? 0.5f * p.softcap / p.scale : -1.0f;
+    a.inv_cap2 = static_cast<float>(1.0 / c2);
+  }
   a.rows = work;
   a.slope_rows = p.dslopes ? work + 2 * p.B * p.H * a.f.Sp : nullptr;
   a.parts = head_parts(p.B, p.H, p.Hkv, p.S);
