@@ -49,7 +49,7 @@ __device__ __forceinline__ bool append_range(const Kv8Append& a, int64_t b, int6
   if (start < 0) return false;
   int64_t n = a.lengths ? a.lengths[b] : a.S;
   n = n < a.S ? n : a.S;
-  blk = start / kTok + touched;
+  blk = (start >> 6) + touched;
   if (n <= 0 || blk >= a.c.NB) return false;
   const int64_t base = blk * kTok, f = start - base, l = start + n - base;
   first = static_cast<int>(f > 0 ? f : 0);
@@ -70,7 +70,7 @@ __device__ __forceinline__ int code_of(float x, float s) {
 }
 // The same for 8 values, by the reciprocal r of s where that decides (rk_rowquant.h: the rounded
 // product, redone by the quotient when one of the 8 lies near a rounding boundary). With the IEEE
-// quotient for every value the divisions bounded the kernel (VVV).
+// quotient for every value the divisions were most of its instructions.
 __device__ __forceinline__ void codes_of(const float (&x)[8], float s, float r, int (&c)[8]) {
   bool exact = false;
 #pragma unroll
@@ -93,7 +93,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   constexpr int PER = D / 8, EACH = kTok * PER / 256, PITCH = kTok + 4;
   __shared__ uint32_t red[4];
   __shared__ __attribute__((aligned(16))) uint8_t tile[D * PITCH];
-  const int64_t bh = blockIdx.y, b = bh / a.c.H, h = bh - b * a.c.H;
+  const uint32_t uh = static_cast<uint32_t>(a.c.H), ub = blockIdx.y / uh;
+  const int64_t bh = blockIdx.y, b = ub, h = blockIdx.y - ub * uh;
   const int tid = threadIdx.x;
   int64_t blk, start;
   int first, last;
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   const float old = first > 0 ? *scale : 0.0f;
 
   // every thread loads, tokens outside first .. last - 1 the nearest one inside: a condition
-  // around the loads let only one be in flight (16 -> NNN us at 4 x 777 tokens, 16 heads of 128)
+  // around the loads let only one be in flight (16 -> 14.5 us at 4 x 777 tokens, 16 heads of 128)
   float x[EACH][8];
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
@@ -370,23 +371,27 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
   __shared__ float sm[NW][16], sl[NW][16];
   const int split = blockIdx.x;
   const int64_t tile = blockIdx.y, bh = blockIdx.z;
-  const int64_t b = bh / a.c.H, kvh = bh - b * a.c.H;
+  const uint32_t uh = static_cast<uint32_t>(a.c.H), ub = blockIdx.z / uh;  // 32-bit divisions
+  const int64_t b = ub, kvh = blockIdx.z - ub * uh;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t start = a.start[b * a.start_step];
   const int64_t cols = a.S * a.G;
   // this lane's column: query i of head kvh * G + hg; lanes past the last take the last's
   const int64_t cc = tile * 16 + col < cols ? tile * 16 + col : cols - 1;
-  const int64_t i = cc / a.G, hd = kvh * a.G + (cc - i * a.G);
+  const uint32_t ug = static_cast<uint32_t>(a.G);  // (the host bounds the columns)
+  const int64_t i = static_cast<uint32_t>(cc) / ug, hd = kvh * a.G + (cc - i * a.G);
   int64_t n = a.lengths ? a.lengths[b] : a.S;
   n = n < a.S ? n : a.S;
   // the blocks that the tile's last active query sees
   const int64_t c_last = tile * 16 + 15 < cols ? tile * 16 + 15 : cols - 1;
-  int64_t i_last = c_last / a.G;
+  int64_t i_last = static_cast<uint32_t>(c_last) / ug;
   i_last = i_last < n ? i_last : n - 1;
-  int64_t nb = start < 0 || n <= 0 || tile * 16 / a.G >= n ? 0 : (start + i_last) / kTok + 1;
+  const bool on = start >= 0 && n > 0 && static_cast<uint32_t>(tile * 16) / ug < n;
+  int64_t nb = on ? ((start + i_last) >> 6) + 1 : 0;
   nb = nb < a.c.NB ? nb : a.c.NB;
-  const int64_t per = (nb + a.nsplit - 1) / a.nsplit;
+  const int64_t per = (static_cast<uint32_t>(nb) + static_cast<uint32_t>(a.nsplit) - 1) /
+                      static_cast<uint32_t>(a.nsplit);
   const int64_t j0 = split * per, j1 = j0 + per < nb ? j0 + per : nb;
 
   float m = -INFINITY, l = 0.0f, o[FT][4];
@@ -581,7 +586,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
       for (int e = 0; e < 4; ++e) r[e] = __builtin_fmaf(x, so[w][c][f + e], r[e]);
     }
     if (a.nsplit == 1) {
-      const int64_t qi = ct / a.G, h = kvh * a.G + (ct - qi * a.G);
+      const int64_t qi = static_cast<uint32_t>(ct) / ug, h = kvh * a.G + (ct - qi * a.G);
       const float factor = row_factor(a, b, qi, ll);
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[e] = factor == 0.0f ? 0.0f : r[e] * factor;
@@ -600,7 +605,8 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
 // grid (columns, B * H), D / 4 threads: the splits of one column.
 template <int D, int ODT>
 __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
-  const int64_t ct = a.col0 + blockIdx.x, bh = blockIdx.y, b = bh / a.c.H, kvh = bh - b * a.c.H;
+  const uint32_t uh = static_cast<uint32_t>(a.c.H), ub = blockIdx.y / uh;
+  const int64_t ct = a.col0 + blockIdx.x, bh = blockIdx.y, b = ub, kvh = blockIdx.y - ub * uh;
   const int f = threadIdx.x * 4;
   const float* w = a.work + (bh * (a.S * a.G - a.col0) + blockIdx.x) * a.nsplit * (D + 4);
   const int64_t step = D + 4;
@@ -634,7 +640,8 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
         r[e] = ms[u] == -INFINITY ? r[e] : __builtin_fmaf(x, o4[e], r[e]);
     }
   }
-  const int64_t qi = ct / a.G, h = kvh * a.G + (ct - qi * a.G);
+  const int64_t qi = static_cast<uint32_t>(ct) / static_cast<uint32_t>(a.G);
+  const int64_t h = kvh * a.G + (ct - qi * a.G);
   const float factor = row_factor(a, b, qi, ll);
 #pragma unroll
   for (int e = 0; e < 4; ++e) r[e] = factor == 0.0f ? 0.0f : r[e] * factor;
@@ -651,7 +658,7 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
 // which a lane holds its probabilities. The next block's codes are in registers meanwhile.
 //
 // Codes converted by each reader instead, or the digits of kv8_attn_kernel for chunks too, cost
-// more: the latter ZZZ us at 4 x 517 tokens behind 1500, 16 heads of 128.
+// more: the latter 176 us at 4 x 517 tokens behind 1500, 16 heads of 128, where this takes QQQ.
 // ---------------------------------------------------------------------------
 template <bool SCALED = false>
 __device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi,
@@ -689,12 +696,14 @@ void kv8_chunk_kernel(Kv8Attn a) {
   constexpr int EACH = kTok * D / 16 / 256;  // 16-code pieces per thread and operand
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * 2 * 2 * TILE];
   // whole tiles first, the last queries, which see most, before the others; heads fastest
-  const int64_t BHq = a.c.B * a.Hq, full = a.S / 128, turn = blockIdx.x / BHq;
-  const bool whole_tile = turn < full * a.nfull;
-  const int64_t qt = whole_tile ? full - 1 - turn / a.nfull : full;
-  const int64_t split = whole_tile ? turn % a.nfull : turn - full * a.nfull;
-  const int64_t nsplit = whole_tile ? a.nfull : a.nsplit;
-  const int64_t bhq = blockIdx.x % BHq, b = bhq / a.Hq, hd = bhq - b * a.Hq, kvh = hd / a.G;
+  const uint32_t uhq = static_cast<uint32_t>(a.Hq), uBHq = static_cast<uint32_t>(a.c.B) * uhq;
+  const uint32_t full = static_cast<uint32_t>(a.S) / 128, nfull = static_cast<uint32_t>(a.nfull);
+  const uint32_t turn = blockIdx.x / uBHq, ubh = blockIdx.x - turn * uBHq, ub = ubh / uhq;
+  const bool whole_tile = turn < full * nfull;
+  const int64_t qt = whole_tile ? full - 1 - turn / nfull : full;
+  const int64_t split = whole_tile ? turn % nfull : turn - full * nfull;
+  const uint32_t nsplit = static_cast<uint32_t>(whole_tile ? a.nfull : a.nsplit);
+  const int64_t b = ub, hd = ubh - ub * uhq, kvh = (ubh - ub * uhq) / static_cast<uint32_t>(a.G);
   const int64_t bh = b * a.c.H + kvh;
   const int tid = threadIdx.x & 255, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -706,9 +715,9 @@ void kv8_chunk_kernel(Kv8Attn a) {
   const int64_t i0 = qt * 128, iw = i0 + 32 * wave, i = iw + l32;
   const bool on = start >= 0 && i0 < n;
   const int64_t last = i0 + 128 < n ? i0 + 127 : n - 1;  // the last active query
-  int64_t nb = on ? (start + last) / kTok + 1 : 0;
+  int64_t nb = on ? ((start + last) >> 6) + 1 : 0;
   nb = nb < a.c.NB ? nb : a.c.NB;
-  const int64_t per = (nb + nsplit - 1) / nsplit;
+  const int64_t per = (static_cast<uint32_t>(nb) + nsplit - 1) / nsplit;
   const int64_t j0 = split * per, j1 = j0 + per < nb ? j0 + per : nb;
   // positions relative to the split's first key
   const int64_t base = start - j0 * kTok;

@@ -20,7 +20,7 @@ namespace rk {
 
 struct ScoredArgs {
   rk_scored_attention_args p;
-  int64_t G;        // query heads per key head
+  uint32_t BH, H, G;  // query heads of all, of a sequence, per key head
   int64_t S32;      // padding words per row
   int64_t Sp;       // S rounded up to 128 (row statistics)
   float dot_scale;  // plain: scale log2(e); capped: 2 log2(e) scale / cap
@@ -123,14 +123,25 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, uint64_t bits, int tid
       *reinterpret_cast<uint4*>(tile + 16 * i) = make_uint4(0, 0, 0, 0);
 }
 
-// What rounding x to bf16 left, in 256ths of the bf16 step (2^-16 of x): the difference of the
-// bit patterns, and the float32 value it restores.
-__device__ __forceinline__ int bf16_rest(float x, uint32_t bf16) {
-  const int d = static_cast<int>(__float_as_uint(x) - (bf16 << 16) + 128) >> 8;
-  return d > 127 ? 127 : d < -128 ? -128 : d;
+// What rounding 4 numbers to the bf16 pairs lo, hi left, a byte each in 256ths of the bf16 step
+// (rounded down, so to 2^-16 of the number): the second byte of the bit patterns' difference,
+// which lies in -2^15 .. 2^15 (the upper end, a tie, taken as the largest byte).
+__device__ __forceinline__ uint32_t bf16_rest4(const float (&x)[4], uint32_t lo, uint32_t hi) {
+  const uint32_t r[4] = {lo << 16, lo & 0xffff0000u, hi << 16, hi & 0xffff0000u};
+  uint32_t d[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int diff = static_cast<int>(__float_as_uint(x[e]) - r[e]);
+    d[e] = static_cast<uint32_t>(diff < 0x7fff ? diff : 0x7fff);
+  }
+  const uint32_t p01 = __builtin_amdgcn_perm(d[1], d[0], 0x0c0c0501u);
+  const uint32_t p23 = __builtin_amdgcn_perm(d[3], d[2], 0x0c0c0501u);
+  return __builtin_amdgcn_perm(p23, p01, 0x05040100u);
 }
-__device__ __forceinline__ float with_rest(uint32_t bf16, int rest) {
-  return __uint_as_float((bf16 << 16) + static_cast<uint32_t>(rest * 256));
+
+// The float32 number, to the middle of its rest's step.
+__device__ __forceinline__ float with_rest(uint32_t bf16_high, int rest) {
+  return __uint_as_float(bf16_high + static_cast<uint32_t>(rest * 256 + 128));
 }
 
 int check_scored(const rk_scored_attention_args& p, bool backward);

@@ -8,7 +8,7 @@
 // Products of bf16 operands summed in float32; p and ds enter the second products rounded to
 // bf16 (half a step); scores, exponentials, delta are float32, o with what its rounding left
 // (`rest`): with the bf16 o alone, dq and dk of concentrated rows were off by 2.7e-3 to 3.2e-3 of
-// their norm instead of XXX, the rounding of ds and of the results. Two launches, as
+// their norm instead of 2.4e-3 (the rounding of ds and of the results). Two launches, as
 // at rk_attention_bwd.hip: the queries' (dq, and delta for the second) and the keys' (dk, dv; the
 // query heads that share a key head are summed by the one wavefront that owns the key, in order),
 // every output summed in a fixed order, so results repeat.
@@ -84,11 +84,10 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   const ScoredArgs& a = ba.f;
   const rk_scored_attention_args& p = a.p;
   const int S = static_cast<int>(p.S);
-  const int64_t BH = p.B * p.H;
   const int nqb = (S + kAttnRows - 1) / kAttnRows;
-  const int blk = static_cast<int>(blockIdx.x / BH);  // heads fastest
-  const int qb = nqb - 1 - blk;                       // longest causal rows first
-  const int64_t bh = blockIdx.x - blk * BH, b = bh / p.H, hd = bh - b * p.H, kvh = hd / a.G;
+  const uint32_t blk = blockIdx.x / a.BH, ubh = blockIdx.x - blk * a.BH, ub = ubh / a.H;
+  const int qb = nqb - 1 - static_cast<int>(blk);  // longest causal rows first; heads fastest
+  const int64_t bh = ubh, b = ub, hd = ubh - ub * a.H, kvh = (ubh - ub * a.H) / a.G;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qw0 = qb * kAttnRows + 32 * wave, qi = qw0 + l32;
@@ -131,8 +130,9 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int8_t r = static_cast<int8_t>((e < 4 ? rest[s].x : rest[s].y) >> (8 * (e % 4)));
-        const float ov = with_rest(pairs[e / 2] >> (16 * (e % 2)) & 0xffffu, r);
-        dot = dot + static_cast<float>(gf[s][e]) * ov;
+        const uint32_t high = e % 2 ? pairs[e / 2] & 0xffff0000u : pairs[e / 2] << 16;
+        const float ov = p.rest ? with_rest(high, r) : __uint_as_float(high);
+        dot = __builtin_fmaf(static_cast<float>(gf[s][e]), ov, dot);
       }
     }
   }
@@ -291,14 +291,14 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
   const ScoredArgs& a = ba.f;
   const rk_scored_attention_args& p = a.p;
   const int S = static_cast<int>(p.S);
-  const int64_t BH = p.B * p.Hkv;
-  const int blk = static_cast<int>(blockIdx.x / (BH * ba.parts));  // heads fastest
-  const int64_t idx = blockIdx.x - blk * (BH * ba.parts);
-  const int64_t bh = idx / ba.parts, part = idx - bh * ba.parts;
-  const int64_t b = bh / p.Hkv, kvh = bh - b * p.Hkv;
-  const int heads = static_cast<int>(a.G / ba.parts);
-  const int64_t hq = kvh * a.G + part * heads;  // the first query head
-  const int k0 = blk * kAttnRows;  // the first keys have the longest walk
+  const uint32_t uparts = static_cast<uint32_t>(ba.parts);
+  const uint32_t ukv = static_cast<uint32_t>(p.Hkv), uBH = static_cast<uint32_t>(p.B) * ukv;
+  const uint32_t blk = blockIdx.x / (uBH * uparts);  // heads fastest
+  const uint32_t uidx = blockIdx.x - blk * (uBH * uparts), ubh = uidx / uparts, ub = ubh / ukv;
+  const int64_t BH = uBH, bh = ubh, part = uidx - ubh * uparts, b = ub, kvh = ubh - ub * ukv;
+  const int heads = static_cast<int>(a.G / uparts);
+  const int64_t hq = kvh * static_cast<int64_t>(a.G) + part * heads;  // the first query head
+  const int k0 = static_cast<int>(blk) * kAttnRows;  // the first keys have the longest walk
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kj = k0 + 32 * wave + l32;
