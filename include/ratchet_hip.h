@@ -722,7 +722,8 @@ int rk_attention_mask(const void* documents, int wide, int64_t sdb, const uint8_
  *   slopes (float32 [H]): s -= slopes[h] |i - j|;
  *   o_i = sum_j softmax_j(s_ij over the keys i sees) v_j,  lse_i = log sum_j exp(s_ij).
  * A query that sees nothing gets zeros (lse 0); what padding positions hold does not matter.
- * rest, written by the forward and read by the backward, makes delta = g . o exact to 2^-16 of o.
+ * rest, written by the forward and read by the backward (a byte per element, in an order of its
+ * own), makes delta = g . o exact to 2^-16 of o.
  * The backward reads o, lse and the gradient g of o, and writes dq, dk, dv and, where given,
  * dslopes (float32 [H]); work: rk_scored_attention_backward_work floats, 16-byte aligned. Scores and softmax run
  * in float32; probabilities and score gradients enter the products rounded to bf16; every sum
@@ -735,7 +736,7 @@ typedef struct rk_scored_attention_args {
   const uint16_t *q, *k, *v;
   uint16_t* o;
   float* lse; /* [B, H, S] contiguous */
-  int8_t* rest; /* [B, S, H, D] contiguous, or NULL: what rounding o left, in 256ths of a step */
+  int8_t* rest; /* what rounding o left, or NULL: rk_scored_attention_rest bytes */
   const int32_t* bounds;
   const uint32_t* padding;
   const float* slopes;
@@ -749,6 +750,7 @@ typedef struct rk_scored_attention_args {
   float scale, softcap;
 } rk_scored_attention_args;
 
+int64_t rk_scored_attention_rest(int64_t B, int64_t H, int64_t S, int64_t D);
 int rk_scored_attention_forward(const rk_scored_attention_args* args, void* stream);
 int64_t rk_scored_attention_backward_work(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D,
                                           int slopes);

@@ -1149,10 +1149,10 @@ std::tuple<Tensor, Tensor, Tensor> scored_attention(const Tensor& q, const Tenso
   Tensor lse = at::empty({a.B, a.H, a.S}, q.options().dtype(at::kFloat));
   a.o = static_cast<uint16_t*>(o.data_ptr());
   a.sob = a.S * a.H * a.D, a.soh = a.D, a.sos = a.H * a.D;
-  Tensor rest = grad ? at::empty({a.B, a.S, a.H, a.D}, q.options().dtype(at::kChar))
-                     : at::empty({0}, q.options().dtype(at::kChar));
+  const int64_t bytes = grad ? rk_scored_attention_rest(a.B, a.H, a.S, a.D) : 0;
+  Tensor rest = at::empty({bytes}, q.options().dtype(at::kChar));
   a.lse = lse.data_ptr<float>();
-  a.rest = grad ? rest.data_ptr<int8_t>() : nullptr;
+  a.rest = bytes > 0 ? rest.data_ptr<int8_t>() : nullptr;
   check_status(rk_scored_attention_forward(&a, stream_of(q)), "rk_scored_attention_forward");
   return {o, lse, rest};
 }
@@ -1182,7 +1182,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> scored_attention_backward(
               "scored attention backward: lse must be a contiguous float32 [B, H, S] tensor");
   same_device(q, rest, "scored attention backward");
   TORCH_CHECK(rest.scalar_type() == at::kChar && rest.is_contiguous() &&
-                  (rest.numel() == 0 || rest.numel() == q.numel()),
+                  (rest.numel() == 0 ||
+                   rest.numel() == rk_scored_attention_rest(a.B, a.H, a.S, a.D)),
               "scored attention backward: rest must be the forward's, or empty");
   TORCH_CHECK(!slope_grad || slopes.has_value(),
               "scored attention backward: a slope gradient needs slopes");

@@ -139,6 +139,15 @@ __device__ __forceinline__ uint32_t bf16_rest4(const float (&x)[4], uint32_t lo,
   return __builtin_amdgcn_perm(p23, p01, 0x05040100u);
 }
 
+// Where the rests of a head's 32 rows from row0 on lie: words [D / 8][64], word r of lane l + 32 h
+// (features 8 r + 4 h .. + 3 of row l) at 64 r + 32 h + l. In rows as o has them the forward's
+// 4-byte stores and the backward's 8-byte loads, each to a row of its own, cost 5 us each at
+// B 8, H 16, S 1024, D 128.
+template <int D>
+__device__ __forceinline__ uint32_t* rest_words(const ScoredArgs& a, int64_t bh, int row0) {
+  return reinterpret_cast<uint32_t*>(a.p.rest + (bh * a.Sp + row0) * D);
+}
+
 // The float32 number, to the middle of its rest's step.
 __device__ __forceinline__ float with_rest(uint32_t bf16_high, int rest) {
   return __uint_as_float(bf16_high + static_cast<uint32_t>(rest * 256 + 128));

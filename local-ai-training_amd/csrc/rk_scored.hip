@@ -169,6 +169,11 @@ void scored_fwd_kernel(ScoredArgs a) {
     }
   }
 
+  uint32_t* const rest = p.rest ? rest_words<D>(a, bh, qw0) + lane : nullptr;
+  if (qi >= S && rest) {
+#pragma unroll
+    for (int r = 0; r < D / 8; ++r) rest[64 * r] = 0;
+  }
   if (qi < S) {
     if (!span.valid) {
 #pragma unroll
@@ -176,7 +181,6 @@ void scored_fwd_kernel(ScoredArgs a) {
     }
     const float factor = span.valid ? 1.0f / l : 0.0f;
     uint16_t* const row = p.o + b * p.sob + hd * p.soh + static_cast<int64_t>(qi) * p.sos;
-    int8_t* const rest = p.rest ? p.rest + ((b * p.S + qi) * p.H + hd) * D + 4 * h : nullptr;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -185,8 +189,7 @@ void scored_fwd_kernel(ScoredArgs a) {
                             o[dt][4 * r + 2] * factor, o[dt][4 * r + 3] * factor};
         const uint32_t lo = bf16_pair(x[0], x[1]), hi = bf16_pair(x[2], x[3]);
         *reinterpret_cast<uint2*>(row + 32 * dt + 8 * r + 4 * h) = make_uint2(lo, hi);
-        if (rest)
-          *reinterpret_cast<uint32_t*>(rest + 32 * dt + 8 * r) = bf16_rest4(x, lo, hi);
+        if (rest) rest[64 * (4 * dt + r)] = bf16_rest4(x, lo, hi);
       }
     if (h == 0)
       p.lse[bh * S + qi] = span.valid ? (m + __log2f(l)) * 0.69314718055994531f : 0.0f;
@@ -433,6 +436,8 @@ int check_scored(const rk_scored_attention_args& p, bool backward) {
     return fail(RK_ERR_ARG, "a mask holds one row or one per sequence");
   if ((p.bounds == nullptr) != (p.padding == nullptr))
     return fail(RK_ERR_ARG, "a mask's intervals and padding bits go together");
+  if (reinterpret_cast<uintptr_t>(p.rest) & 3)
+    return fail(RK_ERR_UNSUPPORTED, "rest needs 4-byte alignment");
   const void* in16[] = {p.q, p.k, p.v, backward ? p.o : p.q, backward ? p.g : p.q};
   for (const void* t : in16)
     if (!t || !aligned16(t)) return fail(RK_ERR_UNSUPPORTED, "operands need 16-byte alignment");
@@ -484,14 +489,17 @@ static void launch_scored_fwd(const ScoredArgs& a, dim3 grid, hipStream_t st) {
 
 using namespace rk;
 
+extern "C" int64_t rk_scored_attention_rest(int64_t B, int64_t H, int64_t S, int64_t D) {
+  if (B <= 0 || H <= 0 || S <= 0 || D <= 0) return 0;
+  return B * H * ((S + kAttnRows - 1) / kAttnRows * kAttnRows) * D;
+}
+
 extern "C" int rk_scored_attention_forward(const rk_scored_attention_args* args, void* stream) {
   clear_error();
   if (!args) return fail(RK_ERR_ARG, "null arguments");
   const rk_scored_attention_args& p = *args;
   if (int e = check_scored(p, false)) return e;
   if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
-  if (reinterpret_cast<uintptr_t>(p.rest) & 3)
-    return fail(RK_ERR_UNSUPPORTED, "rest needs 4-byte alignment");
   if (reinterpret_cast<uintptr_t>(p.o) & 7) return fail(RK_ERR_UNSUPPORTED, "o needs 8-byte alignment");
   const ScoredArgs a = scored_args(p);
   const dim3 grid(static_cast<unsigned>(p.B * p.H * (a.Sp / kAttnRows)));

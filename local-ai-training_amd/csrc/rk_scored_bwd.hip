@@ -117,11 +117,11 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   {
     v8bf_a of[D / 16];
     load_owned<D>(of, p.o + b * p.sob + hd * p.soh, p.sos, S, qi, h);
-    uint2 rest[D / 16] = {};
-    if (p.rest && qi < S) {
-      const int8_t* const at = p.rest + ((b * p.S + qi) * p.H + hd) * D + 8 * h;
+    uint2 rest[D / 16] = {};  // features 16 s + 8 h .. + 7: words 2 s + h of lanes l and l + 32
+    if (p.rest) {
+      const uint32_t* const at = rest_words<D>(a, bh, qw0) + 64 * h + l32;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) rest[s] = *reinterpret_cast<const uint2*>(at + 16 * s);
+      for (int s = 0; s < D / 16; ++s) rest[s] = make_uint2(at[128 * s], at[128 * s + 32]);
     }
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
@@ -555,8 +555,6 @@ extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args
   if (p.dslopes && !p.slopes) return fail(RK_ERR_ARG, "a slope gradient needs slopes");
   if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
   if (!p.dq || !p.dk || !p.dv || !work) return fail(RK_ERR_ARG, "null pointer");
-  if (reinterpret_cast<uintptr_t>(p.rest) & 7)
-    return fail(RK_ERR_UNSUPPORTED, "rest needs 8-byte alignment");
   if (!aligned16(work)) return fail(RK_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
   const void* out8[] = {p.dq, p.dk, p.dv};
   for (const void* t : out8)

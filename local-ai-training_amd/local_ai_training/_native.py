@@ -128,6 +128,7 @@ SIGNATURES: dict[str, list] = {
     "rk_attention_backward": [*([_p, _i64, _i64, _i64] * 5), _p, _i64, _i64, _i64, _i64, _f32,
                               _p, _p, _p, _i64, _i64, _i64, _p, _p],
     "rk_attention_mask": [_p, _i32, _i64, _p, _i64, _i64, _i64, _p, _p, _p],
+    "rk_scored_attention_rest": [_i64, _i64, _i64, _i64],
     "rk_scored_attention_forward": [_p, _p],
     "rk_scored_attention_backward_work": [_i64, _i64, _i64, _i64, _i64, _i32],
     "rk_scored_attention_backward": [_p, _p, _p],
@@ -147,6 +148,7 @@ SIGNATURES: dict[str, list] = {
 RESTYPES = {
     "rk_last_error": ctypes.c_char_p,
     "rk_attention_backward_work": ctypes.c_int64,
+    "rk_scored_attention_rest": ctypes.c_int64,
     "rk_scored_attention_backward_work": ctypes.c_int64,
     "rk_int8_kv_attention_work": ctypes.c_int64,
     "rk_int8_gemm_large_rows": ctypes.c_int64,

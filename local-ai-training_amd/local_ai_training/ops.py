@@ -189,7 +189,7 @@ def _register_fakes() -> None:
     def _scored_attention(q, k, v, bounds, padding, slopes, softcap, scale, grad):
         b, h, sl, d = q.shape
         o = q.new_empty((b, sl, h, d)).permute(0, 2, 1, 3)
-        rest = q.new_empty((b, sl, h, d) if grad else (0,), dtype=torch.int8)
+        rest = q.new_empty((b * h * -(-sl // 128) * 128 * d if grad else 0,), dtype=torch.int8)
         return o, q.new_empty((b, h, sl), dtype=torch.float32), rest
 
     @fake("ratchet::scored_attend")
