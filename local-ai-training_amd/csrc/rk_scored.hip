@@ -453,7 +453,7 @@ int check_scored(const rk_scored_attention_args& p, bool backward) {
   // statistics, lie below 2^31 bytes
   const int64_t rows[] = {p.sqs, p.sks, p.svs, backward ? p.sos : 0, backward ? p.sgs : 0};
   for (int64_t st : rows)
-    if (((p.S + 192) * st + p.D) * 2 >= (int64_t{1} << 31))
+    if (st >= (int64_t{1} << 31) || ((p.S + 192) * st + p.D) * 2 >= (int64_t{1} << 31))
       return fail(RK_ERR_UNSUPPORTED, "sequence extent exceeds 2^31 bytes per head");
   const int64_t blocks = (p.S + kAttnRows - 1) / kAttnRows;
   if (p.S > (int64_t{1} << 27) || p.B > (int64_t{1} << 24) || p.H > (int64_t{1} << 24) ||

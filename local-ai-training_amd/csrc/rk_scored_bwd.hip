@@ -279,7 +279,8 @@ __global__ __launch_bounds__(1024) void scored_slope_kernel(ScoredBwdArgs ba) {
 }
 
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(D == 64 && !CAP ? 3 : 2, D == 64 && !CAP ? 3 : 2)))
 void scored_dkv_kernel(ScoredBwdArgs ba) {
   using T = AttnTile<D, kBwdRows>;
   constexpr int STAGE = 2 * T::BYTES + 256;  // two tiles, 32 log-sum-exp terms, 32 -delta

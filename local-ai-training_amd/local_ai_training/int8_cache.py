@@ -4,7 +4,8 @@ The bf16 cache of ``model.KVCache`` holds 4 bytes per feature of a token and hea
 2, plus one float32 scale per 64 tokens for each of keys and values. A block's scale is its
 largest absolute value / 127 and a code is ``rint(x / scale)``, so a value is off by at most half
 a scale when it is written. Tokens appended to a block that holds some can raise its scale; its
-codes are then rounded again, each time by at most half the scale of that time.
+codes are then rounded again, each time by at most half the scale of that time. A sequence ends
+with the tokens appended last: positions behind them in their block no longer hold anything.
 
 Positions are device tensors (int64, one for the batch or one per sequence), so steps have fixed
 shapes and can be replayed as a HIP graph, and sequences may have different lengths. A negative
@@ -97,12 +98,14 @@ def int8_kv_attention(q: Tensor, cache: Int8KV, start: Tensor, *, lengths: Tenso
     sequence stands at position ``start`` + i and sees positions 0 .. ``start`` + i, which must
     have been appended. The score's cap, bias and scale are those of ``scored_attention``.
     Returns [B, Hq, S, D] in ``out_dtype`` (default q's); queries at or past ``lengths`` are
-    zeros. Not differentiable."""
+    zeros. It has no gradient."""
     b, h, _, _, d = cache.keys.shape
     if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or q.shape[1] % h:
         raise ValueError("q must be [B, Hq, S, D] with heads a multiple of the cache's")
     if not q.is_floating_point():
         raise TypeError("q must be floating point")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("attention over an 8-bit cache has no gradient; call it under no_grad")
     if q.device != cache.keys.device:
         raise ValueError("q must be on the cache's device")
     out_dtype = out_dtype or q.dtype
@@ -110,7 +113,6 @@ def int8_kv_attention(q: Tensor, cache: Int8KV, start: Tensor, *, lengths: Tenso
         raise TypeError("out_dtype must be floating point")
     _check_positions(cache, start, lengths)
     softcap, slopes, scale = score_arguments(q, softcap, slopes, scale)
-    q = q.detach()
     if q.dtype not in (torch.float32, torch.bfloat16):
         q = q.float()
     native = out_dtype if out_dtype in (torch.float32, torch.bfloat16) else torch.float32

@@ -99,6 +99,12 @@ def test_shared_key_heads(cuda, h, hkv, d):
     compare(cuda, 1, h, hkv, 65, d, "", 0.0, False)
 
 
+@pytest.mark.parametrize("b,h", [(128, 8), (64, 16)])
+def test_shared_key_heads_of_large_batches(cuda, b, h):
+    """The query heads of a key head in one workgroup, and in parts of two (small batches: one)."""
+    compare(cuda, b, h, 4, 130, 64, "documents", 0.0, True)
+
+
 def test_scores_that_saturate_the_cap(cuda):
     compare(cuda, 1, 2, 2, 200, 128, "documents", 4.0, True, std=4.0)
 
