@@ -77,7 +77,8 @@ __device__ __forceinline__ float near_capped(const ScoredBwdArgs& a, float x, fl
 template <int D, bool CAP, bool BIAS, bool SG>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void scored_dq_kernel(ScoredBwdArgs ba) {
-  using T = AttnTile<D, kBwdRows>;
+  constexpr int R = D == 64 ? 64 : 32;  // staged keys per step; 32 at a time are computed
+  using T = AttnTile<D, R>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kAttnStages * 2 * T::BYTES];
   __shared__ int box[8];
   const uint32_t lds0 = lds_address(smem);
@@ -99,16 +100,16 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   const WaveSpan ws(span);
   int lo, hi;
   block_range(ws, wave, lane, box, lo, hi);
-  const int first = lo < hi ? lo / kBwdRows : 0;
-  const int end = lo < hi ? (hi + kBwdRows - 1) / kBwdRows : 0;
+  const int first = lo < hi ? lo / R : 0;
+  const int end = lo < hi ? (hi + R - 1) / R : 0;
   const uint32_t width = static_cast<uint32_t>(span.hi - span.lo);
 
-  const TileDma<D, kBwdRows> kd(p.k + b * p.skb + kvh * p.skh, p.sks, S, wave, lane);
-  const TileDma<D, kBwdRows> vd(p.v + b * p.svb + kvh * p.svh, p.svs, S, wave, lane);
+  const TileDma<D, R> kd(p.k + b * p.skb + kvh * p.skh, p.sks, S, wave, lane);
+  const TileDma<D, R> vd(p.v + b * p.svb + kvh * p.svh, p.svs, S, wave, lane);
   auto issue = [&](int step) {
     const uint32_t st = lds0 + (step & 1) * 2 * T::BYTES;
-    kd.issue(st, step * kBwdRows, wave);
-    vd.issue(st + T::BYTES, step * kBwdRows, wave);
+    kd.issue(st, step * R, wave);
+    vd.issue(st + T::BYTES, step * R, wave);
   };
   if (first < end) issue(first);  // under way while delta is formed
 
@@ -153,92 +154,96 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   for (int dt = 0; dt < D / 32; ++dt) dq[dt] = v16f_a{};
   float s_pd = 0.0f, s_pa = 0.0f, s_pda = 0.0f;  // sums of p dp, p |i - j|, p dp |i - j|
   for (int step = first; step < end; ++step) {
-    const uint64_t pad = padding_bits<kBwdRows>(a, b, step * kBwdRows);
+    const uint64_t pad = padding_bits<R>(a, b, step * R);
     dma_wait_barrier<0>();
     if (step + 1 < end) issue(step + 1);
     uint8_t* const kt = smem + (step & 1) * 2 * T::BYTES;
     uint8_t* const vt = kt + T::BYTES;
     if (pad) {  // the keys meet gradients of zero
-      clear_rows<D, kBwdRows>(kt, pad, tid);
+      clear_rows<D, R>(kt, pad, tid);
       __syncthreads();
     }
-    const int key0 = step * kBwdRows;
-    if (ws.none(key0, kBwdRows)) continue;
-    v16f_a st;
+    // (64 staged at head size 128 too: 65 -> 77 us with a bias and slope gradients at B 4, S 1001)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) st[e] = CAP ? 0.0f : term;
+    for (int sub = 0; sub < R; sub += 32) {
+      const int key0 = step * R + sub;
+      if (ws.none(key0, 32)) continue;
+      v16f_a st;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s)
-      st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, 0, s, lane), qf[s], st,
-                                                   0, 0, 0);
-    // the probabilities times the cap's slope (with slope gradients: apart)
-    const bool whole = ws.all(key0, kBwdRows);
-    const int j0 = key0 + 4 * h - span.lo;
-    const float d0 = static_cast<float>(qi - key0 - 4 * h);
-    float slack[CAP && SG ? 16 : 1];
-    bool near = false;
-    if constexpr (CAP && SG) {
-      float most = 0.0f;
+      for (int e = 0; e < 16; ++e) st[e] = CAP ? 0.0f : term;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(st[e]));
-      near = !__any(most > ba.near_limit);
-    }
-    if (near) {  // (never without slope gradients)
+      for (int s = 0; s < D / 16; ++s)
+        st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, sub, s, lane), qf[s], st,
+                                                     0, 0, 0);
+      // the probabilities times the cap's slope (with slope gradients: apart)
+      const bool whole = ws.all(key0, 32);
+      const int j0 = key0 + 4 * h - span.lo;
+      const float d0 = static_cast<float>(qi - key0 - 4 * h);
+      float slack[CAP && SG ? 16 : 1];
+      bool near = false;
+      if constexpr (CAP && SG) {
+        float most = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(st[e]));
+        near = !__any(most > ba.near_limit);
+      }
+      if (near) {  // (never without slope gradients)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float sl;
+          const float t = near_capped(ba, st[e], sl) - term;
+          const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
+          st[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(-slope2, dist, t));
+          if constexpr (CAP && SG) slack[e] = sl;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float sl;
+          st[e] = score_p<CAP, BIAS>(a, st[e], term, slope2,
+                                     d0 - static_cast<float>(8 * (e / 4) + (e % 4)), sl);
+          if constexpr (CAP && SG) slack[e] = sl;
+          else if constexpr (CAP) st[e] = st[e] * sl;
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) st[e] = 0.0f;
+      }
+      v16f_a dp;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[e] = ndelta;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(vt, sub, s, lane), gf[s], dp,
+                                                     0, 0, 0);
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) dp[e] = 0.0f;
+      }
+      float ds[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        float sl;
-        const float t = near_capped(ba, st[e], sl) - term;
-        const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
-        st[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(-slope2, dist, t));
-        if constexpr (CAP && SG) slack[e] = sl;
+        ds[e] = st[e] * dp[e];
+        if constexpr (SG) {
+          const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
+          s_pd = s_pd + ds[e];
+          s_pa = __builtin_fmaf(st[e], dist, s_pa);
+          s_pda = __builtin_fmaf(ds[e], dist, s_pda);
+          if constexpr (CAP) ds[e] = ds[e] * slack[e];
+        }
       }
-    } else {
+      uint4 dsf[2];
+      pack16(dsf, ds);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float sl;
-        st[e] = score_p<CAP, BIAS>(a, st[e], term, slope2,
-                                   d0 - static_cast<float>(8 * (e / 4) + (e % 4)), sl);
-        if constexpr (CAP && SG) slack[e] = sl;
-        else if constexpr (CAP) st[e] = st[e] * sl;
-      }
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+          dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              col_frag<D>(kt, sub + 16 * s2, dt, lane), frag_of(dsf[s2]), dq[dt], 0, 0, 0);
     }
-    if (!whole) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) st[e] = 0.0f;
-    }
-    v16f_a dp;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) dp[e] = ndelta;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s)
-      dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(vt, 0, s, lane), gf[s], dp,
-                                                   0, 0, 0);
-    if (!whole) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) dp[e] = 0.0f;
-    }
-    float ds[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      ds[e] = st[e] * dp[e];
-      if constexpr (SG) {
-        const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
-        s_pd = s_pd + ds[e];
-        s_pa = __builtin_fmaf(st[e], dist, s_pa);
-        s_pda = __builtin_fmaf(ds[e], dist, s_pda);
-        if constexpr (CAP) ds[e] = ds[e] * slack[e];
-      }
-    }
-    uint4 dsf[2];
-    pack16(dsf, ds);
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-        dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            col_frag<D>(kt, 16 * s2, dt, lane), frag_of(dsf[s2]), dq[dt], 0, 0, 0);
   }
   if (!span.valid) {
 #pragma unroll
