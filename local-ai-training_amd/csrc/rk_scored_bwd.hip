@@ -175,42 +175,9 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
       for (int s = 0; s < D / 16; ++s)
         st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, sub, s, lane), qf[s], st,
                                                      0, 0, 0);
-      // the probabilities times the cap's slope (with slope gradients: apart)
       const bool whole = ws.all(key0, 32);
       const int j0 = key0 + 4 * h - span.lo;
       const float d0 = static_cast<float>(qi - key0 - 4 * h);
-      float slack[CAP && SG ? 16 : 1];
-      bool near = false;
-      if constexpr (CAP && SG) {
-        float most = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(st[e]));
-        near = !__any(most > ba.near_limit);
-      }
-      if (near) {  // (never without slope gradients)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float sl;
-          const float t = near_capped(ba, st[e], sl) - term;
-          const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
-          st[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(-slope2, dist, t));
-          if constexpr (CAP && SG) slack[e] = sl;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float sl;
-          st[e] = score_p<CAP, BIAS>(a, st[e], term, slope2,
-                                     d0 - static_cast<float>(8 * (e / 4) + (e % 4)), sl);
-          if constexpr (CAP && SG) slack[e] = sl;
-          else if constexpr (CAP) st[e] = st[e] * sl;
-        }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) st[e] = 0.0f;
-      }
       v16f_a dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[e] = ndelta;
@@ -218,21 +185,51 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
       for (int s = 0; s < D / 16; ++s)
         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(vt, sub, s, lane), gf[s], dp,
                                                      0, 0, 0);
+      // the masks in one uniform branch ahead of straight arithmetic (a masked score of -inf
+      // gives p = 0, a capped one the cap's end, whose gradient is zero with dp)
       if (!whole) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) dp[e] = 0.0f;
+          if (static_cast<uint32_t>(j0 + 8 * (e / 4) + (e % 4)) >= width) {
+            st[e] = -INFINITY;
+            dp[e] = 0.0f;
+          }
+      }
+      bool near = false;
+      if constexpr (CAP && SG) {
+        float most = 0.0f;  // of the scores that count
+#pragma unroll
+        for (int e = 0; e < 16; ++e) most = fmaxf(most, st[e] == -INFINITY ? 0.0f : fabsf(st[e]));
+        near = !__any(most > ba.near_limit);
       }
       float ds[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        ds[e] = st[e] * dp[e];
+      const auto gradient = [&](int e, float p1, float sl) {
+        ds[e] = p1 * dp[e];
         if constexpr (SG) {
           const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
+          const float p2 = CAP && st[e] == -INFINITY ? 0.0f : p1;
           s_pd = s_pd + ds[e];
-          s_pa = __builtin_fmaf(st[e], dist, s_pa);
+          s_pa = __builtin_fmaf(p2, dist, s_pa);
           s_pda = __builtin_fmaf(ds[e], dist, s_pda);
-          if constexpr (CAP) ds[e] = ds[e] * slack[e];
+        }
+        if constexpr (CAP) ds[e] = ds[e] * sl;
+      };
+      if (near) {  // (never without slope gradients)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float sl;
+          const float y = st[e] == -INFINITY ? 0.0f : st[e];
+          const float t = near_capped(ba, y, sl) - term;
+          const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
+          gradient(e, __builtin_amdgcn_exp2f(__builtin_fmaf(-slope2, dist, t)), sl);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float sl;
+          const float p1 = score_p<CAP, BIAS>(
+              a, st[e], term, slope2, d0 - static_cast<float>(8 * (e / 4) + (e % 4)), sl);
+          gradient(e, p1, sl);
         }
       }
       uint4 dsf[2];
@@ -394,34 +391,6 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
     for (int s = 0; s < D / 16; ++s)
       st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(qt, 0, s, lane), kf[s], st,
                                                    0, 0, 0);
-    const bool whole = ws.all(qs, kBwdRows);
-    const int i0 = qs + 4 * h - span.lo;
-    const float d0 = static_cast<float>(qs + 4 * h - kj);
-    // the probabilities, packed, and times the cap's slope
-    uint4 pf[2], dsf[2];
-    {
-      float pr[16];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float4 term{};
-        if constexpr (CAP) term = *reinterpret_cast<const float4*>(rows + 8 * r + 4 * h);
-        const float t4[4] = {term.x, term.y, term.z, term.w};
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int e = 4 * r + x;
-          float sl;
-          pr[e] = score_p<CAP, BIAS>(a, st[e], t4[x], slope2,
-                                     d0 + static_cast<float>(8 * r + x), sl);
-          st[e] = CAP ? pr[e] * sl : pr[e];
-        }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width) st[e] = pr[e] = 0.0f;
-      }
-      pack16(pf, pr);
-    }
     v16f_a dp;
     row_terms(1, dp);
 #pragma unroll
@@ -429,17 +398,54 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
       dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(gt, 0, s, lane),
                                                    row_frag<D>(smem, 32 * wave, s, lane), dp,
                                                    0, 0, 0);
+    // the masks sit in one uniform branch ahead of straight arithmetic: with the probabilities
+    // formed before the second product, and the masks on them, the loop spilled or took a
+    // quarter longer. A masked score of -inf gives p = 0; a capped one gives the cap's end, with
+    // slope 0, and its p is cleared below.
+    const bool whole = ws.all(qs, kBwdRows);
+    const int i0 = qs + 4 * h - span.lo;
     if (!whole) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width) dp[e] = 0.0f;
+        if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width) {
+          st[e] = -INFINITY;
+          dp[e] = 0.0f;
+        }
     }
-    {
-      float ds[16];
+    const float d0 = static_cast<float>(qs + 4 * h - kj);
+    uint4 pf[2], dsf[2];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ds[e] = st[e] * dp[e];
-      pack16(dsf, ds);
+    for (int s2 = 0; s2 < 2; ++s2) {
+      float pr[8], ds[8];
+#pragma unroll
+      for (int r = 2 * s2; r < 2 * s2 + 2; ++r) {
+        float4 term{};
+        if constexpr (CAP) term = *reinterpret_cast<const float4*>(rows + 8 * r + 4 * h);
+        const float t4[4] = {term.x, term.y, term.z, term.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int e = 4 * r + x;
+          float sl;
+          const float p1 = score_p<CAP, BIAS>(a, st[e], t4[x], slope2,
+                                              d0 + static_cast<float>(8 * r + x), sl);
+          pr[e - 8 * s2] = p1;
+          ds[e - 8 * s2] = (CAP ? p1 * sl : p1) * dp[e];
+        }
+      }
+      pf[s2] = make_uint4(bf16_pair(pr[0], pr[1]), bf16_pair(pr[2], pr[3]),
+                          bf16_pair(pr[4], pr[5]), bf16_pair(pr[6], pr[7]));
+      dsf[s2] = make_uint4(bf16_pair(ds[0], ds[1]), bf16_pair(ds[2], ds[3]),
+                           bf16_pair(ds[4], ds[5]), bf16_pair(ds[6], ds[7]));
     }
+    if constexpr (CAP)
+      if (!whole) {
+        uint32_t* const w[8] = {&pf[0].x, &pf[0].y, &pf[0].z, &pf[0].w,
+                                &pf[1].x, &pf[1].y, &pf[1].z, &pf[1].w};
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width)
+            *w[e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
+      }
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
