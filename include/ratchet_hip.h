@@ -725,8 +725,8 @@ int rk_attention_mask(const void* documents, int wide, int64_t sdb, const uint8_
  * rest, written by the forward and read by the backward (a byte per element, in an order of its
  * own), makes delta = g . o exact to 2^-16 of o.
  * The backward reads o, lse and the gradient g of o, and writes dq, dk, dv and, where given,
- * dslopes (float32 [H]); work: rk_scored_attention_backward_work floats, 16-byte aligned. Scores and softmax run
- * in float32; probabilities and score gradients enter the products rounded to bf16; every sum
+ * dslopes (float32 [H]); work: rk_scored_attention_backward_work floats, 16-byte aligned. Scores
+ * and softmax run in float32; probabilities and score gradients enter the products rounded to bf16; every sum
  * has a fixed order. Inputs 16-byte aligned, outputs 8-byte, strides multiples of 8 elements, one
  * head's positions under 2^31 bytes, fewer than 2^24 blocks of 128 positions; otherwise
  * RK_ERR_UNSUPPORTED.
@@ -791,9 +791,10 @@ int rk_int8_kv_read(const rk_int8_kv* cache, int64_t begin, int64_t end, int dty
  * which must have been appended. Scores, softcap and slopes (float32 [Hq]) as in
  * rk_scored_attention_forward. out: [B, S, Hq, D] contiguous, float32 or bf16; zeros for queries
  * at or past lengths and for negative starts, NaN for positions past the cache. The products run
- * in integers on the codes, with queries and probabilities rounded to 23 bits of their row's and
- * block's largest; chunks of 32 bf16 tokens and more with bf16 results take bf16 products, with
- * the probabilities rounded to bf16. work: rk_int8_kv_attention_work floats (0: none), 16-byte aligned.
+ * in integers on the codes, with queries and probabilities rounded to 23 bits (15 for bf16 results)
+ * of their row's and block's largest; chunks of 32 bf16 tokens and more with bf16 results take bf16
+ * products, with the probabilities rounded to bf16. work: rk_int8_kv_attention_work floats (0:
+ * none), 16-byte aligned.
  * No counterpart in the reference (its window is recomputed per token, generate.py:183-201).
  */
 int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S, int qdtype,

@@ -1138,10 +1138,9 @@ rk_scored_attention_args scored_args(const Tensor& q, const Tensor& k, const Ten
 
 // Attention with modified scores (rk_scored_attention_forward): (o, lse, rest), o as a
 // [B, H, S, D] view of [B, S, H, D] memory; rest, for the backward, is empty unless `grad`.
-std::tuple<Tensor, Tensor, Tensor> scored_attention(const Tensor& q, const Tensor& k, const Tensor& v,
-                                            const OptTensor& bounds, const OptTensor& padding,
-                                            const OptTensor& slopes, double softcap,
-                                            double scale, bool grad) {
+std::tuple<Tensor, Tensor, Tensor> scored_attention(
+    const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bounds,
+    const OptTensor& padding, const OptTensor& slopes, double softcap, double scale, bool grad) {
   std::vector<Tensor> keep;
   rk_scored_attention_args a = scored_args(q, k, v, bounds, padding, slopes, softcap, scale, keep);
   const c10::DeviceGuard guard(q.device());
@@ -1375,7 +1374,9 @@ std::tuple<Tensor, Tensor> int8_kv_read(const Tensor& keys, const Tensor& values
   TORCH_CHECK(begin >= 0 && begin <= end && end <= c.blocks * 64,
               "int8 kv read: positions past the cache");
   const c10::DeviceGuard guard(keys.device());
-  const auto out = [&] { return at::empty({c.B, c.H, end - begin, c.D}, keys.options().dtype(dtype)); };
+  const auto out = [&] {
+    return at::empty({c.B, c.H, end - begin, c.D}, keys.options().dtype(dtype));
+  };
   Tensor k = out(), v = out();
   check_status(rk_int8_kv_read(&c, begin, end, code, k.data_ptr(), v.data_ptr(), stream_of(keys)),
                "rk_int8_kv_read");

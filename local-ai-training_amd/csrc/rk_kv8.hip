@@ -19,7 +19,7 @@
 namespace rk {
 
 constexpr int kTok = 64;  // tokens of a block
-constexpr int64_t kChunkTokens = 32;  // chunks from here on take kv8_chunk_kernel
+constexpr int64_t kChunkTokens = 32;  // a wavefront's queries: from here on kv8_chunk_kernel
 constexpr float kLog2e8 = 1.4426950408889634f;
 
 typedef int v4i8 __attribute__((ext_vector_type(4)));
@@ -87,7 +87,9 @@ __device__ __forceinline__ int code_again(int c, float ratio) {
 
 // grid (touched blocks, B * H, 2: keys, values), 256 threads; a thread takes D / 32 pieces of 8
 // features. The block's absmax by the bits of |x| (a NaN is the largest), so a block that takes
-// in a NaN or an infinity has such a scale and reads back as NaN.
+// in a NaN or an infinity has such a scale and reads back as NaN. 4 x 777 tokens, 16 heads of 128:
+// 14.8 us for 39 MB (a load, a reduction and a store in workgroups that are all resident at once;
+// 262 MB of float32 80 us, 4.1 TB/s); a token for 16 sequences 5.4 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   constexpr int PER = D / 8, EACH = kTok * PER / 256, PITCH = kTok + 4;
@@ -205,7 +207,8 @@ struct Kv8Read {
   void* values;
 };
 
-// grid (blocks, B * H, 2), 256 threads: the values codes stand for, code x scale in float32.
+// grid (blocks, B * H, 2), 256 threads: the values codes stand for, code x scale in float32. Bound
+// by its bytes: 64 MB, mostly written, in 12.5 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a) {
   constexpr int PER = D / 8, PITCH = kTok + 4;
@@ -265,13 +268,18 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a) {
 // bits, about a float32 operand's rounding) for float32 results, two (15 bits, against the 8 of
 // the result) for bf16. The matrix unit takes them at a
 // fraction of the time the codes need to arrive, and no code is ever converted: for one query
-// per head, 48 MFMAs and about 500 vector instructions per 16 KB of codes at D = 128.
+// per head, 32 MFMAs (48 with three digits) and a few hundred vector instructions per 16 KB of
+// codes at D = 128.
 //
 // A wavefront walks blocks of 64 tokens with its own running max, sum and output. Lane l holds the
 // scores of column l % 16 against keys 16 (l / 16) .. + 15: key 16 g + 4 t + e is row 4 g + e of
 // product t, and the same 16 keys are the lane's k slots of the second product, whose other
-// operand, 16 tokens of one feature, lies side by side in the cache. The four wavefronts of a
+// operand, 16 tokens of one feature, lies side by side in the cache. The wavefronts of a
 // workgroup are joined in LDS, splits of a long cache by a second launch.
+//
+// 16 sequences of 5 to 16 thousand tokens, 16 heads of 128: 143-147 us, 820 MB of codes at 5.6 TB/s
+// (the device's own copy reaches 5.3); 48 sequences of 2.7 to 8.1 thousand, 32 heads of 64 on 4,
+// capped: 26 + 4 us for 125 MB; one of 1000, 16 heads of 128: 10.6 us, a chain of load latencies.
 // ---------------------------------------------------------------------------
 struct Kv8Attn {
   Kv8 c;
@@ -650,15 +658,20 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
 
 // ---------------------------------------------------------------------------
 // The same for chunks of many bf16 tokens with bf16 results (a prompt's next part): one workgroup
-// takes 128 queries of a head, a wavefront 32, and the products run on the bf16 MFMA as in
+// takes 128 queries of a head, in two halves of four wavefronts that walk every other block; a
+// wavefront takes 32 queries of its half, the halves are joined in LDS at the end, and the products run on the bf16 MFMA as in
 // rk_attention.hip (scores transposed, a lane holds one query). The codes become bf16 once per
-// workgroup and block, exactly (8 bits), on their way into LDS; the key scale goes into the score,
+// half and block, exactly (8 bits), on their way into LDS; the key scale goes into the score,
 // the value scale into the probabilities before they are rounded to bf16. Values lie by feature, so
 // the second product's operand is a row read too: the tokens of a row are stored in the order in
 // which a lane holds its probabilities. The next block's codes are in registers meanwhile.
 //
-// Codes converted by each reader instead, or the digits of kv8_attn_kernel for chunks too, cost
-// more: the latter 176 us at 4 x 517 tokens behind 1500, 16 heads of 128, where this takes QQQ.
+// 4 x 517 tokens behind 1500, 16 heads of 128 (30 GFLOP): 72 us and 5 for the last tile's join; the
+// digits of kv8_attn_kernel 176. A last tile of few queries is split over the keys (attention_plan):
+// its workgroups were 25 of 96 us. Four wavefronts without the halves 82-86; the next block converted
+// between the two products instead of behind them 99. The wavefronts of a half keep step with each
+// other, so its MFMAs (1024 cycles a block and wavefront) and its vector instructions (590) overlap
+// little: those two are what it spends its time on.
 // ---------------------------------------------------------------------------
 template <bool SCALED = false>
 __device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi,
@@ -996,6 +1009,9 @@ static Kv8Plan attention_plan(const rk_int8_kv& c, int64_t Hq, int64_t S, int qd
     return n < 1 || most < 1 ? 1 : n < most ? n : most;
   };
   if (!p.chunk) {
+    // few workgroups: eight wavefronts in each, so that up to 16 blocks need no join (16 heads of
+    // 1000 tokens 10.6 us; four wavefronts in four splits 6.7 + 4.0); otherwise as many
+    // workgroups as the device holds (twice as many gained nothing)
     p.waves = have <= 128 ? 8 : 4;
     p.splits = splits(c.D == 64 ? 1024 : 512, p.waves == 8 ? 16 : 4);
     return p;

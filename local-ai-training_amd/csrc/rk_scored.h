@@ -75,7 +75,9 @@ struct WaveSpan {
       s.hi = 0x7fffffff;
     }
   }
-  __device__ __forceinline__ bool none(int r0, int rows) const { return r0 >= hi || r0 + rows <= lo; }
+  __device__ __forceinline__ bool none(int r0, int rows) const {
+    return r0 >= hi || r0 + rows <= lo;
+  }
   __device__ __forceinline__ bool all(int r0, int rows) const {
     return r0 >= all_lo && r0 + rows <= all_hi;
   }

@@ -11,6 +11,13 @@
 //    workgroup are neither loaded nor computed; a wavefront skips tiles none of its rows sees and
 //    tests elements only in tiles that some row does not see whole;
 //  * capped or biased scores are modified before the running max, in base-2 units (rk_scored.h).
+//
+// B 8, H 16, S 1024, D 128: causal 68 us (34 GFLOP, 510 TFLOP/s; rk_attention_forward 55-60), in
+// documents of 400 on average 44, with capped scores 69 and 50; B 32, H 8, S 512, D 64 in
+// documents of 150 20.6 us, where reading q, k, v and writing o and its rest takes 16 at 5.3 TB/s.
+// The vector unit is busy half of the time (829 instructions a step of 64 keys, capped), the
+// matrix unit an eighth: what is left is waiting between a step's dependent parts, and
+// wavefronts of a workgroup that wait for the one whose rows see most.
 #include "rk_scored.h"
 
 namespace rk {
@@ -197,8 +204,8 @@ void scored_fwd_kernel(ScoredArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The plan: one workgroup per row, a thread 8 consecutive positions of a chunk of 8 * NT, scans over
-// the threads' values by wavefront shuffles. From the left: the document's first position and
+// The plan: one workgroup per row, a thread 8 consecutive positions of a chunk of 8 * NT, scans
+// over the threads' values by wavefront shuffles. From the left: the document's first position and
 // whether the run of marked positions it begins with reaches here; from the right: the
 // document's end and the end of that run. Up to one chunk the first pass stays in registers.
 // (In 8-byte loads and stores of one position each, and through memory between the passes, a row
@@ -219,7 +226,8 @@ struct MaskArgs {
 // Two max scans over the threads of the workgroup, left to right or (BACK) right to left: each
 // thread's x, y become those of the threads before it, tx, ty those of all. box: 2 NT / 64 ints.
 template <int NT, bool BACK>
-__device__ __forceinline__ void block_scan_max(int& x, int& y, int& tx, int& ty, int* box, int tid) {
+__device__ __forceinline__ void block_scan_max(int& x, int& y, int& tx, int& ty, int* box,
+                                               int tid) {
   constexpr int NW = NT / 64, kNone = -0x7fffffff;
   const int lane = tid & 63, wave = tid >> 6;
   const int turn = BACK ? 63 - lane : lane, place = BACK ? NW - 1 - wave : wave;
@@ -500,7 +508,8 @@ extern "C" int rk_scored_attention_forward(const rk_scored_attention_args* args,
   const rk_scored_attention_args& p = *args;
   if (int e = check_scored(p, false)) return e;
   if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
-  if (reinterpret_cast<uintptr_t>(p.o) & 7) return fail(RK_ERR_UNSUPPORTED, "o needs 8-byte alignment");
+  if (reinterpret_cast<uintptr_t>(p.o) & 7)
+    return fail(RK_ERR_UNSUPPORTED, "o needs 8-byte alignment");
   const ScoredArgs a = scored_args(p);
   const dim3 grid(static_cast<unsigned>(p.B * p.H * (a.Sp / kAttnRows)));
   if (p.D == 64) launch_scored_fwd<64, 64, 64>(a, grid, as_stream(stream));

@@ -174,7 +174,8 @@ def check_attention(q, cache, start, lengths=None, cap=0.0, slopes=None, out_dty
         p = s.masked_fill(unseen, -math.inf).softmax(-1)
         want = p @ v
         bound = ((2 * delta.masked_fill(unseen, 0.0).amax(-1, keepdim=True) + 2.0**-20
-                  + (2.0**-8 if rounded else 0.0)) * (p @ v.abs()) + 2.0**(5 - r) * v.abs().amax() + step * want.abs())
+                  + (2.0**-8 if rounded else 0.0)) * (p @ v.abs())
+                 + 2.0**(5 - r) * v.abs().amax() + step * want.abs())
         worst = ((got[b, :, :n].double() - want).abs() - bound).max().item()
         assert worst <= 0.0, (b, p0, worst)
 

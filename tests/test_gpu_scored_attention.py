@@ -303,7 +303,8 @@ def test_the_library_refuses(cuda):
     ops = ratchet()
     mask = attention_mask(torch.zeros(1, 8, dtype=torch.int32, device=cuda))
     with pytest.raises(RuntimeError, match="head size"):
-        ops.scored_attention(q[..., :32], q[..., :32], q[..., :32], None, None, None, 0.0, 1.0, False)
+        x = q[..., :32]
+        ops.scored_attention(x, x, x, None, None, None, 0.0, 1.0, False)
     with pytest.raises(RuntimeError, match="scale"):
         ops.scored_attention(q, q, q, None, None, None, 0.0, -1.0, False)
     with pytest.raises(RuntimeError, match="softcap"):
