@@ -34,7 +34,8 @@ __device__ __forceinline__ float half_sum2(float v) {
 }
 
 // R keys are staged per step, U of them make one update of the running max and sum.
-template <int D, int R, int U, bool CAP, bool BIAS>
+// FINE: capped and biased scores of a pass whose gradients are wanted (near_capped).
+template <int D, int R, int U, bool CAP, bool BIAS, bool FINE = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4)))
 void scored_fwd_kernel(ScoredArgs a) {
   using T = AttnTile<D, R>;
@@ -103,19 +104,39 @@ void scored_fwd_kernel(ScoredArgs a) {
     const float mul = CAP || BIAS ? 1.0f : a.dot_scale;
     if constexpr (CAP || BIAS) {
       const float d0 = static_cast<float>(qi - k0 - 4 * h);
+      bool near = false;
+      if constexpr (FINE) {
+        float most = 0.0f;
 #pragma unroll
-      for (int t = 0; t < R / 32; ++t)
+        for (int t = 0; t < R / 32; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x = sc[t][e] * a.dot_scale;
-          if constexpr (CAP) {
-            const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f);
-            x = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
+          for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(sc[t][e]));
+        near = !__any(most > a.near_limit);
+      }
+      if (near) {
+#pragma unroll
+        for (int t = 0; t < R / 32; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float slack;
+            sc[t][e] = __builtin_fmaf(-slope2, fabsf(d0 - (32 * t + 8 * (e / 4) + (e % 4))),
+                                      near_capped(a, sc[t][e], slack));
           }
-          if constexpr (BIAS)
-            x = __builtin_fmaf(-slope2, fabsf(d0 - (32 * t + 8 * (e / 4) + (e % 4))), x);
-          sc[t][e] = x;
-        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < R / 32; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x = sc[t][e] * a.dot_scale;
+            if constexpr (CAP) {
+              const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f);
+              x = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
+            }
+            if constexpr (BIAS)
+              x = __builtin_fmaf(-slope2, fabsf(d0 - (32 * t + 8 * (e / 4) + (e % 4))), x);
+            sc[t][e] = x;
+          }
+      }
     }
     if (!ws.all(k0, R)) {
       const int j0 = k0 + 4 * h - span.lo;
@@ -481,13 +502,27 @@ ScoredArgs scored_args(const rk_scored_attention_args& p) {
   const bool cap = p.softcap > 0.0f;
   a.dot_scale = cap ? 2.0f * kLog2e * (p.scale / p.softcap) : p.scale * kLog2e;
   a.cap2 = p.softcap * kLog2e;
+  if (cap) {
+    const double c2 = static_cast<double>(a.cap2), step = 1.0 / (c2 * c2);
+    const double fit[4] = {-0.3333323001861572, 0.13327749073505402, -0.053165826946496964,
+                           0.0174802765250206};
+    double power = step;
+    for (int i = 0; i < 4; ++i, power *= step) a.near[i] = static_cast<float>(fit[i] * power);
+    a.near_scale = p.scale * kLog2e;
+    // caps whose powers leave float32's range: always the exponential
+    const bool fits = p.softcap > 1e-3f && p.softcap < 1e3f;
+    a.near_limit = fits ? 0.5f * p.softcap / p.scale : -1.0f;
+    a.inv_cap2 = static_cast<float>(1.0 / c2);
+  }
   return a;
 }
 
 template <int D, int R, int U>
 static void launch_scored_fwd(const ScoredArgs& a, dim3 grid, hipStream_t st) {
   const bool cap = a.p.softcap > 0.0f, bias = a.p.slopes != nullptr;
-  if (cap && bias) scored_fwd_kernel<D, R, U, true, true><<<grid, 256, 0, st>>>(a);
+  if (cap && bias && a.p.rest)
+    scored_fwd_kernel<D, R, U, true, true, true><<<grid, 256, 0, st>>>(a);
+  else if (cap && bias) scored_fwd_kernel<D, R, U, true, true><<<grid, 256, 0, st>>>(a);
   else if (cap) scored_fwd_kernel<D, R, U, true, false><<<grid, 256, 0, st>>>(a);
   else if (bias) scored_fwd_kernel<D, R, U, false, true><<<grid, 256, 0, st>>>(a);
   else scored_fwd_kernel<D, R, U, false, false><<<grid, 256, 0, st>>>(a);

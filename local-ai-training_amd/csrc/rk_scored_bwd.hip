@@ -32,9 +32,6 @@ namespace rk {
 struct ScoredBwdArgs {
   ScoredArgs f;
   float inv_scale;  // 1 / scale
-  // capped scores, with slope gradients: scale log2(e), the largest |x| of the polynomial below,
-  // its coefficients by C^-2, C^-4, .. (C = cap log2(e)), and 1 / C
-  float near_scale, near_limit, near[4], inv_cap2;
   float* rows;      // [B H][2][Sp]: log-sum-exp term and -delta (zeros where a row is none)
   float* slope_rows;  // [B H][Sp], or null
   // the query heads of a key head in `parts` workgroups each: their float32 dk, dv [parts][2]
@@ -64,22 +61,6 @@ __device__ __forceinline__ float score_p(const ScoredArgs& a, float x, float ter
           __builtin_fmaf(-slope2, fabsf(dist), x * a.dot_scale));
     return __builtin_amdgcn_exp2f(x * a.dot_scale);
   }
-}
-
-// The capped score in base-2 units by an odd polynomial, y + y z (c1 + c2 z + c3 z^2 + c4 z^3) with
-// y = x scale log2(e), z = y^2: tanh(u) / u fitted by least squares at Chebyshev nodes of
-// |u| <= 1/2, off by 2e-8 there. The exponential form is off by 2^-24 of the cap whatever the
-// score, which the slopes' gradient, a float32 sum over all pairs, shows: 3e-6 of its norm at
-// caps of 50 to 100, against 1.0e-6 to 1.4e-6. The other kernels, whose results are bf16, keep the
-// exponential: with a branch between the two forms they were slower, the forward by a fifth.
-__device__ __forceinline__ float near_capped(const ScoredBwdArgs& a, float x, float& slack) {
-  const float y = x * a.near_scale, z = y * y;
-  float q = __builtin_fmaf(a.near[3], z, a.near[2]);
-  q = __builtin_fmaf(q, z, a.near[1]);
-  q = __builtin_fmaf(q, z, a.near[0]);
-  const float t = __builtin_fmaf(y, z * q, y), th = t * a.inv_cap2;
-  slack = __builtin_fmaf(-th, th, 1.0f);
-  return t;
 }
 
 template <int D, bool CAP, bool BIAS, bool SG>
@@ -147,7 +128,10 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
   }
   dot = dot + __shfl_xor(dot, 32, kWave);
   const float lse = span.valid ? p.lse[bh * S + qi] : 0.0f;
+  // for the keys' launch, as score_p takes it there; this one subtracts lse after the product where
+  // the score is modified (a sum that begins at -lse / scale rounds to its size, 1e-6 of p)
   const float term = CAP ? lse * kLog2e : -lse * ba.inv_scale;
+  const float lse2 = lse * kLog2e;
   const float ndelta = span.valid ? -dot : 0.0f;
   if (h == 0) {  // Sp rows: the padded block's too
     float* const rows = ba.rows + bh * 2 * a.Sp + qi;
@@ -178,7 +162,7 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
       if (ws.none(key0, 32)) continue;
       v16f_a st;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) st[e] = CAP ? 0.0f : term;
+      for (int e = 0; e < 16; ++e) st[e] = CAP || BIAS ? 0.0f : term;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s)
         st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, sub, s, lane), qf[s], st,
@@ -208,7 +192,7 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
         float most = 0.0f;  // of the scores that count
 #pragma unroll
         for (int e = 0; e < 16; ++e) most = fmaxf(most, st[e] == -INFINITY ? 0.0f : fabsf(st[e]));
-        near = !__any(most > ba.near_limit);
+        near = !__any(most > a.near_limit);
       }
       float ds[16];
       const auto gradient = [&](int e, float p1, float sl) {
@@ -227,16 +211,21 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
         for (int e = 0; e < 16; ++e) {
           float sl;
           const float y = st[e] == -INFINITY ? 0.0f : st[e];
-          const float t = near_capped(ba, y, sl) - term;
+          const float t = near_capped(a, y, sl) - lse2;
           const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
           gradient(e, __builtin_amdgcn_exp2f(__builtin_fmaf(-slope2, dist, t)), sl);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float sl;
-          const float p1 = score_p<CAP, BIAS>(
-              a, st[e], term, slope2, d0 - static_cast<float>(8 * (e / 4) + (e % 4)), sl);
+          float sl = 1.0f;
+          const float dist = d0 - static_cast<float>(8 * (e / 4) + (e % 4));
+          float p1;
+          if constexpr (!CAP && BIAS)
+            p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(
+                -slope2, fabsf(dist), __builtin_fmaf(st[e], a.dot_scale, -lse2)));
+          else
+            p1 = score_p<CAP, BIAS>(a, st[e], lse2, slope2, dist, sl);
           gradient(e, p1, sl);
         }
       }
@@ -583,18 +572,6 @@ extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args
   ScoredBwdArgs a{};
   a.f = scored_args(p);
   a.inv_scale = 1.0f / p.scale;
-  if (p.softcap > 0.0f) {
-    const double c2 = static_cast<double>(a.f.cap2), step = 1.0 / (c2 * c2);
-    const double fit[4] = {-0.3333323001861572, 0.13327749073505402, -0.053165826946496964,
-                           0.0174802765250206};
-    double power = step;
-    for (int i = 0; i < 4; ++i, power *= step) a.near[i] = static_cast<float>(fit[i] * power);
-    a.near_scale = p.scale * kLog2e;
-    // caps whose powers leave float32's range: always the exponential
-    const bool fits = p.softcap > 1e-3f && p.softcap < 1e3f;
-    a.near_limit = fits ? 0.5f * p.softcap / p.scale : -1.0f;
-    a.inv_cap2 = static_cast<float>(1.0 / c2);
-  }
   a.rows = work;
   a.slope_rows = p.dslopes ? work + 2 * p.B * p.H * a.f.Sp : nullptr;
   a.parts = head_parts(p.B, p.H, p.Hkv, p.S);
