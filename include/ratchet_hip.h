@@ -718,7 +718,7 @@ int rk_attention_mask(const void* documents, int wide, int64_t sdb, const uint8_
  * (element strides batch, head, position; unit feature stride), H a multiple of Hkv (query head h
  * reads key head h / (H / Hkv)), D = 64 or 128. With bounds as rk_attention_mask writes them
  * (mask_batch 1 or B rows; NULL: causal),
- *   s_ij = scale q_i . k_j;  softcap > 0: s = softcap tanh(s / softcap);
+ *   s_ij = scale q_i . k_j;  softcap > 0 (1e-3 .. 1e3): s = softcap tanh(s / softcap);
  *   slopes (float32 [H]): s -= slopes[h] |i - j|;
  *   o_i = sum_j softmax_j(s_ij over the keys i sees) v_j,  lse_i = log sum_j exp(s_ij).
  * A query that sees nothing gets zeros (lse 0); what padding positions hold does not matter.

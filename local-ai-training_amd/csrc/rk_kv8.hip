@@ -1099,7 +1099,7 @@ extern "C" int rk_int8_kv_append(const rk_int8_kv* cache, const void* k, int64_t
       return fail(RK_ERR_UNSUPPORTED, "rows and strides must be whole 16-byte vectors");
   if (!aligned16(k) || !aligned16(v))
     return fail(RK_ERR_UNSUPPORTED, "keys and values need 16-byte alignment");
-  if (S > (int64_t{1} << 30)) return fail(RK_ERR_UNSUPPORTED, "too many tokens");
+  if (S > (int64_t{1} << 29)) return fail(RK_ERR_UNSUPPORTED, "too many tokens");
   Kv8Append a{cache_args(c), k, v, skb, skh, sks, svb, svh, svs, start, lengths,
               start_count > 1 ? 1 : 0, S};
   // S tokens from any position touch at most this many blocks
@@ -1175,6 +1175,8 @@ extern "C" int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int 
     return fail(RK_ERR_ARG, "scale must be positive and finite");
   if (!(softcap >= 0.0f) || !(softcap < INFINITY))
     return fail(RK_ERR_ARG, "softcap must be finite and not negative (0: none)");
+  if (softcap != 0.0f && !(softcap >= 1e-3f && softcap <= 1e3f))
+    return fail(RK_ERR_UNSUPPORTED, "softcap outside 1e-3 .. 1e3");
   if (c.B == 0 || Hq == 0 || S == 0) return RK_OK;
   if (c.blocks == 0) return fail(RK_ERR_ARG, "an empty cache");
   if (!q || !start || !out) return fail(RK_ERR_ARG, "null pointer");
@@ -1187,9 +1189,9 @@ extern "C" int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int 
     return fail(RK_ERR_UNSUPPORTED, "queries and outputs need 16-byte alignment");
   const int64_t G = Hq / c.H;
   const Kv8Plan plan = attention_plan(c, Hq, S, qdtype, odtype);
-  // a launch holds fewer than 2^24 blocks of 256 threads
+  // a launch holds fewer than 2^23 blocks of 512 threads
   if (S * G >= (int64_t{1} << 24) || (!plan.chunk && plan.tiles > 65535) ||
-      plan.tiles * c.B * Hq * plan.splits >= (int64_t{1} << 24))
+      plan.tiles * c.B * Hq * plan.splits >= (int64_t{1} << 23))
     return fail(RK_ERR_UNSUPPORTED, "too many queries for one launch");
   const int64_t n = plan.splits;
   if (n > 1 && (!work || !aligned16(work) ||

@@ -7,7 +7,8 @@
 //           C = cap log2(e),  c = 2 log2(e) scale / cap;   1 - tanh^2 = 4 r (1 - r)
 //   biased  t - slope log2(e) |i - j|
 // exp2 and the reciprocal are the hardware's (1 ulp): the capped score is off by at most a few
-// 2^-24 of the cap, 2e-5 of a probability at cap 50 against the 2^-9 of its rounding to bf16.
+// 2^-24 of the cap, 2e-5 of a probability at cap 50 against the 2^-9 of its rounding to bf16. Caps
+// lie in 1e-3 .. 1e3 (2e-4 there).
 //
 // A mask is two intervals per position (rk_attention_mask): the keys [key_lo, key_hi) that a
 // query sees and the queries [query_lo, query_hi) that see a key. A position that sees nothing

@@ -460,6 +460,8 @@ int check_scored(const rk_scored_attention_args& p, bool backward) {
     return fail(RK_ERR_ARG, "scale must be positive and finite");
   if (!(p.softcap >= 0.0f) || !(p.softcap < INFINITY))
     return fail(RK_ERR_ARG, "softcap must be finite and not negative (0: none)");
+  if (p.softcap != 0.0f && !(p.softcap >= 1e-3f && p.softcap <= 1e3f))
+    return fail(RK_ERR_UNSUPPORTED, "softcap outside 1e-3 .. 1e3");
   if (!p.q || !p.k || !p.v || !p.o || !p.lse) return fail(RK_ERR_ARG, "null pointer");
   if (p.bounds && p.mask_batch != 1 && p.mask_batch != p.B)
     return fail(RK_ERR_ARG, "a mask holds one row or one per sequence");
@@ -509,9 +511,7 @@ ScoredArgs scored_args(const rk_scored_attention_args& p) {
     double power = step;
     for (int i = 0; i < 4; ++i, power *= step) a.near[i] = static_cast<float>(fit[i] * power);
     a.near_scale = p.scale * kLog2e;
-    // caps whose powers leave float32's range: always the exponential
-    const bool fits = p.softcap > 1e-3f && p.softcap < 1e3f;
-    a.near_limit = fits ? 0.5f * p.softcap / p.scale : -1.0f;
+    a.near_limit = 0.5f * p.softcap / p.scale;
     a.inv_cap2 = static_cast<float>(1.0 / c2);
   }
   return a;

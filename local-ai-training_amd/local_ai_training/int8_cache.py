@@ -113,6 +113,8 @@ def int8_kv_attention(q: Tensor, cache: Int8KV, start: Tensor, *, lengths: Tenso
         raise TypeError("out_dtype must be floating point")
     _check_positions(cache, start, lengths)
     softcap, slopes, scale = score_arguments(q, softcap, slopes, scale)
+    if softcap and not 1e-3 <= softcap <= 1e3:
+        raise ValueError("softcap must lie in 1e-3 .. 1e3")
     if q.dtype not in (torch.float32, torch.bfloat16):
         q = q.float()
     native = out_dtype if out_dtype in (torch.float32, torch.bfloat16) else torch.float32

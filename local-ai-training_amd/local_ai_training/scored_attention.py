@@ -16,8 +16,9 @@ h reads key head ``h // (H // Hkv)``).
 
 On the GPU, bfloat16 with head size 64 or 128 runs on HIP kernels forward and backward
 (``csrc/rk_scored.hip``, ``csrc/rk_scored_bwd.hip``); operands that do not lie as 16-byte rows
-are copied first. Other types, head sizes and devices take the same formulas in torch operations
-(float32, float64 for float64 operands), which hold all [B, H, S, S] scores at once.
+are copied first. Other types, head sizes and devices, and caps outside 1e-3 .. 1e3 (whose scores
+the kernels' exponentials do not resolve), take the same formulas in torch operations (float32,
+float64 for float64 operands), which hold all [B, H, S, S] scores at once.
 """
 
 from __future__ import annotations
@@ -96,7 +97,7 @@ def _torch_mask(documents: Tensor | None, prefix: Tensor | None) -> AttentionMas
     bounds = torch.where(ids >= 0, torch.stack(rows), 0).to(torch.int32)
     bits = torch.zeros(b, -(-s // 32) * 32, dtype=torch.int64, device=like.device)
     bits[:, :s] = ids < 0
-    words = (bits.view(b, -1, 32) << torch.arange(32, device=like.device)).sum(-1)
+    words = (bits.view(b, -(-s // 32), 32) << torch.arange(32, device=like.device)).sum(-1)
     return AttentionMask(bounds, torch.where(words >= 2**31, words - 2**32, words).to(torch.int32))
 
 
@@ -177,7 +178,8 @@ def scored_attention(q: Tensor, k: Tensor, v: Tensor, *, mask: AttentionMask | N
             raise ValueError("the mask must hold one row or one per sequence, of q's length")
         if mask.bounds.device != q.device:
             raise ValueError("the mask must be on the queries' device")
-    if q.is_cuda and q.dtype == torch.bfloat16 and d in (64, 128):
+    if (q.is_cuda and q.dtype == torch.bfloat16 and d in (64, 128)
+            and (softcap == 0.0 or 1e-3 <= softcap <= 1e3)):
         bounds, padding = mask if mask is not None else (None, None)
         return ratchet().scored_attend(q, k, v, bounds, padding, slopes, softcap, scale)
     return _torch_scored_attention(q, k, v, mask, softcap, slopes, scale)

@@ -352,6 +352,8 @@ def test_refusals(cuda):
         int8_kv_attention(q[:, :3], cache, start)
     with pytest.raises(ValueError, match="softcap"):
         int8_kv_attention(q, cache, start, softcap=-1.0)
+    with pytest.raises(ValueError, match="1e-3"):
+        int8_kv_attention(q, cache, start, softcap=1e4)
     with pytest.raises(RuntimeError, match="no gradient"):
         int8_kv_attention(q.clone().requires_grad_(), cache, start)
     with pytest.raises(ValueError, match="past the cache"):

@@ -298,6 +298,19 @@ def test_other_types_and_head_sizes_take_the_torch_form(cuda):
         assert bool(((got.double() - want).abs() <= step * want.abs() + 1e-5).all())
 
 
+@pytest.mark.parametrize("cap", [1e-3, 0.5, 1e3, 1e-5, 1e6])
+def test_small_and_large_caps(cuda, cap):
+    """The ends of what the kernels take, and what goes to the torch form."""
+    compare(cuda, 1, 2, 2, 150, 64, "documents", cap, True)
+
+
+def test_empty_masks(cuda):
+    for b, s in ((0, 3), (2, 0)):
+        for device in ("cpu", cuda):
+            mask = attention_mask(torch.zeros(b, s, dtype=torch.int64, device=device))
+            assert mask.bounds.shape == (4, b, s) and mask.padding.shape == (b, -(-s // 32))
+
+
 def test_the_library_refuses(cuda):
     q = torch.zeros(1, 2, 8, 64, device=cuda, dtype=torch.bfloat16)
     ops = ratchet()
@@ -309,6 +322,8 @@ def test_the_library_refuses(cuda):
         ops.scored_attention(q, q, q, None, None, None, 0.0, -1.0, False)
     with pytest.raises(RuntimeError, match="softcap"):
         ops.scored_attention(q, q, q, None, None, None, -1.0, 1.0, False)
+    with pytest.raises(RuntimeError, match="1e-3"):
+        ops.scored_attention(q, q, q, None, None, None, 1e5, 1.0, False)
     with pytest.raises(RuntimeError, match="go together"):
         ops.scored_attention(q, q, q, mask.bounds, None, None, 0.0, 1.0, False)
     with pytest.raises(RuntimeError, match="bfloat16"):
