@@ -178,7 +178,8 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(vt, sub, s, lane), gf[s], dp,
                                                      0, 0, 0);
       // the masks in one uniform branch ahead of straight arithmetic (a masked score of -inf
-      // gives p = 0, a capped one the cap's end, whose gradient is zero with dp)
+      // gives p = 0, a capped one the cap's end, whose gradient is zero with dp; of a negative
+      // slope its p may be infinite)
       if (!whole) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -196,10 +197,12 @@ void scored_dq_kernel(ScoredBwdArgs ba) {
       }
       float ds[16];
       const auto gradient = [&](int e, float p1, float sl) {
-        ds[e] = p1 * dp[e];
+        const float p2 = CAP && SG && st[e] == -INFINITY ? 0.0f
+                         : CAP && BIAS && !SG            ? fminf(p1, 0x1p100f)
+                                                         : p1;
+        ds[e] = p2 * dp[e];
         if constexpr (SG) {
           const float dist = fabsf(d0 - static_cast<float>(8 * (e / 4) + (e % 4)));
-          const float p2 = CAP && st[e] == -INFINITY ? 0.0f : p1;
           s_pd = s_pd + ds[e];
           s_pa = __builtin_fmaf(p2, dist, s_pa);
           s_pda = __builtin_fmaf(ds[e], dist, s_pda);
@@ -398,7 +401,8 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
     // the masks sit in one uniform branch ahead of straight arithmetic: with the probabilities
     // formed before the second product, and the masks on them, the loop spilled or took a
     // quarter longer. A masked score of -inf gives p = 0; a capped one gives the cap's end, with
-    // slope 0, and its p is cleared below.
+    // slope 0, and its p (infinite beside a negative slope, then with a gradient that is not a
+    // number) is cleared below.
     const bool whole = ws.all(qs, kBwdRows);
     const int i0 = qs + 4 * h - span.lo;
     if (!whole) {
@@ -438,10 +442,15 @@ void scored_dkv_kernel(ScoredBwdArgs ba) {
       if (!whole) {
         uint32_t* const w[8] = {&pf[0].x, &pf[0].y, &pf[0].z, &pf[0].w,
                                 &pf[1].x, &pf[1].y, &pf[1].z, &pf[1].w};
+        uint32_t* const d[8] = {&dsf[0].x, &dsf[0].y, &dsf[0].z, &dsf[0].w,
+                                &dsf[1].x, &dsf[1].y, &dsf[1].z, &dsf[1].w};
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width)
-            *w[e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
+          if (static_cast<uint32_t>(i0 + 8 * (e / 4) + (e % 4)) >= width) {
+            const uint32_t keep = e % 2 ? 0x0000ffffu : 0xffff0000u;
+            *w[e / 2] &= keep;
+            if constexpr (BIAS) *d[e / 2] &= keep;
+          }
       }
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)

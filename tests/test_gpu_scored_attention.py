@@ -109,6 +109,54 @@ def test_scores_that_saturate_the_cap(cuda):
     compare(cuda, 1, 2, 2, 200, 128, "documents", 4.0, True, std=4.0)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("biased", [False, True])
+def test_saturated_scores_with_large_values(cuda, biased, sign, d):
+    """Sums of p 2^100 leave float32's range where every score is near the cap of 50 (2^72)."""
+    b, h, s, scale = 2, 2, 200, 1.0 / math.sqrt(d)
+    print(f"saturated D={d} {biased} sign {sign}", flush=True)
+    q, k, v, g = operands(cuda, b, h, h, s, d)
+    q, k = (q.abs() + 8.0), (k.abs() + 8.0) * sign
+    slopes = slopes_of(cuda, h) if biased else None
+    want = reference(q, k, v, g, seen_keys(None, None, b, s), 50.0, slopes, scale)
+    for power in (0, 100, -60):
+        with torch.no_grad():
+            out = scored_attention(q, k, v * 2.0 ** power, softcap=50.0, slopes=slopes,
+                                   scale=scale)
+        check([out.double() * 2.0 ** -power], want)
+
+
+@pytest.mark.parametrize("kind", ["", "documents prefix"])
+@pytest.mark.parametrize("cap", [0.0, 20.0, 50.0])
+@pytest.mark.parametrize("d", [64, 128])
+def test_negative_slopes(cuda, cap, kind, d):
+    """The farthest visible key counts most, and masked pairs would count more."""
+    b, h, s = 2, 3, 700
+    print(f"negative slopes D={d} cap={cap} {kind!r}", flush=True)
+    q, k, v, g = operands(cuda, b, h, h, s, d)
+    documents, prefix = layout(kind, b, s)
+    mask = None
+    if kind:
+        mask = attention_mask(documents.to(cuda), prefix.to(cuda))
+    slopes = -slopes_of(cuda, h)
+    got = run(q, k, v, g, mask, cap, slopes)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = scored_attention(*leaves, mask=mask, softcap=cap, slopes=slopes)
+    fixed = [out.detach(), *torch.autograd.grad(out, leaves, g)]  # slopes that do not learn
+    with torch.no_grad():
+        plain = scored_attention(q, k, v, mask=mask, softcap=cap, slopes=slopes)
+    want = reference(q, k, v, g, seen_keys(documents, prefix, b, s), cap, slopes,
+                     1.0 / math.sqrt(d))
+    # Slopes of -1/2 over 700 positions take p below 2^-126, float32's smallest normal number,
+    # where it is zero or a denormal: a gradient's S <= 2^10 terms p (|g| . |v| + |g| . |o|) |k|
+    # with vectors of at most 128 numbers below 6 lose at most 2^-126 2^10 2 (128 36) 6 < 2^-99.
+    want = [(ref, bound + 2.0 ** -99) for ref, bound in want]
+    check(got, want)
+    check(fixed, want)
+    check([plain], want)
+
+
 def test_a_long_row(cuda):
     compare(cuda, 1, 2, 1, 2500, 128, "documents prefix", 30.0, True)
 
