@@ -18,8 +18,6 @@
 // The vector unit is busy half of the time (829 instructions a step of 64 keys, capped), the
 // matrix unit an eighth: what is left is waiting between a step's dependent parts, and
 // wavefronts of a workgroup that wait for the one whose rows see most.
-#include <type_traits>
-
 #include "rk_scored.h"
 
 namespace rk {
@@ -37,13 +35,7 @@ __device__ __forceinline__ float half_sum2(float v) {
 
 // R keys are staged per step, U of them make one update of the running max and sum.
 // FINE: capped and biased scores of a pass whose gradients are wanted (near_capped).
-// FIXED: scores capped at 80 or less in base-2 units are taken relative to a reference known
-// beforehand, the largest bias of the row's keys (a query sees itself, at distance 0), and need
-// no running max: probabilities are at most 2^80 and those of the key with that bias at least
-// 2^-80. Rows that leave float32's range all the same (saturated scores with values beyond 2^30)
-// make their workgroup start over with the running max. Packed documents, D 128, capped: 52 ->
-// 49.8 us (1B training shape); capped and biased at S 8192 288 -> 257 (247 without the check).
-template <int D, int R, int U, bool CAP, bool BIAS, bool FINE = false, bool FIXED = false>
+template <int D, int R, int U, bool CAP, bool BIAS, bool FINE = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4)))
 void scored_fwd_kernel(ScoredArgs a) {
   using T = AttnTile<D, R>;
@@ -81,155 +73,128 @@ void scored_fwd_kernel(ScoredArgs a) {
     vd.issue(st + T::BYTES, step * R, wave);
   };
 
-  float m, l;
+  float m = -INFINITY, l = 0.0f;
   v16f_a o[D / 32];
-  const auto pass = [&](auto known) {
-    constexpr bool KNOWN = decltype(known)::value;
-    m = -INFINITY;
-    if constexpr (KNOWN) {
-      const int far = qi - span.lo > span.hi - 1 - qi ? qi - span.lo : span.hi - 1 - qi;
-      m = BIAS && span.valid ? fmaxf(0.0f, -slope2 * static_cast<float>(far)) : 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) o[dt] = v16f_a{};
+  if (first < end) issue(first);
+  for (int step = first; step < end; ++step) {
+    const uint64_t pad = padding_bits<R>(a, b, step * R);
+    dma_wait_barrier<0>();
+    if (step + 1 < end) issue(step + 1);
+    uint8_t* const kt = smem + (step & 1) * 2 * T::BYTES;
+    uint8_t* const vt = kt + T::BYTES;
+    if (pad) {
+      clear_rows<D, R>(vt, pad, tid);
+      __syncthreads();
     }
-    l = 0.0f;
+    const int k0 = step * R;
+    if (ws.none(k0, R)) continue;
+    // S^T: lane holds keys k0 + 32 t + 8 (e / 4) + 4 h + e % 4 of its query
+    v16f_a sc[R / 32];
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) o[dt] = v16f_a{};
-    if (first < end) issue(first);
-    for (int step = first; step < end; ++step) {
-      const uint64_t pad = padding_bits<R>(a, b, step * R);
-      dma_wait_barrier<0>();
-      if (step + 1 < end) issue(step + 1);
-      uint8_t* const kt = smem + (step & 1) * 2 * T::BYTES;
-      uint8_t* const vt = kt + T::BYTES;
-      if (pad) {
-        clear_rows<D, R>(vt, pad, tid);
-        __syncthreads();
-      }
-      const int k0 = step * R;
-      if (ws.none(k0, R)) continue;
-      // S^T: lane holds keys k0 + 32 t + 8 (e / 4) + 4 h + e % 4 of its query
-      v16f_a sc[R / 32];
+    for (int t = 0; t < R / 32; ++t) {
+      sc[t] = v16f_a{};
 #pragma unroll
-      for (int t = 0; t < R / 32; ++t) {
-        sc[t] = v16f_a{};
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, 32 * t, s, lane), qf[s],
-                                                          sc[t], 0, 0, 0);
-      }
-      // capped and biased scores in base-2 units here; plain ones are scaled with the max
-      const float mul = CAP || BIAS ? 1.0f : a.dot_scale;
-      if constexpr (CAP || BIAS) {
-        const float d0 = static_cast<float>(qi - k0 - 4 * h);
-        bool near = false;
-        if constexpr (FINE) {
-          float most = 0.0f;
-#pragma unroll
-          for (int t = 0; t < R / 32; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(sc[t][e]));
-          near = !__any(most > a.near_limit);
-        }
-        if (near) {
-#pragma unroll
-          for (int t = 0; t < R / 32; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float slack;
-              sc[t][e] = __builtin_fmaf(-slope2, fabsf(d0 - (32 * t + 8 * (e / 4) + (e % 4))),
-                                        near_capped(a, sc[t][e], slack));
-            }
-        } else {
-#pragma unroll
-          for (int t = 0; t < R / 32; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float x = sc[t][e] * a.dot_scale;
-              if constexpr (CAP) {
-                const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f);
-                x = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
-              }
-              if constexpr (BIAS)
-                x = __builtin_fmaf(-slope2, fabsf(d0 - (32 * t + 8 * (e / 4) + (e % 4))), x);
-              sc[t][e] = x;
-            }
-        }
-      }
-      if (!ws.all(k0, R)) {
-        const int j0 = k0 + 4 * h - span.lo;
+      for (int s = 0; s < D / 16; ++s)
+        sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(row_frag<D>(kt, 32 * t, s, lane), qf[s],
+                                                        sc[t], 0, 0, 0);
+    }
+    // capped and biased scores in base-2 units here; plain ones are scaled with the max
+    const float mul = CAP || BIAS ? 1.0f : a.dot_scale;
+    if constexpr (CAP || BIAS) {
+      const float d0 = static_cast<float>(qi - k0 - 4 * h);
+      bool near = false;
+      if constexpr (FINE) {
+        float most = 0.0f;
 #pragma unroll
         for (int t = 0; t < R / 32; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (static_cast<uint32_t>(j0 + 32 * t + 8 * (e / 4) + (e % 4)) >= width)
-              sc[t][e] = -INFINITY;
+          for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(sc[t][e]));
+        near = !__any(most > a.near_limit);
       }
-      // the updates' probabilities first, then their products
-      float alpha[R / U], ps[R / U];
-      uint4 pf[R / 32][2];
+      if (near) {
 #pragma unroll
-      for (int u = 0; u < R / U; ++u) {
-        float mref = m;
-        if constexpr (!KNOWN) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int t = u * UT; t < (u + 1) * UT; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[t][e]);
-          mx = half_max2(mx);
-          const float mnew = fmaxf(m, mx * mul);
-          mref = mnew == -INFINITY ? 0.0f : mnew;  // a row with no key yet
-          alpha[u] = __builtin_amdgcn_exp2f(m - mref);
-          m = mnew;
-        }
-        ps[u] = 0.0f;
-#pragma unroll
-        for (int t = u * UT; t < (u + 1) * UT; ++t) {
-          float pr[16];
+        for (int t = 0; t < R / 32; ++t)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            pr[e] = __builtin_amdgcn_exp2f(KNOWN && !BIAS ? sc[t][e]
-                                           : CAP || BIAS ? sc[t][e] - mref
-                                                         : __builtin_fmaf(sc[t][e], mul, -mref));
-            ps[u] = ps[u] + pr[e];
+            float slack;
+            sc[t][e] = __builtin_fmaf(-slope2, fabsf(d0 - (32 * t + 8 * (e / 4) + (e % 4))),
+                                      near_capped(a, sc[t][e], slack));
           }
-          pack16(pf[t], pr);
-        }
-      }
+      } else {
 #pragma unroll
-      for (int u = 0; u < R / U; ++u) {
-        // keys that no row of the wavefront sees: p is zero, but their values may not be finite
-        if (ws.none(k0 + u * U, U)) continue;
-        if constexpr (KNOWN) {
-          l = l + half_sum2(ps[u]);
-        } else {
-          if (__any(alpha[u] != 1.0f)) {
+        for (int t = 0; t < R / 32; ++t)
 #pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * alpha[u];
+          for (int e = 0; e < 16; ++e) {
+            float x = sc[t][e] * a.dot_scale;
+            if constexpr (CAP) {
+              const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f);
+              x = __builtin_fmaf(-2.0f * a.cap2, r, a.cap2);
+            }
+            if constexpr (BIAS)
+              x = __builtin_fmaf(-slope2, fabsf(d0 - (32 * t + 8 * (e / 4) + (e % 4))), x);
+            sc[t][e] = x;
           }
-          l = l * alpha[u] + half_sum2(ps[u]);
-        }
-#pragma unroll
-        for (int t = u * UT; t < (u + 1) * UT; ++t)
-#pragma unroll
-          for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
-              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                  col_frag<D>(vt, 32 * t + 16 * s2, dt, lane), frag_of(pf[t][s2]), o[dt], 0, 0, 0);
       }
     }
-  };
-  pass(std::integral_constant<bool, FIXED>{});
-  if constexpr (FIXED) {
-    float most = 0.0f;  // a sum: not a number if an output is
-    const bool finite = l >= 0x1p-100f;
+    if (!ws.all(k0, R)) {
+      const int j0 = k0 + 4 * h - span.lo;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+      for (int t = 0; t < R / 32; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) most = most + fabsf(o[dt][e]);
-    if (__syncthreads_or(span.valid && !(finite && most < INFINITY))) pass(std::false_type{});
+        for (int e = 0; e < 16; ++e)
+          if (static_cast<uint32_t>(j0 + 32 * t + 8 * (e / 4) + (e % 4)) >= width)
+            sc[t][e] = -INFINITY;
+    }
+    // the updates' probabilities first, then their products
+    float alpha[R / U], ps[R / U];
+    uint4 pf[R / 32][2];
+#pragma unroll
+    for (int u = 0; u < R / U; ++u) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = u * UT; t < (u + 1) * UT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[t][e]);
+      mx = half_max2(mx);
+      const float mnew = fmaxf(m, mx * mul);
+      const float mref = mnew == -INFINITY ? 0.0f : mnew;  // a row with no key yet
+      alpha[u] = __builtin_amdgcn_exp2f(m - mref);
+      m = mnew;
+      ps[u] = 0.0f;
+#pragma unroll
+      for (int t = u * UT; t < (u + 1) * UT; ++t) {
+        float pr[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          pr[e] = __builtin_amdgcn_exp2f(CAP || BIAS ? sc[t][e] - mref
+                                                     : __builtin_fmaf(sc[t][e], mul, -mref));
+          ps[u] = ps[u] + pr[e];
+        }
+        pack16(pf[t], pr);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < R / U; ++u) {
+      // keys that no row of the wavefront sees: every p is zero, but their values may not be finite
+      if (ws.none(k0 + u * U, U)) continue;
+      if (__any(alpha[u] != 1.0f)) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * alpha[u];
+      }
+      l = l * alpha[u] + half_sum2(ps[u]);
+#pragma unroll
+      for (int t = u * UT; t < (u + 1) * UT; ++t)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt)
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                col_frag<D>(vt, 32 * t + 16 * s2, dt, lane), frag_of(pf[t][s2]), o[dt], 0, 0, 0);
+    }
   }
 
   uint32_t* const rest = p.rest ? rest_words<D>(a, bh, qw0) + lane : nullptr;
@@ -554,21 +519,13 @@ ScoredArgs scored_args(const rk_scored_attention_args& p) {
 
 template <int D, int R, int U>
 static void launch_scored_fwd(const ScoredArgs& a, dim3 grid, hipStream_t st) {
-  const bool cap = a.p.softcap > 0.0f, bias = a.p.slopes != nullptr, fixed = a.cap2 <= 80.0f;
-  if (cap && bias && a.p.rest) {
-    if (fixed) scored_fwd_kernel<D, R, U, true, true, true, true><<<grid, 256, 0, st>>>(a);
-    else scored_fwd_kernel<D, R, U, true, true, true><<<grid, 256, 0, st>>>(a);
-  } else if (cap && bias) {
-    if (fixed) scored_fwd_kernel<D, R, U, true, true, false, true><<<grid, 256, 0, st>>>(a);
-    else scored_fwd_kernel<D, R, U, true, true><<<grid, 256, 0, st>>>(a);
-  } else if (cap) {
-    if (fixed) scored_fwd_kernel<D, R, U, true, false, false, true><<<grid, 256, 0, st>>>(a);
-    else scored_fwd_kernel<D, R, U, true, false><<<grid, 256, 0, st>>>(a);
-  } else if (bias) {
-    scored_fwd_kernel<D, R, U, false, true><<<grid, 256, 0, st>>>(a);
-  } else {
-    scored_fwd_kernel<D, R, U, false, false><<<grid, 256, 0, st>>>(a);
-  }
+  const bool cap = a.p.softcap > 0.0f, bias = a.p.slopes != nullptr;
+  if (cap && bias && a.p.rest)
+    scored_fwd_kernel<D, R, U, true, true, true><<<grid, 256, 0, st>>>(a);
+  else if (cap && bias) scored_fwd_kernel<D, R, U, true, true><<<grid, 256, 0, st>>>(a);
+  else if (cap) scored_fwd_kernel<D, R, U, true, false><<<grid, 256, 0, st>>>(a);
+  else if (bias) scored_fwd_kernel<D, R, U, false, true><<<grid, 256, 0, st>>>(a);
+  else scored_fwd_kernel<D, R, U, false, false><<<grid, 256, 0, st>>>(a);
 }
 
 }  // namespace rk
