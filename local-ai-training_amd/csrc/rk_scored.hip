@@ -35,6 +35,9 @@ __device__ __forceinline__ float half_sum2(float v) {
 
 // R keys are staged per step, U of them make one update of the running max and sum.
 // FINE: capped and biased scores of a pass whose gradients are wanted (near_capped).
+// (Without a running max under a cap, relative to a reference known beforehand: 52 -> 49.8 us of
+// the capped training shape, 288 -> 257 capped and biased at S 8192. But the largest p of a row
+// is then no longer 1 and exact in bf16: gradients off by 2.6e-3 against 2.4e-3. Not kept.)
 template <int D, int R, int U, bool CAP, bool BIAS, bool FINE = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 4)))
 void scored_fwd_kernel(ScoredArgs a) {
