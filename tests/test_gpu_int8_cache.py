@@ -169,7 +169,8 @@ def check_attention(q, cache, start, lengths=None, cap=0.0, slopes=None, out_dty
         bias = slopes.double()[:, None, None] * dist.abs() if slopes is not None else 0.0
         s = s - bias
         products = scale * x.abs().amax(-1, keepdim=True) * k.abs().sum(-1)[:, None]
-        delta = 2.0**-21 * (products + s.abs() + cap + bias) + 2.0**-(r + 1) * products
+        size = abs(bias)  # (slopes may be negative)
+        delta = 2.0**-21 * (products + s.abs() + cap + size) + 2.0**-(r + 1) * products
         unseen = dist < 0
         p = s.masked_fill(unseen, -math.inf).softmax(-1)
         want = p @ v
@@ -224,6 +225,17 @@ def test_several_tokens(cuda, new, h, hkv, d):
     check_attention(q, cache, torch.tensor([77], device=cuda), cap=9.0, out_dtype=torch.float32)
     lengths = torch.tensor([new, 1, new - 1], device=cuda)
     check_attention(q, cache, start, lengths=lengths)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 40])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_negative_slopes(cuda, cap, new, d):
+    print(f"int8 attention negative slopes new={new} cap={cap} D={d}", flush=True)
+    cache = filled(cuda, 2, 3, 700, d)
+    q = rows(2, new, 3, d, 7).to(cuda)
+    start = torch.tensor([700 - new, 130], device=cuda)
+    check_attention(q, cache, start, cap=cap, slopes=-slopes_of(cuda, 3))
 
 
 def test_sequences_switched_off_and_positions_past_the_end(cuda):

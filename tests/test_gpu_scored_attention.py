@@ -214,6 +214,28 @@ def test_layouts_and_repeated_runs(cuda):
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_broadcast_slopes_and_gradients(cuda):
+    """One slope for all heads and its gradient, every other slope of a table, a sum's gradient."""
+    b, h, s, d = 2, 4, 200, 64
+    q, k, v, g = operands(cuda, b, h, 2, s, d)
+    seen = seen_keys(None, None, b, s)
+    scale = 1.0 / math.sqrt(d)
+    one = torch.full((1,), 0.125, device=cuda, requires_grad=True)
+    table = slopes_of(cuda, 2 * h).requires_grad_()
+    for leaf, used in ((one, one.expand(h)), (table, table[::2])):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = scored_attention(*leaves, softcap=30.0, slopes=used)
+        got = [out.detach(), *torch.autograd.grad(out.sum(), [*leaves, leaf])]
+        want = reference(q, k, v, torch.ones_like(g), seen, 30.0, used.detach(), scale)
+        slope, bound = want[4]
+        if leaf is one:
+            want = (*want[:4], (slope.sum().reshape(1), bound.sum().reshape(1)))
+        else:
+            got[4], rest = got[4][::2], got[4][1::2]
+            assert not rest.any()
+        check(got, want)
+
+
 def test_gradients_against_differences(cuda):
     """Along one direction, the float64 differences of the float64 formulas at the bf16 operands;
     the kernels' gradients to the bounds of their elements, summed."""
