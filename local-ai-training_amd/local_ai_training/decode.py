@@ -168,6 +168,15 @@ def _step_buffers(model, cache) -> dict[str, Tensor]:
     return bufs
 
 
+def reserve_step(model, cache) -> None:
+    """Allocates what a step over an 8-bit cache keeps: the layers' codes and scales, and the
+    fused step's buffers."""
+    for layer in range(cache.n_layer):
+        cache.store(layer)
+    if model.fused_decode and fused_decode_supported(model, cache):
+        _step_buffers(model, cache)
+
+
 @torch.no_grad()
 def fused_decode_logits(model, tokens: Tensor, cache) -> Tensor:
     """Logits [B, vocab] (float32 holding bf16 values, as the int8 lm_head writes them) of

@@ -24,7 +24,7 @@ from typing import Literal
 import torch
 from torch import Tensor
 
-from .decode import decode_greedy
+from .decode import decode_greedy, reserve_step
 from .model import Int8KVCache, KVCache, ModelConfig, RatchetGPT, build_seeded_model
 from .ratchet import DiscreteRatchetLinear
 
@@ -121,17 +121,17 @@ class DecodeGraph:
     def __init__(self, model: RatchetGPT, cache: KVCache, greedy: bool = False) -> None:
         self.model, self.cache, self.greedy = model, cache, greedy
         self.tokens = torch.zeros((cache.batch, 1), dtype=torch.long, device=cache.device)
-        # warm-up step (allocates the cache buffers), then undo its position advance. Into an
-        # 8-bit cache it appends nothing (position -1): its token could raise a block's scale.
+        # warm-up step: allocates the cache buffers, and its token is overwritten by the first
+        # replay's. In an 8-bit cache that token could raise a block's scale for good, so the
+        # step is warmed up on a cache of its own, of one position.
+        warm = cache
+        if isinstance(cache, Int8KVCache):
+            reserve_step(model, cache)
+            warm = model.new_cache(cache.batch, max_len=1, dtype=torch.int8)
         stream = torch.cuda.Stream(device=cache.device)
         stream.wait_stream(torch.cuda.current_stream(cache.device))
-        position = cache.pos.clone() if isinstance(cache, Int8KVCache) else None
         with torch.cuda.stream(stream), torch.no_grad():
-            if position is not None:
-                cache.pos.fill_(-1)
-            model.decode_logits(self.tokens, cache)
-            if position is not None:
-                cache.pos.copy_(position)
+            model.decode_logits(self.tokens, warm)
         torch.cuda.current_stream(cache.device).wait_stream(stream)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph), torch.no_grad():
