@@ -18,6 +18,7 @@
 // ratchet.py).
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -1294,9 +1295,15 @@ struct ScoredAttend : torch::autograd::Function<ScoredAttend> {
 Tensor scored_attend_autograd(const Tensor& q, const Tensor& k, const Tensor& v,
                               const OptTensor& bounds, const OptTensor& padding,
                               const OptTensor& slopes, double softcap, double scale) {
-  const bool grad = at::GradMode::is_enabled() &&
-                    (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
-                     (slopes.has_value() && slopes->requires_grad()));
+  const auto any = [&](const auto& holds) {
+    return holds(q) || holds(k) || holds(v) || (slopes.has_value() && holds(*slopes));
+  };
+  // operands with a tangent go to the autograd function too, which refuses them: below autograd
+  // the result would come back as if it did not depend on them
+  const bool grad =
+      (at::GradMode::is_enabled() && any([](const Tensor& t) { return t.requires_grad(); })) ||
+      (c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+       any([](const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }));
   if (!grad) {
     const at::AutoDispatchBelowADInplaceOrView guard;
     static const auto op = c10::Dispatcher::singleton()

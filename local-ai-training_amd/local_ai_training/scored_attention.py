@@ -159,7 +159,8 @@ def scored_attention(q: Tensor, k: Tensor, v: Tensor, *, mask: AttentionMask | N
 
     ``mask``: from ``attention_mask`` (None: causal). ``softcap``: the scores' bound (None or 0:
     none). ``slopes`` [H]: the bias per step of distance (differentiable). ``scale``: default
-    1 / sqrt(D). Returns [B, H, S, D] in q's dtype."""
+    1 / sqrt(D). Returns [B, H, S, D] in q's dtype. The kernels have first derivatives in reverse
+    mode; second ones and operands with a forward-mode tangent are refused."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError("scored_attention expects q [B, H, S, D] and k, v [B, Hkv, S, D]")
     b, h, s, d = q.shape
