@@ -119,6 +119,7 @@ class DecodeGraph:
     with no host work between steps."""
 
     def __init__(self, model: RatchetGPT, cache: KVCache, greedy: bool = False) -> None:
+        cache.check_open()
         self.model, self.cache, self.greedy = model, cache, greedy
         self.tokens = torch.zeros((cache.batch, 1), dtype=torch.long, device=cache.device)
         # warm-up step: allocates the cache buffers, and its token is overwritten by the first

@@ -160,6 +160,7 @@ class KVCache:
         self.pos = torch.zeros(1, dtype=torch.long, device=device)
         self._arange = torch.arange(max_len, device=device)
         self._mask: Tensor | None = None
+        self._ended: Tensor | bool = False  # by the mask of a prompt (end_unless_whole)
         self.step_buffers: dict[str, Tensor] = {}  # fixed-shape work buffers of a step
 
     def buffers(self, layer: int, like: Tensor) -> tuple[Tensor, Tensor]:
@@ -222,6 +223,25 @@ class KVCache:
     def advance(self, steps: int) -> None:
         self.length += steps
         self.pos.add_(steps)
+
+    def end_unless_whole(self, mask: AttentionMask) -> None:
+        """Notes, on the device, whether a prompt under `mask` is one document in every row. Of
+        others (several documents, padding) later positions must not see all, and the cache
+        does not know which part."""
+        low, _, _, high = mask.bounds
+        self._ended = ~((low == 0) & (high == mask.bounds.shape[2])).all()
+
+    def reopen(self) -> None:
+        """A prompt at position 0 starts the cache anew."""
+        self._ended = False
+
+    def check_open(self) -> None:
+        """Refuses to go on behind such a prompt (the first call behind a mask waits for it)."""
+        if not isinstance(self._ended, bool):
+            self._ended = bool(self._ended)
+        if self._ended:
+            raise ValueError("a prompt of several documents or padding cannot be continued: "
+                             "later positions would see all of it")
 
 
 class Int8KVCache(KVCache):
@@ -706,11 +726,22 @@ class RatchetGPT(nn.Module):
                 mask: AttentionMask | None = None) -> Tensor:
         """Run `tokens` [B, S] at positions cache.length .. +S, append their keys/values, and
         return the logits of the last position [B, vocab]. `mask`: of a prompt at the start of
-        the cache, for a model trained so (e.g. its prompt as a prefix)."""
+        the cache, for a model trained so (e.g. its prompt as a prefix). Behind a mask of several
+        documents or padding nothing can follow (and logits of padding mean nothing)."""
         start, length = cache.length, tokens.shape[1]
+        if mask is not None and start:
+            raise ValueError("a mask applies to a prompt at the start of the cache")
+        if start + length > cache.max_len:
+            raise ValueError("KV cache is full")
+        if start:
+            cache.check_open()
+        else:
+            cache.reopen()
         hidden = self.token_embedding(tokens) + self.position_encoding[start:start + length]
         for index, block in enumerate(self.blocks):
             hidden = block(hidden, cache=cache, layer=index, mask=mask)
+        if mask is not None:
+            cache.end_unless_whole(mask)
         cache.advance(length)
         return self.lm_head(self.final_norm(hidden[:, -1:]))[:, 0]
 
@@ -731,6 +762,7 @@ class RatchetGPT(nn.Module):
         step); otherwise through the module forwards."""
         from .decode import fused_decode_logits, fused_decode_supported
 
+        cache.check_open()
         if self.fused_decode and fused_decode_supported(self, cache):
             return fused_decode_logits(self, tokens, cache)
         cache.begin_step()
