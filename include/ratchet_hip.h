@@ -725,11 +725,11 @@ int rk_attention_mask(const void* documents, int wide, int64_t sdb, const uint8_
  * rest, written by the forward and read by the backward (a byte per element, in an order of its
  * own), makes delta = g . o exact to 2^-16 of o.
  * The backward reads o, lse and the gradient g of o, and writes dq, dk, dv and, where given,
- * dslopes (float32 [H]); work: rk_scored_attention_backward_work floats, 16-byte aligned. Scores
- * and softmax run in float32; probabilities and score gradients enter the products rounded to bf16; every sum
- * has a fixed order. Inputs 16-byte aligned, outputs 8-byte, strides multiples of 8 elements, one
- * head's positions under 2^31 bytes, fewer than 2^24 blocks of 128 positions; otherwise
- * RK_ERR_UNSUPPORTED.
+ * dslopes (float32 [H]); work: rk_scored_attention_backward_work floats, 16-byte aligned; H = 0
+ * with Hkv > 0 is RK_ERR_ARG there. Scores and softmax run in float32; probabilities and score
+ * gradients enter the products rounded to bf16; every sum has a fixed order. Inputs 16-byte
+ * aligned, outputs 8-byte, strides multiples of 8 elements, one head's positions under 2^31 bytes,
+ * fewer than 2^24 blocks of 128 positions; otherwise RK_ERR_UNSUPPORTED.
  * No counterpart in the reference (it attends without cap, bias or mask, model.py:117-123).
  */
 typedef struct rk_scored_attention_args {

@@ -1193,7 +1193,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> scored_attention_backward(
   };
   Tensor dq = out(a.H), dk = out(a.Hkv), dv = out(a.Hkv);
   Tensor dslopes = at::empty({slope_grad ? a.H : 0}, lse.options());
-  if (q.numel() == 0) return {dq, dk, dv, dslopes.zero_()};
+  // (without query heads the keys and values have gradients, of zero)
+  if (q.numel() == 0) return {dq, dk.zero_(), dv.zero_(), dslopes.zero_()};
   Tensor work = at::empty({rk_scored_attention_backward_work(a.B, a.H, a.Hkv, a.S, a.D,
                                                             slope_grad)},
                           lse.options());

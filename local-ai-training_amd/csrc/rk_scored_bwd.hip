@@ -571,6 +571,8 @@ extern "C" int rk_scored_attention_backward(const rk_scored_attention_args* args
   const rk_scored_attention_args& p = *args;
   if (int e = check_scored(p, true)) return e;
   if (p.dslopes && !p.slopes) return fail(RK_ERR_ARG, "a slope gradient needs slopes");
+  if (p.H == 0 && p.Hkv > 0 && p.B > 0 && p.S > 0)
+    return fail(RK_ERR_ARG, "no query heads: dk and dv would not be written");
   if (p.B == 0 || p.H == 0 || p.S == 0) return RK_OK;
   if (!p.dq || !p.dk || !p.dv || !work) return fail(RK_ERR_ARG, "null pointer");
   if (!aligned16(work)) return fail(RK_ERR_UNSUPPORTED, "the workspace needs 16-byte alignment");
