@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch import Tensor
 
 from .ops import ratchet
@@ -73,15 +74,24 @@ def _check_positions(cache: Int8KV, start: Tensor, lengths: Tensor | None) -> No
             raise ValueError(f"{name} must be on the cache's device")
 
 
+def _refuse_gradients(what: str, *operands: Tensor | None) -> None:
+    for t in operands:
+        if t is not None and ((t.requires_grad and torch.is_grad_enabled())
+                              or forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError(f"{what} an 8-bit cache has no gradient; call it under no_grad, "
+                               "on operands without tangents")
+
+
 def int8_kv_append(cache: Int8KV, k: Tensor, v: Tensor, start: Tensor,
                    lengths: Tensor | None = None) -> None:
     """Writes k and v [B, H, S, D] at positions ``start`` .. of each sequence; of a sequence's S
-    tokens the first ``lengths`` count (None: all)."""
+    tokens the first ``lengths`` count (None: all). It has no gradient."""
     b, h, _, _, d = cache.keys.shape
     if k.dim() != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (b, h, d):
         raise ValueError("k and v must share the cache's [B, H, S, D] shape")
     if k.dtype != v.dtype or not k.is_floating_point():
         raise TypeError("k and v must share a floating-point dtype")
+    _refuse_gradients("appending to", k, v)
     if not k.device == v.device == cache.keys.device:
         raise ValueError("k and v must be on the cache's device")
     _check_positions(cache, start, lengths)
@@ -104,8 +114,7 @@ def int8_kv_attention(q: Tensor, cache: Int8KV, start: Tensor, *, lengths: Tenso
         raise ValueError("q must be [B, Hq, S, D] with heads a multiple of the cache's")
     if not q.is_floating_point():
         raise TypeError("q must be floating point")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("attention over an 8-bit cache has no gradient; call it under no_grad")
+    _refuse_gradients("attention over", q, slopes)
     if q.device != cache.keys.device:
         raise ValueError("q must be on the cache's device")
     out_dtype = out_dtype or q.dtype
