@@ -33,7 +33,8 @@ from .ratchet import DiscreteRatchetLinear
 # rest of the model config is fixed for generation (no dropout) or derived (vocabulary).
 _ARCHITECTURE = (("block_size", int), ("n_layer", int), ("n_head", int), ("n_embd", int))
 _OPTIONAL = (("matmul_mode", str, "fp32"), ("ratchet_embedding", bool, False),
-             ("rms_ema_beta", float, 0.0), ("pressure_leak_period", int, 0))
+             ("rms_ema_beta", float, 0.0), ("pressure_leak_period", int, 0),
+             ("attention_softcap", float, 0.0), ("distance_bias", bool, False))
 
 
 def _checkpoint_files(base_path: str | Path) -> tuple[Path, Path]:
