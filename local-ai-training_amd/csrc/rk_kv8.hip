@@ -265,11 +265,12 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a) {
 // Both products run on the codes as they are, in exact integers: the query is written as a fixed
 // point number of signed base-256 digits relative to its largest feature, the probabilities
 // relative to the block's largest, and each digit's product is its own MFMA. Three digits (23
-// bits, about a float32 operand's rounding) for float32 results, two (15 bits, against the 8 of
-// the result) for bf16. The matrix unit takes them at a
-// fraction of the time the codes need to arrive, and no code is ever converted: for one query
-// per head, 32 MFMAs (48 with three digits) and a few hundred vector instructions per 16 KB of
-// codes at D = 128.
+// bits, about a float32 operand's rounding) for queries, whose largest feature may be thousands of
+// times the others (with two, one of 500 times took bf16 results from 1.7e-3 to 4e-3), and for the
+// probabilities of float32 results; two (15 bits, against the 8 of the result) for those of bf16.
+// The matrix unit takes them at a fraction of the time the codes need to arrive, and no code is ever
+// converted: for one query per head, 40 MFMAs (48 with three digits) and a few hundred vector
+// instructions per 16 KB of codes at D = 128.
 //
 // A wavefront walks blocks of 64 tokens with its own running max, sum and output. Lane l holds the
 // scores of column l % 16 against keys 16 (l / 16) .. + 15: key 16 g + 4 t + e is row 4 g + e of
@@ -374,7 +375,8 @@ __device__ __forceinline__ float row_factor(const Kv8Attn& a, int64_t b, int64_t
 
 template <int D, int QDT, int ODT, int NW, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
-  constexpr int KK = D / 64, FT = D / 16, ND = ODT == RK_F32 ? 3 : 2, NT = 64 * NW;
+  constexpr int KK = D / 64, FT = D / 16, NT = 64 * NW;
+  constexpr int NQ = 3, ND = ODT == RK_F32 ? 3 : 2;  // digits of queries, of probabilities
   __shared__ __attribute__((aligned(16))) float so[NW][16][D + 4];
   __shared__ float sm[NW][16], sl[NW][16];
   const int split = blockIdx.x;
@@ -445,7 +447,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
     load_k(j);
     load_v(j);
     // the query's digits: features 64 kk + 16 g .. + 15
-    v4i8 qd[ND][KK];
+    v4i8 qd[NQ][KK];
     float qscale;
     {
       float x[KK][16];
@@ -464,23 +466,22 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
       }
       most = col_umax(most);
       const float big = __uint_as_float(most);
-      const float up = big > 0.0f ? kFixed<ND> / big : 0.0f;
-      qscale = big / kFixed<ND>;
+      const float up = big > 0.0f ? kFixed<NQ> / big : 0.0f;
+      qscale = big / kFixed<NQ>;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t y[4];
-          int d[ND];
+          int d[NQ];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float v = fminf(fmaxf(x[kk][4 * w + e] * up, -kFixed<ND>), kFixed<ND>);
-            y[e] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v)) +
-                                         (ND == 3 ? 0x8080 : 0x80));
+            const float v = fminf(fmaxf(x[kk][4 * w + e] * up, -kFixed<NQ>), kFixed<NQ>);
+            y[e] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v)) + 0x8080);
           }
-          digits4<ND>(y, d);
+          digits4<NQ>(y, d);
 #pragma unroll
-          for (int n = 0; n < ND; ++n) qd[n][kk][w] = d[n];
+          for (int n = 0; n < NQ; ++n) qd[n][kk][w] = d[n];
         }
     }
     for (; j < j1; j += NW) {
@@ -489,9 +490,9 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
       const float mul = qscale * kscale * a.dot_scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        v4i8 acc[ND];
+        v4i8 acc[NQ];
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
+        for (int d = 0; d < NQ; ++d) {
           acc[d] = v4i8{0, 0, 0, 0};
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk)
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          s[4 * t + e] = from_digits<ND>(acc, e) * mul;
+          s[4 * t + e] = from_digits<NQ>(acc, e) * mul;
       }
       load_k(j + NW);
       const int64_t ahead = pos - (j * kTok + 16 * g);
