@@ -790,11 +790,12 @@ int rk_int8_kv_read(const rk_int8_kv* cache, int64_t begin, int64_t end, int dty
  * cache: query i of a sequence stands at position start + i and sees positions 0 .. start + i,
  * which must have been appended. Scores, softcap and slopes (float32 [Hq]) as in
  * rk_scored_attention_forward. out: [B, S, Hq, D] contiguous, float32 or bf16; zeros for queries
- * at or past lengths and for negative starts, NaN for positions past the cache. The products run
- * in integers on the codes, with queries rounded to 23 bits of their row's largest feature and
- * probabilities to 23 bits (15 for bf16 results) of their block's largest; chunks of 32 bf16 tokens
- * and more with bf16 results take bf16 products, with the probabilities rounded to bf16. work:
- * rk_int8_kv_attention_work floats (0: none), 16-byte aligned.
+ * at or past lengths and for negative starts, NaN for positions past the cache. Scores come from
+ * integer products on the codes, with queries rounded to 23 bits of their row's largest feature;
+ * probabilities enter the second product as sums of bf16 numbers, off by 2^-24 of themselves
+ * (2^-16 for bf16 results). Chunks of 32 bf16 tokens and more with bf16 results take the queries as
+ * they are and the probabilities rounded to bf16. work: rk_int8_kv_attention_work floats (0: none),
+ * 16-byte aligned.
  * No counterpart in the reference (its window is recomputed per token, generate.py:183-201).
  */
 int64_t rk_int8_kv_attention_work(const rk_int8_kv* cache, int64_t Hq, int64_t S, int qdtype,

@@ -23,6 +23,7 @@ constexpr int64_t kChunkTokens = 32;  // a wavefront's queries: from here on kv8
 constexpr float kLog2e8 = 1.4426950408889634f;
 
 typedef int v4i8 __attribute__((ext_vector_type(4)));
+typedef float v4f_a __attribute__((ext_vector_type(4)));
 
 struct Kv8 {
   int8_t* keys;
@@ -262,20 +263,23 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a) {
 // with k_j, v_j what the codes stand for. Columns of a product are the S * G queries that share a
 // key head (G = query heads per key head), 16 at a time; rows are keys, then features.
 //
-// Both products run on the codes as they are, in exact integers: the query is written as a fixed
-// point number of signed base-256 digits relative to its largest feature, the probabilities
-// relative to the block's largest, and each digit's product is its own MFMA. Three digits (23
-// bits, about a float32 operand's rounding) for queries, whose largest feature may be thousands of
-// times the others (with two, one of 500 times took bf16 results from 1.7e-3 to 4e-3), and for the
-// probabilities of float32 results; two (15 bits, against the 8 of the result) for those of bf16.
-// The matrix unit takes them at a fraction of the time the codes need to arrive, and no code is ever
-// converted: for one query per head, 40 MFMAs (48 with three digits) and a few hundred vector
-// instructions per 16 KB of codes at D = 128.
+// The first product runs on the codes as they are, in exact integers: the query is written as a
+// fixed-point number of three signed base-256 digits (23 bits) relative to its largest feature,
+// which may be thousands of times the others (in two, one of 500 times took bf16 results from 1.7e-3
+// to 4e-3), and each digit's product is its own MFMA.
+// The second takes codes widened to bf16, which holds them exactly, and probabilities as sums of bf16
+// numbers: three for float32 results (24 bits of each probability), two for bf16 (16 bits). A
+// probability needs its own exponent: as fixed-point numbers relative to their block's largest, those
+// beside a token that takes nearly all of the attention lost their bits, and where that token's
+// value is small they are the result (with 1e-3 left to the others, bf16 results off by a tenth;
+// widening and splitting cost 137 -> 142 us at 16 sequences of 5 to 16 thousand tokens, 30 -> 33 at
+// 48 of 2.7 to 8.1 thousand with shared heads). For one query per head, 56 MFMAs (72 with three
+// parts) and about 500 vector instructions per 16 KB of codes at D = 128.
 //
 // A wavefront walks blocks of 64 tokens with its own running max, sum and output. Lane l holds the
 // scores of column l % 16 against keys 16 (l / 16) .. + 15: key 16 g + 4 t + e is row 4 g + e of
-// product t, and the same 16 keys are the lane's k slots of the second product, whose other
-// operand, 16 tokens of one feature, lies side by side in the cache. The wavefronts of a
+// product t, and the same 16 keys are the lane's k slots of the second product (8 for each half),
+// whose other operand, 16 tokens of one feature, lies side by side in the cache. The wavefronts of a
 // workgroup are joined in LDS, splits of a long cache by a second launch.
 //
 // 16 sequences of 5 to 16 thousand tokens, 16 heads of 128: 143-147 us, 820 MB of codes at 5.6 TB/s
@@ -320,36 +324,61 @@ __device__ __forceinline__ uint32_t col_umax(uint32_t v) {
   return s[0] > s[1] ? s[0] : s[1];
 }
 
-// A number of ND signed base-256 digits, the largest 127 256^(ND - 1).
-template <int ND>
-constexpr float kFixed = ND == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
+constexpr int kDigits = 3;  // of a query's number, signed, base 256: the largest is kFixed
+constexpr float kFixed = 127.0f * 65536.0f;
 
 // Digits of 4 numbers, each given as the word whose low bytes are the number plus 128 in every
 // digit but the first (which makes them unsigned, without a carry to take back), as one word a
 // digit, the first digit first.
-template <int ND>
-__device__ __forceinline__ void digits4(const uint32_t (&w)[4], int (&d)[ND]) {
+__device__ __forceinline__ void digits4(const uint32_t (&w)[4], int (&d)[kDigits]) {
   const uint32_t p01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);  // low bytes, second bytes
   const uint32_t p23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
   const uint32_t low = __builtin_amdgcn_perm(p23, p01, 0x05040100u);
   const uint32_t mid = __builtin_amdgcn_perm(p23, p01, 0x07060302u);
-  d[ND - 1] = static_cast<int>(low ^ 0x80808080u);
-  if constexpr (ND == 3) {
-    const uint32_t h01 = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602u);
-    const uint32_t h23 = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0602u);
-    d[1] = static_cast<int>(mid ^ 0x80808080u);
-    d[0] = static_cast<int>(__builtin_amdgcn_perm(h23, h01, 0x05040100u));
-  } else {
-    d[0] = static_cast<int>(mid);
-  }
+  const uint32_t h01 = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0602u);
+  const uint32_t h23 = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0602u);
+  d[0] = static_cast<int>(__builtin_amdgcn_perm(h23, h01, 0x05040100u));
+  d[1] = static_cast<int>(mid ^ 0x80808080u);
+  d[2] = static_cast<int>(low ^ 0x80808080u);
 }
 
 // The sum that the digits' sums make (each below 2^22, so two of them fit an integer).
-template <int ND>
-__device__ __forceinline__ float from_digits(const v4i8 (&d)[ND], int e) {
-  const float low = static_cast<float>(d[ND - 2][e] * 256 + d[ND - 1][e]);
-  if constexpr (ND == 3) return __builtin_fmaf(static_cast<float>(d[0][e]), 65536.0f, low);
-  return low;
+__device__ __forceinline__ float from_digits(const v4i8 (&d)[kDigits], int e) {
+  return __builtin_fmaf(static_cast<float>(d[0][e]), 65536.0f,
+                        static_cast<float>(d[1][e] * 256 + d[2][e]));
+}
+
+template <bool SCALED = false>
+__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi,
+                                            float power = 1.0f) {
+  uint32_t f[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float x = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
+    f[e] = __float_as_uint(SCALED ? x * power : x);
+  }
+  lo = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);  // small integers: the low halves are zero
+  hi = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
+}
+
+// 16 probabilities as sums of N bf16 numbers each, the largest parts first: off by 2^-8N of
+// themselves.
+template <int N>
+__device__ __forceinline__ void split_bf16(float (&p)[16], v8bf_a (&part)[N][2]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = bf16_pair(p[2 * i], p[2 * i + 1]);
+      if (n + 1 < N) {  // what is left, exactly
+        p[2 * i] = p[2 * i] - __uint_as_float(w[i] << 16);
+        p[2 * i + 1] = p[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+    part[n][0] = frag_of(make_uint4(w[0], w[1], w[2], w[3]));
+    part[n][1] = frag_of(make_uint4(w[4], w[5], w[6], w[7]));
+  }
 }
 
 template <int QDT>
@@ -376,7 +405,7 @@ __device__ __forceinline__ float row_factor(const Kv8Attn& a, int64_t b, int64_t
 template <int D, int QDT, int ODT, int NW, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
   constexpr int KK = D / 64, FT = D / 16, NT = 64 * NW;
-  constexpr int NQ = 3, ND = ODT == RK_F32 ? 3 : 2;  // digits of queries, of probabilities
+  constexpr int NP = ODT == RK_F32 ? 3 : 2;  // parts of a probability
   __shared__ __attribute__((aligned(16))) float so[NW][16][D + 4];
   __shared__ float sm[NW][16], sl[NW][16];
   const int split = blockIdx.x;
@@ -447,7 +476,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
     load_k(j);
     load_v(j);
     // the query's digits: features 64 kk + 16 g .. + 15
-    v4i8 qd[NQ][KK];
+    v4i8 qd[kDigits][KK];
     float qscale;
     {
       float x[KK][16];
@@ -466,22 +495,22 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
       }
       most = col_umax(most);
       const float big = __uint_as_float(most);
-      const float up = big > 0.0f ? kFixed<NQ> / big : 0.0f;
-      qscale = big / kFixed<NQ>;
+      const float up = big > 0.0f ? kFixed / big : 0.0f;
+      qscale = big / kFixed;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t y[4];
-          int d[NQ];
+          int d[kDigits];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float v = fminf(fmaxf(x[kk][4 * w + e] * up, -kFixed<NQ>), kFixed<NQ>);
+            const float v = fminf(fmaxf(x[kk][4 * w + e] * up, -kFixed), kFixed);
             y[e] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v)) + 0x8080);
           }
-          digits4<NQ>(y, d);
+          digits4(y, d);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) qd[n][kk][w] = d[n];
+          for (int n = 0; n < kDigits; ++n) qd[n][kk][w] = d[n];
         }
     }
     for (; j < j1; j += NW) {
@@ -490,9 +519,9 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
       const float mul = qscale * kscale * a.dot_scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        v4i8 acc[NQ];
+        v4i8 acc[kDigits];
 #pragma unroll
-        for (int d = 0; d < NQ; ++d) {
+        for (int d = 0; d < kDigits; ++d) {
           acc[d] = v4i8{0, 0, 0, 0};
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk)
@@ -500,7 +529,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          s[4 * t + e] = from_digits<NQ>(acc, e) * mul;
+          s[4 * t + e] = from_digits(acc, e) * mul;
       }
       load_k(j + NW);
       const int64_t ahead = pos - (j * kTok + 16 * g);
@@ -524,29 +553,17 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
       const float alpha = __builtin_amdgcn_exp2f(m - nref);
       const float beta = __builtin_amdgcn_exp2f(mx - nref);
       m = mnew;
-      // p as a fixed-point number: 2^23 and the digits' 128s are added in float32, which rounds
-      // it and leaves the digits in the low bytes of the sum
       float sum = 0.0f;
-      v4i8 pd[ND];
-      constexpr float kUnit = ND == 3 ? 8388608.0f + 32896.0f : 8388608.0f + 128.0f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t y[4];
-        int d[ND];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(s[4 * w + e] - ref);
-          sum = sum + p;
-          y[e] = __float_as_uint(__builtin_fmaf(p, kFixed<ND>, kUnit));
-        }
-        digits4<ND>(y, d);
-#pragma unroll
-        for (int n = 0; n < ND; ++n) pd[n][w] = d[n];
+      for (int x = 0; x < 16; ++x) {
+        s[x] = __builtin_amdgcn_exp2f(s[x] - ref);
+        sum = sum + s[x];
       }
+      v8bf_a p[NP][2];
+      split_bf16<NP>(s, p);
       l = l * alpha + beta * col_sum(sum);
       // a block that the column does not see at all adds nothing, whatever its scale
-      const float add =
-          mx == -INFINITY && sum == 0.0f ? 0.0f : beta * vscale * (1.0f / kFixed<ND>);
+      const float add = mx == -INFINITY && sum == 0.0f ? 0.0f : beta * vscale;
       if (__any(alpha != 1.0f)) {
 #pragma unroll
         for (int f = 0; f < FT; ++f)
@@ -555,13 +572,20 @@ __global__ __launch_bounds__(64 * NW) void kv8_attn_kernel(Kv8Attn a) {
       }
 #pragma unroll
       for (int f = 0; f < FT; ++f) {
-        v4i8 acc[ND];
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-          acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[f], pd[d], v4i8{0, 0, 0, 0}, 0, 0, 0);
+        uint32_t w[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          o[f][e] = __builtin_fmaf(from_digits<ND>(acc, e), add, o[f][e]);
+          widen_codes(static_cast<uint32_t>(vf[f][e]), w[2 * e], w[2 * e + 1]);
+        const v8bf_a v[2] = {frag_of(make_uint4(w[0], w[1], w[2], w[3])),
+                             frag_of(make_uint4(w[4], w[5], w[6], w[7]))};
+        v4f_a acc{};
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], p[n][u], acc, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[f][e] = __builtin_fmaf(acc[e], add, o[f][e]);
       }
       load_v(j + NW);
     }
@@ -660,8 +684,8 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
 // ---------------------------------------------------------------------------
 // The same for chunks of many bf16 tokens with bf16 results (a prompt's next part): one workgroup
 // takes 128 queries of a head, in two halves of four wavefronts that walk every other block; a
-// wavefront takes 32 queries of its half, the halves are joined in LDS at the end, and the products run on the bf16 MFMA as in
-// rk_attention.hip (scores transposed, a lane holds one query). The codes become bf16 once per
+// wavefront takes 32 queries of its half, the halves are joined in LDS at the end, and the products
+// run on the bf16 MFMA as in rk_attention.hip (scores transposed, a lane holds one query). The codes become bf16 once per
 // half and block, exactly (8 bits), on their way into LDS; the key scale goes into the score,
 // the value scale into the probabilities before they are rounded to bf16. Values lie by feature, so
 // the second product's operand is a row read too: the tokens of a row are stored in the order in
@@ -674,19 +698,6 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
 // other, so its MFMAs (1024 cycles a block and wavefront) and its vector instructions (590) overlap
 // little: those two are what it spends its time on.
 // ---------------------------------------------------------------------------
-template <bool SCALED = false>
-__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi,
-                                            float power = 1.0f) {
-  uint32_t f[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float x = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
-    f[e] = __float_as_uint(SCALED ? x * power : x);
-  }
-  lo = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);  // small integers: the low halves are zero
-  hi = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
-}
-
 // A block's value scale: `fold` goes into the exponent of its probabilities, whose sum is
 // multiplied by `inv`, and `rest` into its values. Scales whose products could leave float32's
 // range leave a power of two to the values; one that is not finite makes its values zero and the
@@ -1013,7 +1024,9 @@ static Kv8Plan attention_plan(const rk_int8_kv& c, int64_t Hq, int64_t S, int qd
     // few workgroups: eight wavefronts in each, so that up to 16 blocks need no join (16 heads of
     // 1000 tokens 10.6 us; four wavefronts in four splits 6.7 + 4.0); otherwise as many
     // workgroups as the device holds (twice as many gained nothing)
-    p.waves = have <= 128 ? 8 : 4;
+    // (head size 256 needs more registers than eight wavefronts have: 66 us with them, 40 with
+    // four, at 8 sequences of 1.3 to 4 thousand tokens and 16 heads)
+    p.waves = have <= 128 && c.D <= 128 ? 8 : 4;
     p.splits = splits(c.D == 64 ? 1024 : 512, p.waves == 8 ? 16 : 4);
     return p;
   }
@@ -1040,8 +1053,10 @@ static void launch_kv8_attn(const Kv8Attn& a, bool cap, hipStream_t st) {
 
 template <int D, int QDT, int ODT>
 static void launch_kv8_waves(const Kv8Attn& a, const Kv8Plan& plan, bool cap, hipStream_t st) {
-  if (plan.waves == 8) launch_kv8_attn<D, QDT, ODT, 8>(a, cap, st);
-  else launch_kv8_attn<D, QDT, ODT, 4>(a, cap, st);
+  if constexpr (D <= 128) {
+    if (plan.waves == 8) return launch_kv8_attn<D, QDT, ODT, 8>(a, cap, st);
+  }
+  launch_kv8_attn<D, QDT, ODT, 4>(a, cap, st);
 }
 
 template <int D>
