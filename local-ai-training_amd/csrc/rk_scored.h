@@ -146,14 +146,15 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, uint64_t bits, int tid
 }
 
 // What rounding 4 numbers to the bf16 pairs lo, hi left, a byte each in 256ths of the bf16 step
-// (rounded down, so to 2^-16 of the number): the second byte of the bit patterns' difference,
-// which lies in -2^15 .. 2^15 (the upper end, a tie, taken as the largest byte).
+// (to the nearest, so to 2^-16 of the number, and exact where nothing was left: a token that sees
+// only itself gets no gradient from o's own rounding): the second byte of the bit patterns'
+// difference, which lies in -2^15 .. 2^15 (the upper end, a tie, taken as the largest byte).
 __device__ __forceinline__ uint32_t bf16_rest4(const float (&x)[4], uint32_t lo, uint32_t hi) {
   const uint32_t r[4] = {lo << 16, lo & 0xffff0000u, hi << 16, hi & 0xffff0000u};
   uint32_t d[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int diff = static_cast<int>(__float_as_uint(x[e]) - r[e]);
+    const int diff = static_cast<int>(__float_as_uint(x[e]) - r[e]) + 128;
     d[e] = static_cast<uint32_t>(diff < 0x7fff ? diff : 0x7fff);
   }
   const uint32_t p01 = __builtin_amdgcn_perm(d[1], d[0], 0x0c0c0501u);
@@ -170,9 +171,9 @@ __device__ __forceinline__ uint32_t* rest_words(const ScoredArgs& a, int64_t bh,
   return reinterpret_cast<uint32_t*>(a.p.rest + (bh * a.Sp + row0) * D);
 }
 
-// The float32 number, to the middle of its rest's step.
+// The float32 number, to half of its rest's step.
 __device__ __forceinline__ float with_rest(uint32_t bf16_high, int rest) {
-  return __uint_as_float(bf16_high + static_cast<uint32_t>(rest * 256 + 128));
+  return __uint_as_float(bf16_high + static_cast<uint32_t>(rest * 256));
 }
 
 int check_scored(const rk_scored_attention_args& p, bool backward);
