@@ -5,7 +5,7 @@
 //
 // Layout: keys int8 [B, Hkv, NB, 64, D], values int8 [B, Hkv, NB, D, 64] (by feature), one
 // float32 scale per block and head for each. Both products of the attention then read their
-// operand as v_mfma_i32_16x16x64_i8 takes it, 16 bytes per lane straight from memory.
+// operand 16 bytes per lane straight from memory, in the order in which the MFMA takes it.
 //
 // Quantization: s = absmax / 127 over the block's tokens, code = rint(x / s) (IEEE float32
 // quotients, the rule of rk_quantize_rows). Tokens appended to a block that holds some can only
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Kv8Read a) {
 //
 // 16 sequences of 5 to 16 thousand tokens, 16 heads of 128: 143-147 us, 820 MB of codes at 5.6 TB/s
 // (the device's own copy reaches 5.3); 48 sequences of 2.7 to 8.1 thousand, 32 heads of 64 on 4,
-// capped: 26 + 4 us for 125 MB; one of 1000, 16 heads of 128: 10.6 us, a chain of load latencies.
+// capped: 31 + 4 us for 125 MB; one of 1000, 16 heads of 128: 11.4 us, a chain of load latencies.
 // ---------------------------------------------------------------------------
 struct Kv8Attn {
   Kv8 c;
@@ -685,15 +685,16 @@ __global__ __launch_bounds__(64) void kv8_join_kernel(Kv8Attn a) {
 // The same for chunks of many bf16 tokens with bf16 results (a prompt's next part): one workgroup
 // takes 128 queries of a head, in two halves of four wavefronts that walk every other block; a
 // wavefront takes 32 queries of its half, the halves are joined in LDS at the end, and the products
-// run on the bf16 MFMA as in rk_attention.hip (scores transposed, a lane holds one query). The codes become bf16 once per
-// half and block, exactly (8 bits), on their way into LDS; the key scale goes into the score,
-// the value scale into the probabilities before they are rounded to bf16. Values lie by feature, so
-// the second product's operand is a row read too: the tokens of a row are stored in the order in
-// which a lane holds its probabilities. The next block's codes are in registers meanwhile.
+// run on the bf16 MFMA as in rk_attention.hip (scores transposed, a lane holds one query). The codes
+// become bf16 once per half and block, exactly (8 bits), on their way into LDS; the key scale goes
+// into the score, the value scale into the probabilities before they are rounded to bf16. Values lie
+// by feature, so the second product's operand is a row read too: the tokens of a row are stored in
+// the order in which a lane holds its probabilities. The next block's codes are in registers
+// meanwhile.
 //
-// 4 x 517 tokens behind 1500, 16 heads of 128 (30 GFLOP): 72 us and 5 for the last tile's join; the
-// digits of kv8_attn_kernel 176. A last tile of few queries is split over the keys (attention_plan):
-// its workgroups were 25 of 96 us. Four wavefronts without the halves 82-86; the next block converted
+// 4 x 517 tokens behind 1500, 16 heads of 128 (30 GFLOP): 73 us and 5 for the last tile's join;
+// kv8_attn_kernel in its place took 176. A last tile of few queries is split over the keys
+// (attention_plan): its workgroups were 25 of 96 us. Four wavefronts without the halves 82-86; the next block converted
 // between the two products instead of behind them 99. The wavefronts of a half keep step with each
 // other, so its MFMAs (1024 cycles a block and wavefront) and its vector instructions (590) overlap
 // little: those two are what it spends its time on.
@@ -1021,9 +1022,10 @@ static Kv8Plan attention_plan(const rk_int8_kv& c, int64_t Hq, int64_t S, int qd
     return n < 1 || most < 1 ? 1 : n < most ? n : most;
   };
   if (!p.chunk) {
-    // few workgroups: eight wavefronts in each, so that up to 16 blocks need no join (16 heads of
-    // 1000 tokens 10.6 us; four wavefronts in four splits 6.7 + 4.0); otherwise as many
-    // workgroups as the device holds (twice as many gained nothing)
+    // few workgroups: eight wavefronts in each, so that up to 16 blocks need no join (16 and 128
+    // heads of 128, 1000 tokens: 9.3 and 12.7 us a call; four wavefronts in splits 12.7 and 13.2; of
+    // 4000 tokens 12.8 and 26, against 13.0 and 22.7, and above 128 always slower from there on);
+    // otherwise as many workgroups as the device holds (twice as many gained nothing)
     // (head size 256 needs more registers than eight wavefronts have: 66 us with them, 40 with
     // four, at 8 sequences of 1.3 to 4 thousand tokens and 16 heads)
     p.waves = have <= 128 && c.D <= 128 ? 8 : 4;
@@ -1032,7 +1034,8 @@ static Kv8Plan attention_plan(const rk_int8_kv& c, int64_t Hq, int64_t S, int qd
   }
   p.splits = p.full_splits = splits(256, 8);
   // a last tile of less than 64 queries behind whole ones: its few busy wavefronts would be the
-  // launch's tail, so its keys are split
+  // launch's tail, so its keys are split (512 + 5 to 512 + 63 tokens behind 2000, 4 sequences, 16 heads
+  // of 128: 86-91 us, unsplit 108-113; fuller ones would gain as much, 512 + 120: 93, unsplit 116)
   const int64_t full = S / 128, rest = S % 128;
   if (p.splits == 1 && full > 0 && rest > 0 && rest < 64 && c.blocks >= 16) {
     p.splits = c.blocks / 8 < 8 ? c.blocks / 8 : 8;

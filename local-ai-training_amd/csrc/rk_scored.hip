@@ -15,7 +15,7 @@
 // B 8, H 16, S 1024, D 128: causal 68 us (34 GFLOP, 510 TFLOP/s; rk_attention_forward 55-60), in
 // documents of 400 on average 44, with capped scores 69 and 50; B 32, H 8, S 512, D 64 in
 // documents of 150 20.6 us, where reading q, k, v and writing o and its rest takes 16 at 5.3 TB/s.
-// The vector unit is busy half of the time (829 instructions a step of 64 keys, capped), the
+// The vector unit is busy two fifths of the time (719 instructions a step of 64 keys, capped), the
 // matrix unit an eighth: what is left is waiting between a step's dependent parts, and
 // wavefronts of a workgroup that wait for the one whose rows see most.
 #include "rk_scored.h"

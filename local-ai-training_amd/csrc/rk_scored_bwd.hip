@@ -21,8 +21,8 @@
 // B 8, H 16, S 1024, D 128: causal 85 + 115 us (rk_attention_backward 75 + 90 for the same 120
 // GFLOP), in documents of 400 on average 59 + 69, capped as well 67 + 88; B 4, S 1001 with a
 // learned bias 54 + 62; B 32, H 8, S 512, D 64 in documents of 150 29.6 + 29.5 us. Per step a
-// wavefront of the keys' launch waits 60% of its cycles (barriers, LDS operands, dependent
-// products), its vector instructions fill 20 of the 86 us and its MFMAs 13. Three stages of
+// wavefront of the keys' launch waits 58% of its cycles (barriers, LDS operands, dependent
+// products), its vector instructions fill 18 of the 88 us and its MFMAs 12.5. Three stages of
 // tiles for the queries changed nothing, 64 staged rows at D 128 and both products ahead of a
 // p formed in two halves were slower.
 #include "rk_scored.h"
