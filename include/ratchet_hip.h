@@ -806,6 +806,102 @@ int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int qdtype, int
                          const float* slopes, float* work, int64_t work_floats, void* out,
                          int odtype, void* stream);
 
+/*
+ * Appends the accepted nodes of drafted trees to the 8-bit caches of `count` layers at once (the same
+ * shape, each its own buffers): token i < counts[b] of sequence b is node path[b][i] of that layer's k
+ * and v (float32 or bf16 [B, H, N, D] as in rk_int8_kv_append, all layers the same dtype), and goes
+ * to position start + i. path: device int64 [B][P], row stride path_step; counts: device int64 [B],
+ * at most P of which count; nodes outside 0 .. N - 1 are tokens of zeros. Blocks and scales as in
+ * rk_int8_kv_append.
+ * No counterpart in the reference (it drafts nothing, generate.py:183-201).
+ */
+typedef struct rk_int8_kv_commit_layer {
+  rk_int8_kv cache;
+  const void *k, *v;
+  int64_t skb, skh, sks, svb, svh, svs;
+} rk_int8_kv_commit_layer;
+
+int rk_int8_kv_commit(const rk_int8_kv_commit_layer* layers, int64_t count, int64_t N, int dtype,
+                      const int64_t* start, int64_t start_count, const int64_t* path,
+                      int64_t path_step, int64_t P, const int64_t* counts, void* stream);
+
+/*
+ * The plan of R trees of N <= 256 drafted tokens: parents (device int32, or int64 with wide != 0;
+ * row stride ldp) holds -1 for node 0, the root, and an earlier node for every other one. A node
+ * whose parent is not such, and what descends from it, is off. kept [R][N]: the parents, -2 for
+ * nodes that are off; depths [R][N]: steps from the root (0 for nodes that are off); seen
+ * [R][N][(N + 63) / 64]: a bit for the node itself and each of its ancestors (none for nodes that
+ * are off).
+ */
+int rk_draft_tree(const void* parents, int wide, int64_t ldp, int64_t R, int64_t N, int32_t* kept,
+                  int32_t* depths, uint64_t* seen, void* stream);
+
+/*
+ * Attention of the nodes of drafted trees over the 8-bit cache and over themselves: q [B, Hq, N, D],
+ * k, v [B, H, N, D] (one dtype, float32 or bf16; element strides, unit feature stride, rows whole
+ * 16-byte vectors), Hq a multiple of H, N <= 256. Node i of a sequence stands at position
+ * start + depths[i] and sees positions 0 .. start - 1 of the cache and the nodes in seen[i], itself
+ * among them (rk_draft_tree; one tree, or one per sequence). start: device int64, one or one per
+ * sequence. lengths (device int64 [B], or NULL: N): nodes at or past it are not there. Scores,
+ * softcap and slopes (float32 [Hq], by the distance of the positions) as in
+ * rk_scored_attention_forward. out: [B, N, Hq, D] contiguous, float32 or bf16; zeros for nodes that
+ * are off or not there and for negative starts, NaN for starts past the cache. Over the cache bf16
+ * queries enter as they are, float32 ones as sums of three bf16 numbers, probabilities as sums of
+ * two (three for float32 results); the nodes' part is float32. work: rk_tree_attention_work
+ * floats, 16-byte aligned.
+ * No counterpart in the reference (it drafts nothing, generate.py:183-201).
+ */
+typedef struct rk_tree_attention_args {
+  rk_int8_kv cache;
+  const void *q, *k, *v;
+  void* out;
+  const int64_t *start, *lengths;
+  const uint64_t* seen;
+  const int32_t* depths;
+  const float* slopes;
+  int64_t N, Hq, trees, start_count;
+  int64_t sqb, sqh, sqs, skb, skh, sks, svb, svh, svs;
+  float scale, softcap;
+  int dtype, out_dtype;
+} rk_tree_attention_args;
+
+int64_t rk_tree_attention_work(const rk_tree_attention_args* args);
+int rk_tree_attention(const rk_tree_attention_args* args, float* work, int64_t work_floats,
+                      void* stream);
+
+/*
+ * Verification of drafted trees: logits [B, N, V] of the target at every node (float32 or bf16,
+ * element strides lb, ln, unit stride over V) and, or NULL, drafts, those of the drafter (db, dn);
+ * tokens device int64 [B][N], uniforms float32 [B][N] in [0, 1), parents as rk_draft_tree keeps them
+ * (one tree, or one per sequence), lengths device int64 [B] or NULL. With p_n, q_n the softmax of the
+ * logits at node n over the temperature, of those not below the top_k-th largest (0: all),
+ * the walk begins at node 0; a child c of the node reached (in their order, token x) stands if
+ * u_c q(x) < p(x), otherwise p becomes max(p - q, 0) over its sum (a sum up to 2^-40 is rounding:
+ * then p stays); without drafts q is 1 at x. Where no child stands, next is the first token whose cumulated p passes u_0 times its sum. Temperature 0
+ * (else at least 1e-6): a child stands if its token is the first largest logit's, which is next
+ * otherwise; uniforms and drafts are not read. path [B][N]: the nodes that stand from the root on,
+ * then -1; counts [B]: how many; next [B]. A sequence without nodes has count 0 and next -1; a row
+ * that is no distribution (a NaN, +inf, or -inf only) lets no child stand and gives next -1; a
+ * token outside 0 .. V - 1 does not stand. Probabilities and their sums are 64-bit numbers. work:
+ * rk_verify_drafts_work bytes, 16-byte aligned.
+ * Replaces: the draw of one token, generate.py:180-197 (N = 1).
+ */
+typedef struct rk_verify_drafts_args {
+  const void *logits, *drafts;
+  int64_t lb, ln, db, dn, B, N, V, trees, top_k;
+  const int64_t* tokens;
+  const float* uniforms;
+  const int32_t* parents;
+  const int64_t* lengths;
+  double temperature;
+  int64_t *path, *counts, *next;
+  int dtype;
+} rk_verify_drafts_args;
+
+int64_t rk_verify_drafts_work(const rk_verify_drafts_args* args);
+int rk_verify_drafts(const rk_verify_drafts_args* args, void* work, int64_t work_bytes,
+                     void* stream);
+
 /* HBM streaming probe (measurement only; no counterpart in the reference): reads `bytes`
  * (a multiple of 16) from src in 16-byte vectors, `unroll` (1, 2, 4, 8) loads in flight
  * per thread, `blocks` blocks of 256 threads in a grid-stride loop; copy != 0 writes them

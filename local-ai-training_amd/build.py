@@ -58,6 +58,7 @@ SOURCE_FLAGS = {
     "rk_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "rk_scored.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "rk_kv8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "rk_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -1428,6 +1428,187 @@ Tensor int8_kv_attention(const Tensor& q, const Tensor& keys, const Tensor& valu
   return out.permute({0, 2, 1, 3});
 }
 
+// Accepted nodes of drafted trees into the 8-bit caches of several layers (rk_int8_kv_commit).
+void int8_kv_commit(at::TensorList ks, at::TensorList vs, at::TensorList keys,
+                    at::TensorList values, at::TensorList key_scales, at::TensorList value_scales,
+                    const Tensor& start, const Tensor& path, const Tensor& counts) {
+  constexpr const char* what = "int8 kv commit";
+  const size_t n = keys.size();
+  TORCH_CHECK(n > 0 && ks.size() == n && vs.size() == n && values.size() == n &&
+                  key_scales.size() == n && value_scales.size() == n,
+              what, ": one k, v and cache per layer");
+  std::vector<rk_int8_kv_commit_layer> layers(n);
+  std::vector<Tensor> held;  // copies of operands that do not lie as vectors
+  held.reserve(2 * n);
+  const int code = dtype_code(ks[0], what);
+  for (size_t i = 0; i < n; ++i) {
+    const rk_int8_kv c = int8_kv(keys[i], values[i], key_scales[i], value_scales[i], what);
+    same_device(keys[0], keys[i], what);
+    for (const Tensor* t : {&ks[i], &vs[i]}) {
+      same_device(keys[0], *t, what);
+      TORCH_CHECK(t->dim() == 4 && t->size(0) == c.B && t->size(1) == c.H &&
+                      t->size(2) == ks[0].size(2) && t->size(3) == c.D &&
+                      t->scalar_type() == ks[0].scalar_type(),
+                  what, ": k and v must share a dtype and the caches' [B, H, N, D] shape");
+    }
+    held.push_back(vector_rows(ks[i]));
+    held.push_back(vector_rows(vs[i]));
+    const Tensor &k = held[2 * i], &v = held[2 * i + 1];
+    layers[i] = {c, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+                 v.stride(0), v.stride(1), v.stride(2)};
+  }
+  const int64_t B = keys[0].size(0);
+  const int64_t* at = positions(keys[0], start, B, true, what);
+  const int64_t* count = positions(keys[0], counts, B, false, what);
+  same_device(keys[0], path, what);
+  TORCH_CHECK(path.scalar_type() == at::kLong && path.dim() == 2 && path.size(0) == B &&
+                  (path.stride(1) == 1 || path.size(1) <= 1),
+              what, ": path must be int64, one row per sequence");
+  const c10::DeviceGuard guard(keys[0].device());
+  check_status(rk_int8_kv_commit(layers.data(), static_cast<int64_t>(n), ks[0].size(2), code, at,
+                                 start.size(0), path.data_ptr<int64_t>(), ld(path), path.size(1),
+                                 count, stream_of(keys[0])),
+               "rk_int8_kv_commit");
+}
+
+// The plan of trees of drafted tokens (rk_draft_tree): parents, depths, lineage bits.
+std::tuple<Tensor, Tensor, Tensor> draft_tree(const Tensor& parents) {
+  require_gpu(parents, "draft tree");
+  TORCH_CHECK(parents.dim() == 2 &&
+                  (parents.scalar_type() == at::kInt || parents.scalar_type() == at::kLong),
+              "draft tree: parents must be [trees, nodes] int32 or int64");
+  const c10::DeviceGuard guard(parents.device());
+  const Tensor p = unit_columns(parents);
+  const int64_t R = p.size(0), N = p.size(1);
+  Tensor kept = at::empty({R, N}, p.options().dtype(at::kInt)), depths = at::empty_like(kept);
+  Tensor seen = at::empty({R, N, (N + 63) / 64}, p.options().dtype(at::kLong));
+  check_status(rk_draft_tree(p.data_ptr(), p.scalar_type() == at::kLong, ld(p), R, N,
+                             kept.data_ptr<int32_t>(), depths.data_ptr<int32_t>(),
+                             reinterpret_cast<uint64_t*>(seen.data_ptr<int64_t>()), stream_of(p)),
+               "rk_draft_tree");
+  return {kept, depths, seen};
+}
+
+// A tree's tensor: [1 or B, N, ..], contiguous.
+void tree_part(const Tensor& like, const Tensor& t, at::ScalarType type, int64_t B, int64_t N,
+               int64_t dims, const char* what) {
+  same_device(like, t, what);
+  TORCH_CHECK(t.scalar_type() == type && t.dim() == dims && t.is_contiguous() &&
+                  (t.size(0) == 1 || t.size(0) == B) && t.size(1) == N &&
+                  (dims == 2 || t.size(2) == (N + 63) / 64),
+              what, ": the tree must come from draft_tree, one or one per sequence, of N nodes");
+}
+
+// Attention of drafted nodes over the 8-bit cache and themselves (rk_tree_attention):
+// [B, Hq, N, D] as a view of [B, N, Hq, D] memory.
+Tensor tree_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& keys,
+                      const Tensor& values, const Tensor& key_scales, const Tensor& value_scales,
+                      const Tensor& start, const OptTensor& lengths, const Tensor& depths,
+                      const Tensor& seen, double scale, double softcap, const OptTensor& slopes,
+                      at::ScalarType out_dtype) {
+  constexpr const char* what = "tree attention";
+  rk_tree_attention_args a{};
+  a.cache = int8_kv(keys, values, key_scales, value_scales, what);
+  const int64_t B = a.cache.B, H = a.cache.H, D = a.cache.D;
+  for (const Tensor* t : {&q, &k, &v}) same_device(keys, *t, what);
+  TORCH_CHECK(q.dim() == 4 && q.size(0) == B && q.size(3) == D &&
+                  (H > 0 ? q.size(1) % H == 0 : q.size(1) == 0),
+              what, ": q must be [B, Hq, N, D] with heads a multiple of the cache's");
+  const int64_t Hq = q.size(1), N = q.size(2);
+  TORCH_CHECK(k.sizes() == at::IntArrayRef({B, H, N, D}) && v.sizes() == k.sizes() &&
+                  k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+              what, ": k and v must share q's dtype and be [B, H, N, D]");
+  a.dtype = dtype_code(q, what);
+  a.out_dtype = dtype_code(out_dtype);
+  tree_part(keys, depths, at::kInt, B, N, 2, what);
+  tree_part(keys, seen, at::kLong, B, N, 3, what);
+  TORCH_CHECK(seen.size(0) == depths.size(0), what, ": the tree's parts differ");
+  const c10::DeviceGuard guard(q.device());
+  const Tensor qq = vector_rows(q), kk = vector_rows(k), vv = vector_rows(v);
+  a.start = positions(keys, start, B, true, what);
+  a.start_count = start.size(0);
+  a.lengths = lengths.has_value() ? positions(keys, *lengths, B, false, what) : nullptr;
+  a.depths = depths.data_ptr<int32_t>();
+  a.seen = reinterpret_cast<const uint64_t*>(seen.data_ptr<int64_t>());
+  a.trees = seen.size(0);
+  Tensor sl;
+  if (slopes.has_value()) {
+    same_device(keys, *slopes, what);
+    sl = f32_vector(*slopes, Hq, "slopes");
+    a.slopes = sl.data_ptr<float>();
+  }
+  a.q = qq.data_ptr(), a.k = kk.data_ptr(), a.v = vv.data_ptr();
+  a.sqb = qq.stride(0), a.sqh = qq.stride(1), a.sqs = qq.stride(2);
+  a.skb = kk.stride(0), a.skh = kk.stride(1), a.sks = kk.stride(2);
+  a.svb = vv.stride(0), a.svh = vv.stride(1), a.svs = vv.stride(2);
+  a.N = N, a.Hq = Hq;
+  a.scale = static_cast<float>(scale), a.softcap = static_cast<float>(softcap);
+  Tensor out = at::empty({B, N, Hq, D}, q.options().dtype(out_dtype));
+  a.out = out.data_ptr();
+  const int64_t floats = rk_tree_attention_work(&a);
+  Tensor work = at::empty({floats}, key_scales.options());
+  check_status(rk_tree_attention(&a, floats > 0 ? work.data_ptr<float>() : nullptr, floats,
+                                 stream_of(q)),
+               "rk_tree_attention");
+  return out.permute({0, 2, 1, 3});
+}
+
+// Verification of drafted trees (rk_verify_drafts): path, counts, next.
+std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& logits, const Tensor& tokens,
+                                                 const Tensor& parents, const OptTensor& uniforms,
+                                                 const OptTensor& lengths,
+                                                 const OptTensor& draft_logits,
+                                                 double temperature, int64_t top_k) {
+  constexpr const char* what = "verify drafts";
+  require_gpu(logits, what);
+  TORCH_CHECK(logits.dim() == 3, what, ": logits must be [B, N, V]");
+  rk_verify_drafts_args a{};
+  a.B = logits.size(0), a.N = logits.size(1), a.V = logits.size(2);
+  a.dtype = dtype_code(logits, what);
+  const auto rows = [](const Tensor& t) {
+    return t.stride(2) == 1 || t.size(2) <= 1 ? t : t.contiguous();
+  };
+  const c10::DeviceGuard guard(logits.device());
+  const Tensor lg = rows(logits);
+  a.logits = lg.data_ptr(), a.lb = lg.stride(0), a.ln = lg.stride(1);
+  Tensor dg;
+  if (draft_logits.has_value()) {
+    same_device(logits, *draft_logits, what);
+    TORCH_CHECK(draft_logits->sizes() == logits.sizes() &&
+                    draft_logits->scalar_type() == logits.scalar_type(),
+                what, ": the drafter's logits must have the target's shape and dtype");
+    dg = rows(*draft_logits);
+    a.drafts = dg.data_ptr(), a.db = dg.stride(0), a.dn = dg.stride(1);
+  }
+  tree_part(logits, parents, at::kInt, a.B, a.N, 2, what);
+  a.parents = parents.data_ptr<int32_t>(), a.trees = parents.size(0);
+  same_device(logits, tokens, what);
+  TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.sizes() == at::IntArrayRef({a.B, a.N}),
+              what, ": tokens must be int64 [B, N]");
+  const Tensor tk = tokens.contiguous();
+  a.tokens = tk.data_ptr<int64_t>();
+  Tensor un;
+  if (uniforms.has_value()) {
+    same_device(logits, *uniforms, what);
+    TORCH_CHECK(uniforms->scalar_type() == at::kFloat && uniforms->sizes() == tokens.sizes(), what,
+                ": uniforms must be float32 [B, N]");
+    un = uniforms->contiguous();
+    a.uniforms = un.data_ptr<float>();
+  }
+  a.lengths = lengths.has_value() ? positions(logits, *lengths, a.B, false, what) : nullptr;
+  a.temperature = temperature, a.top_k = top_k;
+  Tensor path = at::empty({a.B, a.N}, tk.options()), counts = at::empty({a.B}, tk.options());
+  Tensor next = at::empty({a.B}, tk.options());
+  a.path = path.data_ptr<int64_t>(), a.counts = counts.data_ptr<int64_t>();
+  a.next = next.data_ptr<int64_t>();
+  const int64_t bytes = rk_verify_drafts_work(&a);
+  Tensor work = at::empty({bytes}, tk.options().dtype(at::kByte));
+  check_status(rk_verify_drafts(&a, bytes > 0 ? work.data_ptr() : nullptr, bytes,
+                                stream_of(logits)),
+               "rk_verify_drafts");
+  return {path, counts, next};
+}
+
 // Means of segments [offsets[s], offsets[s + 1]) of a float32 row-rms buffer (rk_row_rms_means).
 Tensor row_rms_means(const Tensor& row_rms, const Tensor& offsets) {
   require_gpu(row_rms, "row rms means");
@@ -1592,6 +1773,16 @@ TORCH_LIBRARY(ratchet, m) {
   m.def("int8_kv_attention(Tensor q, Tensor keys, Tensor values, Tensor key_scales, "
         "Tensor value_scales, Tensor start, Tensor? lengths, float scale, float softcap, "
         "Tensor? slopes, ScalarType out_dtype) -> Tensor");
+  m.def("int8_kv_commit(Tensor[] ks, Tensor[] vs, Tensor(a!)[] keys, Tensor(b!)[] values, "
+        "Tensor(c!)[] key_scales, Tensor(d!)[] value_scales, Tensor start, Tensor path, "
+        "Tensor counts) -> ()");
+  m.def("draft_tree(Tensor parents) -> (Tensor, Tensor, Tensor)");
+  m.def("tree_attention(Tensor q, Tensor k, Tensor v, Tensor keys, Tensor values, "
+        "Tensor key_scales, Tensor value_scales, Tensor start, Tensor? lengths, Tensor depths, "
+        "Tensor seen, float scale, float softcap, Tensor? slopes, ScalarType out_dtype) -> Tensor");
+  m.def("verify_drafts(Tensor logits, Tensor tokens, Tensor parents, Tensor? uniforms, "
+        "Tensor? lengths, Tensor? draft_logits, float temperature, int top_k) -> "
+        "(Tensor, Tensor, Tensor)");
   m.def("kv_append(Tensor k, Tensor v, Tensor(a!) keys, Tensor(b!) values, int start, "
         "int clear_to) -> ()");
   m.def("cross_entropy_forward(Tensor logits, Tensor targets, int ignore_index=-100) -> "
@@ -1643,6 +1834,10 @@ TORCH_LIBRARY_IMPL(ratchet, CUDA, m) {
   m.impl("int8_kv_append", &int8_kv_append);
   m.impl("int8_kv_read", &int8_kv_read);
   m.impl("int8_kv_attention", &int8_kv_attention);
+  m.impl("int8_kv_commit", &int8_kv_commit);
+  m.impl("draft_tree", &draft_tree);
+  m.impl("tree_attention", &tree_attention);
+  m.impl("verify_drafts", &verify_drafts);
   m.impl("kv_append", &kv_append);
   m.impl("cross_entropy_forward", &cross_entropy_forward);
   m.impl("cross_entropy_backward", &cross_entropy_backward);

@@ -11,27 +11,14 @@
 // quotients, the rule of rk_quantize_rows). Tokens appended to a block that holds some can only
 // raise its scale; the codes there are then rounded again, rint(c (s_old / s)). A block's first
 // token starts it anew, whatever it held.
-#include "rk_attention.h"
+#include "rk_kv8.h"
 #include "rk_rowquant.h"
 
 #include <math.h>
 
 namespace rk {
 
-constexpr int kTok = 64;  // tokens of a block
 constexpr int64_t kChunkTokens = 32;  // a wavefront's queries: from here on kv8_chunk_kernel
-constexpr float kLog2e8 = 1.4426950408889634f;
-
-typedef int v4i8 __attribute__((ext_vector_type(4)));
-typedef float v4f_a __attribute__((ext_vector_type(4)));
-
-struct Kv8 {
-  int8_t* keys;
-  int8_t* values;
-  float* ks;
-  float* vs;
-  int64_t B, H, NB;  // H: key heads
-};
 
 struct Kv8Append {
   Kv8 c;
@@ -86,31 +73,18 @@ __device__ __forceinline__ int code_again(int c, float ratio) {
       fminf(fmaxf(__builtin_rintf(static_cast<float>(c) * ratio), -127.0f), 127.0f));
 }
 
-// grid (touched blocks, B * H, 2: keys, values), 256 threads; a thread takes D / 32 pieces of 8
-// features. The block's absmax by the bits of |x| (a NaN is the largest), so a block that takes
-// in a NaN or an infinity has such a scale and reads back as NaN. 4 x 777 tokens, 16 heads of 128:
-// 14.8 us for 39 MB (a load, a reduction and a store in workgroups that are all resident at once;
-// 262 MB of float32 80 us, 4.1 TB/s); a token for 16 sequences 5.4 us.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
+// Tokens into positions first .. last - 1 of one block, by 256 threads; a thread takes D / 32 pieces
+// of 8 features. `rows(t)` is the element offset in `src` of the token for position t, or negative
+// for one of zeros. The block's absmax by the bits of |x| (a NaN is the largest), so a block that takes
+// in a NaN or an infinity has such a scale and reads back as NaN.
+template <int DT, int D, class Rows>
+__device__ __forceinline__ void append_block(bool val, float* scale, int8_t* codes,
+                                             const void* src, int first, int last,
+                                             const Rows& rows) {
   constexpr int PER = D / 8, EACH = kTok * PER / 256, PITCH = kTok + 4;
   __shared__ uint32_t red[4];
   __shared__ __attribute__((aligned(16))) uint8_t tile[D * PITCH];
-  const uint32_t uh = static_cast<uint32_t>(a.c.H), ub = blockIdx.y / uh;
-  const int64_t bh = blockIdx.y, b = ub, h = blockIdx.y - ub * uh;
   const int tid = threadIdx.x;
-  int64_t blk, start;
-  int first, last;
-  if (!append_range(a, b, blockIdx.x, blk, start, first, last)) return;
-  const bool val = blockIdx.z != 0;
-  const int64_t at = (bh * a.c.NB + blk);
-  float* const scale = (val ? a.c.vs : a.c.ks) + at;
-  int8_t* const codes = (val ? a.c.values : a.c.keys) + at * kTok * D;
-  const void* src = val ? a.v : a.k;
-  const int64_t ss = val ? a.svs : a.sks;
-  // element offset of the token at the block's first position (never read before `first`)
-  const int64_t off = b * (val ? a.svb : a.skb) + h * (val ? a.svh : a.skh) +
-                      (blk * kTok - start) * ss;
   const float old = first > 0 ? *scale : 0.0f;
 
   // every thread loads, tokens outside first .. last - 1 the nearest one inside: a condition
@@ -120,8 +94,13 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   for (int i = 0; i < EACH; ++i) {
     const int unit = tid + 256 * i, t = unit / PER, f = unit % PER * 8;
     const int tc = t < first ? first : t < last ? t : last - 1;
-    load_vec16<DT>(src, off + tc * ss + f, x[i]);
-    if constexpr (DT == RK_F32) load_vec16<DT>(src, off + tc * ss + f + 4, x[i] + 4);
+    const int64_t at = rows(tc), from = Rows::kHoles && at < 0 ? 0 : at;
+    load_vec16<DT>(src, from + f, x[i]);
+    if constexpr (DT == RK_F32) load_vec16<DT>(src, from + f + 4, x[i] + 4);
+    if (Rows::kHoles && at < 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+    }
   }
   uint32_t most = 0;
 #pragma unroll
@@ -199,6 +178,80 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
   for (int i = tid; i < D * (kTok / 4); i += 256)
     reinterpret_cast<uint32_t*>(codes)[i] =
         *reinterpret_cast<const uint32_t*>(tile + i / (kTok / 4) * PITCH + 4 * (i % (kTok / 4)));
+}
+
+struct TokenRows {  // tokens that lie one after another
+  static constexpr bool kHoles = false;
+  int64_t off, step;  // off: of the token at the block's first position (never read before `first`)
+  __device__ __forceinline__ int64_t operator()(int t) const { return off + t * step; }
+};
+
+// grid (touched blocks, B * H, 2: keys, values), 256 threads. 4 x 777 tokens, 16 heads of 128:
+// 14.8 us for 39 MB (a load, a reduction and a store in workgroups that are all resident at once;
+// 262 MB of float32 80 us, 4.1 TB/s); a token for 16 sequences 5.4 us.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Append a) {
+  const uint32_t uh = static_cast<uint32_t>(a.c.H), ub = blockIdx.y / uh;
+  const int64_t bh = blockIdx.y, b = ub, h = blockIdx.y - ub * uh;
+  int64_t blk, start;
+  int first, last;
+  if (!append_range(a, b, blockIdx.x, blk, start, first, last)) return;
+  const bool val = blockIdx.z != 0;
+  const int64_t at = (bh * a.c.NB + blk), ss = val ? a.svs : a.sks;
+  const int64_t off = b * (val ? a.svb : a.skb) + h * (val ? a.svh : a.skh) +
+                      (blk * kTok - start) * ss;
+  append_block<DT, D>(val, (val ? a.c.vs : a.c.ks) + at,
+                      (val ? a.c.values : a.c.keys) + at * kTok * D, val ? a.v : a.k, first, last,
+                      TokenRows{off, ss});
+}
+
+// The nodes that a verification left standing, of up to kCommitLayers layers at once: token i of a
+// sequence is node path[i] of its drafts.
+constexpr int kCommitLayers = 32;
+
+struct Kv8Commit {
+  struct Layer {
+    int8_t *keys, *values;
+    float *ks, *vs;
+    const void *k, *v;
+    int64_t skb, skh, sks, svb, svh, svs;
+  } layer[kCommitLayers];
+  int64_t H, NB, N, P, path_step, start_step;
+  const int64_t *start, *path, *counts;
+};
+
+struct PathRows {
+  static constexpr bool kHoles = true;
+  const int64_t* path;  // of the token for the block's first position
+  int64_t base, step, N;
+  __device__ __forceinline__ int64_t operator()(int t) const {
+    const int64_t n = path[t];
+    return n >= 0 && n < N ? base + n * step : -1;
+  }
+};
+
+// grid (touched blocks, B * H, 2 a layer: keys, values), 256 threads.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void kv8_commit_kernel(Kv8Commit a) {
+  const uint32_t uh = static_cast<uint32_t>(a.H), ub = blockIdx.y / uh;
+  const int64_t bh = blockIdx.y, b = ub, h = blockIdx.y - ub * uh;
+  const int64_t start = a.start[b * a.start_step];
+  if (start < 0) return;
+  int64_t n = a.counts[b];
+  n = n < a.P ? n : a.P;
+  const int64_t blk = (start >> 6) + blockIdx.x, base = blk * kTok;
+  if (n <= 0 || blk >= a.NB) return;
+  const int64_t f = start - base, l = start + n - base;
+  const int first = static_cast<int>(f > 0 ? f : 0), last = static_cast<int>(l < kTok ? l : kTok);
+  if (first >= last) return;
+  const Kv8Commit::Layer& y = a.layer[blockIdx.z >> 1];
+  const bool val = (blockIdx.z & 1) != 0;
+  const int64_t at = bh * a.NB + blk;
+  append_block<DT, D>(val, (val ? y.vs : y.ks) + at, (val ? y.values : y.keys) + at * kTok * D,
+                      val ? y.v : y.k, first, last,
+                      PathRows{a.path + b * a.path_step + (base - start),
+                               b * (val ? y.svb : y.skb) + h * (val ? y.svh : y.skh),
+                               val ? y.svs : y.sks, a.N});
 }
 
 struct Kv8Read {
@@ -301,22 +354,6 @@ struct Kv8Attn {
   void* out;    // [B, S, Hq, D], of type ODT
 };
 
-__device__ __forceinline__ float col_max(float v) {  // over the four lanes of a column
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
-                                                  false);
-  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
-                                                  false);
-  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-}
-__device__ __forceinline__ float col_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
-                                                  false);
-  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
-                                                  false);
-  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
-}
 __device__ __forceinline__ uint32_t col_umax(uint32_t v) {
   const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   v = r[0] > r[1] ? r[0] : r[1];
@@ -346,51 +383,6 @@ __device__ __forceinline__ void digits4(const uint32_t (&w)[4], int (&d)[kDigits
 __device__ __forceinline__ float from_digits(const v4i8 (&d)[kDigits], int e) {
   return __builtin_fmaf(static_cast<float>(d[0][e]), 65536.0f,
                         static_cast<float>(d[1][e] * 256 + d[2][e]));
-}
-
-template <bool SCALED = false>
-__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& lo, uint32_t& hi,
-                                            float power = 1.0f) {
-  uint32_t f[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float x = static_cast<float>(static_cast<int8_t>(w >> (8 * e)));
-    f[e] = __float_as_uint(SCALED ? x * power : x);
-  }
-  lo = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);  // small integers: the low halves are zero
-  hi = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
-}
-
-// 16 probabilities as sums of N bf16 numbers each, the largest parts first: off by 2^-8N of
-// themselves.
-template <int N>
-__device__ __forceinline__ void split_bf16(float (&p)[16], v8bf_a (&part)[N][2]) {
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      w[i] = bf16_pair(p[2 * i], p[2 * i + 1]);
-      if (n + 1 < N) {  // what is left, exactly
-        p[2 * i] = p[2 * i] - __uint_as_float(w[i] << 16);
-        p[2 * i + 1] = p[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u);
-      }
-    }
-    part[n][0] = frag_of(make_uint4(w[0], w[1], w[2], w[3]));
-    part[n][1] = frag_of(make_uint4(w[4], w[5], w[6], w[7]));
-  }
-}
-
-template <int QDT>
-__device__ __forceinline__ void store4(void* out, int64_t idx, const float (&x)[4]) {
-  if constexpr (QDT == RK_F32) {
-    *reinterpret_cast<float4*>(static_cast<float*>(out) + idx) =
-        make_float4(x[0], x[1], x[2], x[3]);
-  } else {
-    const uint32_t lo = f32_to_bf16(x[0]) | (static_cast<uint32_t>(f32_to_bf16(x[1])) << 16);
-    const uint32_t hi = f32_to_bf16(x[2]) | (static_cast<uint32_t>(f32_to_bf16(x[3])) << 16);
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + idx) = make_uint2(lo, hi);
-  }
 }
 
 // What a row of the output holds where it is not a plain quotient: zeros for a sequence or token
@@ -984,7 +976,7 @@ void kv8_chunk_kernel(Kv8Attn a) {
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-static int check_cache(const rk_int8_kv& c) {
+int check_cache(const rk_int8_kv& c) {
   if (c.B < 0 || c.H < 0 || c.blocks < 0) return fail(RK_ERR_ARG, "negative size");
   if (c.D != 64 && c.D != 128 && c.D != 256)
     return fail(RK_ERR_UNSUPPORTED, "head size %lld (64, 128 or 256)", static_cast<long long>(c.D));
@@ -997,10 +989,6 @@ static int check_cache(const rk_int8_kv& c) {
   if (c.blocks * kTok * c.D >= (int64_t{1} << 31) - (int64_t{1} << 20))
     return fail(RK_ERR_UNSUPPORTED, "a head's codes reach 2^31 bytes");
   return RK_OK;
-}
-
-static Kv8 cache_args(const rk_int8_kv& c) {
-  return Kv8{c.keys, c.values, c.key_scales, c.value_scales, c.B, c.H, c.blocks};
 }
 
 // How a call is cut up: chunks of 128 queries of a head, or tiles of 16 columns; splits of the
@@ -1134,6 +1122,64 @@ extern "C" int rk_int8_kv_append(const rk_int8_kv* cache, const void* k, int64_t
   if (dtype == RK_F32) run(std::integral_constant<int, RK_F32>{});
   else run(std::integral_constant<int, RK_BF16>{});
   return launch_status("int8_kv_append");
+}
+
+extern "C" int rk_int8_kv_commit(const rk_int8_kv_commit_layer* layers, int64_t count, int64_t N,
+                                 int dtype, const int64_t* start, int64_t start_count,
+                                 const int64_t* path, int64_t path_step, int64_t P,
+                                 const int64_t* counts, void* stream) {
+  clear_error();
+  if (count < 0 || N < 0 || P < 0) return fail(RK_ERR_ARG, "negative size");
+  if (count == 0) return RK_OK;
+  if (!layers) return fail(RK_ERR_ARG, "null layers");
+  if (dtype != RK_F32 && dtype != RK_BF16)
+    return fail(RK_ERR_ARG, "keys and values must be float32 or bfloat16");
+  const rk_int8_kv& c = layers[0].cache;
+  const int64_t per = dtype == RK_F32 ? 4 : 8;
+  for (int64_t i = 0; i < count; ++i) {
+    const rk_int8_kv_commit_layer& y = layers[i];
+    if (int e = check_cache(y.cache)) return e;
+    if (y.cache.B != c.B || y.cache.H != c.H || y.cache.blocks != c.blocks || y.cache.D != c.D)
+      return fail(RK_ERR_ARG, "the layers' caches differ in shape");
+    const int64_t strides[] = {y.skb, y.skh, y.sks, y.svb, y.svh, y.svs};
+    for (int64_t st : strides)
+      if (st < 0 || st % per != 0)
+        return fail(RK_ERR_UNSUPPORTED, "rows and strides must be whole 16-byte vectors");
+    if (!aligned16(y.k) || !aligned16(y.v))
+      return fail(RK_ERR_UNSUPPORTED, "keys and values need 16-byte alignment");
+  }
+  if (start_count != 1 && start_count != c.B)
+    return fail(RK_ERR_ARG, "one start, or one per sequence");
+  if (c.B == 0 || c.H == 0 || c.blocks == 0 || P == 0 || N == 0) return RK_OK;
+  if (!start || !path || !counts) return fail(RK_ERR_ARG, "null pointer");
+  if (path_step < 0) return fail(RK_ERR_ARG, "negative stride");
+  for (int64_t i = 0; i < count; ++i)
+    if (!layers[i].k || !layers[i].v) return fail(RK_ERR_ARG, "null pointer");
+  if (P > (int64_t{1} << 24)) return fail(RK_ERR_UNSUPPORTED, "too many tokens");
+  hipStream_t st = as_stream(stream);
+  for (int64_t i0 = 0; i0 < count; i0 += kCommitLayers) {
+    const int64_t n = count - i0 < kCommitLayers ? count - i0 : kCommitLayers;
+    Kv8Commit a{};
+    for (int64_t i = 0; i < n; ++i) {
+      const rk_int8_kv_commit_layer& y = layers[i0 + i];
+      a.layer[i] = {y.cache.keys, y.cache.values, y.cache.key_scales, y.cache.value_scales,
+                    y.k, y.v, y.skb, y.skh, y.sks, y.svb, y.svh, y.svs};
+    }
+    a.H = c.H; a.NB = c.blocks; a.N = N; a.P = P;
+    a.path_step = path_step; a.start_step = start_count > 1 ? 1 : 0;
+    a.start = start; a.path = path; a.counts = counts;
+    const dim3 grid(static_cast<unsigned>((P + kTok - 2) / kTok + 1),
+                    static_cast<unsigned>(c.B * c.H), static_cast<unsigned>(2 * n));
+    const auto run = [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      if (c.D == 64) kv8_commit_kernel<DT, 64><<<grid, 256, 0, st>>>(a);
+      else if (c.D == 128) kv8_commit_kernel<DT, 128><<<grid, 256, 0, st>>>(a);
+      else kv8_commit_kernel<DT, 256><<<grid, 256, 0, st>>>(a);
+    };
+    if (dtype == RK_F32) run(std::integral_constant<int, RK_F32>{});
+    else run(std::integral_constant<int, RK_BF16>{});
+  }
+  return launch_status("int8_kv_commit");
 }
 
 extern "C" int rk_int8_kv_read(const rk_int8_kv* cache, int64_t begin, int64_t end, int dtype,

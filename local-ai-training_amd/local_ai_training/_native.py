@@ -138,6 +138,12 @@ SIGNATURES: dict[str, list] = {
     "rk_int8_kv_attention_work": [_p, _i64, _i64, _i32, _i32],
     "rk_int8_kv_attention": [_p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _f32, _f32,
                              _p, _p, _i64, _p, _i32, _p],
+    "rk_int8_kv_commit": [_p, _i64, _i64, _i32, _p, _i64, _p, _i64, _i64, _p, _p],
+    "rk_draft_tree": [_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p],
+    "rk_tree_attention_work": [_p],
+    "rk_tree_attention": [_p, _p, _i64, _p],
+    "rk_verify_drafts_work": [_p],
+    "rk_verify_drafts": [_p, _p, _i64, _p],
     "rk_kv_append": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i32, _i64, _i64,
                      _i64, _i64, _i64, _i64, _i64, _p],
     "rk_version": [],
@@ -151,6 +157,8 @@ RESTYPES = {
     "rk_scored_attention_rest": ctypes.c_int64,
     "rk_scored_attention_backward_work": ctypes.c_int64,
     "rk_int8_kv_attention_work": ctypes.c_int64,
+    "rk_tree_attention_work": ctypes.c_int64,
+    "rk_verify_drafts_work": ctypes.c_int64,
     "rk_int8_gemm_large_rows": ctypes.c_int64,
     "rk_decode_attention_splits": ctypes.c_int64,
     "rk_grad_weight_update_counters": ctypes.c_int64,

@@ -222,6 +222,28 @@ def _register_fakes() -> None:
         b, h, sl, d = q.shape
         return q.new_empty((b, sl, h, d), dtype=out_dtype).permute(0, 2, 1, 3)
 
+    @fake("ratchet::int8_kv_commit")
+    def _int8_kv_commit(ks, vs, keys, values, key_scales, value_scales, start, path, counts):
+        return None
+
+    @fake("ratchet::draft_tree")
+    def _draft_tree(parents):
+        r, n = parents.shape
+        return (*(parents.new_empty((r, n), dtype=torch.int32) for _ in range(2)),
+                parents.new_empty((r, n, (n + 63) // 64), dtype=torch.int64))
+
+    @fake("ratchet::tree_attention")
+    def _tree_attention(q, k, v, keys, values, key_scales, value_scales, start, lengths, depths,
+                        seen, scale, softcap, slopes, out_dtype):
+        b, h, n, d = q.shape
+        return q.new_empty((b, n, h, d), dtype=out_dtype).permute(0, 2, 1, 3)
+
+    @fake("ratchet::verify_drafts")
+    def _verify_drafts(logits, tokens, parents, uniforms, lengths, draft_logits, temperature,
+                       top_k):
+        b, n = tokens.shape
+        return tokens.new_empty((b, n)), tokens.new_empty((b,)), tokens.new_empty((b,))
+
     @fake("ratchet::kv_append")
     def _kv_append(k, v, keys, values, start, clear_to):
         return None
@@ -242,8 +264,8 @@ def _register_fakes() -> None:
 
 
 # the operators the library defines (the opcheck tests walk this list), but for
-# attention_backward, kv_append, attention_mask, the scored_attention and the int8_kv
-# operators, whose opchecks are beside their own tests
+# attention_backward, kv_append, attention_mask, the scored_attention and the int8_kv operators
+# and those of drafted trees, whose opchecks are beside their own tests
 OPERATORS = (
     "quantize_rows", "int8_mm_nt", "packed_mm", "packed_mm_residual", "packed_mm_accumulate",
     "packed_mm_t", "unpack_transpose", "unpack", "effective_bf16", "grad_input_bf16",
