@@ -32,6 +32,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _native as nat
+from .drafts import DraftTree, tree_attention
 from .int8_cache import int8_kv_append, int8_kv_attention
 from .ratchet import DiscreteRatchetLinear
 
@@ -124,12 +125,12 @@ def _ratchet_layers(model) -> list:
     return layers
 
 
-def fused_decode_supported(model, cache) -> bool:
+def fused_decode_supported(model, cache, tokens: int = 1) -> bool:
     """True when the fused kernels cover this model and cache: a ROCm device, at most 16
-    sequences, int8 ratchet layers with N % 16 == 0, K % 64 == 0, K <= 6144, head size
+    sequences (times `tokens` of each, of a drafted tree), int8 ratchet layers with N % 16 == 0, K % 64 == 0, K <= 6144, head size
     64/128/256, a plain float32 token embedding, eval mode."""
     config = model.config
-    if cache.device.type != "cuda" or cache.batch > MAX_ROWS or model.training:
+    if cache.device.type != "cuda" or cache.batch * tokens > MAX_ROWS or model.training:
         return False
     if config.modified_scores and not isinstance(cache, _int8_cache()):
         return False  # capped and biased scores are read from the 8-bit cache
@@ -200,21 +201,62 @@ def fused_decode_logits(model, tokens: Tensor, cache) -> Tensor:
              config.n_embd, positions.data_ptr(), positions.shape[0], cache.pos.data_ptr(),
              hidden.data_ptr(), hidden.stride(0), stream)
     for index, block in enumerate(model.blocks):
-        attention, feed_forward = block.attention, block.feed_forward
-        decode_gemv(attention.qkv, qkv, prologue=PRO_RMSNORM, epilogue=EPI_STORE, x=hidden,
-                    norm_weight=block.attention_norm.weight, eps=BLOCK_NORM_EPS)
+        attention = block.attention
+        _fused_qkv(block, hidden, qkv)
         if int8:
             att = int8_decode_attention(qkv, cache.store(index), cache.pos, attention)
         else:
             keys, values = cache.buffers(index, qkv)
             att = decode_attention(qkv, keys, values, cache.pos, config.n_head, bufs["work"],
                                    bufs["attn"])
-        decode_gemv(attention.projection, hidden, prologue=PRO_PLAIN, epilogue=EPI_ADD, x=att)
-        decode_gemv(feed_forward.expand, ffn, prologue=PRO_RMSNORM, epilogue=EPI_GELU,
-                    x=hidden, norm_weight=block.feed_forward_norm.weight, eps=BLOCK_NORM_EPS)
-        decode_gemv(feed_forward.contract, hidden, prologue=PRO_PLAIN, epilogue=EPI_ADD, x=ffn)
+        _fused_rest(block, hidden, att, ffn)
+    return _fused_head(model, hidden, bufs["logits"])
+
+
+def _fused_qkv(block, hidden: Tensor, qkv: Tensor) -> None:
+    decode_gemv(block.attention.qkv, qkv, prologue=PRO_RMSNORM, epilogue=EPI_STORE, x=hidden,
+                norm_weight=block.attention_norm.weight, eps=BLOCK_NORM_EPS)
+
+
+def _fused_rest(block, hidden: Tensor, att: Tensor, ffn: Tensor) -> None:
+    """A block behind its attention: the projection and the feed-forward, added to `hidden`."""
+    attention, feed_forward = block.attention, block.feed_forward
+    decode_gemv(attention.projection, hidden, prologue=PRO_PLAIN, epilogue=EPI_ADD, x=att)
+    decode_gemv(feed_forward.expand, ffn, prologue=PRO_RMSNORM, epilogue=EPI_GELU,
+                x=hidden, norm_weight=block.feed_forward_norm.weight, eps=BLOCK_NORM_EPS)
+    decode_gemv(feed_forward.contract, hidden, prologue=PRO_PLAIN, epilogue=EPI_ADD, x=ffn)
+
+
+def _fused_head(model, hidden: Tensor, logits: Tensor) -> Tensor:
     final_eps = model.final_norm.eps
     if final_eps is None:  # nn.RMSNorm's default: the float32 machine epsilon
         final_eps = torch.finfo(torch.float32).eps
-    return decode_gemv(model.lm_head, bufs["logits"], prologue=PRO_RMSNORM, epilogue=EPI_STORE,
+    return decode_gemv(model.lm_head, logits, prologue=PRO_RMSNORM, epilogue=EPI_STORE,
                        x=hidden, norm_weight=model.final_norm.weight, eps=final_eps)
+
+
+@torch.no_grad()
+def fused_tree_logits(model, tokens: Tensor, tree: DraftTree, cache) -> Tensor:
+    """Logits [B, N, vocab] (float32) of a drafted tree's nodes over an 8-bit cache, on the same
+    kernels with a row for each node: its attention is ``tree_attention``, and the layers' keys and
+    values stay in ``cache.drafted``."""
+    config = model.config
+    batch, nodes = tokens.shape
+    rows, c, heads = batch * nodes, config.n_embd, config.n_head
+    f32 = dict(dtype=torch.float32, device=cache.device)
+    at = (cache.pos + tree.depths).clamp(max=model.position_encoding.shape[0] - 1)
+    hidden = (model.token_embedding(tokens) + model.position_encoding[at]).view(rows, c)
+    ffn = torch.empty(rows, config.hidden_size, **f32)
+    for index, block in enumerate(model.blocks):
+        qkv = torch.empty(rows, 3 * c, dtype=torch.bfloat16, device=cache.device)
+        _fused_qkv(block, hidden, qkv)
+        q, k, v = (t.view(batch, nodes, heads, c // heads).transpose(1, 2)
+                   for t in qkv.view(batch, nodes, 3 * c).chunk(3, dim=2))
+        attention = block.attention
+        out = tree_attention(q, k, v, cache.store(index), cache.pos, tree,
+                             softcap=attention.softcap, slopes=attention.slopes,
+                             out_dtype=torch.float32)
+        cache.drafted[index] = (k, v)
+        _fused_rest(block, hidden, out.transpose(1, 2).reshape(rows, c), ffn)
+    return _fused_head(model, hidden, torch.empty(rows, config.vocab_size, **f32)).view(
+        batch, nodes, -1)

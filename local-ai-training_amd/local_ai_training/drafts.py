@@ -33,6 +33,12 @@ MAX_NODES = 256
 _NOTHING = 2.0**-40  # a residual of this sum is rounding
 
 
+def check_batch(batch: int) -> None:
+    if batch != 1:
+        raise ValueError("a model's cache has one position for the batch: drafts of one sequence "
+                         "can be committed to it (int8_kv_commit takes any)")
+
+
 class DraftTree(NamedTuple):
     """The plan of trees, made by ``draft_tree``: one for all sequences or one for each (R 1 or B).
 

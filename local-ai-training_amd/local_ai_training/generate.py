@@ -12,12 +12,14 @@ every ratchet GEMM, which dispatches to the small-M int8 kernel. Attention is ca
 the last position's logits are the same quantity the full-window forward computes (equal
 up to float summation order). Past ``block_size`` tokens the reference re-positions a
 sliding window every step; positions are absolute, so a cache cannot follow, and this
-module then recomputes the window each step exactly as the reference does.
+module then recomputes the window each step exactly as the reference does. With a draft model
+(``generate(draft=...)``) several tokens are produced by one step over the cache.
 """
 
 from __future__ import annotations
 
 import json
+import math
 from pathlib import Path
 from typing import Literal
 
@@ -25,6 +27,7 @@ import torch
 from torch import Tensor
 
 from .decode import decode_greedy, reserve_step
+from .drafts import MAX_NODES, draft_tree, sample_tokens, verify_drafts
 from .model import Int8KVCache, KVCache, ModelConfig, RatchetGPT, build_seeded_model
 from .ratchet import DiscreteRatchetLinear
 
@@ -183,6 +186,66 @@ class _TokenSampler:
         return int(torch.multinomial(weights, 1, generator=self.generator).item())
 
 
+class _Drafter:
+    """Rounds of drafted generation: a small model proposes a tree of tokens behind the last one, the
+    large one judges all of them in one pass (``drafts.py``). Both caches hold every token but the
+    last one before a round and after it."""
+
+    def __init__(self, model: RatchetGPT, cache: KVCache, draft: RatchetGPT, draft_cache: KVCache,
+                 shape: tuple[int, ...], pick: _TokenSampler, top_k: int | None) -> None:
+        self.model, self.cache, self.draft, self.draft_cache = model, cache, draft, draft_cache
+        self.shape, self.pick, self.top_k = shape, pick, top_k
+        parents, self.levels = [-1], [1]  # the nodes' parents, the nodes up to each level
+        for width in shape:
+            below = self.levels[-2] if len(self.levels) > 1 else 0
+            parents += [p for p in range(below, self.levels[-1]) for _ in range(width)]
+            self.levels.append(len(parents))
+        # the drafter's own passes run over the tree's upper levels
+        self.trees = [draft_tree(parents[:n], cache.device) for n in self.levels]
+
+    def fits(self) -> bool:
+        """Whether a whole way through the tree and the token behind it have positions."""
+        return all(c.length + len(self.shape) < c.max_len for c in (self.cache, self.draft_cache))
+
+    def round(self, token: int) -> list[int]:
+        """The tokens behind `token`: those that stood, and one of the model's own."""
+        device, nodes = self.cache.device, self.levels[-1]
+        pick, top_k = self.pick, self.top_k
+        numbers = None
+        if pick.temperature:
+            numbers = torch.rand(2, nodes, generator=pick.generator).to(device)
+        tokens = torch.zeros(1, nodes, dtype=torch.long, device=device)
+        tokens[0, 0] = token
+        rows, below = [], 0
+        for level, width in enumerate(self.shape):
+            n, behind = self.levels[level], self.levels[level + 1]
+            logits = self.draft.tree_logits(tokens[:, :n], self.trees[level], self.draft_cache,
+                                            deepest=level)[0, below:].float()
+            if numbers is None:
+                tokens[0, n:behind] = logits.topk(width, dim=-1).indices.flatten()
+            else:
+                rows.append(logits)
+                # (-1 where a row is no distribution: any token, which will not stand)
+                tokens[0, n:behind] = sample_tokens(
+                    logits.repeat_interleave(width, dim=0), numbers[1, n:behind],
+                    temperature=pick.temperature, top_k=top_k).clamp(min=0)
+            below = n
+        # the last level's keys and values; nothing is drawn behind it
+        rest = self.draft.tree_logits(tokens, self.trees[-1], self.draft_cache,
+                                      deepest=len(self.shape))[0, below:].float()
+        logits = self.model.tree_logits(tokens, self.trees[-1], self.cache,
+                                        deepest=len(self.shape)).float()
+        found = verify_drafts(
+            logits, tokens, self.trees[-1], numbers[:1] if numbers is not None else None,
+            draft_logits=torch.cat([*rows, rest])[None] if rows else None,
+            temperature=pick.temperature, top_k=top_k)
+        stood, following = self.model.commit_drafts(self.cache, found)
+        self.draft.commit_drafts(self.draft_cache, found)
+        if following < 0:
+            raise RuntimeError("the model's logits are no distribution")
+        return tokens[0, stood[1:]].tolist() + [following]
+
+
 @torch.no_grad()
 def generate(
     model: RatchetGPT,
@@ -196,11 +259,19 @@ def generate(
     device: str | torch.device | None = None,
     use_graph: bool = False,
     cache_dtype: torch.dtype | None = None,
+    draft: RatchetGPT | None = None,
+    draft_shape: tuple[int, ...] = (1, 1, 1, 1),
 ) -> str:
     """Sample `max_new_tokens` characters continuing `prompt` and return only the new text
     (``generate.py:135-206``: same arguments, validation and sampling). `use_graph` replays
     the decode step as a HIP graph (GPU only); `cache_dtype` is the key/value cache's
-    (``RatchetGPT.new_cache``: e.g. torch.bfloat16, or torch.int8 for codes with scales)."""
+    (``RatchetGPT.new_cache``: e.g. torch.bfloat16, or torch.int8 for codes with scales).
+
+    With a `draft` model over the same vocabulary, tokens are proposed by it and judged by `model`, a
+    tree at a time: `draft_shape` gives the children of a node, level by level. The text is
+    distributed as without it (at temperature 0 it is the same, up to logits whose order the
+    summation order decides), but drawn from other random numbers. Near the windows' end, and
+    behind it, tokens are produced one by one."""
     if max_new_tokens < 0:
         raise ValueError("max_new_tokens must be non-negative")
     if temperature < 0:
@@ -209,6 +280,13 @@ def generate(
     missing = sorted(set(prompt) - index.keys())
     if missing:
         raise ValueError(f"prompt characters not in the model vocabulary: {missing!r}")
+    if draft is not None:
+        if draft.config.vocab_size != model.config.vocab_size:
+            raise ValueError("the draft model must share the vocabulary")
+        if not draft_shape or min(draft_shape) < 1 or max(draft_shape) > len(vocabulary):
+            raise ValueError("draft_shape must hold a level's children, 1 to the vocabulary's size")
+        if sum(math.prod(draft_shape[:i]) for i in range(len(draft_shape) + 1)) > MAX_NODES:
+            raise ValueError(f"a drafted tree has at most {MAX_NODES} nodes")
     pick = _TokenSampler(temperature, top_k, seed)
     device = device or next(model.parameters()).device
     window = model.config.block_size
@@ -219,6 +297,21 @@ def generate(
     logits = model.prefill(torch.tensor([history], dtype=torch.long, device=device), cache)
     graph: DecodeGraph | None = None
     produced: list[int] = []
+    if draft is not None and max_new_tokens > 1 and len(history) <= draft.config.block_size:
+        draft_cache = draft.new_cache(1, dtype=cache_dtype)
+        draft.prefill(torch.tensor([history], dtype=torch.long, device=device), draft_cache)
+        drafter = _Drafter(model, cache, draft, draft_cache, draft_shape, pick, top_k)
+        produced.append(pick(logits))
+        while len(produced) < max_new_tokens and drafter.fits():
+            produced += drafter.round(produced[-1])
+        del produced[max_new_tokens:]
+        history += produced
+        if len(produced) < max_new_tokens and cache.length < window:
+            last = torch.tensor([produced[-1:]], dtype=torch.long, device=device)
+            logits = model.decode_step(last, cache)
+        elif len(produced) < max_new_tokens:
+            recent = torch.tensor([history[-window:]], dtype=torch.long, device=device)
+            logits = model(recent)[0][:, -1]
     while len(produced) < max_new_tokens:
         produced.append(pick(logits))
         history.append(produced[-1])

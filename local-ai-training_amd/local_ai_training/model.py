@@ -26,6 +26,8 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from .attention import CausalAttentionFn, attention_supported
 from .cross_entropy import cross_entropy
+from .drafts import (DraftTree, Verified, check_batch, int8_kv_commit, torch_tree_attention,
+                     tree_attention)
 from .int8_cache import HEAD_SIZES as INT8_HEAD_SIZES
 from .int8_cache import Int8KV, int8_kv, int8_kv_append, int8_kv_attention
 from .int8_fused import (
@@ -162,6 +164,8 @@ class KVCache:
         self._mask: Tensor | None = None
         self._ended: Tensor | bool = False  # by the mask of a prompt (end_unless_whole)
         self.step_buffers: dict[str, Tensor] = {}  # fixed-shape work buffers of a step
+        # keys and values of drafted nodes, a layer's [B, H, N, D] each, until they are committed
+        self.drafted: list[tuple[Tensor, Tensor] | None] = [None] * n_layer
 
     def buffers(self, layer: int, like: Tensor) -> tuple[Tensor, Tensor]:
         """The layer's key/value buffers, allocated on first use in the cache dtype
@@ -224,6 +228,28 @@ class KVCache:
         self.length += steps
         self.pos.add_(steps)
 
+    def commit(self, path: Tensor, counts: Tensor, count: int) -> None:
+        """Appends the drafted nodes that stood (``tree_logits``, ``verify_drafts``): the first
+        `count` of `path` [1, N], which `counts` [1] says on the device. One sequence only (its
+        positions are the batch's)."""
+        check_batch(self.batch)
+        if any(kept is None for kept in self.drafted):
+            raise ValueError("no drafts to commit")
+        if not 0 <= count <= path.shape[1] or path.shape[0] != 1:
+            raise ValueError("path must hold the count's nodes of one sequence")
+        if self.length + count > self.max_len:
+            raise ValueError("KV cache is full")
+        self._commit(path, counts, count)
+        self.drafted = [None] * self.n_layer
+        self.advance(count)
+
+    def _commit(self, path: Tensor, counts: Tensor, count: int) -> None:
+        for layer, (k, v) in enumerate(self.drafted):
+            keys, values = self.buffers(layer, k)
+            for buffer, rows in ((keys, k), (values, v)):
+                at = buffer[:, :, self.length:self.length + count]
+                at.copy_(rows.index_select(2, path[0, :count]))
+
     def end_unless_whole(self, mask: AttentionMask) -> None:
         """Notes, on the device, whether a prompt under `mask` is one document in every row. Of
         others (several documents, padding) later positions must not see all, and the cache
@@ -275,6 +301,11 @@ class Int8KVCache(KVCache):
         store = self.store(layer)
         int8_kv_append(store, k, v, self.pos)
         return store
+
+    def _commit(self, path: Tensor, counts: Tensor, count: int) -> None:
+        int8_kv_commit([self.store(layer) for layer in range(self.n_layer)],
+                       [k for k, _ in self.drafted], [v for _, v in self.drafted], self.pos,
+                       path, counts)
 
     def stores_bf16(self, layer: int) -> bool:
         # what it stores is rounded further: bf16 projections are handed over as they are
@@ -379,9 +410,10 @@ class CausalSelfAttention(nn.Module):
     def forward(self, inputs: Tensor, *, inputs_int8: Tensor | None = None,
                 inputs_scale: Tensor | None = None, cache: KVCache | None = None,
                 layer: int = 0, decode: bool = False, mask: AttentionMask | None = None,
-                residual: Tensor | None = None) -> Tensor:
+                tree: DraftTree | None = None, residual: Tensor | None = None) -> Tensor:
         """``residual``: return residual + attention output (int8 projection: added in the
-        GEMM epilogue). ``mask``: the documents of the batch (``attention_mask``)."""
+        GEMM epilogue). ``mask``: the documents of the batch (``attention_mask``). ``tree``: the
+        positions are drafted nodes behind the cache."""
         batch_size, sequence_length, channels = inputs.shape
         projection_kw = {}
         if inputs_int8 is not None:
@@ -409,7 +441,9 @@ class CausalSelfAttention(nn.Module):
 
         q, k, v = heads(query), heads(key), heads(value)
         dropout_p = self.dropout if self.training else 0.0
-        if cache is not None:
+        if tree is not None:
+            attended = self._drafted_attention(q, k, v, cache, layer, tree)
+        elif cache is not None:
             attended = self._cached_attention(q, k, v, cache, layer, decode, mask)
         elif self._scored(mask):
             if dropout_p:
@@ -486,6 +520,19 @@ class CausalSelfAttention(nn.Module):
         out = _attend(q, keys[:, :, :end], values[:, :, :end], attn_mask=mask)
         return out.to(out_dtype)
 
+    def _drafted_attention(self, q: Tensor, k: Tensor, v: Tensor, cache: KVCache, layer: int,
+                           tree: DraftTree) -> Tensor:
+        """Attention of a tree's nodes over the cache and themselves; their keys and values are
+        kept for ``KVCache.commit``."""
+        cache.drafted[layer] = (k, v)
+        if isinstance(cache, Int8KVCache):
+            return tree_attention(q, k, v, cache.store(layer), cache.pos, tree,
+                                  softcap=self.softcap, slopes=self.slopes)
+        keys, values = cache.buffers(layer, k)
+        out = torch_tree_attention(q.to(keys.dtype), k, v, keys, values, cache.length, tree,
+                                   self.softcap, self.slopes, 1.0 / math.sqrt(self.head_size))
+        return out.to(q.dtype)
+
     def _score_buffer(self, q: Tensor, keys: Tensor, values: Tensor, at: Tensor,
                       key_at: Tensor) -> Tensor:
         """Capped and biased attention of positions `at` over a bf16 / float32 buffer, in torch
@@ -561,10 +608,13 @@ class TransformerBlock(nn.Module):
         self.feed_forward = FeedForward(config, max_code=max_code)
 
     def forward(self, inputs: Tensor, *, cache: KVCache | None = None, layer: int = 0,
-                decode: bool = False, mask: AttentionMask | None = None) -> Tensor:
+                decode: bool = False, mask: AttentionMask | None = None,
+                tree: DraftTree | None = None) -> Tensor:
         kv = dict(cache=cache, layer=layer, decode=decode) if cache is not None else {}
         if mask is not None:
             kv["mask"] = mask
+        if tree is not None:
+            kv["tree"] = tree
         fuse_grad = self.fuse_residual and self.fuse_residual_grad
         if _is_int8(self.attention.qkv):
             if fuse_grad:
@@ -771,6 +821,44 @@ class RatchetGPT(nn.Module):
         for index, block in enumerate(self.blocks):
             hidden = block(hidden, cache=cache, layer=index, decode=True)
         return self.lm_head(self.final_norm(hidden))[:, 0]
+
+    @torch.no_grad()
+    def tree_logits(self, tokens: Tensor, tree: DraftTree, cache: KVCache, *,
+                    deepest: int | None = None) -> Tensor:
+        """Logits [B, N, vocab] of the tokens that follow each node of a drafted `tree`
+        (``drafts.py``), whose node 0 is the last token that is known. `tokens` [B, N] stand
+        behind the cache's, at position ``cache.length`` + depth; the cache keeps their keys and
+        values until ``commit_drafts`` appends those that stand, and nothing else changes.
+        `deepest`: the steps from the root to the deepest node (default: as in a chain), which
+        must fit the cache. On a ROCm GPU with an 8-bit cache, int8 ratchet layers of supported
+        shapes and at most 16 nodes in all the step runs on the fused decode kernels."""
+        from .decode import fused_decode_supported, fused_tree_logits
+
+        if tokens.dim() != 2 or tokens.shape[0] != cache.batch:
+            raise ValueError("tokens must be [B, N] with the cache's batch")
+        deepest = tokens.shape[1] - 1 if deepest is None else deepest
+        if cache.length + deepest >= cache.max_len:
+            raise ValueError("KV cache is full")
+        cache.check_open()
+        if (self.fused_decode and isinstance(cache, Int8KVCache)
+                and fused_decode_supported(self, cache, tokens.shape[1])):
+            return fused_tree_logits(self, tokens, tree, cache)
+        at = (cache.pos + tree.depths).clamp(max=self.position_encoding.shape[0] - 1)
+        hidden = self.token_embedding(tokens) + self.position_encoding[at]
+        for index, block in enumerate(self.blocks):
+            hidden = block(hidden, cache=cache, layer=index, tree=tree)
+        return self.lm_head(self.final_norm(hidden))
+
+    @torch.no_grad()
+    def commit_drafts(self, cache: KVCache, found: Verified) -> tuple[list[int], int]:
+        """Appends the nodes that stood (``verify_drafts``) to a cache of one sequence and advances
+        it; returns them (the root first) and the next token. Waits for the device. Several models
+        over the same tree commit the same result to their own caches."""
+        check_batch(cache.batch)
+        path, counts, following = found
+        *nodes, count, token = torch.cat([path[0], counts, following]).tolist()
+        cache.commit(path, counts, count)
+        return nodes[:count], token
 
     def _attach_count_slots(self) -> None:
         """One int64 [layers, 4] move-count buffer for every ratchet layer of the model (each
