@@ -25,6 +25,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cmath>
 #include <optional>
 #include <utility>
 #include <vector>
@@ -1428,46 +1429,97 @@ Tensor int8_kv_attention(const Tensor& q, const Tensor& keys, const Tensor& valu
   return out.permute({0, 2, 1, 3});
 }
 
+// ---------------------------------------------------------------------------------------
+// Drafted trees (drafts.py). All checks are made here, with the exceptions a caller of the Python
+// functions gets; on the host too, where the operators then refuse the tensors.
+// ---------------------------------------------------------------------------------------
+// Operands that want a gradient (or carry a tangent) are refused: nothing here has one.
+void no_gradient(const char* what, at::ArrayRef<Tensor> operands) {
+  const bool backward = at::GradMode::is_enabled();
+  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor& t : operands)
+    TORCH_CHECK(!(backward && t.requires_grad()) && !(forward && t._fw_grad(/*level=*/0).defined()),
+                what, " has no gradient; call it under no_grad, on operands without tangents");
+}
+
+void on_device(const Tensor& like, const Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(t.device() == like.device(), what, ": the operands must share a device");
+}
+
+// Whole numbers on the device, one per sequence or, where `one`, one for the batch.
+Tensor one_each(const Tensor& like, const Tensor& t, int64_t B, bool one, const char* name,
+                const char* what) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && t.dim() == 1 &&
+                        (t.size(0) == B || (one && t.size(0) == 1)),
+                    what, ": ", name, " must be int64, one per sequence",
+                    one ? " or one for the batch" : "");
+  on_device(like, t, what);
+  return t.contiguous();
+}
+
+// A tree's tensor: [1 or B, N, ..], contiguous.
+void tree_part(const Tensor& like, const Tensor& t, at::ScalarType type, int64_t B, int64_t N,
+               int64_t dims, const char* what) {
+  TORCH_CHECK_VALUE(t.scalar_type() == type && t.dim() == dims && t.is_contiguous() &&
+                        (t.size(0) == 1 || t.size(0) == B) && t.size(1) == N &&
+                        (dims == 2 || t.size(2) == (N + 63) / 64),
+                    what, ": the tree must come from draft_tree, one or one per sequence, of N nodes");
+  on_device(like, t, what);
+}
+
 // Accepted nodes of drafted trees into the 8-bit caches of several layers (rk_int8_kv_commit).
 void int8_kv_commit(at::TensorList ks, at::TensorList vs, at::TensorList keys,
                     at::TensorList values, at::TensorList key_scales, at::TensorList value_scales,
                     const Tensor& start, const Tensor& path, const Tensor& counts) {
   constexpr const char* what = "int8 kv commit";
   const size_t n = keys.size();
-  TORCH_CHECK(n > 0 && ks.size() == n && vs.size() == n && values.size() == n &&
-                  key_scales.size() == n && value_scales.size() == n,
-              what, ": one k, v and cache per layer");
+  TORCH_CHECK_VALUE(n > 0 && ks.size() == n && vs.size() == n && values.size() == n &&
+                        key_scales.size() == n && value_scales.size() == n,
+                    what, ": one k, one v and one cache per layer are needed");
+  no_gradient(what, ks);
+  no_gradient(what, vs);
+  const at::IntArrayRef shape = keys[0].sizes();
+  TORCH_CHECK_VALUE(shape.size() == 5 && ks[0].dim() == 4, what,
+                    ": keys must be [B, H, blocks, 64, D], k [B, H, N, D]");
+  const int64_t B = shape[0], N = ks[0].size(2);
+  const int64_t kv[] = {B, shape[1], N, shape[4]};
+  TORCH_CHECK_TYPE(ks[0].is_floating_point(), what, ": k and v must be floating point");
+  for (size_t i = 0; i < n; ++i) {
+    TORCH_CHECK_VALUE(keys[i].sizes() == shape, what, ": the layers' caches must share a shape");
+    TORCH_CHECK_VALUE(ks[i].sizes() == at::IntArrayRef(kv) && vs[i].sizes() == at::IntArrayRef(kv),
+                      what, ": k and v must share the caches' [B, H, N, D] shape");
+    TORCH_CHECK_TYPE(ks[i].scalar_type() == ks[0].scalar_type() &&
+                         vs[i].scalar_type() == ks[0].scalar_type(),
+                     what, ": k and v must share a dtype");
+    for (const Tensor* t : {&ks[i], &vs[i], &keys[i]}) on_device(keys[0], *t, what);
+    for (size_t j = 0; j < i && keys[i].numel() > 0; ++j)
+      TORCH_CHECK_VALUE(keys[i].data_ptr() != keys[j].data_ptr(), what,
+                        ": a cache was given twice");
+  }
+  const Tensor at = one_each(keys[0], start, B, true, "start", what);
+  const Tensor count = one_each(keys[0], counts, B, false, "counts", what);
+  TORCH_CHECK_VALUE(path.scalar_type() == at::kLong && path.dim() == 2 && path.size(0) == B, what,
+                    ": path must be int64, one row per sequence");
+  on_device(keys[0], path, what);
+  require_gpu(keys[0], what);
+  const int code = dtype_code(ks[0], what);
+  const c10::DeviceGuard guard(keys[0].device());
+  const Tensor way = unit_columns(path);
   std::vector<rk_int8_kv_commit_layer> layers(n);
   std::vector<Tensor> held;  // copies of operands that do not lie as vectors
   held.reserve(2 * n);
-  const int code = dtype_code(ks[0], what);
   for (size_t i = 0; i < n; ++i) {
-    const rk_int8_kv c = int8_kv(keys[i], values[i], key_scales[i], value_scales[i], what);
-    same_device(keys[0], keys[i], what);
-    for (const Tensor* t : {&ks[i], &vs[i]}) {
-      same_device(keys[0], *t, what);
-      TORCH_CHECK(t->dim() == 4 && t->size(0) == c.B && t->size(1) == c.H &&
-                      t->size(2) == ks[0].size(2) && t->size(3) == c.D &&
-                      t->scalar_type() == ks[0].scalar_type(),
-                  what, ": k and v must share a dtype and the caches' [B, H, N, D] shape");
-    }
     held.push_back(vector_rows(ks[i]));
     held.push_back(vector_rows(vs[i]));
     const Tensor &k = held[2 * i], &v = held[2 * i + 1];
-    layers[i] = {c, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                 v.stride(0), v.stride(1), v.stride(2)};
+    layers[i] = {int8_kv(keys[i], values[i], key_scales[i], value_scales[i], what), k.data_ptr(),
+                 v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1),
+                 v.stride(2)};
   }
-  const int64_t B = keys[0].size(0);
-  const int64_t* at = positions(keys[0], start, B, true, what);
-  const int64_t* count = positions(keys[0], counts, B, false, what);
-  same_device(keys[0], path, what);
-  TORCH_CHECK(path.scalar_type() == at::kLong && path.dim() == 2 && path.size(0) == B &&
-                  (path.stride(1) == 1 || path.size(1) <= 1),
-              what, ": path must be int64, one row per sequence");
-  const c10::DeviceGuard guard(keys[0].device());
-  check_status(rk_int8_kv_commit(layers.data(), static_cast<int64_t>(n), ks[0].size(2), code, at,
-                                 start.size(0), path.data_ptr<int64_t>(), ld(path), path.size(1),
-                                 count, stream_of(keys[0])),
+  check_status(rk_int8_kv_commit(layers.data(), static_cast<int64_t>(n), N, code,
+                                 at.data_ptr<int64_t>(), at.size(0), way.data_ptr<int64_t>(),
+                                 ld(way), way.size(1), count.data_ptr<int64_t>(),
+                                 stream_of(keys[0])),
                "rk_int8_kv_commit");
 }
 
@@ -1489,16 +1541,6 @@ std::tuple<Tensor, Tensor, Tensor> draft_tree(const Tensor& parents) {
   return {kept, depths, seen};
 }
 
-// A tree's tensor: [1 or B, N, ..], contiguous.
-void tree_part(const Tensor& like, const Tensor& t, at::ScalarType type, int64_t B, int64_t N,
-               int64_t dims, const char* what) {
-  same_device(like, t, what);
-  TORCH_CHECK(t.scalar_type() == type && t.dim() == dims && t.is_contiguous() &&
-                  (t.size(0) == 1 || t.size(0) == B) && t.size(1) == N &&
-                  (dims == 2 || t.size(2) == (N + 63) / 64),
-              what, ": the tree must come from draft_tree, one or one per sequence, of N nodes");
-}
-
 // Attention of drafted nodes over the 8-bit cache and themselves (rk_tree_attention):
 // [B, Hq, N, D] as a view of [B, N, Hq, D] memory.
 Tensor tree_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& keys,
@@ -1507,36 +1549,49 @@ Tensor tree_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
                       const Tensor& seen, double scale, double softcap, const OptTensor& slopes,
                       at::ScalarType out_dtype) {
   constexpr const char* what = "tree attention";
-  rk_tree_attention_args a{};
-  a.cache = int8_kv(keys, values, key_scales, value_scales, what);
-  const int64_t B = a.cache.B, H = a.cache.H, D = a.cache.D;
-  for (const Tensor* t : {&q, &k, &v}) same_device(keys, *t, what);
-  TORCH_CHECK(q.dim() == 4 && q.size(0) == B && q.size(3) == D &&
-                  (H > 0 ? q.size(1) % H == 0 : q.size(1) == 0),
-              what, ": q must be [B, Hq, N, D] with heads a multiple of the cache's");
+  TORCH_CHECK_VALUE(keys.dim() == 5 && q.dim() == 4, what,
+                    ": q must be [B, Hq, N, D], the cache's keys [B, H, blocks, 64, D]");
+  const int64_t B = keys.size(0), H = keys.size(1), D = keys.size(4);
   const int64_t Hq = q.size(1), N = q.size(2);
-  TORCH_CHECK(k.sizes() == at::IntArrayRef({B, H, N, D}) && v.sizes() == k.sizes() &&
-                  k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
-              what, ": k and v must share q's dtype and be [B, H, N, D]");
-  a.dtype = dtype_code(q, what);
-  a.out_dtype = dtype_code(out_dtype);
+  TORCH_CHECK_VALUE(q.size(0) == B && q.size(3) == D && (H > 0 ? Hq % H == 0 : Hq == 0), what,
+                    ": q must be [B, Hq, N, D] with heads a multiple of the cache's");
+  TORCH_CHECK_VALUE(k.sizes() == at::IntArrayRef({B, H, N, D}) && v.sizes() == k.sizes(), what,
+                    ": k and v must be [B, H, N, D] with the cache's heads");
+  TORCH_CHECK_TYPE(q.is_floating_point() && k.scalar_type() == q.scalar_type() &&
+                       v.scalar_type() == q.scalar_type(),
+                   what, ": q, k and v must share a floating-point dtype");
+  for (const Tensor* t : {&q, &k, &v}) on_device(keys, *t, what);
+  no_gradient(what, {q, k, v});
+  const Tensor at = one_each(keys, start, B, true, "start", what);
+  Tensor len;
+  if (lengths.has_value()) len = one_each(keys, *lengths, B, false, "lengths", what);
   tree_part(keys, depths, at::kInt, B, N, 2, what);
   tree_part(keys, seen, at::kLong, B, N, 3, what);
-  TORCH_CHECK(seen.size(0) == depths.size(0), what, ": the tree's parts differ");
+  TORCH_CHECK_VALUE(seen.size(0) == depths.size(0), what, ": the tree's parts differ");
+  TORCH_CHECK_VALUE(scale > 0.0 && scale < INFINITY, what, ": scale must be positive and finite");
+  TORCH_CHECK_VALUE(softcap == 0.0 || (softcap >= 1e-3 && softcap <= 1e3), what,
+                    ": softcap must lie in 1e-3 .. 1e3 (0: none)");
+  Tensor sl;
+  if (slopes.has_value()) {
+    TORCH_CHECK_VALUE(slopes->dim() == 1 && slopes->size(0) == Hq, what,
+                      ": slopes must hold one value per query head");
+    TORCH_CHECK_TYPE(slopes->is_floating_point(), what, ": slopes must be floating point");
+    on_device(keys, *slopes, what);
+    no_gradient(what, {*slopes});
+    sl = slopes->to(at::kFloat).contiguous();
+  }
+  rk_tree_attention_args a{};
+  a.cache = int8_kv(keys, values, key_scales, value_scales, what);
+  a.dtype = dtype_code(q, what);
+  a.out_dtype = dtype_code(out_dtype);
   const c10::DeviceGuard guard(q.device());
   const Tensor qq = vector_rows(q), kk = vector_rows(k), vv = vector_rows(v);
-  a.start = positions(keys, start, B, true, what);
-  a.start_count = start.size(0);
-  a.lengths = lengths.has_value() ? positions(keys, *lengths, B, false, what) : nullptr;
+  a.start = at.data_ptr<int64_t>(), a.start_count = at.size(0);
+  a.lengths = len.defined() ? len.data_ptr<int64_t>() : nullptr;
   a.depths = depths.data_ptr<int32_t>();
   a.seen = reinterpret_cast<const uint64_t*>(seen.data_ptr<int64_t>());
   a.trees = seen.size(0);
-  Tensor sl;
-  if (slopes.has_value()) {
-    same_device(keys, *slopes, what);
-    sl = f32_vector(*slopes, Hq, "slopes");
-    a.slopes = sl.data_ptr<float>();
-  }
+  a.slopes = sl.defined() ? sl.data_ptr<float>() : nullptr;
   a.q = qq.data_ptr(), a.k = kk.data_ptr(), a.v = vv.data_ptr();
   a.sqb = qq.stride(0), a.sqh = qq.stride(1), a.sqs = qq.stride(2);
   a.skb = kk.stride(0), a.skh = kk.stride(1), a.sks = kk.stride(2);
@@ -1560,42 +1615,50 @@ std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& logits, const Ten
                                                  const OptTensor& draft_logits,
                                                  double temperature, int64_t top_k) {
   constexpr const char* what = "verify drafts";
-  require_gpu(logits, what);
-  TORCH_CHECK(logits.dim() == 3, what, ": logits must be [B, N, V]");
+  TORCH_CHECK_VALUE(logits.dim() == 3 && logits.is_floating_point(), what,
+                    ": logits must be floating point [B, N, V]");
   rk_verify_drafts_args a{};
   a.B = logits.size(0), a.N = logits.size(1), a.V = logits.size(2);
-  a.dtype = dtype_code(logits, what);
+  TORCH_CHECK_VALUE(a.N > 0 && a.V > 0, what, ": a vocabulary and at least the root are needed");
+  const auto each_node = [&](const Tensor& t, at::ScalarType type, const char* name) {
+    TORCH_CHECK_VALUE(t.scalar_type() == type && t.dim() == 2 && t.size(0) == a.B &&
+                          t.size(1) == a.N,
+                      what, ": ", name, " [B, N]");
+    on_device(logits, t, what);
+    return t.contiguous();
+  };
+  const Tensor tk = each_node(tokens, at::kLong, "tokens must be int64");
+  TORCH_CHECK_VALUE(temperature == 0.0 || (temperature >= 1e-6 && temperature < INFINITY), what,
+                    ": temperature must be finite and at least 1e-6 (0: greedy)");
+  TORCH_CHECK_VALUE(top_k >= 0, what, ": top_k must be positive (0: all)");
+  TORCH_CHECK_VALUE(temperature == 0.0 || uniforms.has_value(), what,
+                    ": sampling needs uniforms");
+  Tensor un, dg, len;
+  if (uniforms.has_value()) un = each_node(*uniforms, at::kFloat, "uniforms must be float32");
   const auto rows = [](const Tensor& t) {
     return t.stride(2) == 1 || t.size(2) <= 1 ? t : t.contiguous();
   };
+  if (draft_logits.has_value()) {
+    TORCH_CHECK_VALUE(draft_logits->sizes() == logits.sizes() &&
+                          draft_logits->scalar_type() == logits.scalar_type(),
+                      what, ": the drafter's logits must have the target's shape and dtype");
+    on_device(logits, *draft_logits, what);
+  }
+  if (lengths.has_value()) len = one_each(logits, *lengths, a.B, false, "lengths", what);
+  tree_part(logits, parents, at::kInt, a.B, a.N, 2, what);
+  require_gpu(logits, what);
   const c10::DeviceGuard guard(logits.device());
+  a.dtype = dtype_code(logits, what);
   const Tensor lg = rows(logits);
   a.logits = lg.data_ptr(), a.lb = lg.stride(0), a.ln = lg.stride(1);
-  Tensor dg;
   if (draft_logits.has_value()) {
-    same_device(logits, *draft_logits, what);
-    TORCH_CHECK(draft_logits->sizes() == logits.sizes() &&
-                    draft_logits->scalar_type() == logits.scalar_type(),
-                what, ": the drafter's logits must have the target's shape and dtype");
     dg = rows(*draft_logits);
     a.drafts = dg.data_ptr(), a.db = dg.stride(0), a.dn = dg.stride(1);
   }
-  tree_part(logits, parents, at::kInt, a.B, a.N, 2, what);
   a.parents = parents.data_ptr<int32_t>(), a.trees = parents.size(0);
-  same_device(logits, tokens, what);
-  TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.sizes() == at::IntArrayRef({a.B, a.N}),
-              what, ": tokens must be int64 [B, N]");
-  const Tensor tk = tokens.contiguous();
   a.tokens = tk.data_ptr<int64_t>();
-  Tensor un;
-  if (uniforms.has_value()) {
-    same_device(logits, *uniforms, what);
-    TORCH_CHECK(uniforms->scalar_type() == at::kFloat && uniforms->sizes() == tokens.sizes(), what,
-                ": uniforms must be float32 [B, N]");
-    un = uniforms->contiguous();
-    a.uniforms = un.data_ptr<float>();
-  }
-  a.lengths = lengths.has_value() ? positions(logits, *lengths, a.B, false, what) : nullptr;
+  a.uniforms = un.defined() ? un.data_ptr<float>() : nullptr;
+  a.lengths = len.defined() ? len.data_ptr<int64_t>() : nullptr;
   a.temperature = temperature, a.top_k = top_k;
   Tensor path = at::empty({a.B, a.N}, tk.options()), counts = at::empty({a.B}, tk.options());
   Tensor next = at::empty({a.B}, tk.options());
@@ -1841,6 +1904,12 @@ TORCH_LIBRARY_IMPL(ratchet, CUDA, m) {
   m.impl("kv_append", &kv_append);
   m.impl("cross_entropy_forward", &cross_entropy_forward);
   m.impl("cross_entropy_backward", &cross_entropy_backward);
+}
+
+// (their checks alone: host tensors are refused behind them)
+TORCH_LIBRARY_IMPL(ratchet, CPU, m) {
+  m.impl("int8_kv_commit", &int8_kv_commit);
+  m.impl("tree_attention", &tree_attention);
 }
 
 TORCH_LIBRARY_IMPL(ratchet, AutogradCUDA, m) { m.impl("scored_attend", &scored_attend_autograd); }

@@ -25,11 +25,12 @@ from typing import NamedTuple, Sequence
 import torch
 from torch import Tensor
 
-from .int8_cache import Int8KV, _check_positions, _refuse_gradients
+from .int8_cache import Int8KV
 from .ops import ratchet
-from .scored_attention import score_arguments, torch_scores
+from .scored_attention import torch_scores
 
 MAX_NODES = 256
+_NATIVE = (torch.float32, torch.bfloat16)
 _NOTHING = 2.0**-40  # a residual of this sum is rounding
 
 
@@ -100,17 +101,6 @@ def _lineage(tree: DraftTree) -> Tensor:
     return (tree.seen[..., None] >> shifts & 1).bool().reshape(r, n, -1)[:, :, :n]
 
 
-def _check_tree(tree: DraftTree, batch: int, nodes: int, like: Tensor) -> None:
-    rows = tree.parents.shape[0]
-    if (rows not in (1, batch) or tree.parents.shape != (rows, nodes)
-            or tree.depths.shape != (rows, nodes)
-            or tree.seen.shape != (rows, nodes, -(-nodes // 64))):
-        raise ValueError("the tree must hold one row or one per sequence, of these nodes")
-    for t in tree:
-        if t.device != like.device:
-            raise ValueError("the tree must be on the operands' device")
-
-
 def tree_attention(q: Tensor, k: Tensor, v: Tensor, cache: Int8KV, start: Tensor,
                    tree: DraftTree, *, lengths: Tensor | None = None,
                    softcap: float | None = None, slopes: Tensor | None = None,
@@ -122,32 +112,20 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, cache: Int8KV, start: Tensor
     cap, bias (by the distance of the positions) and scale are those of ``scored_attention``.
     Returns [B, Hq, N, D] in ``out_dtype`` (default q's); zeros for nodes that are off or not there.
     Nothing is appended to the cache. It has no gradient."""
-    b, h, _, _, d = cache.keys.shape
-    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != d or (q.shape[1] % h if h else q.shape[1]):
-        raise ValueError("q must be [B, Hq, N, D] with heads a multiple of the cache's")
-    n = q.shape[2]
-    if k.shape != (b, h, n, d) or v.shape != k.shape:
-        raise ValueError("k and v must be [B, H, N, D] with the cache's heads")
-    for t in (q, k, v):
-        if not t.is_floating_point():
-            raise TypeError("q, k and v must be floating point")
-        if t.device != cache.keys.device:
-            raise ValueError("q, k and v must be on the cache's device")
-    _refuse_gradients("attention over", q, k, v, slopes)
+    if not (q.dtype == k.dtype == v.dtype and q.dtype in _NATIVE):
+        for t in (q, k, v):
+            if not t.is_floating_point():
+                raise TypeError("q, k and v must be floating point")
+        out_dtype = out_dtype or q.dtype
+        q, k, v = q.float(), k.float(), v.float()
     out_dtype = out_dtype or q.dtype
     if not out_dtype.is_floating_point:
         raise TypeError("out_dtype must be floating point")
-    _check_positions(cache, start, lengths)
-    _check_tree(tree, b, n, q)
-    softcap, slopes, scale = score_arguments(q, softcap, slopes, scale)
-    if softcap and not 1e-3 <= softcap <= 1e3:
-        raise ValueError("softcap must lie in 1e-3 .. 1e3")
-    if not (q.dtype == k.dtype == v.dtype and q.dtype in (torch.float32, torch.bfloat16)):
-        q, k, v = q.float(), k.float(), v.float()
-    native = out_dtype if out_dtype in (torch.float32, torch.bfloat16) else torch.float32
-    out = ratchet().tree_attention(
-        q, k, v, *cache, start.contiguous(), lengths.contiguous() if lengths is not None else None,
-        tree.depths, tree.seen, scale, softcap, slopes.detach() if slopes is not None else None,
+    native = out_dtype if out_dtype in _NATIVE else torch.float32
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if q.shape[-1] else 1.0
+    out = ratchet().tree_attention.default(
+        q, k, v, *cache, start, lengths, tree.depths, tree.seen, scale, softcap or 0.0, slopes,
         native)
     return out if native == out_dtype else out.to(out_dtype)
 
@@ -176,18 +154,6 @@ class Verified(NamedTuple):
     next: Tensor
 
 
-def _choice_arguments(temperature: float, top_k: int | None, uniforms: Tensor | None) -> int:
-    if not 0.0 <= temperature < math.inf:
-        raise ValueError("temperature must be finite and not negative")
-    if 0.0 < temperature < 1e-6:
-        raise ValueError("a temperature below 1e-6 is not supported (0: greedy)")
-    if top_k is not None and top_k <= 0:
-        raise ValueError("top_k must be positive")
-    if temperature and uniforms is None:
-        raise ValueError("sampling needs uniforms")
-    return top_k or 0
-
-
 def verify_drafts(logits: Tensor, tokens: Tensor, tree: DraftTree,
                   uniforms: Tensor | None = None, *, lengths: Tensor | None = None,
                   draft_logits: Tensor | None = None, temperature: float = 1.0,
@@ -206,38 +172,53 @@ def verify_drafts(logits: Tensor, tokens: Tensor, tree: DraftTree,
     Of a sequence's nodes the first ``lengths`` [B] are there (none: count 0, next -1). A row that is
     no distribution (a NaN, an infinity) gives next -1. Decisions are made in 64 bits. Logits of other
     types than float32 and bfloat16 are taken as float32."""
-    if logits.dim() != 3 or not logits.is_floating_point():
-        raise ValueError("logits must be floating point [B, N, V]")
-    b, n, vocab = logits.shape
-    if vocab == 0 or n == 0:
-        raise ValueError("a vocabulary and at least the root are needed")
-    if tokens.shape != (b, n) or tokens.dtype != torch.int64:
-        raise ValueError("tokens must be int64 [B, N]")
-    top_k = _choice_arguments(temperature, top_k, uniforms)
-    if uniforms is not None and (uniforms.shape != (b, n) or uniforms.dtype != torch.float32):
-        raise ValueError("uniforms must be float32 [B, N]")
-    if draft_logits is not None and (draft_logits.shape != logits.shape
-                                     or not draft_logits.is_floating_point()):
-        raise ValueError("the drafter's logits must be floating point, of the target's shape")
-    if lengths is not None and (lengths.shape != (b,) or lengths.dtype != torch.int64):
-        raise ValueError("lengths must be int64, one per sequence")
-    for t in (tokens, uniforms, draft_logits, lengths):
-        if t is not None and t.device != logits.device:
-            raise ValueError("the operands must share a device")
-    _check_tree(tree, b, n, logits)
-    logits = logits.detach()
-    draft_logits = draft_logits.detach() if draft_logits is not None else None
-    known = (torch.float32, torch.bfloat16)
-    if logits.dtype not in known or (draft_logits is not None
-                                     and draft_logits.dtype != logits.dtype):
+    if logits.dtype not in _NATIVE or (draft_logits is not None
+                                       and draft_logits.dtype != logits.dtype):
+        for t in (logits, draft_logits):
+            if t is not None and not t.is_floating_point():
+                raise ValueError("logits must be floating point")
         logits = logits.float()
         draft_logits = draft_logits.float() if draft_logits is not None else None
+    if top_k is not None and top_k <= 0:
+        raise ValueError("top_k must be positive")
     if logits.is_cuda:
-        return Verified(*ratchet().verify_drafts(
-            logits, tokens, tree.parents, uniforms.detach() if uniforms is not None else None,
-            lengths.contiguous() if lengths is not None else None, draft_logits,
-            float(temperature), top_k))
-    return _torch_verify(logits, tokens, tree, uniforms, lengths, draft_logits, temperature, top_k)
+        if logits.requires_grad or (draft_logits is not None and draft_logits.requires_grad):
+            logits = logits.detach()
+            draft_logits = draft_logits.detach() if draft_logits is not None else None
+        return Verified(*ratchet().verify_drafts.default(
+            logits, tokens, tree.parents, uniforms, lengths, draft_logits, temperature,
+            top_k or 0))
+    _check_verification(logits, tokens, tree, uniforms, lengths, draft_logits, temperature)
+    with torch.no_grad():
+        return _torch_verify(logits, tokens, tree, uniforms, lengths, draft_logits, temperature,
+                             top_k or 0)
+
+
+def _check_verification(logits: Tensor, tokens: Tensor, tree: DraftTree,
+                        uniforms: Tensor | None, lengths: Tensor | None,
+                        draft_logits: Tensor | None, temperature: float) -> None:
+    """The operator's own checks, for the torch form."""
+    if logits.dim() != 3 or logits.shape[1] == 0 or logits.shape[2] == 0:
+        raise ValueError("logits must be [B, N, V], of at least the root")
+    b, n, _ = logits.shape
+    if tokens.shape != (b, n) or tokens.dtype != torch.int64:
+        raise ValueError("tokens must be int64 [B, N]")
+    if not (temperature == 0.0 or 1e-6 <= temperature < math.inf):
+        raise ValueError("temperature must be finite and at least 1e-6 (0: greedy)")
+    if temperature and uniforms is None:
+        raise ValueError("sampling needs uniforms")
+    if uniforms is not None and (uniforms.shape != (b, n) or uniforms.dtype != torch.float32):
+        raise ValueError("uniforms must be float32 [B, N]")
+    if draft_logits is not None and draft_logits.shape != logits.shape:
+        raise ValueError("the drafter's logits must have the target's shape")
+    if lengths is not None and (lengths.shape != (b,) or lengths.dtype != torch.int64):
+        raise ValueError("lengths must be int64, one per sequence")
+    for t in (tokens, uniforms, draft_logits, lengths, *tree):
+        if t is not None and t.device != logits.device:
+            raise ValueError("the operands must share a device")
+    rows = tree.parents.shape[0]
+    if rows not in (1, b) or tree.parents.shape != (rows, n):
+        raise ValueError("the tree must hold one row or one per sequence, of these nodes")
 
 
 def _distribution(row: Tensor, temperature: float, top_k: int) -> Tensor:
@@ -326,33 +307,8 @@ def int8_kv_commit(caches: Sequence[Int8KV], ks: Sequence[Tensor], vs: Sequence[
     ``counts`` [B] of a sequence is node ``path`` [B, P] [i] of the layer's k and v [B, H, N, D], and
     goes to position ``start`` + i (as ``int8_kv_append`` puts it there). Nodes outside 0 .. N - 1
     within the counts are tokens of zeros. It has no gradient."""
-    if not caches or not len(caches) == len(ks) == len(vs):
+    if not ks or not len(caches) == len(ks) == len(vs):
         raise ValueError("one k, one v and one cache per layer are needed")
-    shape, device = caches[0].keys.shape, caches[0].keys.device
-    b, h, _, _, d = shape
-    n = ks[0].shape[2] if ks[0].dim() == 4 else -1
-    if caches[0].keys.numel() and len({c.keys.data_ptr() for c in caches}) != len(caches):
-        raise ValueError("a cache was given twice")
-    for cache, k, v in zip(caches, ks, vs):
-        if cache.keys.shape != shape:
-            raise ValueError("the layers' caches must share a shape")
-        if k.shape != (b, h, n, d) or v.shape != k.shape:
-            raise ValueError("k and v must share the caches' [B, H, N, D] shape")
-        if k.dtype != v.dtype or not k.is_floating_point():
-            raise TypeError("k and v must share a floating-point dtype")
-        if not k.device == v.device == cache.keys.device == device:
-            raise ValueError("k, v and the caches must share a device")
-        _refuse_gradients("appending to", k, v)
-    _check_positions(caches[0], start, counts)
-    if path.dtype != torch.int64 or path.dim() != 2 or path.shape[0] != b:
-        raise ValueError("path must be int64, one row per sequence")
-    if path.device != device:
-        raise ValueError("path must be on the caches' device")
-    if {t.dtype for t in (*ks, *vs)} not in ({torch.float32}, {torch.bfloat16}):
+    if ks[0].dtype not in _NATIVE and ks[0].is_floating_point():
         ks, vs = [k.float() for k in ks], [v.float() for v in vs]
-    if path.stride(1) != 1 and path.shape[1] > 1:
-        path = path.contiguous()
-    ratchet().int8_kv_commit([k.detach() for k in ks], [v.detach() for v in vs],
-                             [c.keys for c in caches], [c.values for c in caches],
-                             [c.key_scales for c in caches], [c.value_scales for c in caches],
-                             start.contiguous(), path, counts.contiguous())
+    ratchet().int8_kv_commit.default(ks, vs, *zip(*caches), start, path, counts)

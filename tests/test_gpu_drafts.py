@@ -329,9 +329,9 @@ def test_attention_operator(cuda):
     args = (q, k, v, *cache, ints(cuda, 70), None, tree.depths, tree.seen, 0.125, 0.0, None,
             torch.bfloat16)
     torch.library.opcheck(ratchet().tree_attention, args)
-    with pytest.raises(RuntimeError, match="tree"):
+    with pytest.raises(ValueError, match="tree"):
         ratchet().tree_attention(*args[:9], tree.depths[:, :3], *args[10:])
-    with pytest.raises(RuntimeError, match="device"):
+    with pytest.raises(ValueError, match="device"):
         ratchet().tree_attention(q, k.cpu(), *args[2:])
 
 
@@ -513,15 +513,36 @@ def test_sampled_tokens(cuda):
         assert torch.equal(got.cpu(), want)
 
 
+def test_logits_that_want_gradients(cuda):
+    logits, tokens, uniforms, other = (t.to(cuda) for t in choice(3, 6, 250, 4, True))
+    tree = draft_tree(plain.random_parents(6, 1, 2), cuda)
+    want = verify_drafts(logits, tokens, tree, uniforms, draft_logits=other)
+    got = verify_drafts(logits.requires_grad_(), tokens, tree, uniforms,
+                        draft_logits=other.requires_grad_())
+    assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
+    q, k, v = nodes_of(cuda, 1, 4, 1, 1, 64)
+    cache, tree = filled(cuda, 1, 1, 70, 64), draft_tree([-1, 0, 0, 1], cuda)
+    for t in (q, k, v):
+        t.requires_grad_()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            tree_attention(q, k, v, cache, ints(cuda, 70), tree)
+        with torch.no_grad():
+            tree_attention(q, k, v, cache, ints(cuda, 70), tree)
+        t.requires_grad_(False)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        int8_kv_commit([cache], [k.requires_grad_()], [v], ints(cuda, 0), ints(cuda, [0]),
+                       ints(cuda, 1))
+
+
 def test_verification_operator(cuda):
     logits, tokens, uniforms, other = (t.to(cuda) for t in choice(2, 4, 50, 4, True))
     tree = draft_tree([-1, 0, 0, 1], cuda)
     args = (logits, tokens, tree.parents, uniforms, None, other, 1.0, 0)
     torch.library.opcheck(ratchet().verify_drafts, args)
-    for i, bad, match in ((3, None, "null"), (6, -1.0, "temperature"), (7, -1, "negative"),
+    for i, bad, match in ((3, None, "uniforms"), (6, -1.0, "temperature"), (7, -1, "top_k"),
                           (2, tree.parents[:, :2], "tree"), (5, other[:, :3], "shape"),
                           (1, tokens.int(), "int64")):
-        with pytest.raises(RuntimeError, match=match):
+        with pytest.raises(ValueError, match=match):
             ratchet().verify_drafts(*args[:i], bad, *args[i + 1:])
 
 
@@ -578,9 +599,9 @@ def test_commit_operator(cuda):
     args = ([k], [k], *([t] for t in cache), ints(cuda, 64), ints(cuda, [0, 2, -1]), ints(cuda, 2))
     torch.library.opcheck(ratchet().int8_kv_commit, args,
                           test_utils=("test_schema", "test_faketensor"))
-    with pytest.raises(RuntimeError, match="layer"):
+    with pytest.raises(ValueError, match="layer"):
         ratchet().int8_kv_commit([k, k], *args[1:])
-    with pytest.raises(RuntimeError, match="path"):
+    with pytest.raises(ValueError, match="path"):
         ratchet().int8_kv_commit(*args[:7], args[7].int(), args[8])
 
 
