@@ -10,6 +10,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace rk {
 
 // ---------------------------------------------------------------------------
@@ -77,33 +79,50 @@ struct TreeAttn {
   const int32_t* depths;
   const float* slopes;
   int64_t start_step, tree_step, N, W, Hq, G, nsplit, tiles;
-  float dot_scale, cap2;
+  float dot_scale;        // scale log2(e)
+  float cap2, inv_cap2;   // cap log2(e); 0: none
+  float near[3];          // tree_near
   float* work;  // [B * H][N * G][nsplit][D + 4]: max, sum, 2 pad, unnormalized output
   void* out;    // [B, N, Hq, D]
 };
 
-// The capped score in base-2 units of t = 2 log2(e) scale / cap times the dot product. The
-// exponential form is off by a few 2^-24 of the cap whatever the score; where float32 results show
-// it, scores of up to a third of the cap take tanh's series (its next term is below 2^-26 there).
+// The capped score C tanh(y / C) of a score y, both in base-2 units, C = cap log2(e). The exponential
+// form is off by a few 2^-24 of C whatever the score; where float32 results show it (FINE), scores of
+// up to a third of the cap take tanh's series (its next term is below 2^-26 there).
 template <bool FINE>
-__device__ __forceinline__ float tree_capped(float t, float cap2) {
-  const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(t) + 1.0f);
-  float y = __builtin_fmaf(-2.0f * cap2, r, cap2);
+__device__ __forceinline__ float tree_capped(float y, float cap2, float inv_cap2) {
+  const float u = y * inv_cap2;
+  const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * (2.0f * kLog2e8)) + 1.0f);
+  float t = __builtin_fmaf(-2.0f * cap2, r, cap2);
   if constexpr (FINE) {
-    const float u = t * (0.5f / kLog2e8), z = u * u;
+    const float z = u * u;
     float s = __builtin_fmaf(z, -1382.0f / 155925.0f, 62.0f / 2835.0f);
     s = __builtin_fmaf(z, s, -17.0f / 315.0f);
     s = __builtin_fmaf(z, s, 2.0f / 15.0f);
     s = __builtin_fmaf(z, s, -1.0f / 3.0f);
-    y = fabsf(u) < 0.34f ? cap2 * __builtin_fmaf(u * z, s, u) : y;
+    t = fabsf(u) < 0.34f ? __builtin_fmaf(y * z, s, y) : t;
   }
-  return y;
+  return t;
+}
+// The same for |y| <= kNear C by y (1 + z (c0 + c1 z + c2 z^2)), z = y^2: half the instructions. The
+// host interpolates (tanh(u) / u - 1) / u^2 at Chebyshev nodes of u^2 (off by 2e-7 of the score).
+constexpr float kNear = 0.4f;
+__device__ __forceinline__ float tree_near(float y, const float (&c)[3]) {
+  const float z = y * y;
+  float s = __builtin_fmaf(z, c[2], c[1]);
+  s = __builtin_fmaf(z, s, c[0]);
+  return __builtin_fmaf(y, z * s, y);
 }
 
-template <int D, int CT, int QDT, int ODT>
+// What is done to the scores: nothing; a cap of so little (kBounded) that their exponentials need no
+// maximum, in units of which 2^60 is the most; a cap, a bias or both.
+enum { kPlain, kBounded, kModified };
+constexpr float kBound = 60.0f;
+
+template <int D, int CT, int QDT, int ODT, int NP, int MODE>
 __global__ __launch_bounds__(256) void tree_cache_kernel(TreeAttn a) {
   constexpr int KK = D / 64, FT = D / 16, NW = 4;
-  constexpr int QP = QDT == RK_F32 ? 3 : 1, NP = ODT == RK_F32 ? 3 : 2;
+  constexpr int QP = QDT == RK_F32 ? 3 : 1;
   constexpr bool FINE = ODT == RK_F32;
   __shared__ float box[2][CT * (4 * FT + 2)][64];
   const int split = blockIdx.x;
@@ -121,11 +140,13 @@ __global__ __launch_bounds__(256) void tree_cache_kernel(TreeAttn a) {
                       static_cast<uint32_t>(a.nsplit);
   const int64_t j0 = split * per, j1 = j0 + per < nb ? j0 + per : nb;
 
-  float m[CT], l[CT], o[CT][FT][4];
+  // the sum is a product too, of ones (its four rows are equal): the MFMAs have time for it
+  float m[CT], o[CT][FT][4];
+  v4f_a sums[CT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     m[c] = -INFINITY;
-    l[c] = 0.0f;
+    sums[c] = v4f_a{};
 #pragma unroll
     for (int f = 0; f < FT; ++f)
 #pragma unroll
@@ -193,52 +214,58 @@ __global__ __launch_bounds__(256) void tree_cache_kernel(TreeAttn a) {
         }
       }
     }
+    const uint32_t one2 = 0x3f803f80u;
+    const v8bf_a ones = frag_of(make_uint4(one2, one2, one2, one2));
+    // widened codes: 16 features of a key, 16 tokens of a feature
+    const auto widen = [](const v4i8& codes, v8bf_a (&to)[2]) {
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        widen_codes(static_cast<uint32_t>(codes[e]), w[2 * e], w[2 * e + 1]);
+      to[0] = frag_of(make_uint4(w[0], w[1], w[2], w[3]));
+      to[1] = frag_of(make_uint4(w[4], w[5], w[6], w[7]));
+    };
+    const auto product = [&](int c, const v8bf_a (&kw)[KK][2]) {
+      v4f_a acc{};
+#pragma unroll
+      for (int n = QP - 1; n >= 0; --n)
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kw[kk][u], qf[c][n][kk][u], acc, 0, 0, 0);
+      return acc;
+    };
     for (; j < j1; j += NW) {
       const float vscale = vs[j], mul = ks[j] * a.dot_scale;
-      v4f_a s[CT][4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        v8bf_a kw[KK][2];
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          uint32_t w[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            widen_codes(static_cast<uint32_t>(kf[t][kk][e]), w[2 * e], w[2 * e + 1]);
-          kw[kk][0] = frag_of(make_uint4(w[0], w[1], w[2], w[3]));
-          kw[kk][1] = frag_of(make_uint4(w[4], w[5], w[6], w[7]));
-        }
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          s[c][t] = v4f_a{};
-#pragma unroll
-          for (int n = QP - 1; n >= 0; --n)
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-              for (int u = 0; u < 2; ++u)
-                s[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kw[kk][u], qf[c][n][kk][u],
-                                                                  s[c][t], 0, 0, 0);
-        }
-      }
-      load_k(j + NW);
       // key 16 g + x of the block is cached for x < left
       const int64_t ahead = start - (j * kTok + 16 * g);
       const int left = ahead > 16 ? 16 : ahead < 0 ? 0 : static_cast<int>(ahead);
       const bool whole = (j + 1) * kTok <= start;
       const float first = static_cast<float>(j * kTok + 16 * g);
-      v8bf_a p[CT][NP][2];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
+      // a tile's probabilities from its scores, with the running maximum and sum
+      const auto weigh = [&](int c, const v4f_a (&s)[4], v8bf_a (&p)[NP][2]) {
         float y[16];
-        if (a.cap2 != 0.0f) {
+        // plain scores are scaled with the subtraction of the maximum
+        const float unit = MODE == kPlain ? mul : 1.0f;
 #pragma unroll
-          for (int x = 0; x < 16; ++x) y[x] = tree_capped<FINE>(s[c][x / 4][x % 4] * mul, a.cap2);
-        } else {
+        for (int x = 0; x < 16; ++x) y[x] = s[x / 4][x % 4] * (MODE == kPlain ? 1.0f : mul);
+        if (MODE == kBounded || (MODE == kModified && a.cap2 != 0.0f)) {
+          float far = 0.0f, raw[16];
 #pragma unroll
-          for (int x = 0; x < 16; ++x) y[x] = s[c][x / 4][x % 4] * mul;
+          for (int x = 0; x < 16; ++x) far = fmaxf(far, fabsf(y[x]));
+          const bool near = !FINE && !__any(!(far <= kNear * a.cap2));
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            raw[x] = y[x];
+            if constexpr (!FINE) y[x] = tree_near(y[x], a.near);
+          }
+          if (!near) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) y[x] = tree_capped<FINE>(raw[x], a.cap2, a.inv_cap2);
+          }
         }
-        if (a.slopes) {
+        if (MODE == kModified && a.slopes) {
           const float d0 = pos[c] - first;
 #pragma unroll
           for (int x = 0; x < 16; ++x) y[x] = __builtin_fmaf(-slope2[c], d0 - x, y[x]);
@@ -247,55 +274,104 @@ __global__ __launch_bounds__(256) void tree_cache_kernel(TreeAttn a) {
 #pragma unroll
           for (int x = 0; x < 16; ++x) y[x] = x < left ? y[x] : -INFINITY;
         }
-        float mx = y[0];
+        if constexpr (MODE == kBounded) {
+          m[c] = 0.0f;
 #pragma unroll
-        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, y[x]);
-        mx = col_max(mx);
-        const float mnew = fmaxf(m[c], mx), ref = mnew == -INFINITY ? 0.0f : mnew;
-        const float alpha = __builtin_amdgcn_exp2f(m[c] - ref);
-        m[c] = mnew;
-        float sum = 0.0f;
+          for (int x = 0; x < 16; ++x) y[x] = __builtin_amdgcn_exp2f(y[x]);
+        } else {
+          float mx = y[0];
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          y[x] = __builtin_amdgcn_exp2f(y[x] - ref);
-          sum = sum + y[x];
+          for (int x = 1; x < 16; ++x) mx = fmaxf(mx, y[x]);
+          mx = col_max(mx) * unit;
+          const float mnew = fmaxf(m[c], mx), ref = mnew == -INFINITY ? 0.0f : mnew;
+          const float alpha = __builtin_amdgcn_exp2f(m[c] - ref);
+          m[c] = mnew;
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            y[x] = __builtin_amdgcn_exp2f(MODE == kPlain ? __builtin_fmaf(y[x], unit, -ref)
+                                                         : y[x] - ref);
+          if (MODE == kPlain && !whole) {  // (a zero key scale makes NaN of a masked score)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) y[x] = x < left ? y[x] : 0.0f;
+          }
+          if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[c][e] = sums[c][e] * alpha;
+#pragma unroll
+            for (int f = 0; f < FT; ++f)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[c][f][e] = o[c][f][e] * alpha;
+          }
         }
-        l[c] = l[c] * alpha + sum;  // of this lane's keys
-        if (__any(alpha != 1.0f)) {
+        split_bf16<NP>(y, p);
 #pragma unroll
-          for (int f = 0; f < FT; ++f)
+        for (int n = NP - 1; n >= 0; --n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[c][f][e] = o[c][f][e] * alpha;
-        }
-        split_bf16<NP>(y, p[c]);
-      }
+          for (int u = 0; u < 2; ++u)
+            sums[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[n][u], sums[c], 0, 0, 0);
+      };
+      const auto values = [&](int c, int f, const v8bf_a (&v)[2], const v8bf_a (&p)[NP][2]) {
+        v4f_a acc{};
 #pragma unroll
-      for (int f = 0; f < FT; ++f) {
-        uint32_t w[8];
+        for (int n = NP - 1; n >= 0; --n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          widen_codes(static_cast<uint32_t>(vf[f][e]), w[2 * e], w[2 * e + 1]);
-        const v8bf_a v[2] = {frag_of(make_uint4(w[0], w[1], w[2], w[3])),
-                             frag_of(make_uint4(w[4], w[5], w[6], w[7]))};
+          for (int u = 0; u < 2; ++u)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], p[n][u], acc, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c][f][e] = __builtin_fmaf(acc[e], vscale, o[c][f][e]);
+      };
+      if constexpr (D == 64) {
+        // the widened block fits the registers: a tile at a time, one's products beside the next one's
+        // exponentials
+        v8bf_a kw[4][KK][2], vw[FT][2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) widen(kf[t][kk], kw[t][kk]);
+        load_k(j + NW);
+#pragma unroll
+        for (int f = 0; f < FT; ++f) widen(vf[f], vw[f]);
+        load_v(j + NW);
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          v4f_a acc{};
+          v4f_a s[4];
+          v8bf_a p[NP][2];
 #pragma unroll
-          for (int n = NP - 1; n >= 0; --n)
+          for (int t = 0; t < 4; ++t) s[t] = product(c, kw[t]);
+          weigh(c, s, p);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-              acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u], p[c][n][u], acc, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[c][f][e] = __builtin_fmaf(acc[e], vscale, o[c][f][e]);
+          for (int f = 0; f < FT; ++f) values(c, f, vw[f], p);
         }
+      } else {
+        v4f_a s[CT][4];
+        v8bf_a p[CT][NP][2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          v8bf_a kw[KK][2];
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) widen(kf[t][kk], kw[kk]);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) s[c][t] = product(c, kw);
+        }
+        load_k(j + NW);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) weigh(c, s[c], p[c]);
+#pragma unroll
+        for (int f = 0; f < FT; ++f) {
+          v8bf_a v[2];
+          widen(vf[f], v);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) values(c, f, v, p[c]);
+        }
+        load_v(j + NW);
       }
-      load_v(j + NW);
     }
   }
 
   // the wavefronts: 2 and 3 into 0 and 1, then 1 into 0
+  float l[CT];
 #pragma unroll
-  for (int c = 0; c < CT; ++c) l[c] = col_sum(l[c]);
+  for (int c = 0; c < CT; ++c) l[c] = sums[c][0];
   const auto merge = [&](int half) {
     if (wave >= half && wave < 2 * half) {
       float(*const to)[64] = box[wave - half];
@@ -371,16 +447,19 @@ struct TreeState {
   }
 };
 
-// grid (columns, B * H), one wavefront: the splits of one column and the nodes it sees, in float32.
-// Four groups of 16 lanes, D / 16 features a lane, take every fourth of both.
+// grid (columns / 4, B * H), a wavefront a column: its splits and the nodes it sees, in float32. Four
+// groups of 16 lanes, D / 16 features a lane, take every fourth of both.
 template <int D, int QDT, int ODT>
-__global__ __launch_bounds__(64) void tree_join_kernel(TreeAttn a) {
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeAttn a) {
   constexpr int F = D / 16;
   const uint32_t uh = static_cast<uint32_t>(a.c.H), ub = blockIdx.y / uh;
-  const int64_t ct = blockIdx.x, bh = blockIdx.y, b = ub, kvh = blockIdx.y - ub * uh;
+  const int64_t ct = 4 * static_cast<int64_t>(blockIdx.x) +
+                     __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (ct >= a.N * a.G) return;
+  const int64_t bh = blockIdx.y, b = ub, kvh = blockIdx.y - ub * uh;
   const int64_t i = static_cast<uint32_t>(ct) / static_cast<uint32_t>(a.G);
   const int64_t hd = kvh * a.G + (ct - i * a.G);
-  const int lane = threadIdx.x, grp = lane >> 4, f0 = (lane & 15) * F;
+  const int lane = threadIdx.x & 63, grp = lane >> 4, f0 = (lane & 15) * F;
   const int64_t start = a.start[b * a.start_step];
   const int64_t tree = b * a.tree_step;
   const uint64_t* const seen = a.seen + (tree * a.N + i) * a.W;
@@ -421,28 +500,39 @@ __global__ __launch_bounds__(64) void tree_join_kernel(TreeAttn a) {
     const int depth = depths[i];
     for (int64_t w = 0; w < a.W; ++w) {
       uint64_t left = seen[w] & (w + 1 < a.W ? ~0ull : tail);
-      while (left) {  // the next four nodes, one for each group
-        int node = -1;
+      while (left) {  // the next eight nodes, two for each group, loaded together
+        int node[2] = {-1, -1};
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < 8; ++n) {
           const int at = left ? static_cast<int>(__builtin_ctzll(left)) : -1;
-          if (grp == n) node = at;
+          if (grp == n % 4) node[n / 4] = at;
           left &= left - 1;
         }
-        const int64_t at = 64 * w + (node < 0 ? 0 : node);
-        float k[F], v[F], s = 0.0f;
-        load(a.k, b * a.skb + kvh * a.skh + at * a.sks + f0, k);
-        load(a.v, b * a.svb + kvh * a.svh + at * a.svs + f0, v);
+        float k[2][F], v[2][F], s[2];
+        int depth_at[2];
 #pragma unroll
-        for (int e = 0; e < F; ++e) s = __builtin_fmaf(q[e], k[e], s);
-        s = s + __uint_as_float(dpp_u32<0x128>(__float_as_uint(s)));  // over the group's lanes
-        s = s + __uint_as_float(dpp_u32<0x141>(dpp_u32<0x1b>(__float_as_uint(s))));
-        s = s + __uint_as_float(dpp_u32<0x4e>(__float_as_uint(s)));
-        s = s + __uint_as_float(dpp_u32<0xb1>(__float_as_uint(s)));
-        s = s * a.dot_scale;
-        if (a.cap2 != 0.0f) s = tree_capped<ODT == RK_F32>(s, a.cap2);
-        if (a.slopes) s = __builtin_fmaf(-slope2, static_cast<float>(depth - depths[at]), s);
-        if (node >= 0) st.add(s, 1.0f, v);
+        for (int n = 0; n < 2; ++n) {
+          const int64_t at = 64 * w + (node[n] < 0 ? 0 : node[n]);
+          load(a.k, b * a.skb + kvh * a.skh + at * a.sks + f0, k[n]);
+          load(a.v, b * a.svb + kvh * a.svh + at * a.svs + f0, v[n]);
+          depth_at[n] = depths[at];
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          s[n] = 0.0f;
+#pragma unroll
+          for (int e = 0; e < F; ++e) s[n] = __builtin_fmaf(q[e], k[n][e], s[n]);
+          const auto bits = [&] { return __float_as_uint(s[n]); };
+          s[n] = s[n] + __uint_as_float(dpp_u32<0x128>(bits()));  // over the group's lanes
+          s[n] = s[n] + __uint_as_float(dpp_u32<0x141>(dpp_u32<0x1b>(bits())));
+          s[n] = s[n] + __uint_as_float(dpp_u32<0x4e>(bits()));
+          s[n] = s[n] + __uint_as_float(dpp_u32<0xb1>(bits()));
+          s[n] = s[n] * a.dot_scale;
+          if (a.cap2 != 0.0f) s[n] = tree_capped<ODT == RK_F32>(s[n], a.cap2, a.inv_cap2);
+          if (a.slopes)
+            s[n] = __builtin_fmaf(-slope2, static_cast<float>(depth - depth_at[n]), s[n]);
+          if (node[n] >= 0) st.add(s[n], 1.0f, v[n]);
+        }
       }
     }
   }
@@ -472,7 +562,8 @@ __global__ __launch_bounds__(64) void tree_join_kernel(TreeAttn a) {
 // Host side
 // ---------------------------------------------------------------------------
 struct TreeLaunch {
-  int ct;  // tiles of 16 columns a wavefront holds
+  int ct;   // tiles of 16 columns a wavefront holds
+  bool many;  // so many columns that probabilities of bf16 results are one bf16 number each
   int64_t tiles, splits;
 };
 
@@ -480,35 +571,80 @@ static TreeLaunch tree_launch(const rk_tree_attention_args& p) {
   const rk_int8_kv& c = p.cache;
   const int64_t cols = p.N * (p.Hq / c.H);
   TreeLaunch t{};
-  t.ct = cols > 16 && c.D <= 128 ? 2 : 1;
+  t.many = cols > 32 && p.dtype == RK_BF16 && p.out_dtype == RK_BF16;
+  t.ct = c.D > 128 || cols <= 16 || (c.D == 128 && p.dtype == RK_F32) ? 1 : 2;
   t.tiles = (cols + 16 * t.ct - 1) / (16 * t.ct);
-  const int64_t have = t.tiles * c.B * c.H, want = 512 / (have > 0 ? have : 1);
-  const int64_t most = (c.blocks + 3) / 4;
-  t.splits = want < 1 || most < 1 ? 1 : want < most ? want : most;
+  const int64_t have = t.tiles * c.B * c.H;
+  const auto splits = [&](int64_t wgs, int64_t least) {
+    const int64_t n = wgs / (have > 0 ? have : 1), most = (c.blocks + least - 1) / least;
+    return n < 1 || most < 1 ? 1 : n < most ? n : most;
+  };
+  // Up to 512 workgroups of a block for each wavefront at least; of 16 blocks and more, up to 1024
+  // (2048 with many columns, which are slower): sequences of several lengths are not even. 16
+  // sequences of 2.7 to 8 thousand tokens, 16 heads of 128, 32 nodes: 512 85 us, 1024 82, 2048 88; 8 of
+  // 6 to 15 thousand, 32 heads of 64 on 4, 64 nodes: 1024 125, 2048 116, 4096 125. (4 of 1 to 3
+  // thousand, float32: 512 17 us, 1024 of fewer than 16 blocks 19.)
+  const int64_t few = splits(512, 4), more = splits(t.many ? 2048 : 1024, 16);
+  t.splits = few > more ? few : more;
   return t;
 }
 
-template <int D, int CT>
-static void launch_tree_cache(const TreeAttn& a, int qdt, int odt, hipStream_t st) {
+template <int D, int CT, int MODE>
+static void launch_tree_cache(const TreeAttn& a, bool many, int qdt, int odt, hipStream_t st) {
+  constexpr int F32 = RK_F32, BF16 = RK_BF16;
   const dim3 grid(static_cast<unsigned>(a.nsplit), static_cast<unsigned>(a.tiles),
                   static_cast<unsigned>(a.c.B * a.c.H));
-  if (qdt == RK_F32 && odt == RK_F32) tree_cache_kernel<D, CT, RK_F32, RK_F32><<<grid, 256, 0, st>>>(a);
-  else if (qdt == RK_F32) tree_cache_kernel<D, CT, RK_F32, RK_BF16><<<grid, 256, 0, st>>>(a);
-  else if (odt == RK_F32) tree_cache_kernel<D, CT, RK_BF16, RK_F32><<<grid, 256, 0, st>>>(a);
-  else tree_cache_kernel<D, CT, RK_BF16, RK_BF16><<<grid, 256, 0, st>>>(a);
+  if (qdt == RK_F32) {
+    if constexpr (D != 128 || CT == 1) {
+      if (odt == RK_F32) tree_cache_kernel<D, CT, F32, F32, 3, MODE><<<grid, 256, 0, st>>>(a);
+      else tree_cache_kernel<D, CT, F32, BF16, 2, MODE><<<grid, 256, 0, st>>>(a);
+    }
+  } else if (odt == RK_F32) {
+    tree_cache_kernel<D, CT, BF16, F32, 3, MODE><<<grid, 256, 0, st>>>(a);
+  } else if (many) {
+    tree_cache_kernel<D, CT, BF16, BF16, 1, MODE><<<grid, 256, 0, st>>>(a);
+  } else {
+    tree_cache_kernel<D, CT, BF16, BF16, 2, MODE><<<grid, 256, 0, st>>>(a);
+  }
 }
 
 template <int D>
 static void launch_tree(const TreeAttn& a, const TreeLaunch& t, int qdt, int odt, hipStream_t st) {
-  if constexpr (D <= 128) {
-    if (t.ct == 2) launch_tree_cache<D, 2>(a, qdt, odt, st);
+  const auto run = [&](auto mode) {
+    constexpr int M = decltype(mode)::value;
+    if constexpr (D <= 128) {
+      if (t.ct == 2) return launch_tree_cache<D, 2, M>(a, t.many, qdt, odt, st);
+    }
+    launch_tree_cache<D, 1, M>(a, t.many, qdt, odt, st);
+  };
+  if (a.slopes || a.cap2 > kBound) run(std::integral_constant<int, kModified>{});
+  else if (a.cap2 != 0.0f) run(std::integral_constant<int, kBounded>{});
+  else run(std::integral_constant<int, kPlain>{});
+  const dim3 grid(static_cast<unsigned>((a.N * a.G + 3) / 4),
+                  static_cast<unsigned>(a.c.B * a.c.H));
+  if (qdt == RK_F32 && odt == RK_F32) tree_join_kernel<D, RK_F32, RK_F32><<<grid, 256, 0, st>>>(a);
+  else if (qdt == RK_F32) tree_join_kernel<D, RK_F32, RK_BF16><<<grid, 256, 0, st>>>(a);
+  else if (odt == RK_F32) tree_join_kernel<D, RK_BF16, RK_F32><<<grid, 256, 0, st>>>(a);
+  else tree_join_kernel<D, RK_BF16, RK_BF16><<<grid, 256, 0, st>>>(a);
+}
+
+// tree_near's coefficients: the quadratic through g(z) = (tanh(u) / u - 1) / z, z = u^2, at three
+// Chebyshev nodes of 0 .. kNear^2, in units of C^2.
+static void near_coefficients(double cap2, float (&c)[3]) {
+  double z[3], g[3];
+  for (int i = 0; i < 3; ++i) {
+    z[i] = 0.5 * kNear * kNear * (1.0 + cos((2 * i + 1) * M_PI / 6.0));
+    const double u = sqrt(z[i]);
+    g[i] = (tanh(u) / u - 1.0) / z[i];
   }
-  if (t.ct == 1) launch_tree_cache<D, 1>(a, qdt, odt, st);
-  const dim3 grid(static_cast<unsigned>(a.N * a.G), static_cast<unsigned>(a.c.B * a.c.H));
-  if (qdt == RK_F32 && odt == RK_F32) tree_join_kernel<D, RK_F32, RK_F32><<<grid, 64, 0, st>>>(a);
-  else if (qdt == RK_F32) tree_join_kernel<D, RK_F32, RK_BF16><<<grid, 64, 0, st>>>(a);
-  else if (odt == RK_F32) tree_join_kernel<D, RK_BF16, RK_F32><<<grid, 64, 0, st>>>(a);
-  else tree_join_kernel<D, RK_BF16, RK_BF16><<<grid, 64, 0, st>>>(a);
+  const double d01 = (g[1] - g[0]) / (z[1] - z[0]), d12 = (g[2] - g[1]) / (z[2] - z[1]);
+  const double d = (d12 - d01) / (z[2] - z[0]);
+  const double k[3] = {g[0] - d01 * z[0] + d * z[0] * z[1], d01 - d * (z[0] + z[1]), d};
+  double unit = 1.0;
+  for (int i = 0; i < 3; ++i) {
+    unit /= cap2 * cap2;
+    c[i] = static_cast<float>(k[i] * unit);
+  }
 }
 
 static int check_tree(const rk_tree_attention_args& p) {
@@ -583,13 +719,13 @@ extern "C" int rk_tree_attention(const rk_tree_attention_args* args, float* work
     return fail(RK_ERR_UNSUPPORTED, "too many queries for one launch");
   if (!work || !aligned16(work) || work_floats < rk_tree_attention_work(args))
     return fail(RK_ERR_ARG, "attention workspace too small");
-  const bool cap = p.softcap > 0.0f;
-  const TreeAttn a{cache_args(c), p.q, p.k, p.v, p.sqb, p.sqh, p.sqs, p.skb, p.skh, p.sks, p.svb,
-                   p.svh, p.svs, p.start, p.lengths, p.seen, p.depths, p.slopes,
-                   p.start_count > 1 ? 1 : 0, p.trees > 1 ? 1 : 0, p.N, (p.N + 63) / 64, p.Hq, G,
-                   t.splits, t.tiles,
-                   cap ? 2.0f * kLog2e8 * (p.scale / p.softcap) : p.scale * kLog2e8,
-                   p.softcap * kLog2e8, work, p.out};
+  const float cap2 = p.softcap * kLog2e8;
+  TreeAttn a{cache_args(c), p.q, p.k, p.v, p.sqb, p.sqh, p.sqs, p.skb, p.skh, p.sks, p.svb,
+             p.svh, p.svs, p.start, p.lengths, p.seen, p.depths, p.slopes,
+             p.start_count > 1 ? 1 : 0, p.trees > 1 ? 1 : 0, p.N, (p.N + 63) / 64, p.Hq, G,
+             t.splits, t.tiles, p.scale * kLog2e8, cap2, cap2 > 0.0f ? 1.0f / cap2 : 0.0f, {},
+             work, p.out};
+  if (cap2 > 0.0f) near_coefficients(cap2, a.near);
   hipStream_t st = as_stream(stream);
   if (c.D == 64) launch_tree<64>(a, t, p.dtype, p.out_dtype, st);
   else if (c.D == 128) launch_tree<128>(a, t, p.dtype, p.out_dtype, st);

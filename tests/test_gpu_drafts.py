@@ -9,7 +9,10 @@ scaling: it is off by at most
 The sums over T tokens run over 64 at a time, then over blocks, wavefronts and splits: at most
 T / 64 + 64 + 32 roundings of 2^-24, twice (numerator and denominator). bfloat16 results take
 probabilities to 2^-16 and are rounded once, by 2^-8 of themselves; float32 ones by 2^-24, their
-probabilities to 2^-24."""
+probabilities to 2^-24. Where more than 32 queries share a key head, bfloat16 results of bfloat16
+queries take each probability over the cache rounded to bfloat16, by at most 2^-8 of itself: numerator
+and denominator are sums of the same rounded numbers w (1 + e), |e| <= 2^-8, so a result moves by
+at most sum p |e| |v - o| <= 2^-8 (sum p |v| + |o|) <= 2^-7 sum p |v|."""
 
 from __future__ import annotations
 
@@ -100,7 +103,7 @@ def check_attention(q, k, v, cache, start, parents, lengths=None, cap=0.0, slope
     got = tree_attention(q, k, v, cache, start, tree, lengths=lengths, softcap=cap or None,
                          slopes=slopes, out_dtype=out_dtype, scale=scale)
     assert got.shape == q.shape and got.dtype == (out_dtype or q.dtype)
-    got = got.double().cpu()
+    got_dtype, got = got.dtype, got.double().cpu()
     n, d = q.shape[2:]
     keys, values = (t.double().cpu() for t in int8_kv_read(cache))
     half = got.dtype, torch.finfo(out_dtype or q.dtype).eps / 2
@@ -117,6 +120,8 @@ def check_attention(q, k, v, cache, start, parents, lengths=None, cap=0.0, slope
             slopes.double().cpu() if slopes is not None else None,
             scale or 1.0 / math.sqrt(d))
         few = 2.0**-16 if (out_dtype or q.dtype) == torch.bfloat16 else 2.0**-24
+        if n * q.shape[1] // k.shape[1] > 32 and q.dtype == torch.bfloat16 == got_dtype:
+            few = 2.0**-7
         bound = ((2 * delta + 2 * (s / 64 + 96) * 2.0**-24 + few) * size + half[1] * want.abs())
         worst = ((got[b, :, :there] - want).abs() - bound).max().item()
         assert worst <= 0.0, (b, s, worst)
