@@ -15,7 +15,8 @@
 namespace rk {
 
 // ---------------------------------------------------------------------------
-// The plan: grid (trees), 256 threads; thread i walks from node i to the root.
+// The plan: grid (trees), 256 threads; thread i walks from node i to the root. A launch's latency
+// bounds it (16 trees of 32 nodes: 4.6 us).
 // ---------------------------------------------------------------------------
 struct TreePlan {
   const void* parents;  // int32 or int64 [R][N], row stride ldp
@@ -66,8 +67,19 @@ __global__ __launch_bounds__(kTreeNodes) void draft_tree_kernel(TreePlan a) {
 // 16 (l / 16) .. + 15: key 16 g + 4 t + e is row 4 g + e of product t, and the same 16 keys are
 // the lane's k slots of the second product (8 for each half), whose other operand, 16 tokens of one
 // feature, lies side by side in the cache. bf16 queries enter as they are, float32 ones as sums of
-// three bf16 numbers; probabilities as sums of two (2^-16 of themselves) for bf16 results, three
-// for float32.
+// three bf16 numbers; probabilities as sums of three for float32 results and of two (2^-16 of
+// themselves) for bf16 ones, but of more than 32 columns as one (2^-8, as a bf16
+// result itself; the sum in the denominator is of the same rounded numbers): there the products of the second
+// part are what the matrix units have no time for (64 nodes of 8 query heads a key head: 160 us with
+// two, 147 with one).
+//
+// What bounds it: up to 32 columns, the cache's bytes (16 sequences of 2.7 to 8 thousand tokens, 16 heads
+// of 128, 32 nodes: 349 MB in 83 us, 4.2 TB/s of the 5.0 that a copy reaches); with more, the vector
+// instructions of the scores, 72 % busy: an exponential, a cap and a bf16 rounding for each (8 sequences
+// of 6 to 15 thousand, 32 heads of 64 on 4, 64 nodes, capped: 116 us; the two products alone, 38 us at the
+// rate of a large matrix product). Few tokens: the latency of one pass, 5 us at 200. Two tiles of
+// columns a wavefront: the codes are widened once for both; four spill or leave one wavefront a SIMD,
+// and are slower. The join takes 4 us for a few rows, 14 for 16384 columns.
 // ---------------------------------------------------------------------------
 struct TreeAttn {
   Kv8 c;

@@ -241,7 +241,7 @@ __device__ __forceinline__ bool all_rows(const Verify& a) { return a.top_k > 0 &
 
 enum { kGreedy, kTopK, kAll };  // what a row's statistics are for
 
-// grid (parts, B * N, 1 or 2: target, drafter): a row's statistics, or a part's.
+// grid (B * N, parts, 1 or 2: target, drafter): a row's statistics, or a part's.
 template <int DT, int kStatThreads, int MODE>
 __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(Verify a) {
   constexpr int WAVES = kStatThreads / 64, VN = Vec<DT>::N, STEP = VN * kStatThreads;
@@ -251,8 +251,8 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(Verify a) {
   __shared__ uint64_t best[WAVES];
   __shared__ double sums[WAVES], ranked[kStatThreads];
   __shared__ int box[3];
-  const uint32_t un = static_cast<uint32_t>(a.N), ub = blockIdx.y / un;
-  const int64_t b = ub, n = blockIdx.y - ub * un, skip = blockIdx.x * a.part;
+  const uint32_t un = static_cast<uint32_t>(a.N), ub = blockIdx.x / un;
+  const int64_t b = ub, n = blockIdx.x - ub * un, skip = blockIdx.y * a.part;
   const int64_t V = a.V - skip < a.part ? a.V - skip : a.part;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool drafter = blockIdx.z != 0;
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(Verify a) {
     if (!__syncthreads_or(child)) return;
   }
   RowStat* const out =
-      a.parts_of + ((drafter ? a.B * a.N : 0) + b * a.N + n) * a.parts + blockIdx.x;
+      a.parts_of + ((drafter ? a.B * a.N : 0) + b * a.N + n) * a.parts + blockIdx.y;
 
   if constexpr (MODE == kGreedy) {  // the first largest
     uint64_t top = 0;
@@ -933,13 +933,13 @@ __global__ __launch_bounds__(LAST ? 1024 : kTreeNodes) void verify_walk_kernel(V
   walk<DT, DRAFTS, LAST>(a, blockIdx.x, begin);
 }
 
-// grid (parts of a row, B), 256 threads: the segments' sums that a sequence's walk asked for. (The
+// grid (B, parts of a row), 256 threads: the segments' sums that a sequence's walk asked for. (The
 // workgroup that ends last going on with the walk itself, behind a fence and a counter, made it
 // 22 to 57 us instead of 9 and a launch of the walk of 6: each workgroup's fence writes a cache back.)
 template <int DT, bool DRAFTS>
 __global__ __launch_bounds__(kPassThreads) void verify_pass_kernel(Verify a) {
   __shared__ double table[kExpSteps];
-  const int64_t b = blockIdx.y;
+  const int64_t b = blockIdx.x;
   WalkState& w = a.states[b];
   const int tid = threadIdx.x, lane = tid & 63;
   const bool wanted = w.request, bare = w.bare;
@@ -948,8 +948,8 @@ __global__ __launch_bounds__(kPassThreads) void verify_pass_kernel(Verify a) {
   exp_table(table, tid);
   __syncthreads();
   const Segments rows(a.V);
-  const int step = static_cast<int>(gridDim.x) * (kPassThreads / 64);
-  for (int s = static_cast<int>(blockIdx.x) * (kPassThreads / 64) + (tid >> 6); s < rows.count;
+  const int step = static_cast<int>(gridDim.y) * (kPassThreads / 64);
+  for (int s = static_cast<int>(blockIdx.y) * (kPassThreads / 64) + (tid >> 6); s < rows.count;
        s += step) {
     float t = 0.0f;
     const double sum = left.segment(s, rows.per, lane, bare, a.c, t);
@@ -993,7 +993,7 @@ static int64_t stat_bytes(const rk_verify_drafts_args& p) {
 template <int DT, bool DRAFTS>
 static void launch_walk(const Verify& a, int rounds, hipStream_t st) {
   const unsigned B = static_cast<unsigned>(a.B);
-  const dim3 grid(static_cast<unsigned>((a.V + 2047) / 2048 < 64 ? (a.V + 2047) / 2048 : 64), B);
+  const dim3 grid(B, static_cast<unsigned>((a.V + 2047) / 2048 < 64 ? (a.V + 2047) / 2048 : 64));
   for (int r = 0; r < rounds; ++r) {
     verify_walk_kernel<DT, DRAFTS, false><<<B, kTreeNodes, 0, st>>>(a, r == 0);
     verify_pass_kernel<DT, DRAFTS><<<grid, kPassThreads, 0, st>>>(a);
@@ -1034,7 +1034,7 @@ extern "C" int rk_verify_drafts(const rk_verify_drafts_args* args, void* work,
   const int64_t strides[] = {p.lb, p.ln, p.db, p.dn};
   for (int64_t st : strides)
     if (st < 0) return fail(RK_ERR_ARG, "negative stride");
-  if (p.V >= (int64_t{1} << 31) - (int64_t{1} << 20) || p.B * p.N > 65535)
+  if (p.V >= (int64_t{1} << 31) - (int64_t{1} << 20) || p.B * p.N >= (int64_t{1} << 22))
     return fail(RK_ERR_UNSUPPORTED, "too many logits for one launch");
   if (!work || !aligned16(work) || work_bytes < rk_verify_drafts_work(args))
     return fail(RK_ERR_ARG, "verification workspace too small");
@@ -1050,7 +1050,7 @@ extern "C" int rk_verify_drafts(const rk_verify_drafts_args* args, void* work,
                         : nullptr,
                  p.path, p.counts, p.next};
   hipStream_t st = as_stream(stream);
-  const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(p.B * p.N), drafts ? 2 : 1);
+  const dim3 grid(static_cast<unsigned>(p.B * p.N), static_cast<unsigned>(parts), drafts ? 2 : 1);
   const int mode = greedy ? kGreedy : p.top_k > 0 && p.top_k < p.V ? kTopK : kAll;
   const auto run = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;

@@ -9,8 +9,9 @@ prologues quantize on the GPU and hand int8 rows straight to the ratchet GEMMs.
 Additions: ``ffn_hidden`` (default ``4 * n_embd``, the reference's hard-coded width,
 ``model.py:137``) so 1B-class shapes with FFN 5632 can be built; ``attention_softcap`` and
 ``distance_bias`` (scores capped by a tanh, and falling with the distance), masks of packed
-documents and their prefixes in ``forward`` (``scored_attention.py``), and a key/value cache in
-8 bits (``new_cache(dtype=torch.int8)``, ``int8_cache.py``).
+documents and their prefixes in ``forward`` (``scored_attention.py``), a key/value cache in
+8 bits (``new_cache(dtype=torch.int8)``, ``int8_cache.py``), and steps over trees of drafted tokens
+(``tree_logits``, ``commit_drafts``, ``drafts.py``).
 """
 
 from __future__ import annotations
@@ -166,6 +167,7 @@ class KVCache:
         self.step_buffers: dict[str, Tensor] = {}  # fixed-shape work buffers of a step
         # keys and values of drafted nodes, a layer's [B, H, N, D] each, until they are committed
         self.drafted: list[tuple[Tensor, Tensor] | None] = [None] * n_layer
+        self.drafted_at = 0  # the length they stand behind
 
     def buffers(self, layer: int, like: Tensor) -> tuple[Tensor, Tensor]:
         """The layer's key/value buffers, allocated on first use in the cache dtype
@@ -233,8 +235,8 @@ class KVCache:
         `count` of `path` [1, N], which `counts` [1] says on the device. One sequence only (its
         positions are the batch's)."""
         check_batch(self.batch)
-        if any(kept is None for kept in self.drafted):
-            raise ValueError("no drafts to commit")
+        if any(kept is None for kept in self.drafted) or self.drafted_at != self.length:
+            raise ValueError("no drafts to commit behind what the cache holds")
         if not 0 <= count <= path.shape[1] or path.shape[0] != 1:
             raise ValueError("path must hold the count's nodes of one sequence")
         if self.length + count > self.max_len:
@@ -840,6 +842,7 @@ class RatchetGPT(nn.Module):
         if cache.length + deepest >= cache.max_len:
             raise ValueError("KV cache is full")
         cache.check_open()
+        cache.drafted_at = cache.length
         if (self.fused_decode and isinstance(cache, Int8KVCache)
                 and fused_decode_supported(self, cache, tokens.shape[1])):
             return fused_tree_logits(self, tokens, tree, cache)

@@ -57,6 +57,10 @@ def test_committed_nodes_are_as_if_prefilled():
     assert (a - b).abs().max() <= 2.0**-14 * b.abs().max()
     with pytest.raises(ValueError, match="no drafts"):
         model.commit_drafts(cache, found)
+    model.tree_logits(tokens, draft_tree(parents), cache)
+    model.decode_step(torch.tensor([[9]]), cache)  # the cache moves on without them
+    with pytest.raises(ValueError, match="no drafts"):
+        model.commit_drafts(cache, found)
 
 
 @pytest.mark.parametrize("shape", [(1,), (1, 1, 1, 1), (3, 2), (2, 1, 2), (4,)])

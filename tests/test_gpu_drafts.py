@@ -539,6 +539,18 @@ def test_logits_that_want_gradients(cuda):
                        ints(cuda, 1))
 
 
+def test_many_sequences(cuda):
+    """More rows than a launch's second and third dimensions hold."""
+    gen = torch.Generator().manual_seed(1)
+    logits = (torch.randn(1, 9, generator=gen) * 2).expand(70_000, 9)
+    u = torch.rand(70_000, generator=gen)
+    got = sample_tokens(logits.to(cuda), u.to(cuda))
+    sums = logits[0].double().softmax(0).cumsum(0)
+    assert (sums[None] - u.double()[:, None] * sums[-1]).abs().min() > 1e-12
+    want = (sums[None] <= u.double()[:, None] * sums[-1]).sum(1)
+    assert torch.equal(got.cpu(), want)
+
+
 def test_verification_operator(cuda):
     logits, tokens, uniforms, other = (t.to(cuda) for t in choice(2, 4, 50, 4, True))
     tree = draft_tree([-1, 0, 0, 1], cuda)
