@@ -70,8 +70,8 @@ __global__ __launch_bounds__(kTreeNodes) void draft_tree_kernel(TreePlan a) {
 // three bf16 numbers; probabilities as sums of three for float32 results and of two (2^-16 of
 // themselves) for bf16 ones, but of more than 32 columns as one (2^-8, as a bf16
 // result itself; the sum in the denominator is of the same rounded numbers): there the products of the second
-// part are what the matrix units have no time for (64 nodes of 8 query heads a key head: 160 us with
-// two, 147 with one).
+// part are what the matrix units have no time for (64 nodes of 8 query heads a key head: 137 us with
+// two, 116 with one).
 //
 // What bounds it: up to 32 columns, the cache's bytes (16 sequences of 2.7 to 8 thousand tokens, 16 heads
 // of 128, 32 nodes: 349 MB in 83 us, 4.2 TB/s of the 5.0 that a copy reaches); with more, the vector

@@ -241,7 +241,10 @@ __device__ __forceinline__ bool all_rows(const Verify& a) { return a.top_k > 0 &
 
 enum { kGreedy, kTopK, kAll };  // what a row's statistics are for
 
-// grid (B * N, parts, 1 or 2: target, drafter): a row's statistics, or a part's.
+// grid (B * N * parts, 1 or 2: target, drafter): a row's statistics, or a part's. A row's parts are
+// neighbours: all rows' first parts one after the other, a power of two of bytes apart, took 101 us
+// where this takes 65 (512 rows of 131072 bf16 logits that are looked at: 134 MB and as many 64-bit
+// exponentials, which bound it). Top-k rows: 25 us for 32 MB, the bins and the candidates' ranks.
 template <int DT, int kStatThreads, int MODE>
 __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(Verify a) {
   constexpr int WAVES = kStatThreads / 64, VN = Vec<DT>::N, STEP = VN * kStatThreads;
@@ -251,11 +254,12 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(Verify a) {
   __shared__ uint64_t best[WAVES];
   __shared__ double sums[WAVES], ranked[kStatThreads];
   __shared__ int box[3];
-  const uint32_t un = static_cast<uint32_t>(a.N), ub = blockIdx.x / un;
-  const int64_t b = ub, n = blockIdx.x - ub * un, skip = blockIdx.y * a.part;
+  const uint32_t un = static_cast<uint32_t>(a.N), up = static_cast<uint32_t>(a.parts);
+  const uint32_t at = blockIdx.x / up, p = blockIdx.x - at * up, ub = at / un;
+  const int64_t b = ub, n = at - ub * un, skip = p * a.part;
   const int64_t V = a.V - skip < a.part ? a.V - skip : a.part;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const bool drafter = blockIdx.z != 0;
+  const bool drafter = blockIdx.y != 0;
   const void* const row = static_cast<const typename Vec<DT>::Elem*>(row_at<DT>(a, drafter, b, n)) +
                           skip;
   float ref = load_elem<DT>(row, 0);
@@ -269,7 +273,7 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(Verify a) {
     if (!__syncthreads_or(child)) return;
   }
   RowStat* const out =
-      a.parts_of + ((drafter ? a.B * a.N : 0) + b * a.N + n) * a.parts + blockIdx.y;
+      a.parts_of + ((drafter ? a.B * a.N : 0) + b * a.N + n) * a.parts + p;
 
   if constexpr (MODE == kGreedy) {  // the first largest
     uint64_t top = 0;
@@ -926,20 +930,22 @@ __device__ __forceinline__ void walk(const Verify& a, int64_t b, bool begin) {
   if (lane == 0) a.next[b] = token >= 0 ? token : weighty;
 }
 
-// grid (B): a walk from its begin, or what the rounds left of it.
+// grid (B): a walk from its begin, or what the rounds left of it. Latencies of dependent reads bound it:
+// 17 us with its own passes over 8192 tokens (26 nodes), 7 a launch between passes of the device's.
 template <int DT, bool DRAFTS, bool LAST>
 __global__ __launch_bounds__(LAST ? 1024 : kTreeNodes) void verify_walk_kernel(Verify a,
                                                                                 bool begin) {
   walk<DT, DRAFTS, LAST>(a, blockIdx.x, begin);
 }
 
-// grid (B, parts of a row), 256 threads: the segments' sums that a sequence's walk asked for. (The
+// grid (B * parts of a row), 256 threads: the segments' sums that a sequence's walk asked for. (The
 // workgroup that ends last going on with the walk itself, behind a fence and a counter, made it
 // 22 to 57 us instead of 9 and a launch of the walk of 6: each workgroup's fence writes a cache back.)
 template <int DT, bool DRAFTS>
-__global__ __launch_bounds__(kPassThreads) void verify_pass_kernel(Verify a) {
+__global__ __launch_bounds__(kPassThreads) void verify_pass_kernel(Verify a, int parts) {
   __shared__ double table[kExpSteps];
-  const int64_t b = blockIdx.x;
+  const int64_t b = blockIdx.x / static_cast<uint32_t>(parts);
+  const int part = static_cast<int>(blockIdx.x - static_cast<uint32_t>(b * parts));
   WalkState& w = a.states[b];
   const int tid = threadIdx.x, lane = tid & 63;
   const bool wanted = w.request, bare = w.bare;
@@ -948,9 +954,8 @@ __global__ __launch_bounds__(kPassThreads) void verify_pass_kernel(Verify a) {
   exp_table(table, tid);
   __syncthreads();
   const Segments rows(a.V);
-  const int step = static_cast<int>(gridDim.y) * (kPassThreads / 64);
-  for (int s = static_cast<int>(blockIdx.y) * (kPassThreads / 64) + (tid >> 6); s < rows.count;
-       s += step) {
+  const int step = parts * (kPassThreads / 64);
+  for (int s = part * (kPassThreads / 64) + (tid >> 6); s < rows.count; s += step) {
     float t = 0.0f;
     const double sum = left.segment(s, rows.per, lane, bare, a.c, t);
     if (lane == 0) {
@@ -993,10 +998,12 @@ static int64_t stat_bytes(const rk_verify_drafts_args& p) {
 template <int DT, bool DRAFTS>
 static void launch_walk(const Verify& a, int rounds, hipStream_t st) {
   const unsigned B = static_cast<unsigned>(a.B);
-  const dim3 grid(B, static_cast<unsigned>((a.V + 2047) / 2048 < 64 ? (a.V + 2047) / 2048 : 64));
+  const int64_t most = 65536 / a.B < 1 ? 1 : 65536 / a.B < 64 ? 65536 / a.B : 64;
+  const int64_t parts = (a.V + 2047) / 2048 < most ? (a.V + 2047) / 2048 : most;
+  const unsigned grid = B * static_cast<unsigned>(parts);
   for (int r = 0; r < rounds; ++r) {
     verify_walk_kernel<DT, DRAFTS, false><<<B, kTreeNodes, 0, st>>>(a, r == 0);
-    verify_pass_kernel<DT, DRAFTS><<<grid, kPassThreads, 0, st>>>(a);
+    verify_pass_kernel<DT, DRAFTS><<<grid, kPassThreads, 0, st>>>(a, static_cast<int>(parts));
   }
   verify_walk_kernel<DT, DRAFTS, true><<<B, 1024, 0, st>>>(a, rounds == 0);
 }
@@ -1050,7 +1057,7 @@ extern "C" int rk_verify_drafts(const rk_verify_drafts_args* args, void* work,
                         : nullptr,
                  p.path, p.counts, p.next};
   hipStream_t st = as_stream(stream);
-  const dim3 grid(static_cast<unsigned>(p.B * p.N), static_cast<unsigned>(parts), drafts ? 2 : 1);
+  const dim3 grid(static_cast<unsigned>(p.B * p.N * parts), drafts ? 2 : 1);
   const int mode = greedy ? kGreedy : p.top_k > 0 && p.top_k < p.V ? kTopK : kAll;
   const auto run = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
