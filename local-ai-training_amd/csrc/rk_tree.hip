@@ -68,18 +68,18 @@ __global__ __launch_bounds__(kTreeNodes) void draft_tree_kernel(TreePlan a) {
 // the lane's k slots of the second product (8 for each half), whose other operand, 16 tokens of one
 // feature, lies side by side in the cache. bf16 queries enter as they are, float32 ones as sums of
 // three bf16 numbers; probabilities as sums of three for float32 results and of two (2^-16 of
-// themselves) for bf16 ones, but of more than 32 columns as one (2^-8, as a bf16
-// result itself; the sum in the denominator is of the same rounded numbers): there the products of the second
-// part are what the matrix units have no time for (64 nodes of 8 query heads a key head: 137 us with
-// two, 116 with one).
+// themselves) for bf16 ones, but of more than 32 columns as one (2^-8, like a bf16 result's own
+// rounding; the denominator sums the same rounded numbers): with many columns the second part's
+// products and roundings are no longer hidden behind the cache's bytes (64 nodes of 8 query heads a key
+// head: 137 us with two, 116 with one).
 //
 // What bounds it: up to 32 columns, the cache's bytes (16 sequences of 2.7 to 8 thousand tokens, 16 heads
-// of 128, 32 nodes: 349 MB in 83 us, 4.2 TB/s of the 5.0 that a copy reaches); with more, the vector
-// instructions of the scores, 72 % busy: an exponential, a cap and a bf16 rounding for each (8 sequences
-// of 6 to 15 thousand, 32 heads of 64 on 4, 64 nodes, capped: 116 us; the two products alone, 38 us at the
-// rate of a large matrix product). Few tokens: the latency of one pass, 5 us at 200. Two tiles of
-// columns a wavefront: the codes are widened once for both; four spill or leave one wavefront a SIMD,
-// and are slower. The join takes 4 us for a few rows, 14 for 16384 columns.
+// of 128, 32 nodes: 349 MB in 82 us, 4.3 TB/s of the 5.0 that a copy reaches); with more, the vector
+// instructions of the scores, 65 % of the time: an exponential, a cap and a bf16 rounding for each (8
+// sequences of 6 to 15 thousand, 32 heads of 64 on 4, 64 nodes, capped: 117 us; the two products alone,
+// 38 us at the rate of a large matrix product). Few tokens: the latency of one pass, 5 us at 300. Two
+// tiles of columns a wavefront: the codes are widened once for both; four spill or leave one wavefront a
+// SIMD (172 us where two took 147). The join takes 4 us for a few rows, 14 for 16384 columns.
 // ---------------------------------------------------------------------------
 struct TreeAttn {
   Kv8 c;
@@ -116,8 +116,9 @@ __device__ __forceinline__ float tree_capped(float y, float cap2, float inv_cap2
   }
   return t;
 }
-// The same for |y| <= kNear C by y (1 + z (c0 + c1 z + c2 z^2)), z = y^2: half the instructions. The
-// host interpolates (tanh(u) / u - 1) / u^2 at Chebyshev nodes of u^2 (off by 2e-7 of the score).
+// The same for |y| <= kNear C by y (1 + z (c0 + c1 z + c2 z^2)), z = y^2: half the instructions (64 nodes
+// of 8 query heads a key head: 160 us with the exponential form, 147 with this one). The host interpolates
+// (tanh(u) / u - 1) / u^2 at Chebyshev nodes of u^2 (off by 2e-7 of the score).
 constexpr float kNear = 0.4f;
 __device__ __forceinline__ float tree_near(float y, const float (&c)[3]) {
   const float z = y * y;
@@ -127,7 +128,8 @@ __device__ __forceinline__ float tree_near(float y, const float (&c)[3]) {
 }
 
 // What is done to the scores: nothing; a cap of so little (kBounded) that their exponentials need no
-// maximum, in units of which 2^60 is the most; a cap, a bias or both.
+// maximum, 2^60 being the most (147 us with the maximum, 120 without, at 64 nodes of 8 query heads a key
+// head); a cap, a bias or both.
 enum { kPlain, kBounded, kModified };
 constexpr float kBound = 60.0f;
 

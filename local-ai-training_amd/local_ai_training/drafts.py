@@ -164,13 +164,14 @@ def verify_drafts(logits: Tensor, tokens: Tensor, tree: DraftTree,
     With p, q the softmax of the target's and the drafter's logits at a node over ``temperature``,
     without logits below the ``top_k``-th largest: the node's children are tried in their order; one of
     token x stands if u q(x) < p(x), otherwise p becomes max(p - q, 0) over its sum (but for sums up to
-    2^-40, of drafts that q does not hold: then p stays). Where none stands, the next token is the first whose cumulated p passes the root's u times its sum. The
-    children of a node must have been drawn from q independently; without ``draft_logits`` each counts
-    as certain (drafts from a lookup, or the drafter's best). At temperature 0 a child stands if its
-    token is the target's first largest logit's.
+    2^-40, of drafts that q does not hold: then p stays). Where none stands, the next token is the first
+    whose cumulated p passes the root's u times its sum. The children of a node must have been drawn
+    from q independently; without ``draft_logits`` each counts as certain (drafts from a lookup, or the
+    drafter's best). At temperature 0 a child stands if its token is the target's first largest logit's.
 
     Of a sequence's nodes the first ``lengths`` [B] are there (none: count 0, next -1). A row that is
-    no distribution (a NaN, an infinity) gives next -1. Decisions are made in 64 bits. Logits of other
+    no distribution (a NaN, +inf, only -inf) gives next -1 (at temperature 0 a NaN is the largest, as
+    in torch's argmax). Decisions are made in 64 bits. Logits of other
     types than float32 and bfloat16 are taken as float32."""
     if logits.dtype not in _NATIVE or (draft_logits is not None
                                        and draft_logits.dtype != logits.dtype):
