@@ -878,12 +878,13 @@ int rk_tree_attention(const rk_tree_attention_args* args, float* work, int64_t w
  * logits at node n over the temperature, of those not below the top_k-th largest (0: all),
  * the walk begins at node 0; a child c of the node reached (in their order, token x) stands if
  * u_c q(x) < p(x), otherwise p becomes max(p - q, 0) over its sum (a sum up to 2^-40 is rounding:
- * then p stays); without drafts q is 1 at x. Where no child stands, next is the first token whose cumulated p passes u_0 times its sum. Temperature 0
- * (else at least 1e-6): a child stands if its token is the first largest logit's, which is next
- * otherwise; uniforms and drafts are not read. path [B][N]: the nodes that stand from the root on,
+ * then p stays); without drafts q is 1 at x. Where no child stands, next is the first token whose
+ * cumulated p passes u_0 times its sum. Temperature 0 (else at least 1e-6): a child stands if its token
+ * is the first largest logit's (a NaN is above all), which is next otherwise; uniforms and drafts are
+ * not read. path [B][N]: the nodes that stand from the root on,
  * then -1; counts [B]: how many; next [B]. A sequence without nodes has count 0 and next -1; a row
  * that is no distribution (a NaN, +inf, or -inf only) lets no child stand and gives next -1; a
- * token outside 0 .. V - 1 does not stand. Probabilities and their sums are 64-bit numbers. work:
+ * child whose token is outside 0 .. V - 1 is taken as not there. Probabilities and their sums are 64-bit numbers. work:
  * rk_verify_drafts_work bytes, 16-byte aligned.
  * Replaces: the draw of one token, generate.py:180-197 (N = 1).
  */

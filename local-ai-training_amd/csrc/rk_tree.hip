@@ -694,7 +694,8 @@ extern "C" int rk_draft_tree(const void* parents, int wide, int64_t ldp, int64_t
   if (N > kTreeNodes) return fail(RK_ERR_UNSUPPORTED, "a tree has at most %d nodes", kTreeNodes);
   if (R == 0 || N == 0) return RK_OK;
   if (!parents || !kept || !depths || !seen) return fail(RK_ERR_ARG, "null pointer");
-  if (R >= (int64_t{1} << 31)) return fail(RK_ERR_UNSUPPORTED, "too many trees");
+  // a launch holds fewer than 2^24 blocks of 256 threads
+  if (R >= (int64_t{1} << 24)) return fail(RK_ERR_UNSUPPORTED, "too many trees");
   const TreePlan a{parents, wide, ldp, N, (N + 63) / 64, kept, depths, seen};
   draft_tree_kernel<<<static_cast<unsigned>(R), kTreeNodes, 0, as_stream(stream)>>>(a);
   return launch_status("draft_tree");

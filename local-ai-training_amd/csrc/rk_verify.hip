@@ -819,6 +819,10 @@ __device__ __forceinline__ void walk(const Verify& a, int64_t b, bool begin) {
   for (i = child(i);;) {
     while (i < n && !(DRAFTS && pending)) {
       bool stands;
+      if (tok[i] < 0) {  // no token: a child that is not there
+        i = child(i + 1);
+        continue;
+      }
       if (greedy) {
         stands = tok[i] == pick;
       } else if constexpr (DRAFTS) {

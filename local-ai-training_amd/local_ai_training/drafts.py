@@ -169,7 +169,8 @@ def verify_drafts(logits: Tensor, tokens: Tensor, tree: DraftTree,
     from q independently; without ``draft_logits`` each counts as certain (drafts from a lookup, or the
     drafter's best). At temperature 0 a child stands if its token is the target's first largest logit's.
 
-    Of a sequence's nodes the first ``lengths`` [B] are there (none: count 0, next -1). A row that is
+    Of a sequence's nodes the first ``lengths`` [B] are there (none: count 0, next -1); a child whose
+    token is outside 0 .. V - 1 is taken as not there. A row that is
     no distribution (a NaN, +inf, only -inf) gives next -1 (at temperature 0 a NaN is the largest, as
     in torch's argmax). Decisions are made in 64 bits. Logits of other
     types than float32 and bfloat16 are taken as float32."""

@@ -3,12 +3,14 @@ target's distribution as it is."""
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import draft_reference as plain
+from local_ai_training import _native as nat
 from local_ai_training import drafts
 from local_ai_training.drafts import (DraftTree, draft_tree, int8_kv_commit, sample_tokens,
                                       torch_tree_attention, tree_attention, verify_drafts)
@@ -32,6 +34,15 @@ def test_plan(nodes):
 def test_parents_on_the_host_are_checked(parents):
     with pytest.raises(ValueError, match="parent"):
         draft_tree(parents)
+
+
+def test_more_trees_than_a_launch_holds():
+    i64, fake = ctypes.c_int64, ctypes.c_void_p(1 << 12)  # never dereferenced
+    lib = nat.load_library()
+    status = lib.rk_draft_tree(fake, 0, i64(1), i64(1 << 24), i64(1), fake, fake, fake, None)
+    assert status == 3 and b"too many trees" in lib.rk_last_error()
+    assert lib.rk_draft_tree(fake, 0, i64(1), i64(0), i64(1), fake, fake, fake, None) == 0
+    assert lib.rk_last_error() == b""
 
 
 def test_plans_that_are_refused():

@@ -486,6 +486,25 @@ def test_unknown_tokens_do_not_stand(cuda):
     assert got.path.tolist() == [[0, 2, -1], [0, 2, -1], [0, -1, -1]]
 
 
+@pytest.mark.parametrize("vocab", [250, 20000])
+@pytest.mark.parametrize("drafter", [False, True])
+def test_unknown_tokens_leave_the_distribution_as_it_is(cuda, drafter, vocab):
+    """Trees filled up with children of no token: what stands and follows is as without them."""
+    gen = torch.Generator().manual_seed(5)
+    logits = torch.randn(40, 6, vocab, generator=gen)
+    other = logits + torch.randn(40, 6, vocab, generator=gen) if drafter else None
+    uniforms = torch.rand(40, 6, generator=gen)
+    tokens = torch.randint(vocab, (40, 6), generator=gen)
+    tokens[:, 1] = -1
+    tokens[::2, 3] = vocab
+    parents = [-1, 0, 0, 0, 1, 2]
+    got = verify_drafts(logits.to(cuda), tokens.to(cuda), draft_tree(parents, cuda),
+                        uniforms.to(cuda),
+                        draft_logits=other.to(cuda) if drafter else None)
+    want = verify_drafts(logits, tokens, draft_tree(parents), uniforms, draft_logits=other)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
 def test_logits_in_strides_and_other_types(cuda):
     logits, tokens, uniforms, other = (t.to(cuda) for t in choice(3, 6, 250, 4, True))
     tree = draft_tree(plain.random_parents(6, 1, 2), cuda)
