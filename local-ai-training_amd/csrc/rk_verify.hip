@@ -525,6 +525,7 @@ struct Residual {
   int64_t V;
   double c32;
   int k;
+  bool few;  // k-th largest logits
   const double *scale, *table;
   const int* rejected;
 
@@ -532,8 +533,8 @@ struct Residual {
                                       const RowStat& ds, const double* scale, const int* rejected,
                                       const double* table)
       : row(row_at<DT>(a, false, b, cur)), drow(DRAFTS ? row_at<DT>(a, true, b, cur) : nullptr),
-        st(st), ds(ds), V(a.V), c32(a.c * kExpSteps), k(k), scale(scale), table(table),
-        rejected(rejected) {}
+        st(st), ds(ds), V(a.V), c32(a.c * kExpSteps), k(k), few(all_rows(a)), scale(scale),
+        table(table), rejected(rejected) {}
 
   __device__ __forceinline__ void load(const void* from, int64_t i, float (&x)[4]) const {
     const auto* const at = static_cast<const typename Vec<DT>::Elem*>(from) + i;
@@ -558,30 +559,33 @@ struct Residual {
     float x[4], y[4];
     load(row, i, x);
     if (DRAFTS && k > 0) load(drow, i, y);
-    // (nothing is left of what p does not hold: most of a row below its k-th largest logit)
-    const float t = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    if (!__any(t >= st.floor) && st.inv == st.inv) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = 0.0;
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = i + e < V ? chance(x[e], st, c32, table) : 0.0;
-    if constexpr (DRAFTS) {
-      if (k > 0) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
+    const auto token = [&](int e) {
+      double t = i + e < V ? chance(x[e], st, c32, table) : 0.0;
+      if constexpr (DRAFTS) {
+        if (k > 0) {
           const double q = chance(y[e], ds, c32, table);
-          double t = r[e];
 #pragma unroll 1
           for (int j = 0; j < k; ++j) {
             t = t - q;
             t = (t < 0.0 ? 0.0 : t) * (j + 1 < k ? scale[j] : 1.0);
           }
-          r[e] = t;
         }
       }
+      r[e] = t;
+    };
+    if (few) {
+      // nothing is left of what p does not hold, most of a row below its k-th largest logit: a
+      // wavefront's 64 tokens at a time (a walk of some passes over 8192 tokens 17 -> 15 us)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        r[e] = 0.0;
+        if (__any(x[e] >= st.floor) || st.inv != st.inv) token(e);
+      }
     } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) token(e);
+    }
+    if constexpr (!DRAFTS) {
       for (int j = 0; j < k; ++j) {
         const int64_t gone = rejected[j] - i;
 #pragma unroll
@@ -935,7 +939,7 @@ __device__ __forceinline__ void walk(const Verify& a, int64_t b, bool begin) {
 }
 
 // grid (B): a walk from its begin, or what the rounds left of it. Latencies of dependent reads bound it:
-// 17 us with its own passes over 8192 tokens (26 nodes), 7 a launch between passes of the device's.
+// 15 us with its own passes over 8192 tokens (26 nodes), 7 a launch between passes of the device's.
 template <int DT, bool DRAFTS, bool LAST>
 __global__ __launch_bounds__(LAST ? 1024 : kTreeNodes) void verify_walk_kernel(Verify a,
                                                                                 bool begin) {
@@ -969,14 +973,17 @@ __global__ __launch_bounds__(kPassThreads) void verify_pass_kernel(Verify a, int
   }
 }
 
-// Passes over rows of up to kOwnPass tokens are the walk's own workgroup's (4 to 5 us at 8192, 25 at
-// 32003 with a drafter, where the device's with the launches it takes is 20); over larger ones the device
-// shares them, so many of a sequence's one after the other. A chain needs one; a tree's walk one more for
-// each rejected child but its last. A round that no sequence needs takes 4 us; one too few, of 131072
+// Passes over rows of up to kOwnPass tokens, or twice as many of which few have a probability (top_k),
+// are the walk's own workgroup's (4 to 5 us at 8192, 25 at 32003 with a drafter, where the device's with
+// the launches it takes is 20; a call with top_k and a drafter, 16 sequences of 13 nodes: 42 us at 32000
+// tokens where the device's passes make it 47, 58 and 55 at 50000). Over larger ones the device shares
+// them, so many of a sequence's one after the other. A chain needs one; a tree's walk one more for each
+// rejected child but its last. A round that no sequence needs takes 4 us; one too few, of 131072
 // tokens, 60.
 constexpr int64_t kOwnPass = 16384;
 static int verify_rounds(const rk_verify_drafts_args& p) {
-  if (p.temperature == 0.0 || p.V <= kOwnPass) return 0;
+  const bool few = p.top_k > 0 && p.top_k < p.V;
+  if (p.temperature == 0.0 || p.V <= (few ? 2 : 1) * kOwnPass) return 0;
   return !p.drafts ? 1 : p.V <= 4 * kOwnPass ? 2 : 6;
 }
 
