@@ -979,12 +979,13 @@ __global__ __launch_bounds__(kPassThreads) void verify_pass_kernel(Verify a, int
 // tokens where the device's passes make it 47, 58 and 55 at 50000). Over larger ones the device shares
 // them, so many of a sequence's one after the other. A chain needs one; a tree's walk one more for each
 // rejected child but its last. A round that no sequence needs takes 4 us; one too few, of 131072
-// tokens, 60.
+// tokens, up to 60. (16 trees of 64 nodes with four children each, eight sets of drafts: 141 to 267 us
+// with six rounds, 160 on the average; with eight 148 to 176, 156; with eleven 160 to 188, 167.)
 constexpr int64_t kOwnPass = 16384;
 static int verify_rounds(const rk_verify_drafts_args& p) {
   const bool few = p.top_k > 0 && p.top_k < p.V;
   if (p.temperature == 0.0 || p.V <= (few ? 2 : 1) * kOwnPass) return 0;
-  return !p.drafts ? 1 : p.V <= 4 * kOwnPass ? 2 : 6;
+  return !p.drafts ? 1 : p.V <= 4 * kOwnPass ? 2 : 8;
 }
 
 // Logits of a part of a row: a multiple of 4096 (what 256 threads have in flight), 8192 at least, up
