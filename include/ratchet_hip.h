@@ -847,9 +847,8 @@ int rk_draft_tree(const void* parents, int wide, int64_t ldp, int64_t R, int64_t
  * rk_scored_attention_forward. out: [B, N, Hq, D] contiguous, float32 or bf16; zeros for nodes that
  * are off or not there and for negative starts, NaN for starts past the cache. Over the cache bf16
  * queries enter as they are, float32 ones as sums of three bf16 numbers; probabilities as sums of
- * three for float32 results, of two for bf16 ones, and as one if the queries are bf16 too and more
- * than 32 share a key head (N Hq / H); the nodes' part is float32. work: rk_tree_attention_work
- * floats, 16-byte aligned.
+ * three for float32 results, of two for bf16 ones; the nodes' part is float32. work:
+ * rk_tree_attention_work floats, 16-byte aligned.
  * No counterpart in the reference (it drafts nothing, generate.py:183-201).
  */
 typedef struct rk_tree_attention_args {

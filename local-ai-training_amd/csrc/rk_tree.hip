@@ -68,18 +68,18 @@ __global__ __launch_bounds__(kTreeNodes) void draft_tree_kernel(TreePlan a) {
 // the lane's k slots of the second product (8 for each half), whose other operand, 16 tokens of one
 // feature, lies side by side in the cache. bf16 queries enter as they are, float32 ones as sums of
 // three bf16 numbers; probabilities as sums of three for float32 results and of two (2^-16 of
-// themselves) for bf16 ones, but of more than 32 columns as one (2^-8, like a bf16 result's own
-// rounding; the denominator sums the same rounded numbers): with many columns the second part's
-// products and roundings are no longer hidden behind the cache's bytes (64 nodes of 8 query heads a key
-// head: 137 us with two, 116 with one).
+// themselves) for bf16 ones, whatever the tree's size. (One, 2^-8 of themselves, beside more than 32
+// columns took 116 us where two take 137 at 64 nodes of 8 query heads a key head, and left a result off
+// by 2.2e-3 of the norm instead of the 1.7e-3 of its own rounding.)
 //
 // What bounds it: up to 32 columns, the cache's bytes (16 sequences of 2.7 to 8 thousand tokens, 16 heads
-// of 128, 32 nodes: 349 MB in 82 us, 4.3 TB/s of the 5.0 that a copy reaches); with more, the vector
-// instructions of the scores, 65 % of the time: an exponential, a cap and a bf16 rounding for each (8
-// sequences of 6 to 15 thousand, 32 heads of 64 on 4, 64 nodes, capped: 117 us; the two products alone,
-// 38 us at the rate of a large matrix product). Few tokens: the latency of one pass, 5 us at 300. Two
-// tiles of columns a wavefront: the codes are widened once for both; four spill or leave one wavefront a
-// SIMD (172 us where two took 147). The join takes 4 us for a few rows, 14 for 16384 columns.
+// of 128, 32 nodes: 349 MB in 82 us, 4.3 TB/s of the 5.0 that a copy reaches); with more, vector
+// instructions (8 sequences of 6 to 15 thousand, 32 heads of 64 on 4, 64 nodes, capped: 137 us a call;
+// the two products alone, 38 us at the rate of a large matrix product). Of a block and two tiles of
+// columns a lane widens 128 codes with 192 instructions, 6 for each of its 32 scores, more than a cap (5), an
+// exponential (1) or the two roundings (3) take; every two tiles widen the block anew. Few tokens: the
+// latency of one pass, 5 us at 300. Two tiles of columns a wavefront: the codes are widened once for both;
+// four spill or leave one wavefront a SIMD (172 us where two took 147). The join takes 4 us for a few rows, 14 for 16384 columns.
 // ---------------------------------------------------------------------------
 struct TreeAttn {
   Kv8 c;
@@ -117,7 +117,7 @@ __device__ __forceinline__ float tree_capped(float y, float cap2, float inv_cap2
   return t;
 }
 // The same for |y| <= kNear C by y (1 + z (c0 + c1 z + c2 z^2)), z = y^2: half the instructions (64 nodes
-// of 8 query heads a key head: 160 us with the exponential form, 147 with this one). The host interpolates
+// of 8 query heads a key head: 146 us with the exponential form, 137 with this one). The host interpolates
 // (tanh(u) / u - 1) / u^2 at Chebyshev nodes of u^2 (off by 2e-7 of the score).
 constexpr float kNear = 0.4f;
 __device__ __forceinline__ float tree_near(float y, const float (&c)[3]) {
@@ -128,16 +128,17 @@ __device__ __forceinline__ float tree_near(float y, const float (&c)[3]) {
 }
 
 // What is done to the scores: nothing; a cap of so little (kBounded) that their exponentials need no
-// maximum, 2^60 being the most (147 us with the maximum, 120 without, at 64 nodes of 8 query heads a key
+// maximum, 2^60 being the most (155 us with the maximum, 137 without, at 64 nodes of 8 query heads a key
 // head); a cap, a bias or both.
 enum { kPlain, kBounded, kModified };
 constexpr float kBound = 60.0f;
 
-template <int D, int CT, int QDT, int ODT, int NP, int MODE>
+template <int D, int CT, int QDT, int ODT, int MODE>
 __global__ __launch_bounds__(256) void tree_cache_kernel(TreeAttn a) {
   constexpr int KK = D / 64, FT = D / 16, NW = 4;
   constexpr int QP = QDT == RK_F32 ? 3 : 1;
   constexpr bool FINE = ODT == RK_F32;
+  constexpr int NP = FINE ? 3 : 2;  // bf16 numbers of a probability
   __shared__ float box[2][CT * (4 * FT + 2)][64];
   const int split = blockIdx.x;
   const int64_t tile = blockIdx.y, bh = blockIdx.z;
@@ -576,8 +577,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttn a) {
 // Host side
 // ---------------------------------------------------------------------------
 struct TreeLaunch {
-  int ct;   // tiles of 16 columns a wavefront holds
-  bool many;  // so many columns that probabilities of bf16 results are one bf16 number each
+  int ct;  // tiles of 16 columns a wavefront holds
   int64_t tiles, splits;
 };
 
@@ -585,7 +585,7 @@ static TreeLaunch tree_launch(const rk_tree_attention_args& p) {
   const rk_int8_kv& c = p.cache;
   const int64_t cols = p.N * (p.Hq / c.H);
   TreeLaunch t{};
-  t.many = cols > 32 && p.dtype == RK_BF16 && p.out_dtype == RK_BF16;
+  const bool many = cols > 32 && p.dtype == RK_BF16 && p.out_dtype == RK_BF16;
   t.ct = c.D > 128 || cols <= 16 || (c.D == 128 && p.dtype == RK_F32) ? 1 : 2;
   t.tiles = (cols + 16 * t.ct - 1) / (16 * t.ct);
   const int64_t have = t.tiles * c.B * c.H;
@@ -596,29 +596,27 @@ static TreeLaunch tree_launch(const rk_tree_attention_args& p) {
   // Up to 512 workgroups of a block for each wavefront at least; of 16 blocks and more, up to 1024
   // (2048 with many columns, which are slower): sequences of several lengths are not even. 16
   // sequences of 2.7 to 8 thousand tokens, 16 heads of 128, 32 nodes: 512 85 us, 1024 82, 2048 88; 8 of
-  // 6 to 15 thousand, 32 heads of 64 on 4, 64 nodes: 1024 125, 2048 116, 4096 125. (4 of 1 to 3
+  // 6 to 15 thousand, 32 heads of 64 on 4, 64 nodes: 1024 155, 2048 137, 4096 146. (4 of 1 to 3
   // thousand, float32: 512 17 us, 1024 of fewer than 16 blocks 19.)
-  const int64_t few = splits(512, 4), more = splits(t.many ? 2048 : 1024, 16);
+  const int64_t few = splits(512, 4), more = splits(many ? 2048 : 1024, 16);
   t.splits = few > more ? few : more;
   return t;
 }
 
 template <int D, int CT, int MODE>
-static void launch_tree_cache(const TreeAttn& a, bool many, int qdt, int odt, hipStream_t st) {
+static void launch_tree_cache(const TreeAttn& a, int qdt, int odt, hipStream_t st) {
   constexpr int F32 = RK_F32, BF16 = RK_BF16;
   const dim3 grid(static_cast<unsigned>(a.nsplit), static_cast<unsigned>(a.tiles),
                   static_cast<unsigned>(a.c.B * a.c.H));
   if (qdt == RK_F32) {
     if constexpr (D != 128 || CT == 1) {
-      if (odt == RK_F32) tree_cache_kernel<D, CT, F32, F32, 3, MODE><<<grid, 256, 0, st>>>(a);
-      else tree_cache_kernel<D, CT, F32, BF16, 2, MODE><<<grid, 256, 0, st>>>(a);
+      if (odt == RK_F32) tree_cache_kernel<D, CT, F32, F32, MODE><<<grid, 256, 0, st>>>(a);
+      else tree_cache_kernel<D, CT, F32, BF16, MODE><<<grid, 256, 0, st>>>(a);
     }
   } else if (odt == RK_F32) {
-    tree_cache_kernel<D, CT, BF16, F32, 3, MODE><<<grid, 256, 0, st>>>(a);
-  } else if (many) {
-    tree_cache_kernel<D, CT, BF16, BF16, 1, MODE><<<grid, 256, 0, st>>>(a);
+    tree_cache_kernel<D, CT, BF16, F32, MODE><<<grid, 256, 0, st>>>(a);
   } else {
-    tree_cache_kernel<D, CT, BF16, BF16, 2, MODE><<<grid, 256, 0, st>>>(a);
+    tree_cache_kernel<D, CT, BF16, BF16, MODE><<<grid, 256, 0, st>>>(a);
   }
 }
 
@@ -627,9 +625,9 @@ static void launch_tree(const TreeAttn& a, const TreeLaunch& t, int qdt, int odt
   const auto run = [&](auto mode) {
     constexpr int M = decltype(mode)::value;
     if constexpr (D <= 128) {
-      if (t.ct == 2) return launch_tree_cache<D, 2, M>(a, t.many, qdt, odt, st);
+      if (t.ct == 2) return launch_tree_cache<D, 2, M>(a, qdt, odt, st);
     }
-    launch_tree_cache<D, 1, M>(a, t.many, qdt, odt, st);
+    launch_tree_cache<D, 1, M>(a, qdt, odt, st);
   };
   if (a.slopes || a.cap2 > kBound) run(std::integral_constant<int, kModified>{});
   else if (a.cap2 != 0.0f) run(std::integral_constant<int, kBounded>{});
