@@ -884,7 +884,7 @@ int rk_tree_attention(const rk_tree_attention_args* args, float* work, int64_t w
  * then -1; counts [B]: how many; next [B]. A sequence without nodes has count 0 and next -1; a row
  * that is no distribution (a NaN, +inf, or -inf only) lets no child stand and gives next -1; a
  * child whose token is outside 0 .. V - 1 is taken as not there. Probabilities and their sums are 64-bit numbers. work:
- * rk_verify_drafts_work bytes, 16-byte aligned.
+ * rk_verify_drafts_work bytes (0 for sizes that the call refuses), 16-byte aligned.
  * Replaces: the draw of one token, generate.py:180-197 (N = 1).
  */
 typedef struct rk_verify_drafts_args {

@@ -990,6 +990,12 @@ static int verify_rounds(const rk_verify_drafts_args& p) {
   return !p.drafts ? 1 : p.V <= 4 * kOwnPass ? 2 : 8;
 }
 
+// Rows of a launch: fewer than 2^22. (Each factor by itself first: a product may not fit 64 bits.)
+static bool too_many(const rk_verify_drafts_args& p) {
+  constexpr int64_t kRows = int64_t{1} << 22;
+  return p.B >= kRows || p.B * p.N >= kRows || p.V >= (int64_t{1} << 31) - (int64_t{1} << 20);
+}
+
 // Logits of a part of a row: a multiple of 4096 (what 256 threads have in flight), 8192 at least, up
 // to eight parts a row and some thousand workgroups. (With one of 256 threads a row, 512 rows of
 // 131072 had two wavefronts a SIMD: 106 us, in four parts 62.)
@@ -1027,7 +1033,9 @@ static void launch_walk(const Verify& a, int rounds, hipStream_t st) {
 using namespace rk;
 
 extern "C" int64_t rk_verify_drafts_work(const rk_verify_drafts_args* args) {
-  if (!args || args->B <= 0 || args->N <= 0) return 0;
+  if (!args || args->B <= 0 || args->N <= 0 || args->V <= 0 || args->N > kTreeNodes ||
+      too_many(*args))
+    return 0;
   return stat_bytes(*args) +
          (verify_rounds(*args) ? args->B * static_cast<int64_t>(sizeof(WalkState)) : 0);
 }
@@ -1055,7 +1063,7 @@ extern "C" int rk_verify_drafts(const rk_verify_drafts_args* args, void* work,
   const int64_t strides[] = {p.lb, p.ln, p.db, p.dn};
   for (int64_t st : strides)
     if (st < 0) return fail(RK_ERR_ARG, "negative stride");
-  if (p.V >= (int64_t{1} << 31) - (int64_t{1} << 20) || p.B * p.N >= (int64_t{1} << 22))
+  if (too_many(p))
     return fail(RK_ERR_UNSUPPORTED, "too many logits for one launch");
   if (!work || !aligned16(work) || work_bytes < rk_verify_drafts_work(args))
     return fail(RK_ERR_ARG, "verification workspace too small");
