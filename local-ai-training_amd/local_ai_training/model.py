@@ -838,6 +838,8 @@ class RatchetGPT(nn.Module):
 
         if tokens.dim() != 2 or tokens.shape[0] != cache.batch:
             raise ValueError("tokens must be [B, N] with the cache's batch")
+        if tree.depths.shape not in ((1, tokens.shape[1]), tokens.shape):
+            raise ValueError("the tree must hold one row or one per sequence, of these nodes")
         deepest = tokens.shape[1] - 1 if deepest is None else deepest
         if cache.length + deepest >= cache.max_len:
             raise ValueError("KV cache is full")

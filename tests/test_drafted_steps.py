@@ -1,0 +1,42 @@
+"""A tree's step on the host: trees and tokens that do not belong together, and steps that fail."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from local_ai_training.drafts import Verified, draft_tree
+from local_ai_training.model import ModelConfig, build_seeded_model
+
+
+def model_of(n_layer=2):
+    config = ModelConfig(vocab_size=40, block_size=48, n_layer=n_layer, n_head=2, n_embd=32,
+                         ffn_hidden=64)
+    return build_seeded_model(config, max_code=2, seed=3).eval()
+
+
+def tokens_of(b, s):
+    return torch.randint(0, 40, (b, s), generator=torch.Generator().manual_seed(s))
+
+
+@pytest.mark.parametrize("batch,nodes,parents", [
+    (1, 1, [-1, 0, 1]), (1, 4, [-1]), (1, 3, [-1, 0]), (1, 2, [[-1, 0]] * 2), (2, 2, [[-1, 0]] * 3),
+    (2, 1, [-1, 0])])
+@pytest.mark.parametrize("past", [0, 5])
+def test_trees_of_other_sizes_than_the_tokens_are_refused(past, batch, nodes, parents):
+    model = model_of()
+    cache = model.new_cache(batch)
+    if past:
+        model.prefill(tokens_of(batch, past), cache)
+    with pytest.raises(ValueError, match="tree"):
+        model.tree_logits(tokens_of(batch, nodes), draft_tree(parents), cache)
+    assert cache.length == past and cache.drafted == [None, None]
+
+
+def test_one_tree_for_all_or_one_for_each():
+    model = model_of()
+    cache, tokens = model.new_cache(2), tokens_of(2, 3)
+    model.prefill(tokens_of(2, 5), cache)
+    one = model.tree_logits(tokens, draft_tree([-1, 0, 0]), cache)
+    each = model.tree_logits(tokens, draft_tree([[-1, 0, 0], [-1, 0, 1]]), cache)
+    assert torch.equal(one[0], each[0]) and not torch.equal(one[1, 2], each[1, 2])
