@@ -844,7 +844,8 @@ class RatchetGPT(nn.Module):
         if cache.length + deepest >= cache.max_len:
             raise ValueError("KV cache is full")
         cache.check_open()
-        cache.drafted_at = cache.length
+        # (a step that fails half-way leaves nothing to commit)
+        cache.drafted, cache.drafted_at = [None] * cache.n_layer, cache.length
         if (self.fused_decode and isinstance(cache, Int8KVCache)
                 and fused_decode_supported(self, cache, tokens.shape[1])):
             return fused_tree_logits(self, tokens, tree, cache)

@@ -40,3 +40,26 @@ def test_one_tree_for_all_or_one_for_each():
     one = model.tree_logits(tokens, draft_tree([-1, 0, 0]), cache)
     each = model.tree_logits(tokens, draft_tree([[-1, 0, 0], [-1, 0, 1]]), cache)
     assert torch.equal(one[0], each[0]) and not torch.equal(one[1, 2], each[1, 2])
+
+
+def test_a_step_that_fails_leaves_nothing_to_commit():
+    """Half a step's keys and values beside those of an earlier one are not committed."""
+    model = model_of()
+    cache, tree = model.new_cache(1), draft_tree([-1, 0, 1])
+    model.prefill(tokens_of(1, 5), cache)
+    model.tree_logits(tokens_of(1, 3), tree, cache)
+
+    def refuse(*args, **kw):
+        raise RuntimeError("out of memory")
+
+    last = model.blocks[1]
+    forward, last.forward = last.forward, refuse
+    with pytest.raises(RuntimeError, match="memory"):
+        model.tree_logits((tokens_of(1, 3) + 1) % 40, tree, cache)
+    last.forward = forward
+    found = Verified(torch.tensor([[0, 1, -1]]), torch.tensor([2]), torch.tensor([9]))
+    with pytest.raises(ValueError, match="no drafts"):
+        model.commit_drafts(cache, found)
+    assert cache.length == 5
+    model.tree_logits(tokens_of(1, 3), tree, cache)
+    assert model.commit_drafts(cache, found) == ([0, 1], 9) and cache.length == 7
