@@ -811,7 +811,7 @@ int rk_int8_kv_attention(const rk_int8_kv* cache, const void* q, int qdtype, int
  * shape, each its own buffers): token i < counts[b] of sequence b is node path[b][i] of that layer's k
  * and v (float32 or bf16 [B, H, N, D] as in rk_int8_kv_append, all layers the same dtype), and goes
  * to position start + i. path: device int64 [B][P], row stride path_step; counts: device int64 [B],
- * at most P of which count; nodes outside 0 .. N - 1 are tokens of zeros. Blocks and scales as in
+ * at most P of which count; nodes outside 0 .. N - 1 (N > 0) are tokens of zeros. Blocks and scales as in
  * rk_int8_kv_append.
  * No counterpart in the reference (it drafts nothing, generate.py:183-201).
  */

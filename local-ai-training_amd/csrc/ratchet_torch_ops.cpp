@@ -1482,6 +1482,7 @@ void int8_kv_commit(at::TensorList ks, at::TensorList vs, at::TensorList keys,
   TORCH_CHECK_VALUE(shape.size() == 5 && ks[0].dim() == 4, what,
                     ": keys must be [B, H, blocks, 64, D], k [B, H, N, D]");
   const int64_t B = shape[0], N = ks[0].size(2);
+  TORCH_CHECK_VALUE(N > 0, what, ": at least the root is needed");
   const int64_t kv[] = {B, shape[1], N, shape[4]};
   TORCH_CHECK_TYPE(ks[0].is_floating_point(), what, ": k and v must be floating point");
   for (size_t i = 0; i < n; ++i) {

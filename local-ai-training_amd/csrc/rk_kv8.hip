@@ -1153,7 +1153,8 @@ extern "C" int rk_int8_kv_commit(const rk_int8_kv_commit_layer* layers, int64_t 
   }
   if (start_count != 1 && start_count != c.B)
     return fail(RK_ERR_ARG, "one start, or one per sequence");
-  if (c.B == 0 || c.H == 0 || c.blocks == 0 || P == 0 || N == 0) return RK_OK;
+  if (c.B == 0 || c.H == 0 || c.blocks == 0 || P == 0) return RK_OK;
+  if (N == 0) return fail(RK_ERR_ARG, "no nodes");
   if (!start || !path || !counts) return fail(RK_ERR_ARG, "null pointer");
   if (path_step < 0) return fail(RK_ERR_ARG, "negative stride");
   for (int64_t i = 0; i < count; ++i)
