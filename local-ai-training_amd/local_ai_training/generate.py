@@ -242,7 +242,7 @@ class _Drafter:
         stood, following = self.model.commit_drafts(self.cache, found)
         self.draft.commit_drafts(self.draft_cache, found)
         if following < 0:
-            raise RuntimeError("the model's logits are no distribution")
+            raise RuntimeError("the model's or the drafter's logits are no distribution")
         return tokens[0, stood[1:]].tolist() + [following]
 
 

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from local_ai_training.drafts import Verified, draft_tree
+from local_ai_training.generate import generate
 from local_ai_training.model import ModelConfig, build_seeded_model
 
 
@@ -63,3 +64,16 @@ def test_a_step_that_fails_leaves_nothing_to_commit():
     assert cache.length == 5
     model.tree_logits(tokens_of(1, 3), tree, cache)
     assert model.commit_drafts(cache, found) == ([0, 1], 9) and cache.length == 7
+
+
+@pytest.mark.parametrize("broken", ["model", "draft"])
+def test_rows_that_are_no_distribution_name_both_sides(broken):
+    """A residual needs both distributions: the error does not blame the model for its drafter."""
+    letters = tuple(chr(48 + i) for i in range(40))
+    sides = {"model": model_of(), "draft": model_of(1)}
+    model, draft = sides["model"], sides["draft"]
+    cached = sides[broken].tree_logits  # (a prompt's logits stay whole)
+    sides[broken].tree_logits = lambda *args, **kw: cached(*args, **kw) * torch.nan
+    with pytest.raises(RuntimeError, match="model's or the drafter's logits"):
+        generate(model, letters, "01", max_new_tokens=6, temperature=0.9, seed=1, draft=draft,
+                 draft_shape=(1, 1))
