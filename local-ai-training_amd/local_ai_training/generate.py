@@ -269,9 +269,12 @@ def generate(
 
     With a `draft` model over the same vocabulary, tokens are proposed by it and judged by `model`, a
     tree at a time: `draft_shape` gives the children of a node, level by level. The text is
-    distributed as without it (at temperature 0 it is the same, up to logits whose order the
-    summation order decides), but drawn from other random numbers. Near the windows' end, and
-    behind it, tokens are produced one by one."""
+    distributed by the logits of `model`'s tree steps (at temperature 0 it follows their largest), but
+    drawn from other random numbers than without a draft. Those logits are the single steps' up to the
+    order of float32 sums, which int8 layers can turn into another code of an activation; over an 8-bit
+    cache, nodes are also seen as they are until they are committed, where a single step sees its own
+    token's codes. Near the windows' end, and behind it, tokens are produced one by one. Rounds are not
+    captured (`use_graph` replays what is produced one by one) and wait for the device."""
     if max_new_tokens < 0:
         raise ValueError("max_new_tokens must be non-negative")
     if temperature < 0:
