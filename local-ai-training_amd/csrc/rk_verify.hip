@@ -245,8 +245,8 @@ enum { kGreedy, kTopK, kAll };  // what a row's statistics are for
 
 // grid (B * N * parts, 1 or 2: target, drafter): a row's statistics, or a part's. A row's parts are
 // neighbours: all rows' first parts one after the other, a power of two of bytes apart, took 101 us
-// where this takes 65 (512 rows of 131072 bf16 logits that are looked at: 134 MB and as many 64-bit
-// exponentials, which bound it). Top-k rows: 25 us for 32 MB, the bins and the candidates' ranks.
+// where this took 65, 70 with the exponential's fifth power (512 rows of 131072 bf16 logits that are
+// looked at: 134 MB and 67 million 64-bit exponentials, whose instructions take 47 us to issue). Top-k rows: 25 us for 32 MB, the bins and the candidates' ranks.
 template <int DT, int kStatThreads, int MODE>
 __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(Verify a) {
   constexpr int WAVES = kStatThreads / 64, VN = Vec<DT>::N, STEP = VN * kStatThreads;
@@ -979,10 +979,13 @@ __global__ __launch_bounds__(kPassThreads) void verify_pass_kernel(Verify a, int
 // are the walk's own workgroup's (4 to 5 us at 8192, 25 at 32003 with a drafter, where the device's with
 // the launches it takes is 20; a call with top_k and a drafter, 16 sequences of 13 nodes: 42 us at 32000
 // tokens where the device's passes make it 47, 58 and 55 at 50000). Over larger ones the device shares
-// them, so many of a sequence's one after the other. A chain needs one; a tree's walk one more for each
-// rejected child but its last. A round that no sequence needs takes 4 us; one too few, of 131072
-// tokens, up to 60. (16 trees of 64 nodes with four children each, eight sets of drafts: 141 to 267 us
-// with six rounds, 160 on the average; with eight 148 to 176, 156; with eleven 160 to 188, 167.)
+// them, so many of a sequence's one after the other. A chain's walk needs one pass, a tree's one more for each
+// rejected child but its last, so up to the number of nodes but the root; the rule does not look at the
+// nodes. A round that no sequence needs takes 4 us, so a chain or a single draft over a large vocabulary
+// beside a drafter waits 28 us for seven (a sequence of 13 nodes, top_k: 36 us at 50000 tokens, 62 at
+// 100000); one too few, of 131072 tokens, up to 60. (16 trees of 64 nodes with four children each, eight
+// sets of drafts: 141 to 267 us with six rounds, 160 on the average; with eight 148 to 176, 156, and 151
+// to 180, 159, in another run; with eleven 160 to 188, 167.)
 constexpr int64_t kOwnPass = 16384;
 static int verify_rounds(const rk_verify_drafts_args& p) {
   const bool few = p.top_k > 0 && p.top_k < p.V;
