@@ -202,14 +202,15 @@ __global__ __launch_bounds__(256) void tree_cache_kernel(TreeAttn a) {
     load_v(j);
     // the queries: features 64 kk + 16 g .. + 15 of each tile's column
     v8bf_a qf[CT][QP][KK][2];
-    float slope2[CT], pos[CT];
+    float slope2[CT];
+    int depth[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const int64_t ct = (tile * CT + c) * 16 + col, cc = ct < cols ? ct : cols - 1;
       const int64_t i = static_cast<uint32_t>(cc) / ug, hd = kvh * a.G + (cc - i * a.G);
       const int64_t base = b * a.sqb + hd * a.sqh + i * a.sqs + 16 * g;
       slope2[c] = a.slopes ? a.slopes[hd] * kLog2e8 : 0.0f;
-      pos[c] = static_cast<float>(start + a.depths[b * a.tree_step * a.N + i]);
+      depth[c] = a.depths[b * a.tree_step * a.N + i];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         if constexpr (QDT == RK_BF16) {
@@ -258,7 +259,6 @@ __global__ __launch_bounds__(256) void tree_cache_kernel(TreeAttn a) {
       const int64_t ahead = start - (j * kTok + 16 * g);
       const int left = ahead > 16 ? 16 : ahead < 0 ? 0 : static_cast<int>(ahead);
       const bool whole = (j + 1) * kTok <= start;
-      const float first = static_cast<float>(j * kTok + 16 * g);
       // a tile's probabilities from its scores, with the running maximum and sum
       const auto weigh = [&](int c, const v4f_a (&s)[4], v8bf_a (&p)[NP][2]) {
         float y[16];
@@ -282,7 +282,8 @@ __global__ __launch_bounds__(256) void tree_cache_kernel(TreeAttn a) {
           }
         }
         if (MODE == kModified && a.slopes) {
-          const float d0 = pos[c] - first;
+          // (whole numbers: positions pass 2^24; a head's codes bound them to 2^25)
+          const float d0 = static_cast<float>(static_cast<int>(ahead) + depth[c]);
 #pragma unroll
           for (int x = 0; x < 16; ++x) y[x] = __builtin_fmaf(-slope2[c], d0 - x, y[x]);
         }
