@@ -12,6 +12,15 @@ from local_ai_training.model import ModelConfig, build_seeded_model
 LETTERS = tuple("abcdef")
 
 
+@pytest.fixture(autouse=True)
+def one_thread():
+    """Rows of 32 numbers: threads only wait for each other."""
+    threads = torch.get_num_threads()
+    torch.set_num_threads(1)
+    yield
+    torch.set_num_threads(threads)
+
+
 def model_of(seed, **kw):
     config = ModelConfig(**{"vocab_size": 6, "block_size": 12, "n_layer": 1, "n_head": 2,
                             "n_embd": 32, "ffn_hidden": 64, **kw})
