@@ -673,7 +673,9 @@ __device__ __forceinline__ void walk(const Verify& a, int64_t b, bool begin) {
   bool served = false;   // the pass that the walk stopped for is there
   bool bare = false;     // the row of `cur` has no statistics
   float most = 0.0f;     // its largest logit then
-  double rest = 1.0;     // without a drafter: what the rejected tokens left
+  // without a drafter: what the rejected tokens left, off by some 2^-48 (a rejected token leaves 2^-24 of
+  // it at least, the step of the numbers below 1)
+  double rest = 1.0;
   RowStat own{}, other{};  // of the row of `cur` where the walk began again
   int own_of = -1;
   if (!begin) {
